@@ -318,6 +318,164 @@ int tg_gat_aggregate(tg_spmm_plan_t plan, int64_t n, int64_t heads, int64_t f,
                      tg_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Element types of the entry points below that take void* data.
+ * ------------------------------------------------------------------------ */
+enum { TG_TYPE_F32 = 0, TG_TYPE_BF16 = 1, TG_TYPE_F16 = 2 };
+
+/* ------------------------------------------------------------------------
+ * Layer norm over the rows of x [rows x cols] (no counterpart in the
+ * reference): y = (x - mean) * rstd * gamma + beta, with mean and variance of
+ * the row (the variance about the mean, divided by cols) and rstd =
+ * 1 / sqrt(variance + eps), all in fp32; y is rounded to `type` once.
+ * gamma / beta: cols values of `weight_type` (TG_TYPE_F32 or `type`), NULL = 1
+ * / 0.  mean / rstd: rows floats for the backward pass, or NULL.  Leading
+ * dimensions are in elements, at least cols; any alignment.  y may be x (with
+ * the same leading dimension).
+ *
+ * tg_layer_norm_backward: from dy and the forward's x, mean, rstd
+ *   t = dy * gamma, xh = (x - mean) * rstd,
+ *   dx = rstd * (t - mean(t) - xh * mean(t * xh)),
+ *   dgamma = sum over rows of dy * xh, dbeta = sum over rows of dy,
+ * the sums in fp32 in an order that depends on the sizes only (the results of
+ * equal calls are the same bits).  dx, dgamma, dbeta may be NULL; dx may be dy.
+ * dgamma / dbeta have `weight_type`.  With no rows they are zeros.
+ * workspace: tg_layer_norm_backward_workspace_size bytes (0 where neither
+ * dgamma nor dbeta is wanted), or NULL.
+ * ------------------------------------------------------------------------ */
+int tg_layer_norm(int64_t rows, int64_t cols, int type, const void* x, int64_t ldx,
+                  const void* gamma, const void* beta, int weight_type, float eps, void* y,
+                  int64_t ldy, float* mean, float* rstd, tg_stream_t stream);
+size_t tg_layer_norm_backward_workspace_size(int64_t rows, int64_t cols);
+int tg_layer_norm_backward(int64_t rows, int64_t cols, int type, const void* dy, int64_t lddy,
+                           const void* x, int64_t ldx, const void* gamma, int weight_type,
+                           const float* mean, const float* rstd, void* dx, int64_t lddx,
+                           void* dgamma, void* dbeta, void* workspace, size_t workspace_bytes,
+                           tg_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Routing rows to experts (no counterpart in the reference).
+ *
+ * tg_route: p = softmax of each row of logits [tokens x experts] in fp32; the
+ * k largest logits of a row are its experts, in falling order, the lower index
+ * first among equals; weights[t*k + j] = p of the j-th, or with renormalize
+ * that divided by the sum over the k.  A logit of -inf (a masked expert) is
+ * never chosen: where a row has fewer than k others, the places left over hold
+ * expert -1 and weight 0 (a row of -inf alone goes nowhere).  A NaN is not
+ * chosen either; it, and a logit of +inf, make the row's weights NaN.
+ * At most 1,024 experts, k at most 32 and at most experts.
+ *
+ * The plan lists the rows in expert order, for the grouped products: slot
+ * t*k + j of expert e goes to place p in [offsets[e], offsets[e + 1]), in the
+ * order of the slots; rows[p] = t and position[t*k + j] = p; slots of no
+ * expert have position -1, and the places from offsets[experts] on rows -1.
+ * offsets [experts + 1], rows and position [tokens * k].  All three may be NULL
+ * together (weights and experts only).
+ *
+ * tg_route_plan: the plan of n slots whose groups are given (node types: k = 1):
+ * rows[p] = slot / k.  An id outside [0, groups) is a slot of no group.
+ *
+ * tg_route_backward: dlogits from dweights, the logits and tg_route's weights
+ * and experts: p_i * (g_i - sum_j dweights_j * w_j), g_i = dweights_j where i
+ * is the j-th expert and 0 elsewhere; with renormalize w_j * (dweights_j -
+ * sum_j dweights_j * w_j) at the chosen and 0 elsewhere.  dweights of places
+ * without an expert are not used.
+ * ------------------------------------------------------------------------ */
+size_t tg_route_workspace_size(int64_t tokens, int64_t experts, int64_t k);
+int tg_route(int64_t tokens, int64_t experts, int64_t k, int type, const void* logits,
+             int64_t ld, int renormalize, float* weights, int32_t* expert_ids,
+             int32_t* offsets, int32_t* rows, int32_t* position, void* workspace,
+             size_t workspace_bytes, tg_stream_t stream);
+size_t tg_route_plan_workspace_size(int64_t n, int64_t groups);
+int tg_route_plan(int64_t n, int64_t groups, int64_t k, const int32_t* ids, int32_t* offsets,
+                  int32_t* rows, int32_t* position, void* workspace, size_t workspace_bytes,
+                  tg_stream_t stream);
+int tg_route_backward(int64_t tokens, int64_t experts, int64_t k, int type, const void* logits,
+                      int64_t ld, int renormalize, const float* weights,
+                      const int32_t* expert_ids, const float* dweights, void* dlogits,
+                      int64_t lddl, tg_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Joining the experts' results: out[t] = sum over j < k of weights[t*k + j] *
+ * y[position[t*k + j]] over rows of `cols` elements, in fp32, j ascending,
+ * rounded once; weights NULL = all 1 (the gradient of gathered rows).  A
+ * position outside [0, y_rows) adds nothing; a row without any is 0.
+ * Backward: dy[position[t*k + j]] = weights[t*k + j] * dout[t]; rows of dy that
+ * no position names are left as they are; dweights[t*k + j] = dot of dout[t]
+ * and y[position[t*k + j]] in fp32, 0 without a position.  dy or dweights may
+ * be NULL (y is read for dweights only).  No position may occur twice.
+ * ------------------------------------------------------------------------ */
+int tg_route_combine(int64_t tokens, int64_t k, int64_t cols, int type, const void* y,
+                     int64_t y_rows, int64_t ldy, const int32_t* position,
+                     const float* weights, void* out, int64_t ldo, tg_stream_t stream);
+int tg_route_combine_backward(int64_t tokens, int64_t k, int64_t cols, int type,
+                              const void* dout, int64_t lddo, const void* y, int64_t y_rows,
+                              int64_t ldy, const int32_t* position, const float* weights,
+                              void* dy, int64_t lddy, float* dweights, tg_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Products grouped by expert or node type (no counterpart in the reference):
+ * rows [offsets[g], offsets[g + 1]) of x times matrix g.
+ *
+ * tg_grouped_matmul: y[p] = epilogue(x[p] * w_g + bias_g) for the rows p of
+ * group g; x is [x_rows x k] and with `rows` (m indices) x[rows[p]] takes the
+ * place of x[p] (an index outside [0, x_rows) is a row of zeros).  w_g is
+ * w + g * w_stride: [k x n] with leading dimension ldw or, transposed,
+ * [n x k]; the gradient of x is this product of dy with the other flag.
+ * bias [groups x n] or NULL; epilogue TG_EPI_*.  x, w, bias and y have `type`;
+ * sums are in fp32 and rounded once.  offsets: groups + 1 int32 on the device,
+ * not falling, within [0, m]; rows outside all groups are not written (of a
+ * falling or outside offset, only rows within [0, m) are ever touched).  At
+ * most 1,024 groups; m < 2^31.
+ *
+ * tg_grouped_matmul_wgrad: dw_g = (rows of x of group g)^T * (those of dy),
+ * [groups x k x n] contiguous, and dbias_g = sum of those rows of dy
+ * [groups x n] (either may be NULL); zeros for an empty group.  Deterministic.
+ * workspace: the size function's bytes, or NULL.
+ * ------------------------------------------------------------------------ */
+int tg_grouped_matmul(int64_t m, int64_t k, int64_t n, int64_t groups, int type, const void* x,
+                      int64_t x_rows, int64_t ldx, const int32_t* rows, const int32_t* offsets,
+                      const void* w, int64_t ldw, int64_t w_stride, int transposed,
+                      const void* bias, int epilogue, void* y, int64_t ldy,
+                      tg_stream_t stream);
+size_t tg_grouped_matmul_wgrad_workspace_size(int64_t m, int64_t k, int64_t n, int64_t groups,
+                                              int type);
+int tg_grouped_matmul_wgrad(int64_t m, int64_t k, int64_t n, int64_t groups, int type,
+                            const void* x, int64_t x_rows, int64_t ldx, const int32_t* rows,
+                            const void* dy, int64_t lddy, const int32_t* offsets, void* dw,
+                            void* dbias, void* workspace, size_t workspace_bytes,
+                            tg_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Products in 8-bit floating point (e4m3: OCP, largest 448) with a scale for
+ * each block of 128 (no counterpart in the reference).
+ *
+ * A scale is max(largest |x| of the block * (1/448 in fp32), 2^-126) and a
+ * value e4m3(x / scale), product and quotient rounded to fp32, the quotient then
+ * to nearest even; a NaN stays NaN, and an infinity makes its block NaN.
+ * tg_quantize: x [rows x cols] to q [rows x kp], kp = cols rounded up to whole
+ *   128 (zeros there), and scale [kp/128 x rows]: row r, block b at b*rows + r.
+ * tg_quantize_weight: w [groups][k x n] (ldw, w_stride; transposed: [n x k]) to
+ *   q [groups][n x kp] and scale [groups][ceil(n/128) x kp/128].
+ * tg_matmul_fp8: y[p] = epilogue(sum over b of xscale_b[p] * wscale_b[n/128] *
+ *   (the products of block b), + bias), sums in fp32, y and bias of `type`.
+ *   With a 16-bit `type` the products of a block go through the e4m3 matrix
+ *   instructions, whose sum is within 2^-12 of the sum of the products' sizes
+ *   (normal operands: 2^-16); with TG_TYPE_F32 it is that of an fp32 sum;
+ *   offsets NULL: one matrix for all m rows (groups = 1), else groups as for
+ *   tg_grouped_matmul; rows as there, over x_rows quantised rows.  xq and wq
+ *   are 16-byte aligned (as allocated).
+ * ------------------------------------------------------------------------ */
+int tg_quantize(int64_t rows, int64_t cols, int type, const void* x, int64_t ldx, void* q,
+                float* scale, tg_stream_t stream);
+int tg_quantize_weight(int64_t groups, int64_t k, int64_t n, int type, const void* w,
+                       int64_t ldw, int64_t w_stride, int transposed, void* q, float* scale,
+                       tg_stream_t stream);
+int tg_matmul_fp8(int64_t m, int64_t k, int64_t n, int64_t groups, const void* xq,
+                  const float* xscale, int64_t x_rows, const int32_t* rows,
+                  const int32_t* offsets, const void* wq, const float* wscale, int type,
+                  const void* bias, int epilogue, void* y, int64_t ldy, tg_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * Model -- replaces tinygnn::Model (include/tinygnn/model.hpp:89-164,
  * src/model.cpp:191-439): a sequential GCN / SAGE / GAT layer graph with
  * device-resident weights.

@@ -24,6 +24,7 @@ EPI_NONE, EPI_RELU, EPI_ELU = 0, 1, 2
 SAGE_AUTO, SAGE_CONCAT, SAGE_TRANSFORM_FIRST = 0, 1, 2
 FORWARD_REFERENCE, FORWARD_CACHED = 0, 1
 PRECISION_FAST, PRECISION_EXACT = 0, 1
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
 
 
 def _torch():
@@ -387,6 +388,452 @@ def gat_aggregate(plan: SpmmPlan, a_sl: DeviceCSR, wh, heads: int, f: int, src, 
                                    dptr(out), out.stride(0), None, 0, stream_handle(stream)))
     _finish(stream)
     return out
+
+
+# ---------------------------------------------------------------------------
+# Expert layers: norm, routing, grouped and 8-bit products.  Tensors are
+# float32, bfloat16 or float16 on one device, rows contiguous (any row stride).
+# A call runs on `stream`, or on the current stream of its tensors' device;
+# given a `stream` that is not the current one, it returns finished results.
+# Outputs and workspaces are torch memory, so the calls can be captured.
+# ---------------------------------------------------------------------------
+_TYPES: dict = {}
+
+
+def _type_of(t, what: str) -> int:
+    if not _TYPES:
+        torch = _torch()
+        _TYPES.update({torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16,
+                       torch.float16: TYPE_F16})
+    code = _TYPES.get(t.dtype)
+    if code is None:
+        raise InvalidArgument(1, f"{what}: float32, bfloat16 or float16 tensors expected, got "
+                                 f"{t.dtype}.")
+    return code
+
+
+class _Call:
+    """The device and stream of a call: every tensor on one GPU, which is made
+    the current device for the call where it is not."""
+
+    def __init__(self, what: str, stream, *tensors):
+        torch = _torch()
+        dev = tensors[0].device
+        for t in tensors:
+            if t is None:
+                continue
+            if not t.is_cuda:
+                raise ValueError("tinygnn_amd expects device (cuda) tensors")
+            if t.device != dev:
+                raise InvalidArgument(1, f"{what}: tensors on {dev} and {t.device}.")
+        self.what, self.stream, self.guard = what, stream, None
+        if dev.index != torch.cuda.current_device():
+            self.guard = torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        self.handle = stream_handle(self.stream)
+        return self
+
+    def __exit__(self, kind, value, trace):
+        try:
+            if kind is None:
+                _finish(self.stream)
+        finally:
+            if self.guard is not None:
+                self.guard.__exit__(kind, value, trace)
+        return False
+
+    def require(self, ok: bool, message: str) -> None:
+        if not ok:
+            raise InvalidArgument(1, f"{self.what}: {message}")
+
+    def rows(self, t, name: str):
+        """A 2-D tensor whose rows are contiguous, and its leading dimension."""
+        self.require(t.dim() == 2, f"{name} must be a matrix, got {tuple(t.shape)}.")
+        self.require(t.stride(1) == 1 or t.shape[1] <= 1 or t.numel() == 0,
+                     f"{name} must have contiguous rows, got strides {t.stride()}.")
+        if t.shape[0] <= 1:
+            return t.data_ptr(), max(t.shape[1], 1)
+        self.require(t.numel() == 0 or t.stride(0) >= t.shape[1],
+                     f"{name} has overlapping rows (strides {t.stride()}).")
+        return t.data_ptr(), max(t.stride(0), t.shape[1])
+
+    def flat(self, t, name: str, shape, dtype):
+        """A contiguous tensor of a given shape and type, or None."""
+        if t is None:
+            return 0
+        self.require(tuple(t.shape) == tuple(shape),
+                     f"{name} must be {tuple(shape)}, got {tuple(t.shape)}.")
+        self.require(t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}.")
+        self.require(t.is_contiguous(), f"{name} must be contiguous.")
+        return t.data_ptr()
+
+    def out(self, t, name: str, shape, like):
+        if t is None:
+            return _torch().empty(shape, dtype=like.dtype, device=like.device)
+        self.require(tuple(t.shape) == tuple(shape),
+                     f"{name} must be {tuple(shape)}, got {tuple(t.shape)}.")
+        self.require(t.dtype == like.dtype, f"{name} must be {like.dtype}, got {t.dtype}.")
+        return t
+
+    def workspace(self, size: int, device):
+        """`size` bytes of torch memory (0: none)."""
+        if not size:
+            return None, 0
+        return _torch().empty(size, dtype=_torch().uint8, device=device), size
+
+
+def _norm_weights(call, x, gamma, beta):
+    """gamma's and beta's pointers and type: both x's type, or both float32."""
+    torch = _torch()
+    given = [t for t in (gamma, beta) if t is not None]
+    kind = given[0].dtype if given else x.dtype
+    call.require(kind in (x.dtype, torch.float32),
+                 f"gamma and beta must be {x.dtype} or torch.float32, got {kind}.")
+    cols = (x.shape[1],)
+    return (call.flat(gamma, "gamma", cols, kind), call.flat(beta, "beta", cols, kind), kind)
+
+
+def layer_norm(x, gamma=None, beta=None, eps: float = 1e-5, with_stats: bool = False, out=None,
+               stream=None):
+    """The rows of x [rows, cols] to mean 0 and variance 1, times gamma, plus
+    beta (tg_layer_norm).  gamma / beta: [cols] of x's type or float32.
+    with_stats: (y, mean, rstd), float32 [rows], for layer_norm_backward."""
+    torch = _torch()
+    with _Call("layer_norm", stream, x, gamma, beta, out) as c:
+        kind = _type_of(x, "layer_norm")
+        px, ldx = c.rows(x, "x")
+        rows, cols = x.shape
+        pg, pb, wk = _norm_weights(c, x, gamma, beta)
+        y = c.out(out, "out", x.shape, x)
+        py, ldy = c.rows(y, "out")
+        mean = rstd = None
+        if with_stats:
+            mean = torch.empty(rows, dtype=torch.float32, device=x.device)
+            rstd = torch.empty_like(mean)
+        lib.check(lib.tg_layer_norm(rows, cols, kind, px, ldx, pg, pb, _TYPES[wk], eps, py, ldy,
+                                    mean.data_ptr() if with_stats else 0,
+                                    rstd.data_ptr() if with_stats else 0, c.handle))
+    return (y, mean, rstd) if with_stats else y
+
+
+def layer_norm_backward(dy, x, mean, rstd, gamma=None, out=None, stream=None):
+    """(dx, dgamma, dbeta) of layer_norm from dy, its x, mean and rstd
+    (tg_layer_norm_backward); dgamma and dbeta have gamma's type (x's without
+    gamma).  out takes dx (it may be dy)."""
+    torch = _torch()
+    what = "layer_norm_backward"
+    with _Call(what, stream, x, dy, mean, rstd, gamma, out) as c:
+        kind = _type_of(x, what)
+        rows, cols = x.shape if x.dim() == 2 else (-1, -1)
+        px, ldx = c.rows(x, "x")
+        c.require(dy.shape == x.shape and dy.dtype == x.dtype,
+                  f"dy must be {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}.")
+        pdy, lddy = c.rows(dy, "dy")
+        pg, _, wk = _norm_weights(c, x, gamma, None)
+        pm = c.flat(mean, "mean", (rows,), torch.float32)
+        pr = c.flat(rstd, "rstd", (rows,), torch.float32)
+        dx = c.out(out, "out", x.shape, x)
+        pdx, lddx = c.rows(dx, "out")
+        dgamma = torch.empty(cols, dtype=wk, device=x.device)
+        dbeta = torch.empty_like(dgamma)
+        ws, size = c.workspace(lib.tg_layer_norm_backward_workspace_size(rows, cols), x.device)
+        lib.check(lib.tg_layer_norm_backward(
+            rows, cols, kind, pdy, lddy, px, ldx, pg, _TYPES[wk], pm, pr, pdx, lddx,
+            dgamma.data_ptr(), dbeta.data_ptr(), ws.data_ptr() if size else None, size, c.handle))
+    return dx, dgamma, dbeta
+
+
+@dataclass
+class RoutePlan:
+    """Rows in group order (tg_route, tg_route_plan).  Group g holds the
+    places [offsets[g], offsets[g + 1]); rows[p] is the row at place p (-1 past
+    the last group), position[t, j] the place of row t's j-th choice (-1: none)."""
+    offsets: object
+    rows: object
+    position: object
+
+
+def route(logits, k: int, renormalize: bool = False, stream=None):
+    """Softmax of each row of logits [tokens, experts] and its k largest, with
+    the plan of the rows by expert (tg_route): (weights float32 [tokens, k],
+    experts int32 [tokens, k], RoutePlan).  A logit of -inf masks its expert;
+    places without an expert hold -1 and weight 0."""
+    torch = _torch()
+    with _Call("route", stream, logits) as c:
+        kind = _type_of(logits, "route")
+        pl, ld = c.rows(logits, "logits")
+        tokens, experts = logits.shape
+        dev = logits.device
+        c.require(1 <= k <= 32 and k <= experts <= 1024,
+                  f"k must be between 1 and min(32, experts) and experts at most 1024, got k={k} "
+                  f"of {experts}.")
+        weights = torch.empty((tokens, k), dtype=torch.float32, device=dev)
+        ids = torch.empty((tokens, k), dtype=torch.int32, device=dev)
+        plan = RoutePlan(torch.empty(experts + 1, dtype=torch.int32, device=dev),
+                         torch.empty(tokens * k, dtype=torch.int32, device=dev),
+                         torch.empty((tokens, k), dtype=torch.int32, device=dev))
+        ws, size = c.workspace(lib.tg_route_workspace_size(tokens, experts, k), dev)
+        lib.check(lib.tg_route(tokens, experts, k, kind, pl, ld, int(renormalize),
+                               weights.data_ptr(), ids.data_ptr(), plan.offsets.data_ptr(),
+                               plan.rows.data_ptr(), plan.position.data_ptr(),
+                               ws.data_ptr() if size else None, size, c.handle))
+    return weights, ids, plan
+
+
+def route_plan(ids, groups: int, stream=None) -> RoutePlan:
+    """The plan of rows whose groups are known (tg_route_plan): ids int32
+    [rows] (node types) or [rows, k]; an id outside [0, groups) is in none."""
+    torch = _torch()
+    with _Call("route_plan", stream, ids) as c:
+        c.require(ids.dim() in (1, 2) and ids.dtype == torch.int32 and ids.is_contiguous(),
+                  f"ids must be a contiguous int32 vector or matrix, got {tuple(ids.shape)} "
+                  f"{ids.dtype}.")
+        c.require(1 <= groups <= 1024, f"between 1 and 1024 groups, got {groups}.")
+        n, k, dev = ids.numel(), ids.shape[1] if ids.dim() == 2 else 1, ids.device
+        plan = RoutePlan(torch.empty(groups + 1, dtype=torch.int32, device=dev),
+                         torch.empty(n, dtype=torch.int32, device=dev), torch.empty_like(ids))
+        ws, size = c.workspace(lib.tg_route_plan_workspace_size(n, groups), dev)
+        lib.check(lib.tg_route_plan(n, groups, max(k, 1), ids.data_ptr(), plan.offsets.data_ptr(),
+                                    plan.rows.data_ptr(), plan.position.data_ptr(),
+                                    ws.data_ptr() if size else None, size, c.handle))
+    return plan
+
+
+def route_backward(dweights, logits, weights, experts, renormalize: bool = False, stream=None):
+    """dlogits of route from the gradient of its weights (tg_route_backward)."""
+    torch = _torch()
+    what = "route_backward"
+    with _Call(what, stream, logits, dweights, weights, experts) as c:
+        kind = _type_of(logits, what)
+        pl, ld = c.rows(logits, "logits")
+        tokens, n = logits.shape
+        c.require(weights.dim() == 2, "weights must be [tokens, k].")
+        k = weights.shape[1]
+        shape = (tokens, k)
+        pw = c.flat(weights, "weights", shape, torch.float32)
+        pe = c.flat(experts, "experts", shape, torch.int32)
+        pd = c.flat(dweights, "dweights", shape, torch.float32)
+        out = torch.empty((tokens, n), dtype=logits.dtype, device=logits.device)
+        lib.check(lib.tg_route_backward(tokens, n, k, kind, pl, ld, int(renormalize), pw, pe, pd,
+                                        out.data_ptr(), n, c.handle))
+    return out
+
+
+def _places(c, position):
+    c.require(position.dim() == 2, f"position must be [tokens, k], got {tuple(position.shape)}.")
+    return c.flat(position, "position", position.shape, _torch().int32)
+
+
+def route_combine(y, position, weights=None, out=None, stream=None):
+    """out[t] = sum over j of weights[t, j] * y[position[t, j]], weights of 1
+    if None (tg_route_combine); a position of -1 adds nothing."""
+    torch = _torch()
+    with _Call("route_combine", stream, y, position, weights, out) as c:
+        kind = _type_of(y, "route_combine")
+        py, ldy = c.rows(y, "y")
+        pp = _places(c, position)
+        tokens, k = position.shape
+        pw = c.flat(weights, "weights", position.shape, torch.float32)
+        o = c.out(out, "out", (tokens, y.shape[1]), y)
+        po, ldo = c.rows(o, "out")
+        lib.check(lib.tg_route_combine(tokens, k, y.shape[1], kind, py, y.shape[0], ldy, pp, pw,
+                                       po, ldo, c.handle))
+    return o
+
+
+def route_combine_backward(dout, y, position, weights=None, out=None, stream=None):
+    """(dy, dweights) of route_combine (tg_route_combine_backward).  out takes
+    dy; rows that no position names are left as they are (zeros without out)."""
+    torch = _torch()
+    what = "route_combine_backward"
+    with _Call(what, stream, y, dout, position, weights, out) as c:
+        kind = _type_of(y, what)
+        py, ldy = c.rows(y, "y")
+        pp = _places(c, position)
+        tokens, k = position.shape
+        cols = y.shape[1]
+        c.require(tuple(dout.shape) == (tokens, cols) and dout.dtype == y.dtype,
+                  f"dout must be {(tokens, cols)} {y.dtype}, got {tuple(dout.shape)} "
+                  f"{dout.dtype}.")
+        pd, lddo = c.rows(dout, "dout")
+        pw = c.flat(weights, "weights", position.shape, torch.float32)
+        if out is None and position.numel() != y.shape[0]:
+            out = torch.zeros(y.shape, dtype=y.dtype, device=y.device)
+        dy = c.out(out, "out", y.shape, y)
+        pdy, lddy = c.rows(dy, "out")
+        dw = torch.empty((tokens, k), dtype=torch.float32, device=y.device)
+        lib.check(lib.tg_route_combine_backward(tokens, k, cols, kind, pd, lddo, py, y.shape[0],
+                                                ldy, pp, pw, pdy, lddy, dw.data_ptr(), c.handle))
+    return dy, dw
+
+
+def _offsets(c, offsets):
+    torch = _torch()
+    c.require(offsets.dim() == 1 and offsets.numel() >= 1, "offsets must be [groups + 1].")
+    return c.flat(offsets, "offsets", offsets.shape, torch.int32), offsets.numel() - 1
+
+
+def _row_index(c, rows, x):
+    """The rows' pointer and the number of rows of the product."""
+    if rows is None:
+        return 0, x.shape[0]
+    c.require(rows.dim() == 1, "rows must be a vector.")
+    return c.flat(rows, "rows", rows.shape, _torch().int32), rows.numel()
+
+
+def grouped_matmul(x, w, offsets, rows=None, bias=None, epilogue: int = EPI_NONE,
+                   transpose: bool = False, out=None, stream=None):
+    """y[p] = epilogue(x[p] @ w[g] + bias[g]) for the rows p of group g, those
+    in [offsets[g], offsets[g + 1]) (tg_grouped_matmul); with rows, x[rows[p]]
+    in the place of x[p].  w: [groups, k, n], or [groups, n, k] with transpose
+    (the gradient of x: grouped_matmul(dy, w, offsets, transpose=True)).  Rows
+    in no group are not written."""
+    with _Call("grouped_matmul", stream, x, w, offsets, rows, bias, out) as c:
+        kind = _type_of(x, "grouped_matmul")
+        px, ldx = c.rows(x, "x")
+        po, groups = _offsets(c, offsets)
+        pr, m = _row_index(c, rows, x)
+        c.require(w.dim() == 3 and w.dtype == x.dtype and w.shape[0] == groups,
+                  f"w must be [{groups}, k, n] {x.dtype}, got {tuple(w.shape)} {w.dtype}.")
+        k, n = (w.shape[2], w.shape[1]) if transpose else (w.shape[1], w.shape[2])
+        c.require(x.shape[1] == k, f"dimension mismatch: x has {x.shape[1]} columns, w {k}.")
+        c.require(w.numel() == 0 or w.shape[2] == 1 or w.stride(2) == 1,
+                  f"w must have contiguous rows, got strides {w.stride()}.")
+        ldw = max(w.stride(1) if w.shape[1] > 1 else 0, w.shape[2], 1)
+        c.require(w.numel() == 0 or w.shape[1] == 1 or w.stride(1) >= w.shape[2],
+                  f"w has overlapping rows (strides {w.stride()}).")
+        pb = c.flat(bias, "bias", (groups, n), x.dtype)
+        y = c.out(out, "out", (m, n), x)
+        py, ldy = c.rows(y, "out")
+        lib.check(lib.tg_grouped_matmul(m, k, n, groups, kind, px, x.shape[0], ldx, pr, po,
+                                        w.data_ptr(), ldw, w.stride(0) if groups > 1 else 0,
+                                        int(transpose), pb, epilogue, py, ldy, c.handle))
+    return y
+
+
+def grouped_matmul_wgrad(x, dy, offsets, rows=None, bias: bool = False, stream=None):
+    """(dw, dbias) of grouped_matmul from x (and rows) and the gradient before
+    its epilogue (tg_grouped_matmul_wgrad): dw [groups, k, n], dbias [groups,
+    n] or None."""
+    torch = _torch()
+    what = "grouped_matmul_wgrad"
+    with _Call(what, stream, x, dy, offsets, rows) as c:
+        kind = _type_of(x, what)
+        px, ldx = c.rows(x, "x")
+        po, groups = _offsets(c, offsets)
+        pr, m = _row_index(c, rows, x)
+        c.require(dy.dim() == 2 and dy.shape[0] == m and dy.dtype == x.dtype,
+                  f"dy must be [{m}, n] {x.dtype}, got {tuple(dy.shape)} {dy.dtype}.")
+        pd, lddy = c.rows(dy, "dy")
+        k, n = x.shape[1], dy.shape[1]
+        dw = torch.empty((groups, k, n), dtype=x.dtype, device=x.device)
+        db = torch.empty((groups, n), dtype=x.dtype, device=x.device) if bias else None
+        ws, size = c.workspace(lib.tg_grouped_matmul_wgrad_workspace_size(m, k, n, groups, kind),
+                               x.device)
+        lib.check(lib.tg_grouped_matmul_wgrad(
+            m, k, n, groups, kind, px, x.shape[0], ldx, pr, pd, lddy, po, dw.data_ptr(),
+            db.data_ptr() if bias else None, ws.data_ptr() if size else None, size, c.handle))
+    return dw, db
+
+
+@dataclass
+class BlockRows:
+    """Rows in e4m3 with a scale for each 128 columns (tg_quantize): q
+    float8_e4m3fn [rows, columns rounded up to 128], scale float32 [blocks,
+    rows], and the columns they stand for."""
+    q: object
+    scale: object
+    cols: int
+
+
+@dataclass
+class BlockWeight:
+    """Weights in e4m3 with a scale for each 128 x 128 (tg_quantize_weight): q
+    float8_e4m3fn [n, k rounded up to 128] and scale float32 [blocks of n,
+    blocks of k], or [groups, ...] of both, and k."""
+    q: object
+    scale: object
+    k: int
+
+
+def _blocks(n: int) -> int:
+    return -(-n // 128)
+
+
+def quantize(x, stream=None) -> BlockRows:
+    """x [rows, cols] in e4m3 with a scale for each row and 128 columns."""
+    torch = _torch()
+    with _Call("quantize", stream, x) as c:
+        kind = _type_of(x, "quantize")
+        px, ldx = c.rows(x, "x")
+        rows, cols = x.shape
+        blocks = _blocks(cols)
+        q = torch.empty((rows, blocks * 128), dtype=torch.float8_e4m3fn, device=x.device)
+        scale = torch.empty((blocks, rows), dtype=torch.float32, device=x.device)
+        lib.check(lib.tg_quantize(rows, cols, kind, px, ldx, q.data_ptr(), scale.data_ptr(),
+                                  c.handle))
+    return BlockRows(q, scale, cols)
+
+
+def quantize_weight(w, transpose: bool = False, stream=None) -> BlockWeight:
+    """w [k, n] or [groups, k, n] (transpose: [.., n, k]) in e4m3 with a scale
+    for each 128 x 128 block, laid out for matmul_fp8 once."""
+    torch = _torch()
+    with _Call("quantize_weight", stream, w) as c:
+        kind = _type_of(w, "quantize_weight")
+        c.require(w.dim() in (2, 3), f"w must be [k, n] or [groups, k, n], got {tuple(w.shape)}.")
+        many = w.dim() == 3
+        w3 = w if many else w[None]
+        groups = w3.shape[0]
+        k, n = (w3.shape[2], w3.shape[1]) if transpose else (w3.shape[1], w3.shape[2])
+        c.require(w.numel() == 0 or w3.shape[2] == 1 or w3.stride(2) == 1,
+                  f"w must have contiguous rows, got strides {w.stride()}.")
+        c.require(w.numel() == 0 or w3.shape[1] == 1 or w3.stride(1) >= w3.shape[2],
+                  f"w has overlapping rows (strides {w.stride()}).")
+        ldw = max(w3.stride(1) if w3.shape[1] > 1 else 0, w3.shape[2], 1)
+        q = torch.empty((groups, n, _blocks(k) * 128), dtype=torch.float8_e4m3fn, device=w.device)
+        scale = torch.empty((groups, _blocks(n), _blocks(k)), dtype=torch.float32,
+                            device=w.device)
+        lib.check(lib.tg_quantize_weight(groups, k, n, kind, w.data_ptr(), ldw,
+                                         w3.stride(0) if groups > 1 else 0, int(transpose),
+                                         q.data_ptr(), scale.data_ptr(), c.handle))
+    return BlockWeight(q if many else q[0], scale if many else scale[0], k)
+
+
+def matmul_fp8(x: BlockRows, w: BlockWeight, offsets=None, rows=None, bias=None,
+               epilogue: int = EPI_NONE, dtype=None, out=None, stream=None):
+    """The product of quantised rows and weights (tg_matmul_fp8), rounded once
+    to `dtype` (float32 if None, or out's).  With offsets, w and bias [groups,
+    n] are one for each group, as in grouped_matmul (rows too)."""
+    torch = _torch()
+    what = "matmul_fp8"
+    f8 = torch.float8_e4m3fn
+    with _Call(what, stream, x.q, x.scale, w.q, w.scale, offsets, rows, bias, out) as c:
+        kb = _blocks(x.cols)
+        c.require(x.cols == w.k, f"dimension mismatch: x has {x.cols} columns, w {w.k}.")
+        pq = c.flat(x.q, "x.q", (x.q.shape[0], kb * 128), f8)
+        ps = c.flat(x.scale, "x.scale", (kb, x.q.shape[0]), torch.float32)
+        c.require(w.q.dim() == (2 if offsets is None else 3),
+                  f"w.q must be {'[n, k]' if offsets is None else '[groups, n, k]'}, got "
+                  f"{tuple(w.q.shape)}.")
+        n = w.q.shape[-2]
+        po, groups = (0, 1) if offsets is None else _offsets(c, offsets)
+        lead = () if offsets is None else (groups,)
+        pw = c.flat(w.q, "w.q", (*lead, n, kb * 128), f8)
+        pws = c.flat(w.scale, "w.scale", (*lead, _blocks(n), kb), torch.float32)
+        pr, m = _row_index(c, rows, x.q)
+        kind = dtype or (out.dtype if out is not None else torch.float32)
+        like = torch.empty(0, dtype=kind, device=x.q.device)
+        code = _type_of(like, what)
+        pb = c.flat(bias, "bias", (*lead, n), kind)
+        y = c.out(out, "out", (m, n), like)
+        py, ldy = c.rows(y, "out")
+        lib.check(lib.tg_matmul_fp8(m, x.cols, n, groups, pq, ps, x.q.shape[0], pr, po, pw, pws,
+                                    code, pb, epilogue, py, ldy, c.handle))
+    return y
 
 
 # ---------------------------------------------------------------------------

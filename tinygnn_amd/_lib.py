@@ -95,6 +95,27 @@ SIGNATURES = {
     "tg_gat_workspace_size": (sz, [vp, i64, i64, i64, i32]),
     "tg_gat_aggregate": (i32, [vp, i64, i64, i64, vp, vp, vp, i64, vp, vp, f32, vp, i32, i32,
                                i32, vp, i64, vp, sz, vp]),
+    "tg_layer_norm": (i32, [i64, i64, i32, vp, i64, vp, vp, i32, f32, vp, i64, vp, vp, vp]),
+    "tg_layer_norm_backward_workspace_size": (sz, [i64, i64]),
+    "tg_layer_norm_backward": (i32, [i64, i64, i32, vp, i64, vp, i64, vp, i32, vp, vp, vp, i64,
+                                     vp, vp, vp, sz, vp]),
+    "tg_route_workspace_size": (sz, [i64, i64, i64]),
+    "tg_route": (i32, [i64, i64, i64, i32, vp, i64, i32, vp, vp, vp, vp, vp, vp, sz, vp]),
+    "tg_route_plan_workspace_size": (sz, [i64, i64]),
+    "tg_route_plan": (i32, [i64, i64, i64, vp, vp, vp, vp, vp, sz, vp]),
+    "tg_route_backward": (i32, [i64, i64, i64, i32, vp, i64, i32, vp, vp, vp, vp, i64, vp]),
+    "tg_route_combine": (i32, [i64, i64, i64, i32, vp, i64, i64, vp, vp, vp, i64, vp]),
+    "tg_route_combine_backward": (i32, [i64, i64, i64, i32, vp, i64, vp, i64, i64, vp, vp, vp,
+                                        i64, vp, vp]),
+    "tg_grouped_matmul": (i32, [i64, i64, i64, i64, i32, vp, i64, i64, vp, vp, vp, i64, i64, i32,
+                                vp, i32, vp, i64, vp]),
+    "tg_grouped_matmul_wgrad_workspace_size": (sz, [i64, i64, i64, i64, i32]),
+    "tg_grouped_matmul_wgrad": (i32, [i64, i64, i64, i64, i32, vp, i64, i64, vp, vp, i64, vp, vp,
+                                      vp, vp, sz, vp]),
+    "tg_quantize": (i32, [i64, i64, i32, vp, i64, vp, vp, vp]),
+    "tg_quantize_weight": (i32, [i64, i64, i64, i32, vp, i64, i64, i32, vp, vp, vp]),
+    "tg_matmul_fp8": (i32, [i64, i64, i64, i64, vp, vp, i64, vp, vp, vp, vp, i32, vp, i32, vp,
+                            i64, vp]),
     "tg_model_create": (i32, [C.POINTER(vp)]),
     "tg_model_destroy": (i32, [vp]),
     "tg_model_add_gcn_layer": (i32, [vp, i64, i64, i32, i32, i32, pi64]),

@@ -1,0 +1,71 @@
+// grouped.hpp -- shared by the grouped products: arguments and the tiles of
+// ragged groups.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "common.hpp"
+#include "device_utils.hpp"
+#include "tinygnn_amd.h"
+
+namespace tg {
+
+constexpr int64_t kMaxGroups = 1024;
+
+// Rows [offsets[g], offsets[g + 1]), whatever the offsets hold within [0, m].
+__device__ __forceinline__ void group_rows(const int32_t* __restrict__ offsets, int g, int m,
+                                           int* lo, int* hi) {
+    const int a = offsets[g], b = offsets[g + 1];
+    *lo = a < 0 ? 0 : a > m ? m : a;
+    *hi = b < *lo ? *lo : b > m ? m : b;
+}
+
+// The tile of `unit` rows with number t over all groups, each cut from its own
+// first row: its group and rows [*r0, *r1); false past the last.  Every
+// wavefront finds it by itself, 64 groups at a time (offsets come from L2).
+// offsets null: one group of all m rows.
+__device__ __forceinline__ bool find_tile(const int32_t* __restrict__ offsets, int groups, int m,
+                                          int unit, int t, int* g, int* r0, int* r1) {
+    if (offsets == nullptr) {
+        *g = 0;
+        *r0 = t * unit;
+        *r1 = m - *r0 > unit ? *r0 + unit : m;
+        return *r0 < m;
+    }
+    const int lane = threadIdx.x & (kWave - 1);
+    for (int base = 0; base < groups; base += kWave) {
+        int lo = 0, hi = 0;
+        if (base + lane < groups) group_rows(offsets, base + lane, m, &lo, &hi);
+        const int n = static_cast<int>((static_cast<int64_t>(hi) - lo + unit - 1) / unit);
+        const int upto = wave_inclusive_scan(n);
+        const uint64_t past = __ballot(upto > t);
+        if (past) {
+            const int w = __ffsll(static_cast<unsigned long long>(past)) - 1;
+            const int first = __builtin_amdgcn_readlane(upto - n, w);
+            const int a = __builtin_amdgcn_readlane(lo, w), b = __builtin_amdgcn_readlane(hi, w);
+            *g = base + w;
+            *r0 = a + (t - first) * unit;
+            *r1 = b - *r0 > unit ? *r0 + unit : b;
+            return true;
+        }
+        t -= __builtin_amdgcn_readlane(upto, kWave - 1);
+    }
+    return false;
+}
+
+// Most tiles of `unit` rows that m rows in `groups` groups can make.
+inline int64_t most_tiles(int64_t m, int64_t groups, int64_t unit) {
+    return m / unit + std::min(groups, m);
+}
+
+// x + bias, then TG_EPI_* (expm1: exp(x) - 1 loses the small x's digits).
+__device__ __forceinline__ float grouped_epilogue(float x, float bias, int epi) {
+    x += bias;
+    if (epi == TG_EPI_RELU) return 0.0f < x ? x : 0.0f;
+    if (epi == TG_EPI_ELU) return x < 0.0f ? expm1f(x) : x;
+    return x;
+}
+
+}  // namespace tg
