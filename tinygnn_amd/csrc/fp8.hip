@@ -3,6 +3,7 @@
 
 #include <string>
 
+#include "tiles.hpp"
 #include "types.hpp"
 
 namespace tg {
@@ -103,18 +104,24 @@ struct Fp8Args {
     int epi;
     void* y;
     int64_t ldy;
+    uint32_t mt, nt;  // row tiles (most) and column tiles
 };
 
-typedef float v4f __attribute__((ext_vector_type(4)));
 typedef f16 v2h __attribute__((ext_vector_type(2)));
-typedef f16 v8h __attribute__((ext_vector_type(8)));
+typedef int v8i __attribute__((ext_vector_type(8)));
+
+// A wavefront's operand of one tile of 16 rows: the lane's chunks q and 4 + q
+// of a block, 32 values in all.
+struct Operand {
+    Frag c[2];
+};
 
 // Eight e4m3 values as fp16, which holds each of them exactly.
-__device__ __forceinline__ v8h to_f16(uint2 b) {
-    const v2h x[4] = {__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b.x, 1.0f, false),
-                      __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b.x, 1.0f, true),
-                      __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b.y, 1.0f, false),
-                      __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b.y, 1.0f, true)};
+__device__ __forceinline__ v8h to_f16(uint32_t lo, uint32_t hi) {
+    const v2h x[4] = {__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false),
+                      __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true),
+                      __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false),
+                      __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true)};
     v8h v;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -124,61 +131,267 @@ __device__ __forceinline__ v8h to_f16(uint2 b) {
     return v;
 }
 
-// One wavefront: 16 rows x 16 columns.  The e4m3 matrix instructions line the
-// products up with the largest of them and drop what lies far below it: against
-// 64 bits a block's sum is off by up to 2^-12.8 of the sum of its products'
-// sizes for operands of random bits, 2^-16.3 (2^-18.9 in the mean) for normal
-// ones.  That is below a 16-bit result's own rounding; for fp32 results the
-// operands are widened to fp16, exactly, whose products are added in fp32.
-template <typename T>
-__global__ __launch_bounds__(64) void fp8_kernel(Fp8Args a) {
-    int g, r0, r1;
-    if (!find_tile(a.offsets, a.groups, a.m, 16, blockIdx.y, &g, &r0, &r1)) return;
-    const int lane = threadIdx.x, r = lane % 16, q = lane / 16;
-    const int n0 = blockIdx.x * 16;
-    auto source = [&](int i) -> int64_t {
-        const int p = r0 + i < r1 ? r0 + i : r1 - 1;
-        const int64_t s = a.rows ? a.rows[p] : p;
-        return s < 0 || s >= a.x_rows ? -1 : s;
-    };
-    const int64_t ra = source(r);
-    const int col = n0 + r < a.n ? n0 + r : a.n - 1;
-    const int64_t kp = static_cast<int64_t>(a.kb) * kBlock;
-    const uint8_t* pa = a.xq + (ra < 0 ? 0 : ra) * kp;
-    const uint8_t* pb = a.wq + (static_cast<int64_t>(g) * a.n + col) * kp;
-    const float* ws = a.wscale + (static_cast<int64_t>(g) * ((a.n + 127) / 128) + col / 128) * a.kb;
-    v4f acc = {};
-    for (int b = 0; b < a.kb; ++b) {
-        v4f part = {};
+// The sum of a block's products, 16 x 16.  The e4m3 matrix instructions line
+// the products up with the largest of them and drop what lies far below it:
+// against 64 bits a block's sum is off by up to 2^-12.8 of the sum of its
+// products' sizes for operands of random bits, 2^-16.3 (2^-18.9 in the mean) for
+// normal ones.  That is below a 16-bit result's own rounding; for fp32 results
+// (WIDE) the operands are widened to fp16, exactly, at half the rate.
+template <bool WIDE>
+__device__ __forceinline__ v4f block_products(const Operand& a, const Operand& b) {
+    v4f p = {0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (WIDE) {
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            const int64_t c = b * kBlock + s * 32 + q * 8;
-            const uint2 av = *reinterpret_cast<const uint2*>(pa + c);
-            const uint2 bv = *reinterpret_cast<const uint2*>(pb + c);
-            if constexpr (sizeof(T) == 4)
-                part = __builtin_amdgcn_mfma_f32_16x16x32_f16(to_f16(av), to_f16(bv), part, 0, 0,
-                                                              0);
-            else
-                part = __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8(
-                    __builtin_bit_cast(long, av), __builtin_bit_cast(long, bv), part, 0, 0, 0);
+            const v4u& x = a.c[s / 2].u;
+            const v4u& y = b.c[s / 2].u;
+            p = __builtin_amdgcn_mfma_f32_16x16x32_f16(to_f16(x[s % 2 * 2], x[s % 2 * 2 + 1]),
+                                                       to_f16(y[s % 2 * 2], y[s % 2 * 2 + 1]), p,
+                                                       0, 0, 0);
         }
+    } else {
+        v8i x, y;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t rr = source(4 * q + i);
-            const float xs = rr < 0 ? 0.0f : a.xscale[static_cast<int64_t>(b) * a.x_rows + rr];
-            acc[i] = rr < 0 ? 0.0f : __builtin_fmaf(xs * ws[b], part[i], acc[i]);
+        for (int e = 0; e < 8; ++e) {
+            x[e] = static_cast<int>(a.c[e / 4].u[e % 4]);
+            y[e] = static_cast<int>(b.c[e / 4].u[e % 4]);
         }
+        p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, p, 0, 0, 0, 0, 0, 0);
+    }
+    return p;
+}
+
+// x's quantised row for row p of the product, or -1.
+__device__ __forceinline__ int source_row(const Fp8Args& a, int p) {
+    const int r = a.rows ? a.rows[p] : p;
+    return r < 0 || r >= a.x_rows ? -1 : r;
+}
+
+// bias n .. n + 3 of group g.
+template <typename T>
+__device__ __forceinline__ v4f bias_of(const Fp8Args& a, int g, int n) {
+    float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (a.bias)
+        load_floats<T, 4>(static_cast<const T*>(a.bias) + static_cast<int64_t>(g) * a.n + n,
+                          a.n - n, b);
+    return v4f{b[0], b[1], b[2], b[3]};
+}
+
+// Columns n .. n + 3 of row p: bias, epilogue, store.
+template <typename T, int EPI>
+__device__ __forceinline__ void store_outputs(const Fp8Args& a, int p, int n, const v4f& acc,
+                                              const v4f& bias) {
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = grouped_epilogue<EPI>(acc[e], bias[e]);
+    store_floats<T, 4>(static_cast<T*>(a.y) + p * a.ldy + n, a.n - n, v);
+}
+
+// BM x BN outputs, a tile a block of 128: the products of a block go to fresh
+// registers and from there, times x's scale of the row and w's of the columns,
+// to the sums (16 multiply-adds beside each 32-cycle instruction).  As in the
+// 16-bit products the outputs are computed transposed, so a lane's row of x is
+// one; x's scales of the block come to LDS with its tile.
+template <typename T, typename S>
+__global__ __launch_bounds__(S::kThreads) void fp8_kernel(Fp8Args a) {
+    constexpr int kScales = S::kM * kRowBytes;  // behind x's tile
+    __shared__ __attribute__((aligned(16))) char a0[kScales + S::kM * 4];
+    __shared__ __attribute__((aligned(16))) char b0[S::kN * kRowBytes];
+    __shared__ __attribute__((aligned(16))) char a1[kScales + S::kM * 4];
+    __shared__ __attribute__((aligned(16))) char b1[S::kN * kRowBytes];
+    constexpr bool WIDE = sizeof(T) == 4;
+    uint32_t mt, ntile;
+    tile_of(blockIdx.x, gridDim.x, a.nt, a.mt, &mt, &ntile);
+    int g, r0, r1;
+    if (!find_tile(a.offsets, a.groups, a.m, S::kM, static_cast<int>(mt), &g, &r0, &r1)) return;
+    const int n0 = static_cast<int>(ntile) * S::kN;
+    const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, r = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / S::kWC * S::kMI * 16, wn = wave % S::kWC * S::kNJ * 16;
+    const int64_t kp = static_cast<int64_t>(a.kb) * kBlock;
+    const uint8_t* w = a.wq + static_cast<int64_t>(g) * a.n * kp;
+    static_assert(S::kNJ * 16 <= kBlock && kBlock % (S::kNJ * 16) == 0, "one scale of w a wavefront");
+    const int nb = (a.n + kBlock - 1) / kBlock;
+    const int wblock = (n0 + wn) / kBlock < nb ? (n0 + wn) / kBlock : nb - 1;
+    const float* ws = a.wscale + (static_cast<int64_t>(g) * nb + wblock) * a.kb;
+
+    // a tile's rows of x from its first (gathered: from x's first), w's columns
+    const uint8_t* xb = a.rows ? a.xq : a.xq + static_cast<int64_t>(r0) * kp;
+    const uint8_t* wb = w + static_cast<int64_t>(n0) * kp;
+    uint32_t ao[S::kCA], bo[S::kCB];
+#pragma unroll
+    for (int t = 0; t < S::kCA; ++t) {
+        int row, c;
+        chunk_place<uint8_t, S::kM, false>(t * S::kThreads + tid, &row, &c);
+        const int src = r0 + row < r1 ? source_row(a, r0 + row) : -1;
+        ao[t] = src < 0 ? kOutside
+                        : static_cast<uint32_t>((a.rows ? src : row) * kp + c);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int p = r0 + 4 * q + i;
-        if (p >= r1 || n0 + r >= a.n) continue;
-        const float bias = a.bias ? static_cast<float>(static_cast<const T*>(
-                                        a.bias)[static_cast<int64_t>(g) * a.n + n0 + r])
-                                  : 0.0f;
-        static_cast<T*>(a.y)[p * a.ldy + n0 + r] =
-            static_cast<T>(grouped_epilogue(acc[i], bias, a.epi));
+    for (int t = 0; t < S::kCB; ++t) {
+        int col, c;
+        chunk_place<uint8_t, S::kN, false>(t * S::kThreads + tid, &col, &c);
+        bo[t] = n0 + col < a.n ? static_cast<uint32_t>(col * kp + c) : kOutside;
     }
+    // one row's scale for each thread of the first wavefronts; outside: 0
+    uint32_t so = kOutside;
+    if (tid < S::kM && r0 + tid < r1) {
+        const int src = source_row(a, r0 + tid);
+        if (src >= 0) so = static_cast<uint32_t>(src) * 4;
+    }
+    auto load = [&](int kt, char* la, char* lb) {
+        const auto xbuf = buffer_of(xb + static_cast<int64_t>(kt) * kBlock, kDirectBytes);
+        const auto wbuf = buffer_of(wb + static_cast<int64_t>(kt) * kBlock, kDirectBytes);
+        if (wave * 64 < S::kM)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                buffer_of(a.xscale + static_cast<int64_t>(kt) * a.x_rows, 4 * a.x_rows),
+                (TG_LDS void*)(la + kScales + wave * 256), 4, static_cast<int>(so), 0, 0, 0);
+#pragma unroll
+        for (int t = 0; t < S::kCA; ++t)
+            load_to_lds(xbuf, la + (t * S::kThreads + wave * 64) * 16, ao[t]);
+#pragma unroll
+        for (int t = 0; t < S::kCB; ++t)
+            load_to_lds(wbuf, lb + (t * S::kThreads + wave * 64) * 16, bo[t]);
+    };
+    Acc<S> acc = {};
+    const Reader<uint8_t, S::kM, false, S::kMI> ra(wm, lane);
+    const Reader<uint8_t, S::kN, false, S::kNJ> rb(wn, lane);
+    int kt = 0;
+    auto compute = [&](const char* la, const char* lb) {
+        const float scale = ws[kt++];
+        const float* xs = reinterpret_cast<const float*>(la + kScales) + wm + r;
+        Operand b[S::kNJ];
+#pragma unroll
+        for (int j = 0; j < S::kNJ; ++j)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) b[j].c[s] = rb.read(lb, j, s);
+        // row tile i's products run while those of i - 1 are scaled and added;
+        // no more than that may be live (registers)
+        v4f part[2][S::kNJ];
+#pragma unroll
+        for (int i = 0; i <= S::kMI; ++i) {
+            if (i < S::kMI) {
+                Operand x;
+#pragma unroll
+                for (int s = 0; s < 2; ++s) x.c[s] = ra.read(la, i, s);
+#pragma unroll
+                for (int j = 0; j < S::kNJ; ++j)
+                    part[i & 1][j] = block_products<WIDE>(b[j], x);
+            }
+            if (i > 0) {
+                const float f = xs[(i - 1) * 16] * scale;
+#pragma unroll
+                for (int j = 0; j < S::kNJ; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        acc[i - 1][j][e] = __builtin_fmaf(part[(i - 1) & 1][j][e], f,
+                                                          acc[i - 1][j][e]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    pipeline<true>(a.kb, a0, b0, a1, b1, load, [](char*, char*) {}, compute);
+    v4f bias[S::kNJ];
+#pragma unroll
+    for (int j = 0; j < S::kNJ; ++j) bias[j] = bias_of<T>(a, g, n0 + wn + j * 16 + 4 * q);
+    with_epilogue(a.epi, [&](auto epi) {
+#pragma unroll
+        for (int i = 0; i < S::kMI; ++i) {
+            const int p = r0 + wm + i * 16 + r;
+            if (p >= r1) continue;
+#pragma unroll
+            for (int j = 0; j < S::kNJ; ++j)
+                store_outputs<T, decltype(epi)::value>(a, p, n0 + wn + j * 16 + 4 * q, acc[i][j],
+                                                       bias[j]);
+        }
+    });
+}
+
+// Few rows: 16 rows x 16 columns, each of four wavefronts a quarter of the
+// blocks straight from memory (w is read once, and that is what counts), four
+// blocks in flight; their sums are joined in LDS, in order.
+constexpr int kThinWaves = 4, kThinAhead = 4;
+
+template <typename T>
+__global__ __launch_bounds__(64 * kThinWaves) void fp8_thin_kernel(Fp8Args a) {
+    __shared__ v4f join[kThinWaves - 1][64];
+    constexpr bool WIDE = sizeof(T) == 4;
+    uint32_t mt, ntile;
+    tile_of(blockIdx.x, gridDim.x, a.nt, a.mt, &mt, &ntile);
+    int g, r0, r1;
+    if (!find_tile(a.offsets, a.groups, a.m, 16, static_cast<int>(mt), &g, &r0, &r1)) return;
+    const int n0 = static_cast<int>(ntile) * 16;
+    const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t kp = static_cast<int64_t>(a.kb) * kBlock;
+    const int src = r0 + r < r1 ? source_row(a, r0 + r) : -1;
+    const int col = n0 + r < a.n ? n0 + r : a.n - 1;  // past the last: computed, not stored
+    const int nb = (a.n + kBlock - 1) / kBlock;
+    const uint8_t* px = a.xq + (src < 0 ? 0 : src) * kp + 16 * q;
+    const uint8_t* pw = a.wq + (static_cast<int64_t>(g) * a.n + col) * kp + 16 * q;
+    const float* xs = a.xscale + (src < 0 ? 0 : src);
+    const float* ws = a.wscale + (static_cast<int64_t>(g) * nb + n0 / kBlock) * a.kb;
+    const int share = (a.kb + kThinWaves - 1) / kThinWaves;
+    const int b0 = wave * share, b1 = b0 + share < a.kb ? b0 + share : a.kb;
+    v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int base = b0; base < b1; base += kThinAhead) {
+        Operand x[kThinAhead], w[kThinAhead];
+        float s[kThinAhead];
+#pragma unroll
+        for (int u = 0; u < kThinAhead; ++u) {
+            const int b = base + u < b1 ? base + u : b1 - 1;  // again, for nothing
+            const int64_t at = static_cast<int64_t>(b) * kBlock;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                w[u].c[h].u = *reinterpret_cast<const v4u*>(pw + at + 64 * h);
+                x[u].c[h].u = *reinterpret_cast<const v4u*>(px + at + 64 * h);
+            }
+            s[u] = xs[static_cast<int64_t>(b) * a.x_rows] * ws[b];
+        }
+#pragma unroll
+        for (int u = 0; u < kThinAhead; ++u) {
+            const v4f p = block_products<WIDE>(w[u], x[u]);
+            if (base + u >= b1) break;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(p[e], s[u], acc[e]);
+        }
+    }
+    if (wave > 0) join[wave - 1][lane] = acc;
+    __syncthreads();
+    if (wave > 0 || r0 + r >= r1) return;
+#pragma unroll
+    for (int u = 0; u < kThinWaves - 1; ++u) acc += join[u][lane];
+    if (src < 0) acc = v4f{0.0f, 0.0f, 0.0f, 0.0f};  // a row of zeros
+    const v4f bias = bias_of<T>(a, g, n0 + 4 * q);
+    with_epilogue(a.epi, [&](auto epi) {
+        store_outputs<T, decltype(epi)::value>(a, r0 + r, n0 + 4 * q, acc, bias);
+    });
+}
+
+using Medium = Shape<128, 128, 2, 2>;
+
+unsigned set_grid(Fp8Args& a, int bm, int bn) {
+    a.mt = static_cast<uint32_t>(most_tiles(a.m, a.groups, bm));
+    a.nt = static_cast<uint32_t>(ceil_div(a.n, bn));
+    const int64_t grid = static_cast<int64_t>(a.mt) * a.nt;
+    require(grid < (int64_t(1) << 31), "matmul_fp8: too many tiles");
+    return static_cast<unsigned>(grid);
+}
+
+template <typename T>
+void launch_fp8(Fp8Args& a, hipStream_t s) {
+    const int64_t kp = static_cast<int64_t>(a.kb) * kBlock;
+    // tiles' offsets have 31 bits
+    const bool fits = (a.rows ? a.x_rows : 256) * kp < kDirectBytes &&
+                      256 * kp < kDirectBytes && 4 * a.x_rows < kDirectBytes;
+    if (!fits || a.m <= 32 * a.groups) {
+        const unsigned grid = set_grid(a, 16, 16);
+        fp8_thin_kernel<T><<<grid, 64 * kThinWaves, 0, s>>>(a);
+    } else {
+        const unsigned grid = set_grid(a, Medium::kM, Medium::kN);
+        fp8_kernel<T, Medium><<<grid, Medium::kThreads, 0, s>>>(a);
+    }
+    TG_LAUNCH_CHECK();
 }
 
 }  // namespace
@@ -281,12 +494,9 @@ int tg_matmul_fp8(int64_t m, int64_t k, int64_t n, int64_t groups, const void* x
         a.y = y;
         a.ldy = ldy;
         if (x_rows == 0) a.kb = 0;  // every row is one of zeros
-        const dim3 grid(static_cast<unsigned>(tg::ceil_div(n, 16)),
-                        static_cast<unsigned>(tg::most_tiles(m, groups, 16)));
         tg::with_type(type, "matmul_fp8", [&](auto t) {
-            tg::fp8_kernel<decltype(t)><<<grid, 64, 0, static_cast<hipStream_t>(stream)>>>(a);
+            tg::launch_fp8<decltype(t)>(a, static_cast<hipStream_t>(stream));
         });
-        TG_LAUNCH_CHECK();
     });
 }
 

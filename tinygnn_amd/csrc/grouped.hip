@@ -1,8 +1,14 @@
 // grouped.hip -- products grouped by expert or node type, with ragged groups.
+//
+// Every product is cut into row tiles of its own groups (find_tile), so no
+// group's size is known to the host and nothing waits for it.  16-bit types go
+// through v_mfma_f32_16x16x32, floats through v_mfma_f32_16x16x4f32 (tiles.hpp);
+// sums are fp32 and rounded once.
 #include "grouped.hpp"
 
 #include <string>
 
+#include "tiles.hpp"
 #include "types.hpp"
 
 namespace tg {
@@ -16,109 +22,375 @@ struct GroupedArgs {
     const int32_t* offsets;
     const void* w;  // forward
     int64_t ldw, w_stride;
-    int transposed;
     const void* bias;
     int epi;
     void* y;
     int64_t ldy;
-    const void* dy;  // gradient of w
+    uint32_t mt, nt;  // row tiles (most) and column tiles
+    const void* dy;   // gradient of w
     int64_t lddy;
     void* dw;
     void* dbias;
+    int unit;    // rows of a part of a group, 0: whole groups
+    float* part;  // [parts][k][n] sums of the parts, [parts][n] of dy's
+    float* part_bias;
 };
 
-constexpr int kT = 64, kTK = 16;  // tile edge and depth
-
-// One 64 x 64 tile, 4 x 4 outputs a thread: a(i, c), b(c, j) give the operands
-// (0 outside), out(i, j, v) takes the sums.
-template <typename A, typename B, typename O>
-__device__ void plain_tile(int depth, A&& a, B&& b, O&& out) {
-    __shared__ float as[kTK][kT + 4], bs[kTK][kT + 4];
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    float acc[4][4] = {};
-    for (int c0 = 0; c0 < depth; c0 += kTK) {
-        for (int i = threadIdx.x; i < kT * kTK; i += 256) {
-            as[i % kTK][i / kTK] = a(i / kTK, c0 + i % kTK);
-            bs[i / kT][i % kT] = b(c0 + i / kT, i % kT);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < kTK; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    acc[i][j] = __builtin_fmaf(as[c][ty * 4 + i], bs[c][tx * 4 + j], acc[i][j]);
-        __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) out(ty * 4 + i, tx * 4 + j, acc[i][j]);
+// x's row for row p of the product, or -1.
+__device__ __forceinline__ int64_t source_row(const GroupedArgs& a, int p) {
+    const int64_t r = a.rows ? a.rows[p] : p;
+    return r < 0 || r >= a.x_rows ? -1 : r;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
+// ---------------------------------------------------------------------------
+// BM x BN outputs by WR x WC wavefronts, two tiles of both operands in LDS: while the matrix instructions read one, the other is loaded.
+// The wavefront's outputs are computed transposed (columns of w as the rows of
+// the instruction), so a lane holds four consecutive columns of y.
+//
+// DIRECT: the tiles come by loads that write to LDS; else through registers,
+// for operands that are not 16-byte aligned or reach past 2 GB.
+// ---------------------------------------------------------------------------
+// The products of one tile pair.
+template <typename T, typename S, typename RA, typename RB>
+__device__ __forceinline__ void multiply(const RA& ra, const RB& rb, const char* la, const char* lb,
+                                         Acc<S>& acc) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        Frag b[S::kNJ];
+#pragma unroll
+        for (int j = 0; j < S::kNJ; ++j) b[j] = rb.read(lb, j, s);
+#pragma unroll
+        for (int i = 0; i < S::kMI; ++i) {
+            const Frag a = ra.read(la, i, s);
+#pragma unroll
+            for (int j = 0; j < S::kNJ; ++j) acc[i][j] = mfma<T>(b[j], a, acc[i][j]);
+        }
+    }
+}
+
+template <typename T, typename S, bool ALONG_W, bool DIRECT>
+__global__ __launch_bounds__(S::kThreads) void grouped_kernel(GroupedArgs a) {
+    __shared__ __attribute__((aligned(16))) char a0[S::kM * kRowBytes];
+    __shared__ __attribute__((aligned(16))) char b0[S::kN * kRowBytes];
+    __shared__ __attribute__((aligned(16))) char a1[S::kM * kRowBytes];
+    __shared__ __attribute__((aligned(16))) char b1[S::kN * kRowBytes];
+    constexpr int Z = sizeof(T);
+    uint32_t mt, ntile;
+    tile_of(blockIdx.x, gridDim.x, a.nt, a.mt, &mt, &ntile);
     int g, r0, r1;
-    if (!find_tile(a.offsets, a.groups, a.m, kT, blockIdx.y, &g, &r0, &r1)) return;
-    const int n0 = blockIdx.x * kT;
+    if (!find_tile(a.offsets, a.groups, a.m, S::kM, static_cast<int>(mt), &g, &r0, &r1)) return;
+    const int n0 = static_cast<int>(ntile) * S::kN;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / S::kWC * S::kMI * 16, wn = wave % S::kWC * S::kNJ * 16;
     const T* x = static_cast<const T*>(a.x);
     const T* w = static_cast<const T*>(a.w) + g * a.w_stride;
-    plain_tile(
-        a.k,
-        [&](int i, int c) {
-            if (r0 + i >= r1 || c >= a.k) return 0.0f;
-            const int64_t r = a.rows ? a.rows[r0 + i] : r0 + i;
-            return r < 0 || r >= a.x_rows ? 0.0f : static_cast<float>(x[r * a.ldx + c]);
-        },
-        [&](int c, int j) {
-            if (c >= a.k || n0 + j >= a.n) return 0.0f;
-            return static_cast<float>(a.transposed ? w[(n0 + j) * a.ldw + c]
-                                                   : w[c * a.ldw + n0 + j]);
-        },
-        [&](int i, int j, float v) {
-            if (r0 + i >= r1 || n0 + j >= a.n) return;
-            const float b = a.bias ? static_cast<float>(static_cast<const T*>(
-                                         a.bias)[static_cast<int64_t>(g) * a.n + n0 + j])
-                                   : 0.0f;
-            static_cast<T*>(a.y)[(r0 + i) * a.ldy + n0 + j] =
-                static_cast<T>(grouped_epilogue(v, b, a.epi));
-        });
+    const int tiles = (a.k + kDepth<T> - 1) / kDepth<T>;
+
+    // chunk t of this thread: its row and first value of x's tile, ...
+    int ac[S::kCA], bmaj[S::kCB], bmin[S::kCB];
+    int64_t ar[S::kCA];  // x's row, -1: zeros
+#pragma unroll
+    for (int t = 0; t < S::kCA; ++t) {
+        int row;
+        chunk_place<T, S::kM, false>(t * S::kThreads + tid, &row, &ac[t]);
+        ar[t] = r0 + row < r1 ? source_row(a, r0 + row) : -1;
+    }
+#pragma unroll
+    for (int t = 0; t < S::kCB; ++t)
+        chunk_place<T, S::kN, !ALONG_W>(t * S::kThreads + tid, &bmaj[t], &bmin[t]);
+
+    Acc<S> acc = {};
+    const Reader<T, S::kM, false, S::kMI> ra(wm, lane);
+    const Reader<T, S::kN, !ALONG_W, S::kNJ> rb(wn, lane);
+    auto compute = [&](const char* la, const char* lb) { multiply<T, S>(ra, rb, la, lb, acc); };
+    if constexpr (DIRECT) {
+        // offsets from the tile's first row (gathered: x's) and w's tile
+        const T* xb = a.rows ? x : x + static_cast<int64_t>(r0) * a.ldx;
+        uint32_t ao[S::kCA], bo[S::kCB];
+#pragma unroll
+        for (int t = 0; t < S::kCA; ++t) {
+            const int64_t row = a.rows ? ar[t] : ar[t] - r0;
+            ao[t] = ar[t] < 0 ? kOutside : static_cast<uint32_t>(Z * (row * a.ldx + ac[t]));
+        }
+#pragma unroll
+        for (int t = 0; t < S::kCB; ++t) {
+            if (ALONG_W)
+                bo[t] = n0 + bmaj[t] < a.n
+                            ? static_cast<uint32_t>(Z * (bmaj[t] * a.ldw + bmin[t]))
+                            : kOutside;
+            else
+                bo[t] = n0 + bmin[t] < a.n
+                            ? static_cast<uint32_t>(Z * (bmaj[t] * a.ldw + bmin[t]))
+                            : kOutside;
+        }
+        const T* wb = ALONG_W ? w + n0 * a.ldw : w + n0;
+        auto load = [&](int kt, char* la, char* lb) {
+            const int k0 = kt * kDepth<T>;
+            const auto xbuf = buffer_of(xb + k0, kDirectBytes);
+            const auto wbuf = buffer_of(ALONG_W ? wb + k0 : wb + k0 * a.ldw, kDirectBytes);
+            const bool part = k0 + kDepth<T> > a.k;  // the last tile: what lies behind k is 0
+#pragma unroll
+            for (int t = 0; t < S::kCA; ++t)
+                load_to_lds(xbuf, la + (t * S::kThreads + wave * 64) * 16,
+                            part && k0 + ac[t] >= a.k ? kOutside : ao[t]);
+#pragma unroll
+            for (int t = 0; t < S::kCB; ++t)
+                load_to_lds(wbuf, lb + (t * S::kThreads + wave * 64) * 16,
+                            part && k0 + (ALONG_W ? bmin[t] : bmaj[t]) >= a.k ? kOutside : bo[t]);
+        };
+        pipeline<true>(tiles, a0, b0, a1, b1, load, [](char*, char*) {}, compute);
+    } else {
+        v4u av[S::kCA], bv[S::kCB];
+        auto load = [&](int kt, char*, char*) {
+            const int k0 = kt * kDepth<T>;
+#pragma unroll
+            for (int t = 0; t < S::kCA; ++t) {
+                const int k = k0 + ac[t];
+                av[t] = load_chunk(x + (ar[t] < 0 ? 0 : ar[t]) * a.ldx + k,
+                                   ar[t] < 0 ? 0 : a.k - k);
+            }
+#pragma unroll
+            for (int t = 0; t < S::kCB; ++t) {
+                const int n = n0 + (ALONG_W ? bmaj[t] : bmin[t]);
+                const int k = k0 + (ALONG_W ? bmin[t] : bmaj[t]);
+                if (ALONG_W)
+                    bv[t] = load_chunk(w + n * a.ldw + k, n < a.n ? a.k - k : 0);
+                else
+                    bv[t] = load_chunk(w + k * a.ldw + n, k < a.k ? a.n - n : 0);
+            }
+        };
+        auto store = [&](char* la, char* lb) {
+#pragma unroll
+            for (int t = 0; t < S::kCA; ++t)
+                *reinterpret_cast<v4u*>(la + (t * S::kThreads + tid) * 16) = av[t];
+#pragma unroll
+            for (int t = 0; t < S::kCB; ++t)
+                *reinterpret_cast<v4u*>(lb + (t * S::kThreads + tid) * 16) = bv[t];
+        };
+        pipeline<false>(tiles, a0, b0, a1, b1, load, store, compute);
+    }
+
+    // lane (q, r): row r of a tile, columns 4 q .. 4 q + 3
+    const int q = lane >> 4, r = lane & 15;
+    float bias[S::kNJ][4];
+#pragma unroll
+    for (int j = 0; j < S::kNJ; ++j) {
+        const int n = n0 + wn + j * 16 + 4 * q;
+        if (a.bias)
+            load_floats<T, 4>(static_cast<const T*>(a.bias) + static_cast<int64_t>(g) * a.n + n,
+                              a.n - n, bias[j]);
+        else
+            bias[j][0] = bias[j][1] = bias[j][2] = bias[j][3] = 0.0f;
+    }
+    with_epilogue(a.epi, [&](auto epi) {
+#pragma unroll
+        for (int i = 0; i < S::kMI; ++i) {
+            const int p = r0 + wm + i * 16 + r;
+            if (p >= r1) continue;
+            T* y = static_cast<T*>(a.y) + p * a.ldy;
+#pragma unroll
+            for (int j = 0; j < S::kNJ; ++j) {
+                const int n = n0 + wn + j * 16 + 4 * q;
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    v[e] = grouped_epilogue<decltype(epi)::value>(acc[i][j][e], bias[j][e]);
+                store_floats<T, 4>(y + n, a.n - n, v);
+            }
+        }
+    });
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void wgrad_kernel(GroupedArgs a) {
-    const int g = blockIdx.z, k0 = blockIdx.y * kT, n0 = blockIdx.x * kT;
-    int lo, hi;
-    group_rows(a.offsets, g, a.m, &lo, &hi);
+// dw_g = x_g^T dy_g and, from the workgroups of dw's first row tile, dbias: dy's
+// columns times ones on the matrix units.  With a.unit a workgroup sums that
+// many of a group's rows to fp32 parts, which parts_kernel adds in order: where
+// the groups' own tiles are too few for the CUs (233K rows of 7 types, 602 x 256:
+// 70 tiles), and the chains over 33K rows too long for fp32's digits.
+template <typename T, typename S, bool DIRECT, bool BIAS>
+__global__ __launch_bounds__(S::kThreads) void wgrad_kernel(GroupedArgs a) {
+    __shared__ __attribute__((aligned(16))) char a0[S::kM * kRowBytes];
+    __shared__ __attribute__((aligned(16))) char b0[S::kN * kRowBytes];
+    __shared__ __attribute__((aligned(16))) char a1[S::kM * kRowBytes];
+    __shared__ __attribute__((aligned(16))) char b1[S::kN * kRowBytes];
+    constexpr int Z = sizeof(T);
+    const uint32_t per = a.mt * a.nt;
+    const int part = static_cast<int>(blockIdx.x / per);
+    uint32_t mt, ntile;
+    tile_of(blockIdx.x % per, per, a.nt, a.mt, &mt, &ntile);
+    int g = part, lo, hi;
+    if (a.unit == 0)
+        group_rows(a.offsets, g, a.m, &lo, &hi);
+    else if (!find_tile(a.offsets, a.groups, a.m, a.unit, part, &g, &lo, &hi))
+        return;
+    const int k0 = static_cast<int>(mt) * S::kM, n0 = static_cast<int>(ntile) * S::kN;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / S::kWC * S::kMI * 16, wn = wave % S::kWC * S::kNJ * 16;
     const T* x = static_cast<const T*>(a.x);
     const T* dy = static_cast<const T*>(a.dy);
-    auto grad = [&](int c, int j) {
-        return lo + c >= hi || n0 + j >= a.n
-                   ? 0.0f
-                   : static_cast<float>(dy[(lo + c) * a.lddy + n0 + j]);
+    const int tiles = (hi - lo + kDepth<T> - 1) / kDepth<T>;
+
+    int ap[S::kCA], ac[S::kCA], bp[S::kCB], bc[S::kCB];
+#pragma unroll
+    for (int t = 0; t < S::kCA; ++t)
+        chunk_place<T, S::kM, true>(t * S::kThreads + tid, &ap[t], &ac[t]);
+#pragma unroll
+    for (int t = 0; t < S::kCB; ++t)
+        chunk_place<T, S::kN, true>(t * S::kThreads + tid, &bp[t], &bc[t]);
+
+    Acc<S> acc = {};
+    v4f sum[BIAS ? S::kNJ : 1] = {};
+    const bool sums = BIAS && mt == 0 && wm == 0;  // uniform
+    const Frag one = ones<T>();
+    const Reader<T, S::kM, true, S::kMI> ra(wm, lane);
+    const Reader<T, S::kN, true, S::kNJ> rb(wn, lane);
+    auto compute = [&](const char* la, const char* lb) {
+        multiply<T, S>(ra, rb, la, lb, acc);
+        if (BIAS && sums) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int j = 0; j < S::kNJ; ++j)
+                    sum[j] = mfma<T>(rb.read(lb, j, s), one, sum[j]);
+        }
     };
-    if (a.dw)
-        plain_tile(
-            hi - lo,
-            [&](int i, int c) {
-                if (lo + c >= hi || k0 + i >= a.k) return 0.0f;
-                const int64_t r = a.rows ? a.rows[lo + c] : lo + c;
-                return r < 0 || r >= a.x_rows ? 0.0f : static_cast<float>(x[r * a.ldx + k0 + i]);
-            },
-            grad,
-            [&](int i, int j, float v) {
-                if (k0 + i < a.k && n0 + j < a.n)
-                    static_cast<T*>(
-                        a.dw)[(static_cast<int64_t>(g) * a.k + k0 + i) * a.n + n0 + j] =
-                        static_cast<T>(v);
-            });
-    if (a.dbias && blockIdx.y == 0 && threadIdx.x < kT && n0 + threadIdx.x < a.n) {
-        float s = 0.0f;
-        for (int c = 0; c < hi - lo; ++c) s += grad(c, threadIdx.x);
-        static_cast<T*>(a.dbias)[static_cast<int64_t>(g) * a.n + n0 + threadIdx.x] =
-            static_cast<T>(s);
+    if constexpr (DIRECT) {
+        uint32_t ao[S::kCA], bo[S::kCB];
+        int idx[S::kCA];  // the next tile's gathered rows
+#pragma unroll
+        for (int t = 0; t < S::kCA; ++t)
+            ao[t] = k0 + ac[t] < a.k ? static_cast<uint32_t>(Z * (ap[t] * a.ldx + k0 + ac[t]))
+                                     : kOutside;
+#pragma unroll
+        for (int t = 0; t < S::kCB; ++t)
+            bo[t] = n0 + bc[t] < a.n ? static_cast<uint32_t>(Z * (bp[t] * a.lddy + n0 + bc[t]))
+                                     : kOutside;
+        auto fetch = [&](int kt) {
+#pragma unroll
+            for (int t = 0; t < S::kCA; ++t) {
+                const int p = lo + kt * kDepth<T> + ap[t];
+                idx[t] = p < hi ? a.rows[p] : -1;
+            }
+        };
+        if (a.rows) fetch(0);
+        auto load = [&](int kt, char* la, char* lb) {
+            const int p0 = lo + kt * kDepth<T>;
+            const int64_t left = hi - p0;  // rows: the buffers end with them
+            const auto dbuf = buffer_of(dy + p0 * a.lddy, Z * ((left - 1) * a.lddy + a.n));
+            if (a.rows) {
+                const auto xbuf = buffer_of(x, kDirectBytes);
+#pragma unroll
+                for (int t = 0; t < S::kCA; ++t) {
+                    const bool in = idx[t] >= 0 && idx[t] < a.x_rows && k0 + ac[t] < a.k;
+                    load_to_lds(xbuf, la + (t * S::kThreads + wave * 64) * 16,
+                                in ? static_cast<uint32_t>(
+                                         Z * (idx[t] * a.ldx + k0 + ac[t]))
+                                   : kOutside);
+                }
+                fetch(kt + 1);
+            } else {
+                const auto xbuf = buffer_of(x + p0 * a.ldx, Z * ((left - 1) * a.ldx + a.k));
+#pragma unroll
+                for (int t = 0; t < S::kCA; ++t)
+                    load_to_lds(xbuf, la + (t * S::kThreads + wave * 64) * 16, ao[t]);
+            }
+#pragma unroll
+            for (int t = 0; t < S::kCB; ++t)
+                load_to_lds(dbuf, lb + (t * S::kThreads + wave * 64) * 16, bo[t]);
+        };
+        pipeline<true>(tiles, a0, b0, a1, b1, load, [](char*, char*) {}, compute);
+    } else {
+        v4u av[S::kCA], bv[S::kCB];
+        auto load = [&](int kt, char*, char*) {
+#pragma unroll
+            for (int t = 0; t < S::kCA; ++t) {
+                const int p = lo + kt * kDepth<T> + ap[t];
+                const int64_t row = p < hi ? source_row(a, p) : -1;
+                av[t] = load_chunk(x + (row < 0 ? 0 : row) * a.ldx + k0 + ac[t],
+                                   row < 0 ? 0 : a.k - k0 - ac[t]);
+            }
+#pragma unroll
+            for (int t = 0; t < S::kCB; ++t) {
+                const int p = lo + kt * kDepth<T> + bp[t];
+                bv[t] = load_chunk(dy + p * a.lddy + n0 + bc[t], p < hi ? a.n - n0 - bc[t] : 0);
+            }
+        };
+        auto store = [&](char* la, char* lb) {
+#pragma unroll
+            for (int t = 0; t < S::kCA; ++t)
+                *reinterpret_cast<v4u*>(la + (t * S::kThreads + tid) * 16) = av[t];
+#pragma unroll
+            for (int t = 0; t < S::kCB; ++t)
+                *reinterpret_cast<v4u*>(lb + (t * S::kThreads + tid) * 16) = bv[t];
+        };
+        pipeline<false>(tiles, a0, b0, a1, b1, load, store, compute);
     }
+
+    const int q = lane >> 4, r = lane & 15;
+    if (a.dw) {
+#pragma unroll
+        for (int i = 0; i < S::kMI; ++i) {
+            const int k = k0 + wm + i * 16 + r;
+            if (k >= a.k) continue;
+            const int64_t row = (static_cast<int64_t>(part) * a.k + k) * a.n;
+#pragma unroll
+            for (int j = 0; j < S::kNJ; ++j) {
+                const int n = n0 + wn + j * 16 + 4 * q;
+                const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                if (a.unit)
+                    store_floats<float, 4>(a.part + row + n, a.n - n, v);
+                else
+                    store_floats<T, 4>(static_cast<T*>(a.dw) + row + n, a.n - n, v);
+            }
+        }
+    }
+    if (BIAS && sums && r == 0) {
+        const int64_t row = static_cast<int64_t>(part) * a.n;
+#pragma unroll
+        for (int j = 0; j < S::kNJ; ++j) {
+            const int n = n0 + wn + j * 16 + 4 * q;
+            const float v[4] = {sum[j][0], sum[j][1], sum[j][2], sum[j][3]};
+            if (a.unit)
+                store_floats<float, 4>(a.part_bias + row + n, a.n - n, v);
+            else
+                store_floats<T, 4>(static_cast<T*>(a.dbias) + row + n, a.n - n, v);
+        }
+    }
+}
+
+// out[g] = the sum of group g's parts, in order: `size` values each.
+template <typename T>
+__global__ __launch_bounds__(256) void parts_kernel(const int32_t* __restrict__ offsets, int m,
+                                                    int unit, int most,
+                                                    const float* __restrict__ part, int64_t size,
+                                                    T* __restrict__ out) {
+    const int g = blockIdx.y, lane = threadIdx.x & (kWave - 1);
+    int first = 0, lo, hi;
+    for (int base = 0; base < g; base += kWave) {
+        int n = 0;
+        if (base + lane < g) {
+            group_rows(offsets, base + lane, m, &lo, &hi);
+            n = (hi - lo + unit - 1) / unit;
+        }
+        first += wave_sum(n);
+    }
+    group_rows(offsets, g, m, &lo, &hi);
+    // (falling offsets may name more parts than there are)
+    int parts = (hi - lo + unit - 1) / unit;
+    parts = parts < most - first ? parts : most - first;
+    const int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+    if (at >= size) return;
+    const float* p = part + first * size + at;
+    float s[4] = {};
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) {
+        float v[4];
+        load_floats<float, 4>(p + i * size, size - at, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += v[e];
+    }
+    store_floats<T, 4>(out + static_cast<int64_t>(g) * size + at, size - at, s);
 }
 
 void check_grouped(const std::string& w, int64_t m, int64_t k, int64_t n, int64_t groups, int type,
@@ -130,6 +402,96 @@ void check_grouped(const std::string& w, int64_t m, int64_t k, int64_t n, int64_
     require(groups <= kMaxGroups, w + ": at most 1024 groups, got " + std::to_string(groups));
     require(type >= TG_TYPE_F32 && type <= TG_TYPE_F16, w + ": unknown element type " +
                                                             std::to_string(type));
+}
+
+// Whether an operand's tiles of up to `major` rows of `ld` elements can come by
+// loads to LDS: whole, aligned 16-byte chunks within 2 GB of the tile's start.
+bool direct_operand(const void* p, int64_t ld, int64_t cols, int64_t stride, int64_t z,
+                    int64_t major) {
+    const int64_t epc = 16 / z;
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % epc == 0 && cols % epc == 0 &&
+           stride % epc == 0 && (major * ld + cols) * z < kDirectBytes;
+}
+
+using Large = Shape<256, 256, 2, 4>;
+using Medium = Shape<128, 128, 2, 2>;
+using Small = Shape<32, 128, 1, 4>;
+
+unsigned grid_of(const std::string& w, int64_t tiles) {
+    require(tiles < (int64_t(1) << 31), w + ": too many tiles");
+    return static_cast<unsigned>(tiles);
+}
+
+template <typename T, typename S>
+void launch_grouped(GroupedArgs& a, bool along, bool direct, hipStream_t s) {
+    a.mt = static_cast<uint32_t>(most_tiles(a.m, a.groups, S::kM));
+    a.nt = static_cast<uint32_t>(ceil_div(a.n, S::kN));
+    const unsigned grid = grid_of("grouped_matmul", static_cast<int64_t>(a.mt) * a.nt);
+    if (along)
+        direct ? grouped_kernel<T, S, true, true><<<grid, S::kThreads, 0, s>>>(a)
+               : grouped_kernel<T, S, true, false><<<grid, S::kThreads, 0, s>>>(a);
+    else
+        direct ? grouped_kernel<T, S, false, true><<<grid, S::kThreads, 0, s>>>(a)
+               : grouped_kernel<T, S, false, false><<<grid, S::kThreads, 0, s>>>(a);
+    TG_LAUNCH_CHECK();
+}
+
+// How a gradient of w is cut.  Whole groups where their tiles are two for each
+// of the 256 CUs; else parts of `unit` rows for about four, 256 rows at least.
+struct WgradPlan {
+    int64_t mt, nt, unit, parts;  // parts: most of them
+    size_t bytes(int64_t k, int64_t n, float** part, float** part_bias, void* ws, size_t size) const {
+        Carver c(ws, size);
+        if (unit == 0) return 0;
+        float* p = c.take<float>(static_cast<size_t>(parts * k * n));
+        float* b = c.take<float>(static_cast<size_t>(parts * n));
+        if (part) *part = p;
+        if (part_bias) *part_bias = b;
+        return c.bytes();
+    }
+};
+
+using WgradShape = Medium;
+
+WgradPlan wgrad_plan(int64_t m, int64_t k, int64_t n, int64_t groups) {
+    WgradPlan p{};
+    p.mt = std::max<int64_t>(1, ceil_div(k, WgradShape::kM));
+    p.nt = ceil_div(n, WgradShape::kN);
+    p.parts = groups;
+    const int64_t tiles = p.mt * p.nt;
+    if (tiles * groups >= 512) return p;
+    const int64_t unit = std::max<int64_t>(256, ceil_div(ceil_div(m * tiles, 1024), 64) * 64);
+    if (unit >= m) return p;
+    p.unit = unit;
+    p.parts = most_tiles(m, groups, unit);
+    return p;
+}
+
+template <typename T>
+void launch_wgrad(GroupedArgs& a, const WgradPlan& p, bool direct, hipStream_t s) {
+    using S = WgradShape;
+    a.mt = static_cast<uint32_t>(p.mt);
+    a.nt = static_cast<uint32_t>(p.nt);
+    a.unit = static_cast<int>(p.unit);
+    const unsigned grid = grid_of("grouped_matmul_wgrad", p.mt * p.nt * p.parts);
+    if (a.dbias)
+        direct ? wgrad_kernel<T, S, true, true><<<grid, S::kThreads, 0, s>>>(a)
+               : wgrad_kernel<T, S, false, true><<<grid, S::kThreads, 0, s>>>(a);
+    else
+        direct ? wgrad_kernel<T, S, true, false><<<grid, S::kThreads, 0, s>>>(a)
+               : wgrad_kernel<T, S, false, false><<<grid, S::kThreads, 0, s>>>(a);
+    TG_LAUNCH_CHECK();
+    if (!p.unit) return;
+    auto add = [&](const float* part, int64_t size, void* out) {
+        const dim3 blocks(grid_of("grouped_matmul_wgrad", ceil_div(size, 1024)),
+                          static_cast<unsigned>(a.groups));
+        parts_kernel<T><<<blocks, 256, 0, s>>>(a.offsets, a.m, a.unit,
+                                               static_cast<int>(p.parts), part, size,
+                                               static_cast<T*>(out));
+        TG_LAUNCH_CHECK();
+    };
+    if (a.dw) add(a.part, static_cast<int64_t>(a.k) * a.n, a.dw);
+    if (a.dbias) add(a.part_bias, a.n, a.dbias);
 }
 
 }  // namespace
@@ -168,27 +530,39 @@ int tg_grouped_matmul(int64_t m, int64_t k, int64_t n, int64_t groups, int type,
         a.w = w;
         a.ldw = ldw;
         a.w_stride = w_stride;
-        a.transposed = transposed != 0;
         a.bias = bias;
         a.epi = epilogue;
         a.y = y;
         a.ldy = ldy;
+        const bool along = transposed != 0;
+        const int64_t z = tg::type_size(type);
+        const bool direct =
+            tg::direct_operand(x, ldx, k, 0, z, rows ? x_rows : 256) &&
+            tg::direct_operand(w, ldw, along ? k : n, groups > 1 ? w_stride : 0, z, 256);
         hipStream_t s = static_cast<hipStream_t>(stream);
-        const dim3 grid(static_cast<unsigned>(tg::ceil_div(n, tg::kT)),
-                        static_cast<unsigned>(tg::most_tiles(m, groups, tg::kT)));
         tg::with_type(type, "grouped_matmul", [&](auto t) {
-            tg::grouped_kernel<decltype(t)><<<grid, 256, 0, s>>>(a);
+            using T = decltype(t);
+            if (m <= 32 * groups)
+                tg::launch_grouped<T, tg::Small>(a, along, direct, s);
+            else if (type == TG_TYPE_F32 || !direct)
+                tg::launch_grouped<T, tg::Medium>(a, along, direct, s);
+            else if constexpr (sizeof(T) == 2)
+                tg::launch_grouped<T, tg::Large>(a, along, direct, s);
         });
-        TG_LAUNCH_CHECK();
     });
 }
 
-size_t tg_grouped_matmul_wgrad_workspace_size(int64_t, int64_t, int64_t, int64_t, int) { return 0; }
+size_t tg_grouped_matmul_wgrad_workspace_size(int64_t m, int64_t k, int64_t n, int64_t groups,
+                                              int) {
+    if (m <= 0 || k < 0 || n <= 0 || groups <= 0 || groups > tg::kMaxGroups) return 0;
+    return tg::wgrad_plan(m, k, n, groups).bytes(k, n, nullptr, nullptr, nullptr, 0);
+}
 
 int tg_grouped_matmul_wgrad(int64_t m, int64_t k, int64_t n, int64_t groups, int type,
                             const void* x, int64_t x_rows, int64_t ldx, const int32_t* rows,
                             const void* dy, int64_t lddy, const int32_t* offsets, void* dw,
-                            void* dbias, void*, size_t, tg_stream_t stream) {
+                            void* dbias, void* workspace, size_t workspace_bytes,
+                            tg_stream_t stream) {
     return guard([&] {
         const std::string what = "grouped_matmul_wgrad";
         tg::check_grouped(what, m, k, n, groups, type, x_rows);
@@ -199,7 +573,7 @@ int tg_grouped_matmul_wgrad(int64_t m, int64_t k, int64_t n, int64_t groups, int
         require(lddy >= n && (!dw || ldx >= k), what + ": leading dimension below the columns");
         tg::GroupedArgs a{};
         a.m = static_cast<int>(m);
-        a.k = static_cast<int>(k);
+        a.k = static_cast<int>(dw ? k : 0);
         a.n = static_cast<int>(n);
         a.groups = static_cast<int>(groups);
         a.x = x;
@@ -211,14 +585,24 @@ int tg_grouped_matmul_wgrad(int64_t m, int64_t k, int64_t n, int64_t groups, int
         a.lddy = lddy;
         a.dw = dw;
         a.dbias = dbias;
+        const int64_t z = tg::type_size(type);
+        const bool direct = tg::direct_operand(x, ldx, a.k, 0, z, rows ? x_rows : 64) &&
+                            tg::direct_operand(dy, lddy, n, 0, z, 64);
         hipStream_t s = static_cast<hipStream_t>(stream);
-        const dim3 grid(static_cast<unsigned>(tg::ceil_div(n, tg::kT)),
-                        static_cast<unsigned>(dw ? tg::ceil_div(k, tg::kT) : 1),
-                        static_cast<unsigned>(groups));
+        const tg::WgradPlan plan = tg::wgrad_plan(m, a.k, n, groups);
+        tg::TempBuffer temp;
+        if (plan.unit) {
+            const size_t need = plan.bytes(a.k, n, nullptr, nullptr, nullptr, 0);
+            if (!workspace) {
+                temp.allocate(need, s);
+                workspace = temp.get();
+                workspace_bytes = need;
+            }
+            plan.bytes(a.k, n, &a.part, &a.part_bias, workspace, workspace_bytes);
+        }
         tg::with_type(type, "grouped_matmul_wgrad", [&](auto t) {
-            tg::wgrad_kernel<decltype(t)><<<grid, 256, 0, s>>>(a);
+            tg::launch_wgrad<decltype(t)>(a, plan, direct, s);
         });
-        TG_LAUNCH_CHECK();
     });
 }
 

@@ -1,0 +1,240 @@
+// tiles.hpp -- operand tiles of the matrix products in LDS: how they lie
+// there, how they come from memory and how the matrix instructions' operands
+// are read.
+//
+// A tile holds 128 bytes of values along the contraction (64 of 16 bits, 32
+// floats, 128 of 8 bits) for each of its R rows (of x) or columns (of w).  Two
+// forms:
+//   * along: the contraction runs along memory.  [R][128 bytes], a row's eight
+//     16-byte chunks at positions c ^ (row & 7): sixteen lanes that read one
+//     chunk each of sixteen rows meet every bank equally.
+//   * across: the contraction runs across memory (w [k x n] in x * w; both
+//     operands in x^T * dy).  [depth][R], in slots of 16 values that are
+//     permuted within a row of the tile by its k, so that what the lanes of an
+//     operand read (one slot in several rows) falls in different banks.  Floats
+//     are read one by one; 16-bit values by the transposing LDS load, whose
+//     sixteen lanes cover four rows of one slot: lane l reads 8 bytes of row
+//     l / 4 and gets column l of the four rows.
+// A thread moves the same 16-byte chunks in every tile, chunk (t threads + its
+// number) to LDS address 16 x that: what the loads that write straight to LDS
+// need (a wavefront's 64 chunks are consecutive there), so the permutations are
+// applied to the addresses in memory.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "device_utils.hpp"
+#include "types.hpp"
+
+namespace tg {
+
+constexpr int kRowBytes = 128;    // of a tile along the contraction
+template <typename T>
+constexpr int kDepth = kRowBytes / static_cast<int>(sizeof(T));
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef f16 v8h __attribute__((ext_vector_type(8)));
+#define TG_LDS __attribute__((address_space(3)))
+
+// 16 bytes of consecutive contraction values of a row or column.
+union Frag {
+    v4u u;
+    v4f f;
+    v4s s[2];
+    v8bf b;
+    v8h h;
+};
+
+template <typename T>
+__device__ __forceinline__ Frag ones() {
+    Frag v;
+    if constexpr (std::is_same_v<T, float>) {
+        v.f = v4f{1.0f, 1.0f, 1.0f, 1.0f};
+    } else {
+        const uint32_t one = std::is_same_v<T, bf16> ? 0x3F80u : 0x3C00u;
+        v.u = v4u{one * 0x10001u, one * 0x10001u, one * 0x10001u, one * 0x10001u};
+    }
+    return v;
+}
+
+// c + the products of 64 (16 floats) contraction values' fragments.
+template <typename T>
+__device__ __forceinline__ v4f mfma(const Frag& a, const Frag& b, v4f c) {
+    if constexpr (std::is_same_v<T, bf16>) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.b, b.b, c, 0, 0, 0);
+    } else if constexpr (std::is_same_v<T, f16>) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.h, b.h, c, 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.f[e], b.f[e], c, 0, 0, 0);
+        return c;
+    }
+}
+
+// The permutation of an across tile's slots in row k (of R / 16 slots).  16-bit
+// operands: a read covers rows 8 q + 0 .. 3 of lanes' quarters q; floats: row
+// 4 q of each.
+template <typename T, int R>
+__device__ __forceinline__ int slot_swizzle(int k) {
+    const int s = sizeof(T) == 2 ? (k & 3) | ((k >> 3) & 1) << 2 : (k >> 2) & 3;
+    return s & (R / 16 - 1);
+}
+
+// Where a thread's chunk number e lies in the tile: (row, first value), the
+// permutation undone.  ACROSS: (k, first column).
+template <typename T, int R, bool ACROSS>
+__device__ __forceinline__ void chunk_place(int e, int* major, int* minor) {
+    constexpr int EPC = kVec<T>;
+    if constexpr (ACROSS) {
+        constexpr int CPR = R / EPC, CPS = 16 / EPC;  // chunks of a row, of a slot
+        const int k = e / CPR, p = e % CPR;
+        *major = k;
+        *minor = ((p / CPS) ^ slot_swizzle<T, R>(k)) * 16 + p % CPS * EPC;
+    } else {
+        *major = e >> 3;
+        *minor = ((e & 7) ^ (*major & 7)) * EPC;
+    }
+}
+
+// A wavefront's operands of N tiles of 16 rows (columns) from row `first` on.
+template <typename T, int R, bool ACROSS, int N>
+struct Reader {
+    int at[ACROSS ? N : 2];
+    __device__ __forceinline__ Reader(int first, int lane) {
+        const int q = lane >> 4, r = lane & 15;
+        if constexpr (ACROSS) {
+            const int k = sizeof(T) == 2 ? 8 * q + (r >> 2) : 4 * q;
+            const int in = sizeof(T) == 2 ? (r & 3) * 8 : r * 4;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                at[i] = (k * R + (((first >> 4) + i) ^ slot_swizzle<T, R>(k)) * 16) *
+                            static_cast<int>(sizeof(T)) +
+                        in;
+        } else {
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+                at[s] = (first + r) * kRowBytes + (((4 * s + q) ^ (r & 7)) << 4);
+        }
+    }
+    // Tile i, chunk 4 s + q of the contraction (s = 0, 1).
+    __device__ __forceinline__ Frag read(const char* lds, int i, int s) const {
+        Frag f;
+        if constexpr (!ACROSS) {
+            f.u = *reinterpret_cast<const v4u*>(lds + at[s] + i * 16 * kRowBytes);
+        } else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                f.s[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (TG_LDS v4s*)(lds + at[i] + (32 * s + 4 * h) * R * 2));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                f.f[e] = *reinterpret_cast<const float*>(lds + at[i] + (16 * s + e) * R * 4);
+        }
+        return f;
+    }
+};
+
+// The memory side.  `Direct`: buffer loads that write to LDS by themselves,
+// zeros for what lies outside the buffer: offsets of 32 bits from a base that
+// moves with the tile, 16-byte aligned chunks that are whole or outside.
+constexpr uint32_t kOutside = 0x80000000u;  // added to an offset: outside any buffer below
+constexpr int64_t kDirectBytes = int64_t(1) << 31;
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, int64_t bytes) {
+    const int64_t n = bytes < 0 ? 0 : bytes > kDirectBytes ? kDirectBytes : bytes;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, static_cast<int>(n),
+                                             0x00020000);
+}
+
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t b, char* lds, uint32_t offset) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (TG_LDS void*)lds, 16, static_cast<int>(offset), 0,
+                                             0, 0);
+}
+
+// 16 bytes of T's values at any address of theirs, zeros from `left` values on.
+template <typename T>
+__device__ __forceinline__ v4u load_chunk(const T* p, int64_t left) {
+    constexpr int EPC = kVec<T>;
+    v4u v = {0, 0, 0, 0};
+    if (left >= EPC) {
+        typedef T Whole __attribute__((ext_vector_type(EPC)));
+        v = __builtin_bit_cast(v4u, static_cast<Whole>(
+                                        *reinterpret_cast<const typename Pack<T, EPC>::V*>(p)));
+    } else if (left > 0) {
+        if constexpr (sizeof(T) == 4) {
+            const uint32_t* e = reinterpret_cast<const uint32_t*>(p);
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                if (i < left) v[i] = e[i];
+        } else {
+            const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+            for (int i = 0; i < 7; ++i)
+                if (i < left) v[i / 2] |= static_cast<uint32_t>(e[i]) << (i % 2 * 16);
+        }
+    }
+    return v;
+}
+
+// The tile that workgroup `b` of `grid` takes of `mt` x `nt`: each XCD (every
+// eighth workgroup) has a run of consecutive tiles, taken `kBand` row tiles by
+// all columns at a time, so that the tiles in flight on an XCD share their rows
+// and columns in its L2.
+constexpr int kBand = 4;
+__device__ __forceinline__ void tile_of(uint32_t b, uint32_t grid, uint32_t nt, uint32_t mt,
+                                        uint32_t* i, uint32_t* j) {
+    const uint32_t per = grid / 8, rest = grid % 8, x = b % 8;
+    uint32_t t = x * per + (x < rest ? x : rest) + b / 8;
+    const uint32_t band = t / (kBand * nt), first = band * kBand;
+    const uint32_t high = mt - first < kBand ? mt - first : kBand;
+    t -= band * kBand * nt;
+    *i = first + t % high;
+    *j = t / high;
+}
+
+// BM x BN outputs by WR x WC wavefronts.
+template <int BM, int BN, int WR, int WC>
+struct Shape {
+    static constexpr int kM = BM, kN = BN, kWR = WR, kWC = WC, kThreads = 64 * WR * WC;
+    static constexpr int kMI = BM / WR / 16, kNJ = BN / WC / 16;
+    static constexpr int kCA = BM * 8 / kThreads, kCB = BN * 8 / kThreads;  // chunks a thread
+    static_assert(kCA * kThreads == BM * 8 && kCB * kThreads == BN * 8, "chunks");
+};
+
+template <typename S>
+using Acc = v4f[S::kMI][S::kNJ];
+
+// The loop over `tiles` tiles: load(kt, la, lb) brings tile kt.  With DIRECT
+// the loads are in flight until the barrier; else load keeps them in registers
+// and store(la, lb) writes them.
+template <bool DIRECT, typename L, typename W, typename C>
+__device__ __forceinline__ void pipeline(int tiles, char* a0, char* b0, char* a1, char* b1,
+                                         L&& load, W&& store, C&& compute) {
+    if (tiles == 0) return;
+    load(0, a0, b0);
+    if (!DIRECT) store(a0, b0);
+    int kt = 0;
+    for (; kt + 1 < tiles; kt += 2) {
+        __syncthreads();
+        load(kt + 1, a1, b1);
+        compute(a0, b0);
+        if (!DIRECT) store(a1, b1);
+        __syncthreads();
+        if (kt + 2 < tiles) load(kt + 2, a0, b0);
+        compute(a1, b1);
+        if (!DIRECT && kt + 2 < tiles) store(a0, b0);
+    }
+    if (kt < tiles) {
+        __syncthreads();
+        compute(a0, b0);
+    }
+}
+
+}  // namespace tg
