@@ -166,6 +166,9 @@ class _Fake(torch.Tensor):
     is_cuda = True
     device = torch.device("cuda", 0)
 
+    def get_device(self):
+        return 0
+
 
 def fake(*shape, dtype=torch.float32):
     return torch.zeros(*shape, dtype=dtype).as_subclass(_Fake)
@@ -209,6 +212,8 @@ I32 = torch.int32
 def test_shapes_are_refused(monkeypatch, call, text):
     import tinygnn_amd as tg
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
-    monkeypatch.setattr(tg, "stream_handle", lambda stream=None: 0)
+    names = tg._Torch()
+    names.raw_stream = lambda index: 0
+    monkeypatch.setattr(tg, "_pt", names)
     with pytest.raises(tg.InvalidArgument, match=text):
         call(tg)

@@ -396,153 +396,173 @@ def gat_aggregate(plan: SpmmPlan, a_sl: DeviceCSR, wh, heads: int, f: int, src, 
 # A call runs on `stream`, or on the current stream of its tensors' device;
 # given a `stream` that is not the current one, it returns finished results.
 # Outputs and workspaces are torch memory, so the calls can be captured.
+# (Small calls are bound by this code: messages are made when they are needed.)
 # ---------------------------------------------------------------------------
-_TYPES: dict = {}
+class _Torch:
+    """What the calls below use of torch, looked up once."""
 
-
-def _type_of(t, what: str) -> int:
-    if not _TYPES:
+    def __init__(self):
         torch = _torch()
-        _TYPES.update({torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16,
-                       torch.float16: TYPE_F16})
-    code = _TYPES.get(t.dtype)
+        self.torch = torch
+        self.empty = torch.empty
+        self.f32, self.i32, self.u8 = torch.float32, torch.int32, torch.uint8
+        self.f8 = torch.float8_e4m3fn
+        self.types = {torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16,
+                      torch.float16: TYPE_F16}
+        self.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+_pt: _Torch | None = None
+
+
+def _refuse(what: str, message: str):
+    raise InvalidArgument(1, f"{what}: {message}")
+
+
+def _device_call(fn):
+    """The first tensor's GPU is the current device for the call."""
+    import functools
+
+    @functools.wraps(fn)
+    def call(first, *args, **kwargs):
+        global _pt
+        if _pt is None:
+            _pt = _Torch()
+        index = getattr(first, "q", first).get_device()
+        if index < 0:
+            raise ValueError("tinygnn_amd expects device (cuda) tensors")
+        cuda = _pt.torch.cuda
+        if index != cuda.current_device():
+            with cuda.device(index):
+                return fn(first, *args, **kwargs)
+        return fn(first, *args, **kwargs)
+
+    return call
+
+
+def _stream_of(what: str, stream, first, *others) -> int:
+    """The stream's handle; every tensor must be on the first one's GPU."""
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            if t.get_device() < 0:
+                raise ValueError("tinygnn_amd expects device (cuda) tensors")
+            _refuse(what, f"tensors on {first.device} and {t.device}.")
+    if stream is not None or _pt.raw_stream is None:
+        return stream_handle(stream)
+    return _pt.raw_stream(index)
+
+
+def _type_of(what: str, t) -> int:
+    code = _pt.types.get(t.dtype)
     if code is None:
-        raise InvalidArgument(1, f"{what}: float32, bfloat16 or float16 tensors expected, got "
-                                 f"{t.dtype}.")
+        _refuse(what, f"float32, bfloat16 or float16 tensors expected, got {t.dtype}.")
     return code
 
 
-class _Call:
-    """The device and stream of a call: every tensor on one GPU, which is made
-    the current device for the call where it is not."""
-
-    def __init__(self, what: str, stream, *tensors):
-        torch = _torch()
-        dev = tensors[0].device
-        for t in tensors:
-            if t is None:
-                continue
-            if not t.is_cuda:
-                raise ValueError("tinygnn_amd expects device (cuda) tensors")
-            if t.device != dev:
-                raise InvalidArgument(1, f"{what}: tensors on {dev} and {t.device}.")
-        self.what, self.stream, self.guard = what, stream, None
-        if dev.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        self.handle = stream_handle(self.stream)
-        return self
-
-    def __exit__(self, kind, value, trace):
-        try:
-            if kind is None:
-                _finish(self.stream)
-        finally:
-            if self.guard is not None:
-                self.guard.__exit__(kind, value, trace)
-        return False
-
-    def require(self, ok: bool, message: str) -> None:
-        if not ok:
-            raise InvalidArgument(1, f"{self.what}: {message}")
-
-    def rows(self, t, name: str):
-        """A 2-D tensor whose rows are contiguous, and its leading dimension."""
-        self.require(t.dim() == 2, f"{name} must be a matrix, got {tuple(t.shape)}.")
-        self.require(t.stride(1) == 1 or t.shape[1] <= 1 or t.numel() == 0,
-                     f"{name} must have contiguous rows, got strides {t.stride()}.")
-        if t.shape[0] <= 1:
-            return t.data_ptr(), max(t.shape[1], 1)
-        self.require(t.numel() == 0 or t.stride(0) >= t.shape[1],
-                     f"{name} has overlapping rows (strides {t.stride()}).")
-        return t.data_ptr(), max(t.stride(0), t.shape[1])
-
-    def flat(self, t, name: str, shape, dtype):
-        """A contiguous tensor of a given shape and type, or None."""
-        if t is None:
-            return 0
-        self.require(tuple(t.shape) == tuple(shape),
-                     f"{name} must be {tuple(shape)}, got {tuple(t.shape)}.")
-        self.require(t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}.")
-        self.require(t.is_contiguous(), f"{name} must be contiguous.")
-        return t.data_ptr()
-
-    def out(self, t, name: str, shape, like):
-        if t is None:
-            return _torch().empty(shape, dtype=like.dtype, device=like.device)
-        self.require(tuple(t.shape) == tuple(shape),
-                     f"{name} must be {tuple(shape)}, got {tuple(t.shape)}.")
-        self.require(t.dtype == like.dtype, f"{name} must be {like.dtype}, got {t.dtype}.")
-        return t
-
-    def workspace(self, size: int, device):
-        """`size` bytes of torch memory (0: none)."""
-        if not size:
-            return None, 0
-        return _torch().empty(size, dtype=_torch().uint8, device=device), size
+def _rows_of(what: str, name: str, t):
+    """Pointer and leading dimension of a matrix whose rows are contiguous."""
+    if t.dim() != 2:
+        _refuse(what, f"{name} must be a matrix, got {tuple(t.shape)}.")
+    ld, step = t.stride()
+    rows, cols = t.shape
+    if step == 1 and ld >= cols:
+        return t.data_ptr(), ld
+    if step != 1 and cols > 1 and rows > 0:
+        _refuse(what, f"{name} must have contiguous rows, got strides {t.stride()}.")
+    if rows > 1 and cols > 0 and ld < cols:
+        _refuse(what, f"{name} has overlapping rows (strides {t.stride()}).")
+    return t.data_ptr(), max(ld, cols, 1) if rows > 1 else max(cols, 1)
 
 
-def _norm_weights(call, x, gamma, beta):
+def _flat(what: str, name: str, t, shape, dtype):
+    """Pointer of a contiguous tensor of a given shape and type; None's."""
+    if t is None:
+        return None
+    if t.shape != shape or t.dtype is not dtype or not t.is_contiguous():
+        _refuse(what, f"{name} must be contiguous, {tuple(shape)} {dtype}, got {tuple(t.shape)} "
+                      f"{t.dtype}, strides {t.stride()}.")
+    return t.data_ptr()
+
+
+def _out(what: str, name: str, t, shape, like, dtype):
+    """An output: `t` if it fits, or new memory; with pointer and leading
+    dimension."""
+    if t is None:
+        t = _pt.empty(shape, dtype=dtype, device=like.device)
+        return t, t.data_ptr(), max(shape[1], 1)
+    if t.shape != shape or t.dtype is not dtype:
+        _refuse(what, f"{name} must be {tuple(shape)} {dtype}, got {tuple(t.shape)} {t.dtype}.")
+    return (t, *_rows_of(what, name, t))
+
+
+def _workspace(size: int, like):
+    """`size` bytes of torch memory: the tensor and its pointer (0: none)."""
+    if not size:
+        return None, None
+    t = _pt.empty(size, dtype=_pt.u8, device=like.device)
+    return t, t.data_ptr()
+
+
+def _norm_weights(what: str, x, gamma, beta):
     """gamma's and beta's pointers and type: both x's type, or both float32."""
-    torch = _torch()
-    given = [t for t in (gamma, beta) if t is not None]
-    kind = given[0].dtype if given else x.dtype
-    call.require(kind in (x.dtype, torch.float32),
-                 f"gamma and beta must be {x.dtype} or torch.float32, got {kind}.")
+    given = gamma if gamma is not None else beta
+    kind = x.dtype if given is None else given.dtype
+    if kind is not x.dtype and kind is not _pt.f32:
+        _refuse(what, f"gamma and beta must be {x.dtype} or torch.float32, got {kind}.")
     cols = (x.shape[1],)
-    return (call.flat(gamma, "gamma", cols, kind), call.flat(beta, "beta", cols, kind), kind)
+    return (_flat(what, "gamma", gamma, cols, kind), _flat(what, "beta", beta, cols, kind), kind)
 
 
+@_device_call
 def layer_norm(x, gamma=None, beta=None, eps: float = 1e-5, with_stats: bool = False, out=None,
                stream=None):
     """The rows of x [rows, cols] to mean 0 and variance 1, times gamma, plus
     beta (tg_layer_norm).  gamma / beta: [cols] of x's type or float32.
     with_stats: (y, mean, rstd), float32 [rows], for layer_norm_backward."""
-    torch = _torch()
-    with _Call("layer_norm", stream, x, gamma, beta, out) as c:
-        kind = _type_of(x, "layer_norm")
-        px, ldx = c.rows(x, "x")
-        rows, cols = x.shape
-        pg, pb, wk = _norm_weights(c, x, gamma, beta)
-        y = c.out(out, "out", x.shape, x)
-        py, ldy = c.rows(y, "out")
-        mean = rstd = None
-        if with_stats:
-            mean = torch.empty(rows, dtype=torch.float32, device=x.device)
-            rstd = torch.empty_like(mean)
-        lib.check(lib.tg_layer_norm(rows, cols, kind, px, ldx, pg, pb, _TYPES[wk], eps, py, ldy,
-                                    mean.data_ptr() if with_stats else 0,
-                                    rstd.data_ptr() if with_stats else 0, c.handle))
+    what = "layer_norm"
+    s = _stream_of(what, stream, x, gamma, beta, out)
+    kind = _type_of(what, x)
+    px, ldx = _rows_of(what, "x", x)
+    rows, cols = x.shape
+    pg, pb, wk = _norm_weights(what, x, gamma, beta)
+    y, py, ldy = _out(what, "out", out, x.shape, x, x.dtype)
+    mean = rstd = pm = pr = None
+    if with_stats:
+        mean = _pt.empty(rows, dtype=_pt.f32, device=x.device)
+        rstd = _pt.empty(rows, dtype=_pt.f32, device=x.device)
+        pm, pr = mean.data_ptr(), rstd.data_ptr()
+    lib.check(lib.tg_layer_norm(rows, cols, kind, px, ldx, pg, pb, _pt.types[wk], eps, py, ldy,
+                                pm, pr, s))
+    _finish(stream)
     return (y, mean, rstd) if with_stats else y
 
 
+@_device_call
 def layer_norm_backward(dy, x, mean, rstd, gamma=None, out=None, stream=None):
     """(dx, dgamma, dbeta) of layer_norm from dy, its x, mean and rstd
     (tg_layer_norm_backward); dgamma and dbeta have gamma's type (x's without
     gamma).  out takes dx (it may be dy)."""
-    torch = _torch()
     what = "layer_norm_backward"
-    with _Call(what, stream, x, dy, mean, rstd, gamma, out) as c:
-        kind = _type_of(x, what)
-        rows, cols = x.shape if x.dim() == 2 else (-1, -1)
-        px, ldx = c.rows(x, "x")
-        c.require(dy.shape == x.shape and dy.dtype == x.dtype,
-                  f"dy must be {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}.")
-        pdy, lddy = c.rows(dy, "dy")
-        pg, _, wk = _norm_weights(c, x, gamma, None)
-        pm = c.flat(mean, "mean", (rows,), torch.float32)
-        pr = c.flat(rstd, "rstd", (rows,), torch.float32)
-        dx = c.out(out, "out", x.shape, x)
-        pdx, lddx = c.rows(dx, "out")
-        dgamma = torch.empty(cols, dtype=wk, device=x.device)
-        dbeta = torch.empty_like(dgamma)
-        ws, size = c.workspace(lib.tg_layer_norm_backward_workspace_size(rows, cols), x.device)
-        lib.check(lib.tg_layer_norm_backward(
-            rows, cols, kind, pdy, lddy, px, ldx, pg, _TYPES[wk], pm, pr, pdx, lddx,
-            dgamma.data_ptr(), dbeta.data_ptr(), ws.data_ptr() if size else None, size, c.handle))
+    s = _stream_of(what, stream, dy, x, mean, rstd, gamma, out)
+    kind = _type_of(what, x)
+    px, ldx = _rows_of(what, "x", x)
+    rows, cols = x.shape
+    if dy.shape != x.shape or dy.dtype is not x.dtype:
+        _refuse(what, f"dy must be {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}.")
+    pdy, lddy = _rows_of(what, "dy", dy)
+    pg, _, wk = _norm_weights(what, x, gamma, None)
+    pm = _flat(what, "mean", mean, (rows,), _pt.f32)
+    pr = _flat(what, "rstd", rstd, (rows,), _pt.f32)
+    dx, pdx, lddx = _out(what, "out", out, x.shape, x, x.dtype)
+    dgamma = _pt.empty(cols, dtype=wk, device=x.device)
+    dbeta = _pt.empty(cols, dtype=wk, device=x.device)
+    size = lib.tg_layer_norm_backward_workspace_size(rows, cols)
+    ws, pws = _workspace(size, x)
+    lib.check(lib.tg_layer_norm_backward(rows, cols, kind, pdy, lddy, px, ldx, pg, _pt.types[wk],
+                                         pm, pr, pdx, lddx, dgamma.data_ptr(), dbeta.data_ptr(),
+                                         pws, size, s))
+    _finish(stream)
     return dx, dgamma, dbeta
 
 
@@ -556,134 +576,159 @@ class RoutePlan:
     position: object
 
 
+@_device_call
 def route(logits, k: int, renormalize: bool = False, stream=None):
     """Softmax of each row of logits [tokens, experts] and its k largest, with
     the plan of the rows by expert (tg_route): (weights float32 [tokens, k],
     experts int32 [tokens, k], RoutePlan).  A logit of -inf masks its expert;
     places without an expert hold -1 and weight 0."""
-    torch = _torch()
-    with _Call("route", stream, logits) as c:
-        kind = _type_of(logits, "route")
-        pl, ld = c.rows(logits, "logits")
-        tokens, experts = logits.shape
-        dev = logits.device
-        c.require(1 <= k <= 32 and k <= experts <= 1024,
-                  f"k must be between 1 and min(32, experts) and experts at most 1024, got k={k} "
-                  f"of {experts}.")
-        weights = torch.empty((tokens, k), dtype=torch.float32, device=dev)
-        ids = torch.empty((tokens, k), dtype=torch.int32, device=dev)
-        plan = RoutePlan(torch.empty(experts + 1, dtype=torch.int32, device=dev),
-                         torch.empty(tokens * k, dtype=torch.int32, device=dev),
-                         torch.empty((tokens, k), dtype=torch.int32, device=dev))
-        ws, size = c.workspace(lib.tg_route_workspace_size(tokens, experts, k), dev)
-        lib.check(lib.tg_route(tokens, experts, k, kind, pl, ld, int(renormalize),
-                               weights.data_ptr(), ids.data_ptr(), plan.offsets.data_ptr(),
-                               plan.rows.data_ptr(), plan.position.data_ptr(),
-                               ws.data_ptr() if size else None, size, c.handle))
-    return weights, ids, plan
+    what = "route"
+    s = _stream_of(what, stream, logits)
+    kind = _type_of(what, logits)
+    pl, ld = _rows_of(what, "logits", logits)
+    tokens, experts = logits.shape
+    if not (1 <= k <= 32 and k <= experts <= 1024):
+        _refuse(what, f"k must be between 1 and min(32, experts) and experts at most 1024, got "
+                      f"k={k} of {experts}.")
+    dev = logits.device
+    weights = _pt.empty((tokens, k), dtype=_pt.f32, device=dev)
+    ids = _pt.empty((tokens, k), dtype=_pt.i32, device=dev)
+    offsets = _pt.empty(experts + 1, dtype=_pt.i32, device=dev)
+    rows = _pt.empty(tokens * k, dtype=_pt.i32, device=dev)
+    position = _pt.empty((tokens, k), dtype=_pt.i32, device=dev)
+    size = lib.tg_route_workspace_size(tokens, experts, k)
+    ws, pws = _workspace(size, logits)
+    lib.check(lib.tg_route(tokens, experts, k, kind, pl, ld, 1 if renormalize else 0,
+                           weights.data_ptr(), ids.data_ptr(), offsets.data_ptr(),
+                           rows.data_ptr(), position.data_ptr(), pws, size, s))
+    _finish(stream)
+    return weights, ids, RoutePlan(offsets, rows, position)
 
 
+@_device_call
 def route_plan(ids, groups: int, stream=None) -> RoutePlan:
     """The plan of rows whose groups are known (tg_route_plan): ids int32
     [rows] (node types) or [rows, k]; an id outside [0, groups) is in none."""
-    torch = _torch()
-    with _Call("route_plan", stream, ids) as c:
-        c.require(ids.dim() in (1, 2) and ids.dtype == torch.int32 and ids.is_contiguous(),
-                  f"ids must be a contiguous int32 vector or matrix, got {tuple(ids.shape)} "
-                  f"{ids.dtype}.")
-        c.require(1 <= groups <= 1024, f"between 1 and 1024 groups, got {groups}.")
-        n, k, dev = ids.numel(), ids.shape[1] if ids.dim() == 2 else 1, ids.device
-        plan = RoutePlan(torch.empty(groups + 1, dtype=torch.int32, device=dev),
-                         torch.empty(n, dtype=torch.int32, device=dev), torch.empty_like(ids))
-        ws, size = c.workspace(lib.tg_route_plan_workspace_size(n, groups), dev)
-        lib.check(lib.tg_route_plan(n, groups, max(k, 1), ids.data_ptr(), plan.offsets.data_ptr(),
-                                    plan.rows.data_ptr(), plan.position.data_ptr(),
-                                    ws.data_ptr() if size else None, size, c.handle))
-    return plan
+    what = "route_plan"
+    s = _stream_of(what, stream, ids)
+    if ids.dim() not in (1, 2) or ids.dtype is not _pt.i32 or not ids.is_contiguous():
+        _refuse(what, f"ids must be a contiguous int32 vector or matrix, got {tuple(ids.shape)} "
+                      f"{ids.dtype}.")
+    if not 1 <= groups <= 1024:
+        _refuse(what, f"between 1 and 1024 groups, got {groups}.")
+    n, k, dev = ids.numel(), ids.shape[1] if ids.dim() == 2 else 1, ids.device
+    offsets = _pt.empty(groups + 1, dtype=_pt.i32, device=dev)
+    rows = _pt.empty(n, dtype=_pt.i32, device=dev)
+    position = _pt.empty(ids.shape, dtype=_pt.i32, device=dev)
+    size = lib.tg_route_plan_workspace_size(n, groups)
+    ws, pws = _workspace(size, ids)
+    lib.check(lib.tg_route_plan(n, groups, max(k, 1), ids.data_ptr(), offsets.data_ptr(),
+                                rows.data_ptr(), position.data_ptr(), pws, size, s))
+    _finish(stream)
+    return RoutePlan(offsets, rows, position)
 
 
+@_device_call
 def route_backward(dweights, logits, weights, experts, renormalize: bool = False, stream=None):
     """dlogits of route from the gradient of its weights (tg_route_backward)."""
-    torch = _torch()
     what = "route_backward"
-    with _Call(what, stream, logits, dweights, weights, experts) as c:
-        kind = _type_of(logits, what)
-        pl, ld = c.rows(logits, "logits")
-        tokens, n = logits.shape
-        c.require(weights.dim() == 2, "weights must be [tokens, k].")
-        k = weights.shape[1]
-        shape = (tokens, k)
-        pw = c.flat(weights, "weights", shape, torch.float32)
-        pe = c.flat(experts, "experts", shape, torch.int32)
-        pd = c.flat(dweights, "dweights", shape, torch.float32)
-        out = torch.empty((tokens, n), dtype=logits.dtype, device=logits.device)
-        lib.check(lib.tg_route_backward(tokens, n, k, kind, pl, ld, int(renormalize), pw, pe, pd,
-                                        out.data_ptr(), n, c.handle))
+    s = _stream_of(what, stream, dweights, logits, weights, experts)
+    kind = _type_of(what, logits)
+    pl, ld = _rows_of(what, "logits", logits)
+    tokens, n = logits.shape
+    if weights.dim() != 2:
+        _refuse(what, f"weights must be [tokens, k], got {tuple(weights.shape)}.")
+    k = weights.shape[1]
+    shape = (tokens, k)
+    pw = _flat(what, "weights", weights, shape, _pt.f32)
+    pe = _flat(what, "experts", experts, shape, _pt.i32)
+    pd = _flat(what, "dweights", dweights, shape, _pt.f32)
+    out = _pt.empty((tokens, n), dtype=logits.dtype, device=logits.device)
+    lib.check(lib.tg_route_backward(tokens, n, k, kind, pl, ld, 1 if renormalize else 0, pw, pe,
+                                    pd, out.data_ptr(), n, s))
+    _finish(stream)
     return out
 
 
-def _places(c, position):
-    c.require(position.dim() == 2, f"position must be [tokens, k], got {tuple(position.shape)}.")
-    return c.flat(position, "position", position.shape, _torch().int32)
+def _places(what: str, position):
+    if position.dim() != 2:
+        _refuse(what, f"position must be [tokens, k], got {tuple(position.shape)}.")
+    return _flat(what, "position", position, position.shape, _pt.i32)
 
 
+@_device_call
 def route_combine(y, position, weights=None, out=None, stream=None):
     """out[t] = sum over j of weights[t, j] * y[position[t, j]], weights of 1
     if None (tg_route_combine); a position of -1 adds nothing."""
-    torch = _torch()
-    with _Call("route_combine", stream, y, position, weights, out) as c:
-        kind = _type_of(y, "route_combine")
-        py, ldy = c.rows(y, "y")
-        pp = _places(c, position)
-        tokens, k = position.shape
-        pw = c.flat(weights, "weights", position.shape, torch.float32)
-        o = c.out(out, "out", (tokens, y.shape[1]), y)
-        po, ldo = c.rows(o, "out")
-        lib.check(lib.tg_route_combine(tokens, k, y.shape[1], kind, py, y.shape[0], ldy, pp, pw,
-                                       po, ldo, c.handle))
+    what = "route_combine"
+    s = _stream_of(what, stream, y, position, weights, out)
+    kind = _type_of(what, y)
+    py, ldy = _rows_of(what, "y", y)
+    pp = _places(what, position)
+    tokens, k = position.shape
+    rows, cols = y.shape
+    pw = _flat(what, "weights", weights, position.shape, _pt.f32)
+    o, po, ldo = _out(what, "out", out, (tokens, cols), y, y.dtype)
+    lib.check(lib.tg_route_combine(tokens, k, cols, kind, py, rows, ldy, pp, pw, po, ldo, s))
+    _finish(stream)
     return o
 
 
+@_device_call
 def route_combine_backward(dout, y, position, weights=None, out=None, stream=None):
     """(dy, dweights) of route_combine (tg_route_combine_backward).  out takes
-    dy; rows that no position names are left as they are (zeros without out)."""
-    torch = _torch()
+    dy; its rows that no position names are left as they are (without out and
+    with fewer places than rows of y: zeros)."""
     what = "route_combine_backward"
-    with _Call(what, stream, y, dout, position, weights, out) as c:
-        kind = _type_of(y, what)
-        py, ldy = c.rows(y, "y")
-        pp = _places(c, position)
-        tokens, k = position.shape
-        cols = y.shape[1]
-        c.require(tuple(dout.shape) == (tokens, cols) and dout.dtype == y.dtype,
-                  f"dout must be {(tokens, cols)} {y.dtype}, got {tuple(dout.shape)} "
-                  f"{dout.dtype}.")
-        pd, lddo = c.rows(dout, "dout")
-        pw = c.flat(weights, "weights", position.shape, torch.float32)
-        if out is None and position.numel() != y.shape[0]:
-            out = torch.zeros(y.shape, dtype=y.dtype, device=y.device)
-        dy = c.out(out, "out", y.shape, y)
-        pdy, lddy = c.rows(dy, "out")
-        dw = torch.empty((tokens, k), dtype=torch.float32, device=y.device)
-        lib.check(lib.tg_route_combine_backward(tokens, k, cols, kind, pd, lddo, py, y.shape[0],
-                                                ldy, pp, pw, pdy, lddy, dw.data_ptr(), c.handle))
+    s = _stream_of(what, stream, dout, y, position, weights, out)
+    kind = _type_of(what, y)
+    py, ldy = _rows_of(what, "y", y)
+    pp = _places(what, position)
+    tokens, k = position.shape
+    rows, cols = y.shape
+    if dout.shape != (tokens, cols) or dout.dtype is not y.dtype:
+        _refuse(what, f"dout must be {(tokens, cols)} {y.dtype}, got {tuple(dout.shape)} "
+                      f"{dout.dtype}.")
+    pd, lddo = _rows_of(what, "dout", dout)
+    pw = _flat(what, "weights", weights, position.shape, _pt.f32)
+    dy, pdy, lddy = _out(what, "out", out, y.shape, y, y.dtype)
+    if out is None and tokens * k != rows:
+        dy.zero_()
+    dw = _pt.empty((tokens, k), dtype=_pt.f32, device=y.device)
+    lib.check(lib.tg_route_combine_backward(tokens, k, cols, kind, pd, lddo, py, rows, ldy, pp,
+                                            pw, pdy, lddy, dw.data_ptr(), s))
+    _finish(stream)
     return dy, dw
 
 
-def _offsets(c, offsets):
-    torch = _torch()
-    c.require(offsets.dim() == 1 and offsets.numel() >= 1, "offsets must be [groups + 1].")
-    return c.flat(offsets, "offsets", offsets.shape, torch.int32), offsets.numel() - 1
+def _offsets(what: str, offsets):
+    if offsets.dim() != 1 or offsets.numel() < 1:
+        _refuse(what, f"offsets must be [groups + 1], got {tuple(offsets.shape)}.")
+    return _flat(what, "offsets", offsets, offsets.shape, _pt.i32), offsets.numel() - 1
 
 
-def _row_index(c, rows, x):
+def _row_index(what: str, rows, x):
     """The rows' pointer and the number of rows of the product."""
     if rows is None:
-        return 0, x.shape[0]
-    c.require(rows.dim() == 1, "rows must be a vector.")
-    return c.flat(rows, "rows", rows.shape, _torch().int32), rows.numel()
+        return None, x.shape[0]
+    if rows.dim() != 1:
+        _refuse(what, f"rows must be a vector, got {tuple(rows.shape)}.")
+    return _flat(what, "rows", rows, rows.shape, _pt.i32), rows.numel()
 
 
+def _matrices(what: str, w):
+    """Leading dimension and stride of matrices [groups, rows, cols]."""
+    groups, rows, cols = w.shape
+    each, ld, step = w.stride()
+    if w.numel():
+        if step != 1 and cols > 1:
+            _refuse(what, f"w must have contiguous rows, got strides {w.stride()}.")
+        if rows > 1 and ld < cols:
+            _refuse(what, f"w has overlapping rows (strides {w.stride()}).")
+    return max(ld if rows > 1 else 0, cols, 1), each if groups > 1 else 0
+
+
+@_device_call
 def grouped_matmul(x, w, offsets, rows=None, bias=None, epilogue: int = EPI_NONE,
                    transpose: bool = False, out=None, stream=None):
     """y[p] = epilogue(x[p] @ w[g] + bias[g]) for the rows p of group g, those
@@ -691,51 +736,50 @@ def grouped_matmul(x, w, offsets, rows=None, bias=None, epilogue: int = EPI_NONE
     in the place of x[p].  w: [groups, k, n], or [groups, n, k] with transpose
     (the gradient of x: grouped_matmul(dy, w, offsets, transpose=True)).  Rows
     in no group are not written."""
-    with _Call("grouped_matmul", stream, x, w, offsets, rows, bias, out) as c:
-        kind = _type_of(x, "grouped_matmul")
-        px, ldx = c.rows(x, "x")
-        po, groups = _offsets(c, offsets)
-        pr, m = _row_index(c, rows, x)
-        c.require(w.dim() == 3 and w.dtype == x.dtype and w.shape[0] == groups,
-                  f"w must be [{groups}, k, n] {x.dtype}, got {tuple(w.shape)} {w.dtype}.")
-        k, n = (w.shape[2], w.shape[1]) if transpose else (w.shape[1], w.shape[2])
-        c.require(x.shape[1] == k, f"dimension mismatch: x has {x.shape[1]} columns, w {k}.")
-        c.require(w.numel() == 0 or w.shape[2] == 1 or w.stride(2) == 1,
-                  f"w must have contiguous rows, got strides {w.stride()}.")
-        ldw = max(w.stride(1) if w.shape[1] > 1 else 0, w.shape[2], 1)
-        c.require(w.numel() == 0 or w.shape[1] == 1 or w.stride(1) >= w.shape[2],
-                  f"w has overlapping rows (strides {w.stride()}).")
-        pb = c.flat(bias, "bias", (groups, n), x.dtype)
-        y = c.out(out, "out", (m, n), x)
-        py, ldy = c.rows(y, "out")
-        lib.check(lib.tg_grouped_matmul(m, k, n, groups, kind, px, x.shape[0], ldx, pr, po,
-                                        w.data_ptr(), ldw, w.stride(0) if groups > 1 else 0,
-                                        int(transpose), pb, epilogue, py, ldy, c.handle))
+    what = "grouped_matmul"
+    s = _stream_of(what, stream, x, w, offsets, rows, bias, out)
+    kind = _type_of(what, x)
+    px, ldx = _rows_of(what, "x", x)
+    po, groups = _offsets(what, offsets)
+    pr, m = _row_index(what, rows, x)
+    if w.dim() != 3 or w.dtype is not x.dtype or w.shape[0] != groups:
+        _refuse(what, f"w must be [{groups}, k, n] {x.dtype}, got {tuple(w.shape)} {w.dtype}.")
+    n, k = (w.shape[1], w.shape[2]) if transpose else (w.shape[2], w.shape[1])
+    if x.shape[1] != k:
+        _refuse(what, f"dimension mismatch: x has {x.shape[1]} columns, w {k}.")
+    ldw, each = _matrices(what, w)
+    pb = _flat(what, "bias", bias, (groups, n), x.dtype)
+    y, py, ldy = _out(what, "out", out, (m, n), x, x.dtype)
+    lib.check(lib.tg_grouped_matmul(m, k, n, groups, kind, px, x.shape[0], ldx, pr, po,
+                                    w.data_ptr(), ldw, each, 1 if transpose else 0, pb, epilogue,
+                                    py, ldy, s))
+    _finish(stream)
     return y
 
 
+@_device_call
 def grouped_matmul_wgrad(x, dy, offsets, rows=None, bias: bool = False, stream=None):
     """(dw, dbias) of grouped_matmul from x (and rows) and the gradient before
     its epilogue (tg_grouped_matmul_wgrad): dw [groups, k, n], dbias [groups,
     n] or None."""
-    torch = _torch()
     what = "grouped_matmul_wgrad"
-    with _Call(what, stream, x, dy, offsets, rows) as c:
-        kind = _type_of(x, what)
-        px, ldx = c.rows(x, "x")
-        po, groups = _offsets(c, offsets)
-        pr, m = _row_index(c, rows, x)
-        c.require(dy.dim() == 2 and dy.shape[0] == m and dy.dtype == x.dtype,
-                  f"dy must be [{m}, n] {x.dtype}, got {tuple(dy.shape)} {dy.dtype}.")
-        pd, lddy = c.rows(dy, "dy")
-        k, n = x.shape[1], dy.shape[1]
-        dw = torch.empty((groups, k, n), dtype=x.dtype, device=x.device)
-        db = torch.empty((groups, n), dtype=x.dtype, device=x.device) if bias else None
-        ws, size = c.workspace(lib.tg_grouped_matmul_wgrad_workspace_size(m, k, n, groups, kind),
-                               x.device)
-        lib.check(lib.tg_grouped_matmul_wgrad(
-            m, k, n, groups, kind, px, x.shape[0], ldx, pr, pd, lddy, po, dw.data_ptr(),
-            db.data_ptr() if bias else None, ws.data_ptr() if size else None, size, c.handle))
+    s = _stream_of(what, stream, x, dy, offsets, rows)
+    kind = _type_of(what, x)
+    px, ldx = _rows_of(what, "x", x)
+    po, groups = _offsets(what, offsets)
+    pr, m = _row_index(what, rows, x)
+    if dy.dim() != 2 or dy.shape[0] != m or dy.dtype is not x.dtype:
+        _refuse(what, f"dy must be [{m}, n] {x.dtype}, got {tuple(dy.shape)} {dy.dtype}.")
+    pd, lddy = _rows_of(what, "dy", dy)
+    k, n = x.shape[1], dy.shape[1]
+    dw = _pt.empty((groups, k, n), dtype=x.dtype, device=x.device)
+    db = _pt.empty((groups, n), dtype=x.dtype, device=x.device) if bias else None
+    size = lib.tg_grouped_matmul_wgrad_workspace_size(m, k, n, groups, kind)
+    ws, pws = _workspace(size, x)
+    lib.check(lib.tg_grouped_matmul_wgrad(m, k, n, groups, kind, px, x.shape[0], ldx, pr, pd,
+                                          lddy, po, dw.data_ptr(),
+                                          db.data_ptr() if bias else None, pws, size, s))
+    _finish(stream)
     return dw, db
 
 
@@ -763,76 +807,81 @@ def _blocks(n: int) -> int:
     return -(-n // 128)
 
 
+@_device_call
 def quantize(x, stream=None) -> BlockRows:
     """x [rows, cols] in e4m3 with a scale for each row and 128 columns."""
-    torch = _torch()
-    with _Call("quantize", stream, x) as c:
-        kind = _type_of(x, "quantize")
-        px, ldx = c.rows(x, "x")
-        rows, cols = x.shape
-        blocks = _blocks(cols)
-        q = torch.empty((rows, blocks * 128), dtype=torch.float8_e4m3fn, device=x.device)
-        scale = torch.empty((blocks, rows), dtype=torch.float32, device=x.device)
-        lib.check(lib.tg_quantize(rows, cols, kind, px, ldx, q.data_ptr(), scale.data_ptr(),
-                                  c.handle))
+    what = "quantize"
+    s = _stream_of(what, stream, x)
+    kind = _type_of(what, x)
+    px, ldx = _rows_of(what, "x", x)
+    rows, cols = x.shape
+    blocks = _blocks(cols)
+    q = _pt.empty((rows, blocks * 128), dtype=_pt.f8, device=x.device)
+    scale = _pt.empty((blocks, rows), dtype=_pt.f32, device=x.device)
+    lib.check(lib.tg_quantize(rows, cols, kind, px, ldx, q.data_ptr(), scale.data_ptr(), s))
+    _finish(stream)
     return BlockRows(q, scale, cols)
 
 
+@_device_call
 def quantize_weight(w, transpose: bool = False, stream=None) -> BlockWeight:
     """w [k, n] or [groups, k, n] (transpose: [.., n, k]) in e4m3 with a scale
     for each 128 x 128 block, laid out for matmul_fp8 once."""
-    torch = _torch()
-    with _Call("quantize_weight", stream, w) as c:
-        kind = _type_of(w, "quantize_weight")
-        c.require(w.dim() in (2, 3), f"w must be [k, n] or [groups, k, n], got {tuple(w.shape)}.")
-        many = w.dim() == 3
-        w3 = w if many else w[None]
-        groups = w3.shape[0]
-        k, n = (w3.shape[2], w3.shape[1]) if transpose else (w3.shape[1], w3.shape[2])
-        c.require(w.numel() == 0 or w3.shape[2] == 1 or w3.stride(2) == 1,
-                  f"w must have contiguous rows, got strides {w.stride()}.")
-        c.require(w.numel() == 0 or w3.shape[1] == 1 or w3.stride(1) >= w3.shape[2],
-                  f"w has overlapping rows (strides {w.stride()}).")
-        ldw = max(w3.stride(1) if w3.shape[1] > 1 else 0, w3.shape[2], 1)
-        q = torch.empty((groups, n, _blocks(k) * 128), dtype=torch.float8_e4m3fn, device=w.device)
-        scale = torch.empty((groups, _blocks(n), _blocks(k)), dtype=torch.float32,
-                            device=w.device)
-        lib.check(lib.tg_quantize_weight(groups, k, n, kind, w.data_ptr(), ldw,
-                                         w3.stride(0) if groups > 1 else 0, int(transpose),
-                                         q.data_ptr(), scale.data_ptr(), c.handle))
+    what = "quantize_weight"
+    s = _stream_of(what, stream, w)
+    kind = _type_of(what, w)
+    if w.dim() not in (2, 3):
+        _refuse(what, f"w must be [k, n] or [groups, k, n], got {tuple(w.shape)}.")
+    many = w.dim() == 3
+    w3 = w if many else w[None]
+    groups = w3.shape[0]
+    n, k = (w3.shape[1], w3.shape[2]) if transpose else (w3.shape[2], w3.shape[1])
+    ldw, each = _matrices(what, w3)
+    q = _pt.empty((groups, n, _blocks(k) * 128), dtype=_pt.f8, device=w.device)
+    scale = _pt.empty((groups, _blocks(n), _blocks(k)), dtype=_pt.f32, device=w.device)
+    lib.check(lib.tg_quantize_weight(groups, k, n, kind, w.data_ptr(), ldw, each,
+                                     1 if transpose else 0, q.data_ptr(), scale.data_ptr(), s))
+    _finish(stream)
     return BlockWeight(q if many else q[0], scale if many else scale[0], k)
 
 
+@_device_call
 def matmul_fp8(x: BlockRows, w: BlockWeight, offsets=None, rows=None, bias=None,
                epilogue: int = EPI_NONE, dtype=None, out=None, stream=None):
     """The product of quantised rows and weights (tg_matmul_fp8), rounded once
     to `dtype` (float32 if None, or out's).  With offsets, w and bias [groups,
     n] are one for each group, as in grouped_matmul (rows too)."""
-    torch = _torch()
     what = "matmul_fp8"
-    f8 = torch.float8_e4m3fn
-    with _Call(what, stream, x.q, x.scale, w.q, w.scale, offsets, rows, bias, out) as c:
-        kb = _blocks(x.cols)
-        c.require(x.cols == w.k, f"dimension mismatch: x has {x.cols} columns, w {w.k}.")
-        pq = c.flat(x.q, "x.q", (x.q.shape[0], kb * 128), f8)
-        ps = c.flat(x.scale, "x.scale", (kb, x.q.shape[0]), torch.float32)
-        c.require(w.q.dim() == (2 if offsets is None else 3),
-                  f"w.q must be {'[n, k]' if offsets is None else '[groups, n, k]'}, got "
-                  f"{tuple(w.q.shape)}.")
-        n = w.q.shape[-2]
-        po, groups = (0, 1) if offsets is None else _offsets(c, offsets)
-        lead = () if offsets is None else (groups,)
-        pw = c.flat(w.q, "w.q", (*lead, n, kb * 128), f8)
-        pws = c.flat(w.scale, "w.scale", (*lead, _blocks(n), kb), torch.float32)
-        pr, m = _row_index(c, rows, x.q)
-        kind = dtype or (out.dtype if out is not None else torch.float32)
-        like = torch.empty(0, dtype=kind, device=x.q.device)
-        code = _type_of(like, what)
-        pb = c.flat(bias, "bias", (*lead, n), kind)
-        y = c.out(out, "out", (m, n), like)
-        py, ldy = c.rows(y, "out")
-        lib.check(lib.tg_matmul_fp8(m, x.cols, n, groups, pq, ps, x.q.shape[0], pr, po, pw, pws,
-                                    code, pb, epilogue, py, ldy, c.handle))
+    q, wq = x.q, w.q
+    s = _stream_of(what, stream, q, x.scale, wq, w.scale, offsets, rows, bias, out)
+    cols = x.cols
+    kb = _blocks(cols)
+    if cols != w.k:
+        _refuse(what, f"dimension mismatch: x has {cols} columns, w {w.k}.")
+    x_rows = q.shape[0]
+    pq = _flat(what, "x.q", q, (x_rows, kb * 128), _pt.f8)
+    ps = _flat(what, "x.scale", x.scale, (kb, x_rows), _pt.f32)
+    if wq.dim() != (2 if offsets is None else 3):
+        _refuse(what, f"w.q must be {'[n, k]' if offsets is None else '[groups, n, k]'}, got "
+                      f"{tuple(wq.shape)}.")
+    n = wq.shape[-2]
+    if offsets is None:
+        po, groups, lead = None, 1, ()
+    else:
+        po, groups = _offsets(what, offsets)
+        lead = (groups,)
+    pw = _flat(what, "w.q", wq, (*lead, n, kb * 128), _pt.f8)
+    pws = _flat(what, "w.scale", w.scale, (*lead, _blocks(n), kb), _pt.f32)
+    pr, m = _row_index(what, rows, q)
+    kind = dtype or (out.dtype if out is not None else _pt.f32)
+    code = _pt.types.get(kind)
+    if code is None:
+        _refuse(what, f"float32, bfloat16 or float16 results expected, got {kind}.")
+    pb = _flat(what, "bias", bias, (*lead, n), kind)
+    y, py, ldy = _out(what, "out", out, (m, n), q, kind)
+    lib.check(lib.tg_matmul_fp8(m, cols, n, groups, pq, ps, x_rows, pr, po, pw, pws, code, pb,
+                                epilogue, py, ldy, s))
+    _finish(stream)
     return y
 
 

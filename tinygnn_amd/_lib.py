@@ -182,7 +182,8 @@ class _Lib:
 
     def __getattr__(self, name):
         if name.startswith("tg_"):
-            return getattr(self.load(), name)
+            fn = self.__dict__[name] = getattr(self.load(), name)
+            return fn
         raise AttributeError(name)
 
     def check(self, status: int) -> None:
