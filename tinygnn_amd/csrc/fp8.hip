@@ -201,7 +201,7 @@ __global__ __launch_bounds__(S::kThreads) void fp8_kernel(Fp8Args a) {
     __shared__ __attribute__((aligned(16))) char b1[S::kN * kRowBytes];
     constexpr bool WIDE = sizeof(T) == 4;
     uint32_t mt, ntile;
-    tile_of(blockIdx.x, gridDim.x, a.nt, a.mt, &mt, &ntile);
+    if (!tile_of(blockIdx.x, count_tiles(a.offsets, a.groups, a.m, S::kM), a.nt, &mt, &ntile)) return;
     int g, r0, r1;
     if (!find_tile(a.offsets, a.groups, a.m, S::kM, static_cast<int>(mt), &g, &r0, &r1)) return;
     const int n0 = static_cast<int>(ntile) * S::kN;
@@ -317,7 +317,7 @@ __global__ __launch_bounds__(64 * kThinWaves) void fp8_thin_kernel(Fp8Args a) {
     __shared__ v4f join[kThinWaves - 1][64];
     constexpr bool WIDE = sizeof(T) == 4;
     uint32_t mt, ntile;
-    tile_of(blockIdx.x, gridDim.x, a.nt, a.mt, &mt, &ntile);
+    if (!tile_of(blockIdx.x, count_tiles(a.offsets, a.groups, a.m, 16), a.nt, &mt, &ntile)) return;
     int g, r0, r1;
     if (!find_tile(a.offsets, a.groups, a.m, 16, static_cast<int>(mt), &g, &r0, &r1)) return;
     const int n0 = static_cast<int>(ntile) * 16;

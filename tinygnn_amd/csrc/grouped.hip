@@ -42,6 +42,80 @@ __device__ __forceinline__ int64_t source_row(const GroupedArgs& a, int p) {
     return r < 0 || r >= a.x_rows ? -1 : r;
 }
 
+// A wavefront's outputs from row p0, column n0 of group g: bias, epilogue and
+// stores.  Lane (q, r) holds row r of a tile, columns 4 q .. 4 q + 3.
+template <typename T, int MI, int NJ>
+__device__ __forceinline__ void store_outputs(const GroupedArgs& a, int g, int p0, int r1, int n0,
+                                              int lane, const v4f (&acc)[MI][NJ]) {
+    const int q = lane >> 4, r = lane & 15;
+    float bias[NJ][4];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        const int n = n0 + j * 16 + 4 * q;
+        if (a.bias)
+            load_floats<T, 4>(static_cast<const T*>(a.bias) + static_cast<int64_t>(g) * a.n + n,
+                              a.n - n, bias[j]);
+        else
+            bias[j][0] = bias[j][1] = bias[j][2] = bias[j][3] = 0.0f;
+    }
+    with_epilogue(a.epi, [&](auto epi) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const int p = p0 + i * 16 + r;
+            if (p >= r1) continue;
+            T* y = static_cast<T*>(a.y) + p * a.ldy;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int n = n0 + j * 16 + 4 * q;
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    v[e] = grouped_epilogue<decltype(epi)::value>(acc[i][j][e], bias[j][e]);
+                store_floats<T, 4>(y + n, a.n - n, v);
+            }
+        }
+    });
+}
+
+// A wavefront's sums of dw from row k0, column n0 on: of group (or part) `part`.
+template <typename T, int MI, int NJ>
+__device__ __forceinline__ void store_gradient(const GroupedArgs& a, int part, int k0, int n0,
+                                               int lane, const v4f (&acc)[MI][NJ]) {
+    const int q = lane >> 4, r = lane & 15;
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+        const int k = k0 + i * 16 + r;
+        if (k >= a.k) continue;
+        const int64_t row = (static_cast<int64_t>(part) * a.k + k) * a.n;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int n = n0 + j * 16 + 4 * q;
+            const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+            if (a.unit)
+                store_floats<float, 4>(a.part + row + n, a.n - n, v);
+            else
+                store_floats<T, 4>(static_cast<T*>(a.dw) + row + n, a.n - n, v);
+        }
+    }
+}
+
+template <typename T, int NJ>
+__device__ __forceinline__ void store_bias_gradient(const GroupedArgs& a, int part, int n0,
+                                                    int lane, const v4f (&sum)[NJ]) {
+    const int q = lane >> 4, r = lane & 15;
+    if (r != 0) return;
+    const int64_t row = static_cast<int64_t>(part) * a.n;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        const int n = n0 + j * 16 + 4 * q;
+        const float v[4] = {sum[j][0], sum[j][1], sum[j][2], sum[j][3]};
+        if (a.unit)
+            store_floats<float, 4>(a.part_bias + row + n, a.n - n, v);
+        else
+            store_floats<T, 4>(static_cast<T*>(a.dbias) + row + n, a.n - n, v);
+    }
+}
+
 // ---------------------------------------------------------------------------
 // BM x BN outputs by WR x WC wavefronts, two tiles of both operands in LDS: while the matrix instructions read one, the other is loaded.
 // The wavefront's outputs are computed transposed (columns of w as the rows of
@@ -76,7 +150,7 @@ __global__ __launch_bounds__(S::kThreads) void grouped_kernel(GroupedArgs a) {
     __shared__ __attribute__((aligned(16))) char b1[S::kN * kRowBytes];
     constexpr int Z = sizeof(T);
     uint32_t mt, ntile;
-    tile_of(blockIdx.x, gridDim.x, a.nt, a.mt, &mt, &ntile);
+    if (!tile_of(blockIdx.x, count_tiles(a.offsets, a.groups, a.m, S::kM), a.nt, &mt, &ntile)) return;
     int g, r0, r1;
     if (!find_tile(a.offsets, a.groups, a.m, S::kM, static_cast<int>(mt), &g, &r0, &r1)) return;
     const int n0 = static_cast<int>(ntile) * S::kN;
@@ -171,35 +245,63 @@ __global__ __launch_bounds__(S::kThreads) void grouped_kernel(GroupedArgs a) {
         pipeline<false>(tiles, a0, b0, a1, b1, load, store, compute);
     }
 
-    // lane (q, r): row r of a tile, columns 4 q .. 4 q + 3
-    const int q = lane >> 4, r = lane & 15;
-    float bias[S::kNJ][4];
+    store_outputs<T>(a, g, r0 + wm, r1, n0 + wn, lane, acc);
+}
+
+// The large tile (tiles.hpp): 16-bit operands that can be loaded directly.
+template <typename T, bool ALONG_W>
+__global__ __launch_bounds__(kRingThreads) void grouped_ring_kernel(GroupedArgs a) {
+    TG_RING_LDS;
+    uint32_t mt, ntile;
+    if (!tile_of(blockIdx.x, count_tiles(a.offsets, a.groups, a.m, 256), a.nt, &mt, &ntile)) return;
+    int g, r0, r1;
+    if (!find_tile(a.offsets, a.groups, a.m, 256, static_cast<int>(mt), &g, &r0, &r1)) return;
+    const int n0 = static_cast<int>(ntile) * 256;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / 4 * 128, wn = wave % 4 * 64;
+    const T* w = static_cast<const T*>(a.w) + g * a.w_stride;
+    const T* xb = static_cast<const T*>(a.x) + (a.rows ? 0 : static_cast<int64_t>(r0) * a.ldx);
+    const T* wb = ALONG_W ? w + n0 * a.ldw : w + n0;
+    uint32_t ao[2], bo[2];
+    int ac[2], bk[2];  // the chunks' places along the contraction
 #pragma unroll
-    for (int j = 0; j < S::kNJ; ++j) {
-        const int n = n0 + wn + j * 16 + 4 * q;
-        if (a.bias)
-            load_floats<T, 4>(static_cast<const T*>(a.bias) + static_cast<int64_t>(g) * a.n + n,
-                              a.n - n, bias[j]);
+    for (int t = 0; t < 2; ++t) {
+        int row, col, kk;
+        part_place<false>(t * kRingThreads + tid, &row, &ac[t]);
+        const int64_t src = r0 + row < r1 ? source_row(a, r0 + row) : -1;
+        ao[t] = src < 0 ? kOutside
+                        : static_cast<uint32_t>(2 * ((a.rows ? src : row) * a.ldx + ac[t]));
+        if (ALONG_W)
+            part_place<false>(t * kRingThreads + tid, &col, &kk);
         else
-            bias[j][0] = bias[j][1] = bias[j][2] = bias[j][3] = 0.0f;
+            part_place<true>(t * kRingThreads + tid, &kk, &col);
+        bk[t] = kk;
+        bo[t] = n0 + col < a.n
+                    ? static_cast<uint32_t>(2 * (ALONG_W ? col * a.ldw + kk : kk * a.ldw + col))
+                    : kOutside;
     }
-    with_epilogue(a.epi, [&](auto epi) {
+    auto load = [&](int u, char* la, char* lb) {
+        const int k0 = u * kStep;
+        const int64_t size = k0 < a.k ? kDirectBytes : 0;
+        const auto xbuf = buffer_of(xb + k0, size);
+        const auto wbuf = buffer_of(ALONG_W ? wb + k0 : wb + k0 * a.ldw, size);
+        const bool part = k0 + kStep > a.k;  // what lies behind k is 0
 #pragma unroll
-        for (int i = 0; i < S::kMI; ++i) {
-            const int p = r0 + wm + i * 16 + r;
-            if (p >= r1) continue;
-            T* y = static_cast<T*>(a.y) + p * a.ldy;
+        for (int t = 0; t < 2; ++t)
+            load_to_lds(xbuf, la + (t * kRingThreads + wave * 64) * 16,
+                        part && k0 + ac[t] >= a.k ? kOutside : ao[t]);
 #pragma unroll
-            for (int j = 0; j < S::kNJ; ++j) {
-                const int n = n0 + wn + j * 16 + 4 * q;
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    v[e] = grouped_epilogue<decltype(epi)::value>(acc[i][j][e], bias[j][e]);
-                store_floats<T, 4>(y + n, a.n - n, v);
-            }
-        }
-    });
+        for (int t = 0; t < 2; ++t)
+            load_to_lds(wbuf, lb + (t * kRingThreads + wave * 64) * 16,
+                        part && k0 + bk[t] >= a.k ? kOutside : bo[t]);
+    };
+    v4f acc[8][4] = {};
+    const PartReader<false, 8> ra(wm, lane);
+    const PartReader<!ALONG_W, 4> rb(wn, lane);
+    ring<T>((a.k + kStep - 1) / kStep, ra, rb, load, [](Frag(&)[4]) {}, a0, b0, a1,
+            b1, a2, b2, a3, b3, acc);
+    store_outputs<T>(a, g, r0 + wm, r1, n0 + wn, lane, acc);
 }
 
 // dw_g = x_g^T dy_g and, from the workgroups of dw's first row tile, dbias: dy's
@@ -217,7 +319,7 @@ __global__ __launch_bounds__(S::kThreads) void wgrad_kernel(GroupedArgs a) {
     const uint32_t per = a.mt * a.nt;
     const int part = static_cast<int>(blockIdx.x / per);
     uint32_t mt, ntile;
-    tile_of(blockIdx.x % per, per, a.nt, a.mt, &mt, &ntile);
+    tile_of(blockIdx.x % per, a.mt, a.nt, &mt, &ntile);
     int g = part, lo, hi;
     if (a.unit == 0)
         group_rows(a.offsets, g, a.m, &lo, &hi);
@@ -327,35 +429,91 @@ __global__ __launch_bounds__(S::kThreads) void wgrad_kernel(GroupedArgs a) {
         pipeline<false>(tiles, a0, b0, a1, b1, load, store, compute);
     }
 
-    const int q = lane >> 4, r = lane & 15;
-    if (a.dw) {
+    if (a.dw) store_gradient<T>(a, part, k0 + wm, n0 + wn, lane, acc);
+    if (BIAS && sums) store_bias_gradient<T>(a, part, n0 + wn, lane, sum);
+}
+
+// dw on the large tile: both operands run across memory, the contraction over
+// the group's rows.
+template <typename T, bool BIAS>
+__global__ __launch_bounds__(kRingThreads) void wgrad_ring_kernel(GroupedArgs a) {
+    TG_RING_LDS;
+    const uint32_t per = a.mt * a.nt;
+    const int part = static_cast<int>(blockIdx.x / per);
+    uint32_t mt, ntile;
+    tile_of(blockIdx.x % per, a.mt, a.nt, &mt, &ntile);
+    int g = part, lo, hi;
+    if (a.unit == 0)
+        group_rows(a.offsets, g, a.m, &lo, &hi);
+    else if (!find_tile(a.offsets, a.groups, a.m, a.unit, part, &g, &lo, &hi))
+        return;
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    const int k0 = static_cast<int>(mt) * 256, n0 = static_cast<int>(ntile) * 256;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / 4 * 128, wn = wave % 4 * 64;
+    const T* x = static_cast<const T*>(a.x);
+    const T* dy = static_cast<const T*>(a.dy);
+    // a wavefront's load takes two rows, 32 chunks of each
+    uint32_t ao[2], bo[2], ax[2];
 #pragma unroll
-        for (int i = 0; i < S::kMI; ++i) {
-            const int k = k0 + wm + i * 16 + r;
-            if (k >= a.k) continue;
-            const int64_t row = (static_cast<int64_t>(part) * a.k + k) * a.n;
-#pragma unroll
-            for (int j = 0; j < S::kNJ; ++j) {
-                const int n = n0 + wn + j * 16 + 4 * q;
-                const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-                if (a.unit)
-                    store_floats<float, 4>(a.part + row + n, a.n - n, v);
-                else
-                    store_floats<T, 4>(static_cast<T*>(a.dw) + row + n, a.n - n, v);
-            }
-        }
+    for (int t = 0; t < 2; ++t) {
+        int p, c;
+        part_place<true>(t * kRingThreads + tid, &p, &c);
+        ax[t] = k0 + c < a.k ? static_cast<uint32_t>(2 * (k0 + c)) : kOutside;
+        ao[t] = k0 + c < a.k ? static_cast<uint32_t>(2 * (p * a.ldx + k0 + c)) : kOutside;
+        bo[t] = n0 + c < a.n ? static_cast<uint32_t>(2 * (p * a.lddy + n0 + c)) : kOutside;
     }
-    if (BIAS && sums && r == 0) {
-        const int64_t row = static_cast<int64_t>(part) * a.n;
+    auto load = [&](int u, char* la, char* lb) {
+        const int p0 = lo + u * kStep;
+        const int64_t left = hi - p0;  // rows: the buffers end with them
+        const auto dbuf = buffer_of(dy + p0 * a.lddy, left > 0 ? 2 * ((left - 1) * a.lddy + a.n)
+                                                               : 0);
+        if (a.rows) {
+            const auto xbuf = buffer_of(x, kDirectBytes);
 #pragma unroll
-        for (int j = 0; j < S::kNJ; ++j) {
-            const int n = n0 + wn + j * 16 + 4 * q;
-            const float v[4] = {sum[j][0], sum[j][1], sum[j][2], sum[j][3]};
-            if (a.unit)
-                store_floats<float, 4>(a.part_bias + row + n, a.n - n, v);
-            else
-                store_floats<T, 4>(static_cast<T*>(a.dbias) + row + n, a.n - n, v);
+            for (int t = 0; t < 2; ++t) {
+                uint32_t at[2];  // the two rows' starts
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int p = p0 + t * 16 + wave * 2 + h;
+                    const int r = p < hi ? scalar_load(a.rows + p) : -1;
+                    at[h] = r >= 0 && r < a.x_rows ? static_cast<uint32_t>(2 * r * a.ldx)
+                                                   : kOutside;
+                }
+                const uint32_t row = lane < 32 ? at[0] : at[1];
+                load_to_lds(xbuf, la + (t * kRingThreads + wave * 64) * 16,
+                            (row | ax[t]) >= kOutside ? kOutside : row + ax[t]);
+            }
+        } else {
+            const auto xbuf = buffer_of(x + p0 * a.ldx, left > 0 ? 2 * ((left - 1) * a.ldx + a.k)
+                                                                 : 0);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                load_to_lds(xbuf, la + (t * kRingThreads + wave * 64) * 16, ao[t]);
         }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+            load_to_lds(dbuf, lb + (t * kRingThreads + wave * 64) * 16, bo[t]);
+    };
+    v4f acc[8][4] = {};
+    v4f sum[BIAS ? 4 : 1] = {};
+    const bool sums = BIAS && mt == 0 && wm == 0;  // uniform
+    const Frag one = ones<T>();
+    const PartReader<true, 8> ra(wm, lane);
+    const PartReader<true, 4> rb(wn, lane);
+    ring<T>((hi - lo + kStep - 1) / kStep, ra, rb, load,
+            [&](Frag(&w)[4]) {
+                if (BIAS && sums) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) sum[BIAS ? j : 0] = mfma<T>(w[j], one, sum[BIAS ? j : 0]);
+                }
+            },
+            a0, b0, a1, b1, a2, b2, a3, b3, acc);
+    if (a.dw) store_gradient<T>(a, part, k0 + wm, n0 + wn, lane, acc);
+    if constexpr (BIAS) {
+        if (sums) store_bias_gradient<T>(a, part, n0 + wn, lane, sum);
     }
 }
 
@@ -413,7 +571,6 @@ bool direct_operand(const void* p, int64_t ld, int64_t cols, int64_t stride, int
            stride % epc == 0 && (major * ld + cols) * z < kDirectBytes;
 }
 
-using Large = Shape<256, 256, 2, 4>;
 using Medium = Shape<128, 128, 2, 2>;
 using Small = Shape<32, 128, 1, 4>;
 
@@ -436,10 +593,21 @@ void launch_grouped(GroupedArgs& a, bool along, bool direct, hipStream_t s) {
     TG_LAUNCH_CHECK();
 }
 
-// How a gradient of w is cut.  Whole groups where their tiles are two for each
-// of the 256 CUs; else parts of `unit` rows for about four, 256 rows at least.
+template <typename T>
+void launch_ring(GroupedArgs& a, bool along, hipStream_t s) {
+    a.mt = static_cast<uint32_t>(most_tiles(a.m, a.groups, 256));
+    a.nt = static_cast<uint32_t>(ceil_div(a.n, 256));
+    const unsigned grid = grid_of("grouped_matmul", static_cast<int64_t>(a.mt) * a.nt);
+    along ? grouped_ring_kernel<T, true><<<grid, kRingThreads, 0, s>>>(a)
+          : grouped_ring_kernel<T, false><<<grid, kRingThreads, 0, s>>>(a);
+    TG_LAUNCH_CHECK();
+}
+
+// How a gradient of w is cut: `edge` x `edge` tiles of whole groups where they
+// are two for each of the 256 CUs; else of parts of `unit` rows for about four,
+// 256 rows at least.
 struct WgradPlan {
-    int64_t mt, nt, unit, parts;  // parts: most of them
+    int64_t edge, mt, nt, unit, parts;  // parts: most of them
     size_t bytes(int64_t k, int64_t n, float** part, float** part_bias, void* ws, size_t size) const {
         Carver c(ws, size);
         if (unit == 0) return 0;
@@ -451,12 +619,11 @@ struct WgradPlan {
     }
 };
 
-using WgradShape = Medium;
-
-WgradPlan wgrad_plan(int64_t m, int64_t k, int64_t n, int64_t groups) {
+WgradPlan wgrad_plan(int64_t m, int64_t k, int64_t n, int64_t groups, int type, bool direct) {
     WgradPlan p{};
-    p.mt = std::max<int64_t>(1, ceil_div(k, WgradShape::kM));
-    p.nt = ceil_div(n, WgradShape::kN);
+    p.edge = type != TG_TYPE_F32 && direct && getenv("TGM") ? 256 : 128;
+    p.mt = std::max<int64_t>(1, ceil_div(k, p.edge));
+    p.nt = ceil_div(n, p.edge);
     p.parts = groups;
     const int64_t tiles = p.mt * p.nt;
     if (tiles * groups >= 512) return p;
@@ -469,12 +636,16 @@ WgradPlan wgrad_plan(int64_t m, int64_t k, int64_t n, int64_t groups) {
 
 template <typename T>
 void launch_wgrad(GroupedArgs& a, const WgradPlan& p, bool direct, hipStream_t s) {
-    using S = WgradShape;
+    using S = Medium;
     a.mt = static_cast<uint32_t>(p.mt);
     a.nt = static_cast<uint32_t>(p.nt);
     a.unit = static_cast<int>(p.unit);
     const unsigned grid = grid_of("grouped_matmul_wgrad", p.mt * p.nt * p.parts);
-    if (a.dbias)
+    if (p.edge == 256) {
+        if constexpr (sizeof(T) == 2)
+            a.dbias ? wgrad_ring_kernel<T, true><<<grid, kRingThreads, 0, s>>>(a)
+                    : wgrad_ring_kernel<T, false><<<grid, kRingThreads, 0, s>>>(a);
+    } else if (a.dbias)
         direct ? wgrad_kernel<T, S, true, true><<<grid, S::kThreads, 0, s>>>(a)
                : wgrad_kernel<T, S, false, true><<<grid, S::kThreads, 0, s>>>(a);
     else
@@ -547,15 +718,20 @@ int tg_grouped_matmul(int64_t m, int64_t k, int64_t n, int64_t groups, int type,
             else if (type == TG_TYPE_F32 || !direct)
                 tg::launch_grouped<T, tg::Medium>(a, along, direct, s);
             else if constexpr (sizeof(T) == 2)
-                tg::launch_grouped<T, tg::Large>(a, along, direct, s);
+                tg::launch_ring<T>(a, along, s);
         });
     });
 }
 
 size_t tg_grouped_matmul_wgrad_workspace_size(int64_t m, int64_t k, int64_t n, int64_t groups,
-                                              int) {
+                                              int type) {
     if (m <= 0 || k < 0 || n <= 0 || groups <= 0 || groups > tg::kMaxGroups) return 0;
-    return tg::wgrad_plan(m, k, n, groups).bytes(k, n, nullptr, nullptr, nullptr, 0);
+    // either tile: which one depends on the operands' alignment
+    size_t most = 0;
+    for (const bool direct : {false, true})
+        most = std::max(most, tg::wgrad_plan(m, k, n, groups, type, direct)
+                                  .bytes(k, n, nullptr, nullptr, nullptr, 0));
+    return most;
 }
 
 int tg_grouped_matmul_wgrad(int64_t m, int64_t k, int64_t n, int64_t groups, int type,
@@ -589,7 +765,7 @@ int tg_grouped_matmul_wgrad(int64_t m, int64_t k, int64_t n, int64_t groups, int
         const bool direct = tg::direct_operand(x, ldx, a.k, 0, z, rows ? x_rows : 64) &&
                             tg::direct_operand(dy, lddy, n, 0, z, 64);
         hipStream_t s = static_cast<hipStream_t>(stream);
-        const tg::WgradPlan plan = tg::wgrad_plan(m, a.k, n, groups);
+        const tg::WgradPlan plan = tg::wgrad_plan(m, a.k, n, groups, type, direct);
         tg::TempBuffer temp;
         if (plan.unit) {
             const size_t need = plan.bytes(a.k, n, nullptr, nullptr, nullptr, 0);

@@ -55,6 +55,22 @@ __device__ __forceinline__ bool find_tile(const int32_t* __restrict__ offsets, i
     return false;
 }
 
+// Row tiles of `unit` rows of all groups.  (Their number decides which tiles an
+// XCD takes: with the most that there can be instead, the last XCDs had only
+// tiles that do not exist, and 256 tiles took two rounds of the 256 CUs.)
+__device__ __forceinline__ int count_tiles(const int32_t* __restrict__ offsets, int groups, int m,
+                                           int unit) {
+    if (offsets == nullptr) return static_cast<int>((static_cast<int64_t>(m) + unit - 1) / unit);
+    const int lane = threadIdx.x & (kWave - 1);
+    int n = 0;
+    for (int base = 0; base < groups; base += kWave) {
+        int lo = 0, hi = 0;
+        if (base + lane < groups) group_rows(offsets, base + lane, m, &lo, &hi);
+        n += static_cast<int>((static_cast<int64_t>(hi) - lo + unit - 1) / unit);
+    }
+    return __builtin_amdgcn_readfirstlane(wave_sum(n));
+}
+
 // Most tiles of `unit` rows that m rows in `groups` groups can make.
 inline int64_t most_tiles(int64_t m, int64_t groups, int64_t unit) {
     return m / unit + std::min(groups, m);

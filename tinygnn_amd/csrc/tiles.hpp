@@ -183,20 +183,21 @@ __device__ __forceinline__ v4u load_chunk(const T* p, int64_t left) {
     return v;
 }
 
-// The tile that workgroup `b` of `grid` takes of `mt` x `nt`: each XCD (every
-// eighth workgroup) has a run of consecutive tiles, taken `kBand` row tiles by
-// all columns at a time, so that the tiles in flight on an XCD share their rows
-// and columns in its L2.
+// Tile b of mt x nt, taken `kBand` row tiles by all columns at a time on each
+// of 8 XCDs (every eighth workgroup), whose runs of consecutive tiles share
+// their rows and columns in its L2; false where there are fewer.
 constexpr int kBand = 4;
-__device__ __forceinline__ void tile_of(uint32_t b, uint32_t grid, uint32_t nt, uint32_t mt,
-                                        uint32_t* i, uint32_t* j) {
-    const uint32_t per = grid / 8, rest = grid % 8, x = b % 8;
+__device__ __forceinline__ bool tile_of(uint32_t b, uint32_t mt, uint32_t nt, uint32_t* i,
+                                        uint32_t* j) {
+    const uint32_t all = mt * nt, per = all / 8, rest = all % 8, x = b % 8;
+    if (b / 8 >= per + (x < rest ? 1 : 0)) return false;
     uint32_t t = x * per + (x < rest ? x : rest) + b / 8;
     const uint32_t band = t / (kBand * nt), first = band * kBand;
     const uint32_t high = mt - first < kBand ? mt - first : kBand;
     t -= band * kBand * nt;
     *i = first + t % high;
     *j = t / high;
+    return true;
 }
 
 // BM x BN outputs by WR x WC wavefronts.
@@ -236,5 +237,138 @@ __device__ __forceinline__ void pipeline(int tiles, char* a0, char* b0, char* a1
         compute(a0, b0);
     }
 }
+
+// ---------------------------------------------------------------------------
+// The large tile: 256 x 256 outputs of a 16-bit type by eight wavefronts of 128
+// x 64, two on each SIMD.  The operands lie in a ring of four parts of 32
+// contraction values (64 bytes a row along, 32 rows across).  While a
+// wavefront's 32 matrix instructions of one part run (512 cycles), it reads its
+// operands of the next one from LDS to other registers and asks for the part
+// that takes the place of this one, three steps before it is read; one barrier a
+// step.
+// ---------------------------------------------------------------------------
+constexpr int kStep = 32;                // contraction values of a part
+constexpr int kPartBytes = 256 * 64;     // of one operand
+constexpr int kRingThreads = 512;
+
+template <bool ACROSS>
+__device__ __forceinline__ void part_place(int e, int* major, int* minor) {
+    if constexpr (ACROSS) {
+        chunk_place<bf16, 256, true>(e, major, minor);
+    } else {
+        *major = e >> 2;
+        *minor = ((e & 3) ^ ((*major >> 1) & 3)) * 8;
+    }
+}
+
+template <bool ACROSS, int N>
+struct PartReader {
+    int at[ACROSS ? N : 1];
+    __device__ __forceinline__ PartReader(int first, int lane) {
+        const int q = lane >> 4, r = lane & 15;
+        if constexpr (ACROSS) {
+            const Reader<bf16, 256, true, N> all(first, lane);
+#pragma unroll
+            for (int i = 0; i < N; ++i) at[i] = all.at[i];
+        } else {
+            at[0] = (first + r) * 64 + ((q ^ ((r >> 1) & 3)) << 4);
+        }
+    }
+    __device__ __forceinline__ Frag read(const char* lds, int i) const {
+        Frag f;
+        if constexpr (ACROSS) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                f.s[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (TG_LDS v4s*)(lds + at[i] + 4 * h * 512));
+        } else {
+            f.u = *reinterpret_cast<const v4u*>(lds + at[0] + i * 1024);
+        }
+        return f;
+    }
+};
+
+// A step's border: what this wavefront asked of LDS is there, and all but
+// LOADS of its loads; then the same of every wavefront.
+template <int LOADS>
+__device__ __forceinline__ void step_border() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// acc += the products of `steps` parts; load(u, la, lb) asks for part u (four
+// loads a thread; zeros from `steps` on); also(w) sees the columns' operands.
+template <typename T, typename RA, typename RB, typename L, typename W>
+__device__ __forceinline__ void ring(int steps, const RA& ra, const RB& rb, L&& load, W&& also,
+                                     char* a0, char* b0, char* a1, char* b1, char* a2, char* b2,
+                                     char* a3, char* b3, v4f (&acc)[8][4]) {
+    constexpr int kLoads = 4;
+    if (steps == 0) return;
+    struct Operands {
+        Frag x[8], w[4];
+    };
+    auto read = [&](Operands& o, const char* la, const char* lb) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o.w[j] = rb.read(lb, j);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o.x[i] = ra.read(la, i);
+    };
+    // part u in `now`; part u + 1, in na and nb, to `next`; part u + 4 to u's place
+    auto step = [&](int u, Operands& now, Operands& next, char* la, char* lb, const char* na,
+                    const char* nb) {
+        step_border<2 * kLoads>();
+        load(u + 4, la, lb);
+        read(next, na, nb);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = mfma<T>(now.w[j], now.x[i], acc[i][j]);
+        also(now.w);
+        // an LDS read beside each of the first matrix instructions: the reads
+        // have the rest of the step to arrive (left to itself, the compiler
+        // puts them last, where the border waits for them)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 16, 0);
+    };
+    load(0, a0, b0);
+    load(1, a1, b1);
+    load(2, a2, b2);
+    load(3, a3, b3);
+    step_border<3 * kLoads>();
+    Operands even, odd;
+    read(even, a0, b0);
+    int u = 0;
+    for (; u + 4 <= steps; u += 4) {
+        step(u, even, odd, a0, b0, a1, b1);
+        step(u + 1, odd, even, a1, b1, a2, b2);
+        step(u + 2, even, odd, a2, b2, a3, b3);
+        step(u + 3, odd, even, a3, b3, a0, b0);
+    }
+    if (u < steps) {
+        step(u, even, odd, a0, b0, a1, b1);
+        if (u + 1 < steps) {
+            step(u + 1, odd, even, a1, b1, a2, b2);
+            if (u + 2 < steps) step(u + 2, even, odd, a2, b2, a3, b3);
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+}
+
+#define TG_RING_LDS                                                       \
+    __shared__ __attribute__((aligned(16))) char a0[kPartBytes];          \
+    __shared__ __attribute__((aligned(16))) char b0[kPartBytes];          \
+    __shared__ __attribute__((aligned(16))) char a1[kPartBytes];          \
+    __shared__ __attribute__((aligned(16))) char b1[kPartBytes];          \
+    __shared__ __attribute__((aligned(16))) char a2[kPartBytes];          \
+    __shared__ __attribute__((aligned(16))) char b2[kPartBytes];          \
+    __shared__ __attribute__((aligned(16))) char a3[kPartBytes];          \
+    __shared__ __attribute__((aligned(16))) char b3[kPartBytes]
 
 }  // namespace tg
