@@ -327,15 +327,21 @@ __device__ __forceinline__ void ring(int steps, const RA& ra, const RB& rb, L&& 
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[i][j] = mfma<T>(now.w[j], now.x[i], acc[i][j]);
         also(now.w);
-        // an LDS read beside each of the first matrix instructions: the reads
-        // have the rest of the step to arrive (left to itself, the compiler
-        // puts them last, where the border waits for them)
+        // An LDS read beside each of the first matrix instructions, then a load
+        // beside every fourth: the reads have the rest of the step to arrive
+        // (left to itself, the compiler puts them last, where the border waits
+        // for them), and the loads of eight wavefronts, 16 cycles each, do not
+        // hold back the first products.
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, 16, 0);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+        }
     };
     load(0, a0, b0);
     load(1, a1, b1);
