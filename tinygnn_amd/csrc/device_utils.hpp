@@ -154,8 +154,9 @@ __device__ __forceinline__ uint32_t write_lane(uint32_t s, uint32_t v) {
 
 // A load by the scalar unit from a wave-uniform address, of memory that nothing
 // writes while the kernel runs.
-__device__ __forceinline__ int scalar_load(const int* p) {
-    return *(const __attribute__((address_space(4))) int*)p;
+template <typename T>
+__device__ __forceinline__ T scalar_load(const T* p) {
+    return *(const __attribute__((address_space(4))) T*)p;
 }
 
 // Non-temporal (streaming) loads for data read exactly once.

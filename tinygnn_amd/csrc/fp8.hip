@@ -258,36 +258,49 @@ __global__ __launch_bounds__(S::kThreads) void fp8_kernel(Fp8Args a) {
     const Reader<uint8_t, S::kN, false, S::kNJ> rb(wn, lane);
     int kt = 0;
     auto compute = [&](const char* la, const char* lb) {
-        const float scale = ws[kt++];
+        const float scale = scalar_load(ws + kt++);
         const float* xs = reinterpret_cast<const float*>(la + kScales) + wm + r;
-        Operand b[S::kNJ];
+        // kHalf columns' tiles at a time; while row tile i's products run, x's
+        // operands of i + 1 are read and the products of i - 1 scaled and added.
+        // No more than that may be live (registers; x's operands are read again
+        // for the other half).
+        constexpr int kHalf = S::kNJ;
+        auto row_tile = [&](int i) {
+            Operand x;
 #pragma unroll
-        for (int j = 0; j < S::kNJ; ++j)
+            for (int s = 0; s < 2; ++s) x.c[s] = ra.read(la, i, s);
+            return x;
+        };
 #pragma unroll
-            for (int s = 0; s < 2; ++s) b[j].c[s] = rb.read(lb, j, s);
-        // row tile i's products run while those of i - 1 are scaled and added;
-        // no more than that may be live (registers)
-        v4f part[2][S::kNJ];
+        for (int h = 0; h < S::kNJ / kHalf; ++h) {
+            Operand b[kHalf], x[2];
 #pragma unroll
-        for (int i = 0; i <= S::kMI; ++i) {
-            if (i < S::kMI) {
-                Operand x;
+            for (int j = 0; j < kHalf; ++j)
 #pragma unroll
-                for (int s = 0; s < 2; ++s) x.c[s] = ra.read(la, i, s);
+                for (int s = 0; s < 2; ++s) b[j].c[s] = rb.read(lb, h * kHalf + j, s);
+            x[0] = row_tile(0);
+            v4f part[2][kHalf];
 #pragma unroll
-                for (int j = 0; j < S::kNJ; ++j)
-                    part[i & 1][j] = block_products<WIDE>(b[j], x);
+            for (int i = 0; i <= S::kMI; ++i) {
+                if (i + 1 < S::kMI) x[(i + 1) & 1] = row_tile(i + 1);
+                if (i < S::kMI) {
+#pragma unroll
+                    for (int j = 0; j < kHalf; ++j)
+                        part[i & 1][j] = block_products<WIDE>(b[j], x[i & 1]);
+                }
+                if (i > 0) {
+                    const float f = xs[(i - 1) * 16] * scale;
+#pragma unroll
+                    for (int j = 0; j < kHalf; ++j) {
+                        v4f& sum = acc[i - 1][h * kHalf + j];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            sum[e] = __builtin_fmaf(part[(i - 1) & 1][j][e], f, sum[e]);
+                        asm volatile("" : "+v"(sum));  // here, not at the tile's end
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            if (i > 0) {
-                const float f = xs[(i - 1) * 16] * scale;
-#pragma unroll
-                for (int j = 0; j < S::kNJ; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        acc[i - 1][j][e] = __builtin_fmaf(part[(i - 1) & 1][j][e], f,
-                                                          acc[i - 1][j][e]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
         }
     };
     pipeline<true>(a.kb, a0, b0, a1, b1, load, [](char*, char*) {}, compute);
@@ -368,7 +381,9 @@ __global__ __launch_bounds__(64 * kThinWaves) void fp8_thin_kernel(Fp8Args a) {
     });
 }
 
+using Large = Shape<256, 256, 2, 4>;
 using Medium = Shape<128, 128, 2, 2>;
+using Small = Shape<64, 64, 2, 2>;
 
 unsigned set_grid(Fp8Args& a, int bm, int bn) {
     a.mt = static_cast<uint32_t>(most_tiles(a.m, a.groups, bm));
@@ -384,12 +399,29 @@ void launch_fp8(Fp8Args& a, hipStream_t s) {
     // tiles' offsets have 31 bits
     const bool fits = (a.rows ? a.x_rows : 256) * kp < kDirectBytes &&
                       256 * kp < kDirectBytes && 4 * a.x_rows < kDirectBytes;
-    if (!fits || a.m <= 32 * a.groups) {
+    auto tiled = [&](auto shape) {
+        using S = decltype(shape);
+        const unsigned grid = set_grid(a, S::kM, S::kN);
+        fp8_kernel<T, S><<<grid, S::kThreads, 0, s>>>(a);
+    };
+    auto tiles = [&](int64_t edge) {
+        return most_tiles(a.m, a.groups, edge) * ceil_div(a.n, edge);
+    };
+    // Few rows: the thin form while its workgroups are few (5 rows of 4,096 x
+    // 4,096 7.6 us; 150 rows of 32 groups 46 us against 23).  Large tiles where
+    // they fill the CUs at least twice and the groups do (8,192 x 4,096 x 8,192
+    // 314 us against 389; 10,000 x 1,024 x 512 19 against 13), 128 x 128 where
+    // those do once (10,000 rows 13 against 15), else 64 x 64 (600 x 2,048 x
+    // 1,024 12 against 18).
+    if (!fits || tiles(16) <= 1024) {
         const unsigned grid = set_grid(a, 16, 16);
         fp8_thin_kernel<T><<<grid, 64 * kThinWaves, 0, s>>>(a);
+    } else if (tiles(256) >= 600 && a.m >= 256 * a.groups) {
+        tiled(Large{});
+    } else if (tiles(128) >= 256 && a.m >= 100 * a.groups) {
+        tiled(Medium{});
     } else {
-        const unsigned grid = set_grid(a, Medium::kM, Medium::kN);
-        fp8_kernel<T, Medium><<<grid, Medium::kThreads, 0, s>>>(a);
+        tiled(Small{});
     }
     TG_LAUNCH_CHECK();
 }

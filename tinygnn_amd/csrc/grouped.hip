@@ -299,8 +299,8 @@ __global__ __launch_bounds__(kRingThreads) void grouped_ring_kernel(GroupedArgs 
     v4f acc[8][4] = {};
     const PartReader<false, 8> ra(wm, lane);
     const PartReader<!ALONG_W, 4> rb(wn, lane);
-    ring<T>((a.k + kStep - 1) / kStep, ra, rb, load, [](Frag(&)[4]) {}, a0, b0, a1,
-            b1, a2, b2, a3, b3, acc);
+    ring<T>((a.k + kStep - 1) / kStep, ra, rb, [](int) {}, load, [](Frag(&)[4]) {},
+            a0, b0, a1, b1, a2, b2, a3, b3, acc);
     store_outputs<T>(a, g, r0 + wm, r1, n0 + wn, lane, acc);
 }
 
@@ -433,11 +433,14 @@ __global__ __launch_bounds__(S::kThreads) void wgrad_kernel(GroupedArgs a) {
     if (BIAS && sums) store_bias_gradient<T>(a, part, n0 + wn, lane, sum);
 }
 
+constexpr int kRowParts = 64;
+
 // dw on the large tile: both operands run across memory, the contraction over
 // the group's rows.
 template <typename T, bool BIAS>
 __global__ __launch_bounds__(kRingThreads) void wgrad_ring_kernel(GroupedArgs a) {
     TG_RING_LDS;
+    __shared__ uint32_t row_starts[8 * kRowParts * 4];
     const uint32_t per = a.mt * a.nt;
     const int part = static_cast<int>(blockIdx.x / per);
     uint32_t mt, ntile;
@@ -465,6 +468,21 @@ __global__ __launch_bounds__(kRingThreads) void wgrad_ring_kernel(GroupedArgs a)
         ao[t] = k0 + c < a.k ? static_cast<uint32_t>(2 * (p * a.ldx + k0 + c)) : kOutside;
         bo[t] = n0 + c < a.n ? static_cast<uint32_t>(2 * (p * a.lddy + n0 + c)) : kOutside;
     }
+    // Gathered rows: a wavefront's rows' starts, in LDS for kRowParts parts at a
+    // time.  (The indices loaded a step ahead to scalar registers held every step
+    // back: 866 us against 609 without a gather, 32 groups of 32,768 x 2,048 x
+    // 4,096.)
+    uint32_t* own = row_starts + wave * kRowParts * 4;
+    auto ahead = [&](int u) {
+        if (a.rows == nullptr || u % kRowParts != 0) return;
+#pragma unroll
+        for (int c = 0; c < kRowParts / 16; ++c) {
+            const int e = c * 64 + lane, t = (e >> 1) & 1, h = e & 1;
+            const int p = lo + (u + (e >> 2)) * kStep + t * 16 + wave * 2 + h;
+            const int r = p < hi ? a.rows[p] : -1;
+            own[e] = r >= 0 && r < a.x_rows ? static_cast<uint32_t>(2 * r * a.ldx) : kOutside;
+        }
+    };
     auto load = [&](int u, char* la, char* lb) {
         const int p0 = lo + u * kStep;
         const int64_t left = hi - p0;  // rows: the buffers end with them
@@ -474,15 +492,7 @@ __global__ __launch_bounds__(kRingThreads) void wgrad_ring_kernel(GroupedArgs a)
             const auto xbuf = buffer_of(x, kDirectBytes);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                uint32_t at[2];  // the two rows' starts
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int p = p0 + t * 16 + wave * 2 + h;
-                    const int r = p < hi ? scalar_load(a.rows + p) : -1;
-                    at[h] = r >= 0 && r < a.x_rows ? static_cast<uint32_t>(2 * r * a.ldx)
-                                                   : kOutside;
-                }
-                const uint32_t row = lane < 32 ? at[0] : at[1];
+                const uint32_t row = own[u % kRowParts * 4 + t * 2 + (lane >> 5)];
                 load_to_lds(xbuf, la + (t * kRingThreads + wave * 64) * 16,
                             (row | ax[t]) >= kOutside ? kOutside : row + ax[t]);
             }
@@ -503,7 +513,7 @@ __global__ __launch_bounds__(kRingThreads) void wgrad_ring_kernel(GroupedArgs a)
     const Frag one = ones<T>();
     const PartReader<true, 8> ra(wm, lane);
     const PartReader<true, 4> rb(wn, lane);
-    ring<T>((hi - lo + kStep - 1) / kStep, ra, rb, load,
+    ring<T>((hi - lo + kStep - 1) / kStep, ra, rb, ahead, load,
             [&](Frag(&w)[4]) {
                 if (BIAS && sums) {
 #pragma unroll
@@ -572,7 +582,8 @@ bool direct_operand(const void* p, int64_t ld, int64_t cols, int64_t stride, int
 }
 
 using Medium = Shape<128, 128, 2, 2>;
-using Small = Shape<32, 128, 1, 4>;
+using Small = Shape<64, 64, 2, 2>;
+using Few = Shape<32, 128, 1, 4>;
 
 unsigned grid_of(const std::string& w, int64_t tiles) {
     require(tiles < (int64_t(1) << 31), w + ": too many tiles");
@@ -603,9 +614,13 @@ void launch_ring(GroupedArgs& a, bool along, hipStream_t s) {
     TG_LAUNCH_CHECK();
 }
 
-// How a gradient of w is cut: `edge` x `edge` tiles of whole groups where they
-// are two for each of the 256 CUs; else of parts of `unit` rows for about four,
-// 256 rows at least.
+// How a gradient of w is cut: tiles of `edge` x `edge` of whole groups where they
+// are two for each of the 256 CUs, or the rows few; else of parts of `unit` rows
+// for about four, 512 rows at least.  Edge 256 (16-bit types, direct loads) where
+// that gives two or four tiles a CU of enough rows (32 groups of 40,000 x 1,024
+// x 4,096 375 us against 459 of edge 128; 10,000 rows of 8 groups 122 against
+// 113), 64 where the groups make few tiles (40,000 x 512 x 512 52 us against
+// 69; in 8 groups 88 against 67).
 struct WgradPlan {
     int64_t edge, mt, nt, unit, parts;  // parts: most of them
     size_t bytes(int64_t k, int64_t n, float** part, float** part_bias, void* ws, size_t size) const {
@@ -621,13 +636,23 @@ struct WgradPlan {
 
 WgradPlan wgrad_plan(int64_t m, int64_t k, int64_t n, int64_t groups, int type, bool direct) {
     WgradPlan p{};
-    p.edge = type != TG_TYPE_F32 && direct && getenv("TGM") ? 256 : 128;
+    const auto tiles_of = [&](int64_t edge) {
+        return std::max<int64_t>(1, ceil_div(k, edge)) * ceil_div(n, edge);
+    };
+    const int64_t t256 = groups * tiles_of(256);
+    p.edge = 128;
+    if (type != TG_TYPE_F32 && direct &&
+        ((t256 >= 1024 && m >= 192 * groups) || (t256 >= 512 && m >= 4096 * groups)))
+        p.edge = 256;
+    else if (groups * tiles_of(128) <= 64)
+        p.edge = 64;
+    if (const char* ev = getenv("TGE")) p.edge = atoi(ev);
     p.mt = std::max<int64_t>(1, ceil_div(k, p.edge));
     p.nt = ceil_div(n, p.edge);
     p.parts = groups;
     const int64_t tiles = p.mt * p.nt;
-    if (tiles * groups >= 512) return p;
-    const int64_t unit = std::max<int64_t>(256, ceil_div(ceil_div(m * tiles, 1024), 64) * 64);
+    if (tiles * groups >= 512 || m < 1024) return p;
+    const int64_t unit = std::max<int64_t>(512, ceil_div(ceil_div(m * tiles, 1024), 64) * 64);
     if (unit >= m) return p;
     p.unit = unit;
     p.parts = most_tiles(m, groups, unit);
@@ -636,21 +661,28 @@ WgradPlan wgrad_plan(int64_t m, int64_t k, int64_t n, int64_t groups, int type, 
 
 template <typename T>
 void launch_wgrad(GroupedArgs& a, const WgradPlan& p, bool direct, hipStream_t s) {
-    using S = Medium;
     a.mt = static_cast<uint32_t>(p.mt);
     a.nt = static_cast<uint32_t>(p.nt);
     a.unit = static_cast<int>(p.unit);
     const unsigned grid = grid_of("grouped_matmul_wgrad", p.mt * p.nt * p.parts);
-    if (p.edge == 256) {
-        if constexpr (sizeof(T) == 2)
+    auto tiled = [&](auto shape) {
+        using S = decltype(shape);
+        if (a.dbias)
+            direct ? wgrad_kernel<T, S, true, true><<<grid, S::kThreads, 0, s>>>(a)
+                   : wgrad_kernel<T, S, false, true><<<grid, S::kThreads, 0, s>>>(a);
+        else
+            direct ? wgrad_kernel<T, S, true, false><<<grid, S::kThreads, 0, s>>>(a)
+                   : wgrad_kernel<T, S, false, false><<<grid, S::kThreads, 0, s>>>(a);
+    };
+    if (p.edge == 64)
+        tiled(Small{});
+    else if (p.edge == 128)
+        tiled(Medium{});
+    if constexpr (sizeof(T) == 2) {
+        if (p.edge == 256)
             a.dbias ? wgrad_ring_kernel<T, true><<<grid, kRingThreads, 0, s>>>(a)
                     : wgrad_ring_kernel<T, false><<<grid, kRingThreads, 0, s>>>(a);
-    } else if (a.dbias)
-        direct ? wgrad_kernel<T, S, true, true><<<grid, S::kThreads, 0, s>>>(a)
-               : wgrad_kernel<T, S, false, true><<<grid, S::kThreads, 0, s>>>(a);
-    else
-        direct ? wgrad_kernel<T, S, true, false><<<grid, S::kThreads, 0, s>>>(a)
-               : wgrad_kernel<T, S, false, false><<<grid, S::kThreads, 0, s>>>(a);
+    }
     TG_LAUNCH_CHECK();
     if (!p.unit) return;
     auto add = [&](const float* part, int64_t size, void* out) {
@@ -713,12 +745,29 @@ int tg_grouped_matmul(int64_t m, int64_t k, int64_t n, int64_t groups, int type,
         hipStream_t s = static_cast<hipStream_t>(stream);
         tg::with_type(type, "grouped_matmul", [&](auto t) {
             using T = decltype(t);
-            if (m <= 32 * groups)
+            // Tiles of 32 rows for groups of about 20 (150 rows of 32 groups in
+            // fp32 59 us against 79 of 64 x 64, in bf16 23 both); for 16-bit
+            // types the large tile where there are 160 of them of 1,024 values
+            // (2,500 x 1,024 x 4,096 38 us against 47; 40,000 x 512 x 512 45
+            // against 42) and the groups fill them, 128 x 128 where there are
+            // two for each CU (40,000 x 512 x 512 42 against 50); else, and for
+            // floats always (the matrix units' rate bounds those: 40,000 x 2,048
+            // x 1,024 1.28 ms both), 64 x 64.
+            const auto tiles = [&](int64_t edge) {
+                return tg::most_tiles(m, groups, edge) * tg::ceil_div(n, edge);
+            };
+            if (m <= 24 * groups) {
+                tg::launch_grouped<T, tg::Few>(a, along, direct, s);
+            } else if constexpr (sizeof(T) == 2) {
+                if (direct && k >= 512 && tiles(256) * k >= 160 * 1024 && m >= 192 * groups)
+                    tg::launch_ring<T>(a, along, s);
+                else if (tiles(128) >= 600)
+                    tg::launch_grouped<T, tg::Medium>(a, along, direct, s);
+                else
+                    tg::launch_grouped<T, tg::Small>(a, along, direct, s);
+            } else {
                 tg::launch_grouped<T, tg::Small>(a, along, direct, s);
-            else if (type == TG_TYPE_F32 || !direct)
-                tg::launch_grouped<T, tg::Medium>(a, along, direct, s);
-            else if constexpr (sizeof(T) == 2)
-                tg::launch_ring<T>(a, along, s);
+            }
         });
     });
 }

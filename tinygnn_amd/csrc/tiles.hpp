@@ -300,10 +300,11 @@ __device__ __forceinline__ void step_border() {
 }
 
 // acc += the products of `steps` parts; load(u, la, lb) asks for part u (four
-// loads a thread; zeros from `steps` on); also(w) sees the columns' operands.
-template <typename T, typename RA, typename RB, typename L, typename W>
-__device__ __forceinline__ void ring(int steps, const RA& ra, const RB& rb, L&& load, W&& also,
-                                     char* a0, char* b0, char* a1, char* b1, char* a2, char* b2,
+// loads a thread; zeros from `steps` on), ahead(u) comes before the loads of u ..
+// u + 3; also(w) sees the columns' operands.
+template <typename T, typename RA, typename RB, typename P, typename L, typename W>
+__device__ __forceinline__ void ring(int steps, const RA& ra, const RB& rb, P&& ahead, L&& load,
+                                     W&& also, char* a0, char* b0, char* a1, char* b1, char* a2, char* b2,
                                      char* a3, char* b3, v4f (&acc)[8][4]) {
     constexpr int kLoads = 4;
     if (steps == 0) return;
@@ -343,6 +344,7 @@ __device__ __forceinline__ void ring(int steps, const RA& ra, const RB& rb, L&& 
             __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
         }
     };
+    ahead(0);
     load(0, a0, b0);
     load(1, a1, b1);
     load(2, a2, b2);
@@ -352,12 +354,14 @@ __device__ __forceinline__ void ring(int steps, const RA& ra, const RB& rb, L&& 
     read(even, a0, b0);
     int u = 0;
     for (; u + 4 <= steps; u += 4) {
+        ahead(u + 4);
         step(u, even, odd, a0, b0, a1, b1);
         step(u + 1, odd, even, a1, b1, a2, b2);
         step(u + 2, even, odd, a2, b2, a3, b3);
         step(u + 3, odd, even, a3, b3, a0, b0);
     }
     if (u < steps) {
+        ahead(u + 4);
         step(u, even, odd, a0, b0, a1, b1);
         if (u + 1 < steps) {
             step(u + 1, odd, even, a1, b1, a2, b2);
