@@ -199,19 +199,40 @@ __global__ __launch_bounds__(S::kThreads) void grouped_kernel(GroupedArgs a) {
                             : kOutside;
         }
         const T* wb = ALONG_W ? w + n0 * a.ldw : w + n0;
+        // a chunk of an operand along memory that k ends in: by registers
+        auto last_chunk = [&](const T* base, uint32_t offset, int64_t left, char* to) {
+            const T* p = reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) +
+                                                    (offset == kOutside ? 0 : offset));
+            *reinterpret_cast<v4u*>(to) = load_chunk(p, offset == kOutside ? 0 : left);
+        };
         auto load = [&](int kt, char* la, char* lb) {
             const int k0 = kt * kDepth<T>;
             const auto xbuf = buffer_of(xb + k0, kDirectBytes);
-            const auto wbuf = buffer_of(ALONG_W ? wb + k0 : wb + k0 * a.ldw, kDirectBytes);
+            // (w across memory ends with its last row's columns)
+            const auto wbuf =
+                ALONG_W ? buffer_of(wb + k0, kDirectBytes)
+                        : buffer_of(wb + k0 * a.ldw, Z * ((a.k - k0 - 1) * a.ldw + a.n - n0));
             const bool part = k0 + kDepth<T> > a.k;  // the last tile: what lies behind k is 0
+            const bool split = part && a.k % kVec<T> != 0;
 #pragma unroll
-            for (int t = 0; t < S::kCA; ++t)
-                load_to_lds(xbuf, la + (t * S::kThreads + wave * 64) * 16,
-                            part && k0 + ac[t] >= a.k ? kOutside : ao[t]);
+            for (int t = 0; t < S::kCA; ++t) {
+                if (split)
+                    last_chunk(xb + k0, ao[t], a.k - k0 - ac[t],
+                               la + (t * S::kThreads + tid) * 16);
+                else
+                    load_to_lds(xbuf, la + (t * S::kThreads + wave * 64) * 16,
+                                part && k0 + ac[t] >= a.k ? kOutside : ao[t]);
+            }
 #pragma unroll
-            for (int t = 0; t < S::kCB; ++t)
-                load_to_lds(wbuf, lb + (t * S::kThreads + wave * 64) * 16,
-                            part && k0 + (ALONG_W ? bmin[t] : bmaj[t]) >= a.k ? kOutside : bo[t]);
+            for (int t = 0; t < S::kCB; ++t) {
+                if (ALONG_W && split)
+                    last_chunk(wb + k0, bo[t], a.k - k0 - bmin[t],
+                               lb + (t * S::kThreads + tid) * 16);
+                else
+                    load_to_lds(wbuf, lb + (t * S::kThreads + wave * 64) * 16,
+                                part && k0 + (ALONG_W ? bmin[t] : bmaj[t]) >= a.k ? kOutside
+                                                                                 : bo[t]);
+            }
         };
         pipeline<true>(tiles, a0, b0, a1, b1, load, [](char*, char*) {}, compute);
     } else {
@@ -285,7 +306,10 @@ __global__ __launch_bounds__(kRingThreads) void grouped_ring_kernel(GroupedArgs 
         const int k0 = u * kStep;
         const int64_t size = k0 < a.k ? kDirectBytes : 0;
         const auto xbuf = buffer_of(xb + k0, size);
-        const auto wbuf = buffer_of(ALONG_W ? wb + k0 : wb + k0 * a.ldw, size);
+        const auto wbuf =
+            ALONG_W ? buffer_of(wb + k0, size)
+                    : buffer_of(wb + k0 * a.ldw,
+                                k0 < a.k ? 2 * ((a.k - k0 - 1) * a.ldw + a.n - n0) : 0);
         const bool part = k0 + kStep > a.k;  // what lies behind k is 0
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -381,7 +405,8 @@ __global__ __launch_bounds__(S::kThreads) void wgrad_kernel(GroupedArgs a) {
             const int64_t left = hi - p0;  // rows: the buffers end with them
             const auto dbuf = buffer_of(dy + p0 * a.lddy, Z * ((left - 1) * a.lddy + a.n));
             if (a.rows) {
-                const auto xbuf = buffer_of(x, kDirectBytes);
+                const auto xbuf = buffer_of(x, static_cast<int64_t>(sizeof(T)) *
+                                             ((a.x_rows - 1) * a.ldx + a.k));
 #pragma unroll
                 for (int t = 0; t < S::kCA; ++t) {
                     const bool in = idx[t] >= 0 && idx[t] < a.x_rows && k0 + ac[t] < a.k;
@@ -489,7 +514,8 @@ __global__ __launch_bounds__(kRingThreads) void wgrad_ring_kernel(GroupedArgs a)
         const auto dbuf = buffer_of(dy + p0 * a.lddy, left > 0 ? 2 * ((left - 1) * a.lddy + a.n)
                                                                : 0);
         if (a.rows) {
-            const auto xbuf = buffer_of(x, kDirectBytes);
+            const auto xbuf = buffer_of(x, static_cast<int64_t>(sizeof(T)) *
+                                             ((a.x_rows - 1) * a.ldx + a.k));
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const uint32_t row = own[u % kRowParts * 4 + t * 2 + (lane >> 5)];
@@ -573,12 +599,12 @@ void check_grouped(const std::string& w, int64_t m, int64_t k, int64_t n, int64_
 }
 
 // Whether an operand's tiles of up to `major` rows of `ld` elements can come by
-// loads to LDS: whole, aligned 16-byte chunks within 2 GB of the tile's start.
+// loads to LDS: from dword-aligned rows, within 2 GB of the tile's start; across
+// memory, in whole dwords.
 bool direct_operand(const void* p, int64_t ld, int64_t cols, int64_t stride, int64_t z,
-                    int64_t major) {
-    const int64_t epc = 16 / z;
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % epc == 0 && cols % epc == 0 &&
-           stride % epc == 0 && (major * ld + cols) * z < kDirectBytes;
+                    int64_t major, bool across) {
+    return reinterpret_cast<uintptr_t>(p) % 4 == 0 && ld * z % 4 == 0 && stride * z % 4 == 0 &&
+           (!across || cols * z % 4 == 0) && (major * ld + cols) * z < kDirectBytes;
 }
 
 using Medium = Shape<128, 128, 2, 2>;
@@ -740,8 +766,8 @@ int tg_grouped_matmul(int64_t m, int64_t k, int64_t n, int64_t groups, int type,
         const bool along = transposed != 0;
         const int64_t z = tg::type_size(type);
         const bool direct =
-            tg::direct_operand(x, ldx, k, 0, z, rows ? x_rows : 256) &&
-            tg::direct_operand(w, ldw, along ? k : n, groups > 1 ? w_stride : 0, z, 256);
+            tg::direct_operand(x, ldx, k, 0, z, rows ? x_rows : 256, false) &&
+            tg::direct_operand(w, ldw, along ? k : n, groups > 1 ? w_stride : 0, z, 256, !along);
         hipStream_t s = static_cast<hipStream_t>(stream);
         tg::with_type(type, "grouped_matmul", [&](auto t) {
             using T = decltype(t);
@@ -759,7 +785,7 @@ int tg_grouped_matmul(int64_t m, int64_t k, int64_t n, int64_t groups, int type,
             if (m <= 24 * groups) {
                 tg::launch_grouped<T, tg::Few>(a, along, direct, s);
             } else if constexpr (sizeof(T) == 2) {
-                if (direct && k >= 512 && tiles(256) * k >= 160 * 1024 && m >= 192 * groups)
+                if (direct && k % 8 == 0 && k >= 512 && tiles(256) * k >= 160 * 1024 && m >= 192 * groups)
                     tg::launch_ring<T>(a, along, s);
                 else if (tiles(128) >= 600)
                     tg::launch_grouped<T, tg::Medium>(a, along, direct, s);
@@ -811,8 +837,8 @@ int tg_grouped_matmul_wgrad(int64_t m, int64_t k, int64_t n, int64_t groups, int
         a.dw = dw;
         a.dbias = dbias;
         const int64_t z = tg::type_size(type);
-        const bool direct = tg::direct_operand(x, ldx, a.k, 0, z, rows ? x_rows : 64) &&
-                            tg::direct_operand(dy, lddy, n, 0, z, 64);
+        const bool direct = tg::direct_operand(x, ldx, a.k, 0, z, rows ? x_rows : 64, true) &&
+                            tg::direct_operand(dy, lddy, n, 0, z, 64, true);
         hipStream_t s = static_cast<hipStream_t>(stream);
         const tg::WgradPlan plan = tg::wgrad_plan(m, a.k, n, groups, type, direct);
         tg::TempBuffer temp;

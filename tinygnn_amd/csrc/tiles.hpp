@@ -141,9 +141,9 @@ struct Reader {
     }
 };
 
-// The memory side.  `Direct`: buffer loads that write to LDS by themselves,
-// zeros for what lies outside the buffer: offsets of 32 bits from a base that
-// moves with the tile, 16-byte aligned chunks that are whole or outside.
+// The memory side.  `Direct`: buffer loads that write to LDS by themselves, 16
+// bytes from a dword-aligned address, each dword zero that lies outside the
+// buffer: offsets of 32 bits from a base that moves with the tile.
 constexpr uint32_t kOutside = 0x80000000u;  // added to an offset: outside any buffer below
 constexpr int64_t kDirectBytes = int64_t(1) << 31;
 
