@@ -9,11 +9,12 @@
 // partials in order (no atomics: equal calls give equal bits).  Both are bound
 // by HBM: 2 RC and 3 RC elements.
 //
-// A row is taken by a wavefront up to 1,024 columns (four rows a workgroup, no
-// barrier), by 256 threads up to 4,096 and by 1,024 up to 16,384 -- at most 16
-// values of a row in a thread, which leaves the backward pass (x, dy, the next
-// row's x and dy, gamma, two sums for each value) under 128 registers -- and by
-// 1,024 threads that walk the row, out of L2 after the first time, beyond.
+// A row is taken by as many threads as one 16-byte load of x each covers, 64
+// (four rows a workgroup, no barrier) to 1,024, then by 1,024 with two or four
+// loads each, up to 16,384 columns: few registers, so many wavefronts a SIMD (16
+// values a thread kept the backward pass at two of them: 16,384 x 4,096 bf16 170
+// us against RESULT).  Wider rows are walked by 1,024 threads, out of L2 after the
+// first time.
 #include "common.hpp"
 #include "device_utils.hpp"
 #include "types.hpp"
@@ -23,7 +24,6 @@
 namespace tg {
 namespace {
 
-constexpr int kRowValues = 16;  // values of a row that a thread holds
 constexpr int kWideThreads = 1024;
 
 struct NormArgs {
@@ -60,15 +60,15 @@ __device__ __forceinline__ void load_weights(const void* w, int f32, int64_t c, 
     }
 }
 
-// Sum over the TPR threads of a row, to all of them; for TPR > 64 the
-// workgroup is one row and `lds` holds TPR / 64 values (a barrier before the
+// Sum over the TPR threads of a row, to all of them; for TPR > 64 through `lds`,
+// the row's own, and a barrier that the whole workgroup joins (one before the
 // next use of lds is the caller's: two buffers alternate).
 template <int TPR, int N>
 __device__ __forceinline__ void row_sums(float (&v)[N], float (*lds)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
     if constexpr (TPR > kWave) {
-        const int wave = threadIdx.x / kWave;
+        const int wave = threadIdx.x % TPR / kWave;
         if ((threadIdx.x & (kWave - 1)) == 0) {
 #pragma unroll
             for (int i = 0; i < N; ++i) lds[wave][i] = v[i];
@@ -84,13 +84,13 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float (*lds)[N]) {
     }
 }
 
-template <typename T, int TPR>
+template <typename T, int TPR, int ITEMS>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_kernel(NormArgs a) {
-    constexpr int VEC = kVec<T>, ITEMS = kRowValues / VEC, RPB = TPR > 256 ? 1 : 256 / TPR;
-    __shared__ float lds[2][TPR / kWave][1];
-    const int lane = threadIdx.x % TPR;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * RPB + threadIdx.x / TPR;
-    if (row >= a.rows) return;  // a whole wavefront, or workgroups of one row: none
+    constexpr int VEC = kVec<T>, RPB = TPR > 256 ? 1 : 256 / TPR;
+    __shared__ float lds[2][RPB][TPR / kWave][1];
+    const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * RPB + sub;
+    const int64_t row = at < a.rows ? at : a.rows - 1;  // again, for the barriers
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     float v[ITEMS][VEC];
     float s[1] = {0.0f};
@@ -101,7 +101,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_kernel(NormArgs a)
 #pragma unroll
         for (int u = 0; u < VEC; ++u) s[0] += v[i][u];
     }
-    row_sums<TPR>(s, lds[0]);
+    row_sums<TPR>(s, lds[0][sub]);
     const float n = static_cast<float>(a.cols);
     const float mean = s[0] / n;
     float q[1] = {0.0f};
@@ -115,7 +115,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_kernel(NormArgs a)
             if (c + u < a.cols) q[0] = __builtin_fmaf(d, d, q[0]);
         }
     }
-    row_sums<TPR>(q, lds[1]);
+    row_sums<TPR>(q, lds[1][sub]);
+    if (at >= a.rows) return;
     const float rstd = 1.0f / sqrtf(q[0] / n + a.eps);
     if (lane == 0) {
         if (a.mean) a.mean[row] = mean;
@@ -180,11 +181,11 @@ __global__ __launch_bounds__(kWideThreads) void norm_wide_kernel(NormArgs a) {
 
 // The backward pass of rows b, b + B, ... for workgroup (or, TPR = 64, a
 // quarter of one) b of B; the next row is loaded while this one is summed.
-template <typename T, int TPR>
+template <typename T, int TPR, int ITEMS>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_backward_kernel(NormArgs a) {
-    constexpr int VEC = kVec<T>, ITEMS = kRowValues / VEC, RPB = TPR > 256 ? 1 : 256 / TPR;
-    __shared__ float lds[2][TPR / kWave][2];
-    __shared__ float sums[RPB > 1 ? RPB : 1][RPB > 1 ? TPR * kRowValues : 1];
+    constexpr int VEC = kVec<T>, RPB = TPR > 256 ? 1 : 256 / TPR;
+    __shared__ float lds[2][RPB][TPR / kWave][2];
+    __shared__ float sums[RPB > 1 ? RPB : 1][RPB > 1 ? TPR * ITEMS * VEC : 1];
     const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
     const int64_t step = static_cast<int64_t>(gridDim.x) * RPB;
     const T* x = static_cast<const T*>(a.x);
@@ -208,8 +209,10 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_backward_kernel(No
         load_weights<T, VEC>(a.gamma, a.weight_f32, c, a.cols, 1.0f, g[i]);
     }
     int64_t row = static_cast<int64_t>(blockIdx.x) * RPB + sub;
+    int64_t first = row - sub;  // the workgroup's; rows past the last join its barriers
     if (row < a.rows) fetch(row);
-    for (int buf = 0; row < a.rows; row += step, buf ^= 1) {
+    for (int buf = 0; first < a.rows; first += step, row += step, buf ^= 1) {
+        const bool in = row < a.rows;
         float t[ITEMS][VEC], xh[ITEMS][VEC];
         float s[2] = {0.0f, 0.0f};
         const float r = rstd;
@@ -219,8 +222,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_backward_kernel(No
 #pragma unroll
             for (int u = 0; u < VEC; ++u) {
                 // past the row's end dy and g are 0, and so are the sums' terms
-                const float d = dv[i][u];
-                xh[i][u] = c + u < a.cols ? (xv[i][u] - mean) * r : 0.0f;
+                const float d = in ? dv[i][u] : 0.0f;
+                xh[i][u] = in && c + u < a.cols ? (xv[i][u] - mean) * r : 0.0f;
                 t[i][u] = d * g[i][u];
                 s[0] += t[i][u];
                 s[1] = __builtin_fmaf(t[i][u], xh[i][u], s[1]);
@@ -229,8 +232,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_backward_kernel(No
             }
         }
         if (row + step < a.rows) fetch(row + step);
-        row_sums<TPR>(s, lds[buf]);
-        if (a.dx == nullptr) continue;
+        row_sums<TPR>(s, lds[buf][sub]);
+        if (a.dx == nullptr || !in) continue;
         const float m0 = s[0] / n, m1 = s[1] / n;
         T* dx = static_cast<T*>(a.dx) + row * a.lddx;
 #pragma unroll
@@ -358,17 +361,55 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(const float* __restri
     }
 }
 
-int threads_per_row(int64_t cols) {
-    return cols <= 64 * kRowValues ? 64 : cols <= 256 * kRowValues ? 256 : 1024;
+// Threads of a row and 16-byte loads of each (0: rows that are walked).
+struct RowShape {
+    int threads, items;
+};
+
+RowShape row_shape(int64_t cols, int type) {
+    const int64_t loads = ceil_div(cols, 16 / type_size(type));
+    for (int t = 64; t < 1024; t *= 2)
+        if (loads <= t) return {t, 1};
+    const int items = loads <= 1024 ? 1 : loads <= 2048 ? 2 : 4;
+    return {1024, cols > 16384 ? 0 : items};
 }
 
-bool is_wide(int64_t cols) { return cols > kWideThreads * kRowValues; }
+// The backward pass holds a thread's values of x and dy, of the next row's, of
+// gamma and of two sums: up to 8 of each in registers (16 spilled), wider rows are
+// walked.
+constexpr int kBackwardValues = 8;
+
+bool in_registers(RowShape r, int type) {
+    return r.items > 0 && r.items * 16 / type_size(type) <= kBackwardValues;
+}
+
+// fn(threads, items) as constants, for shapes that hold the row.
+template <typename T, typename F>
+void with_row_shape(RowShape r, F&& fn) {
+    auto call = [&](auto threads, auto items) { fn(threads, items); };
+    std::integral_constant<int, 1> one;
+    if (r.threads == 64)
+        call(std::integral_constant<int, 64>{}, one);
+    else if (r.threads == 128)
+        call(std::integral_constant<int, 128>{}, one);
+    else if (r.threads == 256)
+        call(std::integral_constant<int, 256>{}, one);
+    else if (r.threads == 512)
+        call(std::integral_constant<int, 512>{}, one);
+    else if (r.items == 1)
+        call(std::integral_constant<int, 1024>{}, one);
+    else if (r.items == 2)
+        call(std::integral_constant<int, 1024>{}, std::integral_constant<int, 2>{});
+    else if constexpr (sizeof(T) == 4)
+        call(std::integral_constant<int, 1024>{}, std::integral_constant<int, 4>{});
+}
 
 // Workgroups of the backward pass: enough to fill the 256 CUs, few enough that
 // the partial rows cost little beside the data.
-int64_t backward_blocks(int64_t rows, int64_t cols) {
-    const int64_t rpb = threads_per_row(cols) == 64 ? 4 : 1;
-    const int64_t most = cols <= 64 * kRowValues ? 1024 : cols <= 256 * kRowValues ? 768 : 256;
+int64_t backward_blocks(int64_t rows, int64_t cols, int type) {
+    const RowShape r = row_shape(cols, type);
+    const int64_t rpb = r.threads < 256 ? 256 / r.threads : 1;
+    const int64_t most = 256 * std::max(1, std::min(4, 1024 / r.threads));  // that many fit
     return std::min(ceil_div(rows, rpb), most);
 }
 
@@ -418,14 +459,16 @@ int tg_layer_norm(int64_t rows, int64_t cols, int type, const void* x, int64_t l
         const unsigned n = static_cast<unsigned>(rows);
         tg::with_type(type, "layer_norm", [&](auto t) {
             using T = decltype(t);
-            if (tg::is_wide(cols))
+            const tg::RowShape shape = tg::row_shape(cols, type);
+            if (shape.items == 0) {
                 tg::norm_wide_kernel<T><<<n, tg::kWideThreads, 0, s>>>(a);
-            else if (tg::threads_per_row(cols) == 64)
-                tg::norm_kernel<T, 64><<<(n + 3) / 4, 256, 0, s>>>(a);
-            else if (tg::threads_per_row(cols) == 256)
-                tg::norm_kernel<T, 256><<<n, 256, 0, s>>>(a);
-            else
-                tg::norm_kernel<T, 1024><<<n, 1024, 0, s>>>(a);
+                return;
+            }
+            tg::with_row_shape<T>(shape, [&](auto threads, auto items) {
+                constexpr int TPR = decltype(threads)::value, RPB = TPR > 256 ? 1 : 256 / TPR;
+                tg::norm_kernel<T, TPR, decltype(items)::value>
+                    <<<(n + RPB - 1) / RPB, TPR > 256 ? TPR : 256, 0, s>>>(a);
+            });
         });
         TG_LAUNCH_CHECK();
     });
@@ -433,9 +476,11 @@ int tg_layer_norm(int64_t rows, int64_t cols, int type, const void* x, int64_t l
 
 size_t tg_layer_norm_backward_workspace_size(int64_t rows, int64_t cols) {
     if (rows <= 0 || cols <= 0) return 0;
+    // of any type
+    const int64_t blocks = std::max(tg::backward_blocks(rows, cols, TG_TYPE_F32),
+                                    tg::backward_blocks(rows, cols, TG_TYPE_BF16));
     tg::Carver c(nullptr, 0);
-    c.take<float>(static_cast<size_t>(tg::backward_blocks(rows, cols)) * 2 *
-                  static_cast<size_t>(cols));
+    c.take<float>(static_cast<size_t>(blocks) * 2 * static_cast<size_t>(cols));
     return c.bytes();
 }
 
@@ -452,7 +497,7 @@ int tg_layer_norm_backward(int64_t rows, int64_t cols, int type, const void* dy,
         const bool sums = dgamma || dbeta;
         tg::NormArgs a{};
         tg::TempBuffer temp;
-        const int64_t blocks = tg::backward_blocks(rows, cols);
+        const int64_t blocks = tg::backward_blocks(rows, cols, type);
         if (rows > 0) {
             require(dy && x && mean && rstd, "layer_norm_backward: null pointer");
             require(ldx >= cols && lddy >= cols && (!dx || lddx >= cols),
@@ -485,14 +530,16 @@ int tg_layer_norm_backward(int64_t rows, int64_t cols, int type, const void* dy,
             using T = decltype(t);
             const unsigned n = static_cast<unsigned>(blocks);
             if (rows > 0) {
-                if (tg::is_wide(cols))
+                const tg::RowShape shape = tg::row_shape(cols, type);
+                if (!tg::in_registers(shape, type))
                     tg::norm_backward_wide_kernel<T><<<n, tg::kWideThreads, 0, s>>>(a);
-                else if (tg::threads_per_row(cols) == 64)
-                    tg::norm_backward_kernel<T, 64><<<n, 256, 0, s>>>(a);
-                else if (tg::threads_per_row(cols) == 256)
-                    tg::norm_backward_kernel<T, 256><<<n, 256, 0, s>>>(a);
                 else
-                    tg::norm_backward_kernel<T, 1024><<<n, 1024, 0, s>>>(a);
+                    tg::with_row_shape<T>(shape, [&](auto threads, auto items) {
+                        constexpr int TPR = decltype(threads)::value, I = decltype(items)::value;
+                        if constexpr (I * tg::kVec<T> <= tg::kBackwardValues)
+                            tg::norm_backward_kernel<T, TPR, I>
+                                <<<n, TPR > 256 ? TPR : 256, 0, s>>>(a);
+                    });
                 TG_LAUNCH_CHECK();
             }
             if (sums) {
