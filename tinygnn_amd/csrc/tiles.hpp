@@ -261,26 +261,37 @@ __device__ __forceinline__ void part_place(int e, int* major, int* minor) {
     }
 }
 
-template <bool ACROSS, int N>
+// Tile i's address across memory is the first one's with i in the slot's bits.
+// KEEP: the N addresses stay in registers, else each step makes them: whichever
+// leaves room for the sums and two parts' operands (8192^3, w [k x n]: 10
+// registers spilled with them kept, 1129 TFLOP/s against 1393; the weights'
+// gradient: 11 spilled without, 898 against 1283).
+template <bool ACROSS, int N, bool KEEP>
 struct PartReader {
-    int at[ACROSS ? N : 1];
+    static constexpr int kKept = ACROSS && KEEP ? N : 1;
+    int at[kKept];
     __device__ __forceinline__ PartReader(int first, int lane) {
         const int q = lane >> 4, r = lane & 15;
         if constexpr (ACROSS) {
-            const Reader<bf16, 256, true, N> all(first, lane);
+            const Reader<bf16, 256, true, 1> one(first, lane);
 #pragma unroll
-            for (int i = 0; i < N; ++i) at[i] = all.at[i];
+            for (int i = 0; i < kKept; ++i) at[i] = one.at[0] ^ (i * 32);
         } else {
             at[0] = (first + r) * 64 + ((q ^ ((r >> 1) & 3)) << 4);
         }
     }
+    // Before a step's reads.
+    __device__ __forceinline__ void begin() {
+        if constexpr (ACROSS && !KEEP) asm volatile("" : "+v"(at[0]));
+    }
     __device__ __forceinline__ Frag read(const char* lds, int i) const {
         Frag f;
         if constexpr (ACROSS) {
+            const int a = KEEP ? at[KEEP ? i : 0] : at[0] ^ (i * 32);
 #pragma unroll
             for (int h = 0; h < 2; ++h)
                 f.s[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (TG_LDS v4s*)(lds + at[i] + 4 * h * 512));
+                    (TG_LDS v4s*)(lds + a + 4 * h * 512));
         } else {
             f.u = *reinterpret_cast<const v4u*>(lds + at[0] + i * 1024);
         }
@@ -303,7 +314,7 @@ __device__ __forceinline__ void step_border() {
 // loads a thread; zeros from `steps` on), ahead(u) comes before the loads of u ..
 // u + 3; also(w) sees the columns' operands.
 template <typename T, typename RA, typename RB, typename P, typename L, typename W>
-__device__ __forceinline__ void ring(int steps, const RA& ra, const RB& rb, P&& ahead, L&& load,
+__device__ __forceinline__ void ring(int steps, RA& ra, RB& rb, P&& ahead, L&& load,
                                      W&& also, char* a0, char* b0, char* a1, char* b1, char* a2, char* b2,
                                      char* a3, char* b3, v4f (&acc)[8][4]) {
     constexpr int kLoads = 4;
@@ -312,6 +323,8 @@ __device__ __forceinline__ void ring(int steps, const RA& ra, const RB& rb, P&& 
         Frag x[8], w[4];
     };
     auto read = [&](Operands& o, const char* la, const char* lb) {
+        ra.begin();
+        rb.begin();
 #pragma unroll
         for (int j = 0; j < 4; ++j) o.w[j] = rb.read(lb, j);
 #pragma unroll
