@@ -160,6 +160,52 @@ def test_grouped_many_rows_and_groups(gpu):
         within(got, dw, tolerance(dw, dw_size, m, dt), "dw")
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("k,n,gather", [(512, 2048, True), (520, 2056, False), (544, 1544, True),
+                                        (602, 2048, False)])
+def test_grouped_large_tiles(gpu, dtype, k, n, gather):
+    """Sizes that take the 256-wide tiles and, with k or n of no whole chunks,
+    those of 128: contractions that end inside a part, a group of more rows than
+    their starts kept at once (2,048), empty groups, padded rows."""
+    import tinygnn_amd as tg
+    dt, g = DTYPES[dtype], gen(k)
+    sizes = [200 + 7 * (i % 23) for i in range(64)]
+    sizes[3], sizes[5], sizes[40], sizes[63] = 5003, 0, 1, 0
+    m, off = sum(sizes), offsets_of(sizes)
+    x = padded(randn(g, (m // 2 if gather else m, k), dt), 8)
+    rows = None
+    if gather:
+        rows = torch.randint(0, m // 2, (m,), generator=g, device="cuda", dtype=torch.int32)
+        rows[[0, m // 3]] = torch.tensor([m // 2, -1], dtype=torch.int32, device="cuda")
+    dy = padded(randn(g, (m, n), dt), 8)
+    w, bias = randn(g, (64, k, n), dt, k ** -0.5), randn(g, (64, n), dt)
+    want, size = grouped(x, w, off, rows=rows, bias=bias, epi="elu")
+    y = tg.grouped_matmul(x, w, off, rows=rows, bias=bias, epilogue=tg.EPI_ELU)
+    check_y(y, want, size, k, dt)
+    want, size = grouped(dy, w, off, transpose=True)
+    check_y(tg.grouped_matmul(dy, w, off, transpose=True), want, size, n, dt)
+    dw, dw_size, db, db_size = wgrad(x, dy, off, rows=rows)
+    got_w, got_b = tg.grouped_matmul_wgrad(x, dy, off, rows=rows, bias=True)
+    # the longest chain is the largest group's
+    within(got_w, dw, tolerance(dw, dw_size, 5003, dt), "dw")
+    within(got_b, db, tolerance(db, db_size, 5003, dt), "dbias")
+    again = tg.grouped_matmul_wgrad(x, dy, off, rows=rows, bias=True)
+    assert torch.equal(got_w, again[0]) and torch.equal(got_b, again[1])
+
+
+@pytest.mark.parametrize("groups", [None, 3])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_matmul_fp8_large_tiles(gpu, dtype, groups):
+    import tinygnn_amd as tg
+    dt, g, m, k, n = DTYPES[dtype], gen(17), 5003, 300, 8200
+    xq, wq, xv, wv = fp8_operands(g, m, k, n, groups)
+    off = None if groups is None else offsets_of([2000, 0, 3003])
+    want, size = grouped(xv, wv[None] if groups is None else wv,
+                         torch.tensor([0, m]) if off is None else off)
+    got = tg.matmul_fp8(xq, wq, offsets=off, dtype=dt)
+    check_y(got, want, size, k, dt, tolerance_fp8)
+
+
 def test_grouped_bad_offsets_stay_inside(gpu):
     """Falling or outside offsets: only rows within x and y are touched."""
     import tinygnn_amd as tg

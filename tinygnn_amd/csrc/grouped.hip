@@ -461,19 +461,16 @@ constexpr int kRowParts = 64;
 
 // dw on the large tile: both operands run across memory, the contraction over
 // the group's rows.
-template <typename T, bool BIAS>
+template <typename T>
 __global__ __launch_bounds__(kRingThreads) void wgrad_ring_kernel(GroupedArgs a) {
     TG_RING_LDS;
     __shared__ uint32_t row_starts[8 * kRowParts * 4];
     const uint32_t per = a.mt * a.nt;
-    const int part = static_cast<int>(blockIdx.x / per);
+    const int g = static_cast<int>(blockIdx.x / per);
     uint32_t mt, ntile;
     tile_of(blockIdx.x % per, a.mt, a.nt, &mt, &ntile);
-    int g = part, lo, hi;
-    if (a.unit == 0)
-        group_rows(a.offsets, g, a.m, &lo, &hi);
-    else if (!find_tile(a.offsets, a.groups, a.m, a.unit, part, &g, &lo, &hi))
-        return;
+    int lo, hi;
+    group_rows(a.offsets, g, a.m, &lo, &hi);
     lo = __builtin_amdgcn_readfirstlane(lo);
     hi = __builtin_amdgcn_readfirstlane(hi);
     const int k0 = static_cast<int>(mt) * 256, n0 = static_cast<int>(ntile) * 256;
@@ -533,23 +530,42 @@ __global__ __launch_bounds__(kRingThreads) void wgrad_ring_kernel(GroupedArgs a)
             load_to_lds(dbuf, lb + (t * kRingThreads + wave * 64) * 16, bo[t]);
     };
     v4f acc[8][4] = {};
-    v4f sum[BIAS ? 4 : 1] = {};
-    const bool sums = BIAS && mt == 0 && wm == 0;  // uniform
-    const Frag one = ones<T>();
-    PartReader<true, 8, !BIAS> ra(wm, lane);
-    PartReader<true, 4, !BIAS> rb(wn, lane);
+    PartReader<true, 8, true> ra(wm, lane);
+    PartReader<true, 4, true> rb(wn, lane);
     ring<T>((hi - lo + kStep - 1) / kStep, ra, rb, ahead, load,
-            [&](Frag(&w)[4]) {
-                if (BIAS && sums) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) sum[BIAS ? j : 0] = mfma<T>(w[j], one, sum[BIAS ? j : 0]);
-                }
-            },
+            [](Frag(&)[4]) {},
             a0, b0, a1, b1, a2, b2, a3, b3, acc);
-    if (a.dw) store_gradient<T>(a, part, k0 + wm, n0 + wn, lane, acc);
-    if constexpr (BIAS) {
-        if (sums) store_bias_gradient<T>(a, part, n0 + wn, lane, sum);
+    store_gradient<T>(a, g, k0 + wm, n0 + wn, lane, acc);
+}
+
+// dbias beside the large tiles, which have no registers left for it: the rows of
+// a group over 16 wavefronts, 64 chunks of columns, their sums joined in order.
+template <typename T>
+__global__ __launch_bounds__(1024) void column_sums_kernel(GroupedArgs a) {
+    constexpr int VEC = kVec<T>;
+    __shared__ float join[16][64][VEC];
+    const int g = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int lo, hi;
+    group_rows(a.offsets, g, a.m, &lo, &hi);
+    const int64_t c = (static_cast<int64_t>(blockIdx.x) * 64 + lane) * VEC;
+    const T* dy = static_cast<const T*>(a.dy) + c;
+    float s[VEC] = {};
+#pragma unroll 8
+    for (int p = lo + wave; p < hi; p += 16) {
+        float v[VEC];
+        load_floats<T, VEC>(dy + p * a.lddy, a.n - c, v);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s[e] += v[e];
     }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) join[wave][lane][e] = s[e];
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int w = 1; w < 16; ++w)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s[e] += join[w][lane][e];
+    store_floats<T, VEC>(static_cast<T*>(a.dbias) + static_cast<int64_t>(g) * a.n + c, a.n - c, s);
 }
 
 // out[g] = the sum of group g's parts, in order: `size` values each.
@@ -675,7 +691,6 @@ WgradPlan wgrad_plan(int64_t m, int64_t k, int64_t n, int64_t groups, int type, 
         p.edge = 256;
     else if (groups * tiles_of(128) <= 64)
         p.edge = 64;
-    if (const char* ev = getenv("TGE")) p.edge = atoi(ev);
     p.mt = std::max<int64_t>(1, ceil_div(k, p.edge));
     p.nt = ceil_div(n, p.edge);
     p.parts = groups;
@@ -708,9 +723,15 @@ void launch_wgrad(GroupedArgs& a, const WgradPlan& p, bool direct, hipStream_t s
     else if (p.edge == 128)
         tiled(Medium{});
     if constexpr (sizeof(T) == 2) {
-        if (p.edge == 256)
-            a.dbias ? wgrad_ring_kernel<T, true><<<grid, kRingThreads, 0, s>>>(a)
-                    : wgrad_ring_kernel<T, false><<<grid, kRingThreads, 0, s>>>(a);
+        if (p.edge == 256) {
+            wgrad_ring_kernel<T><<<grid, kRingThreads, 0, s>>>(a);
+            TG_LAUNCH_CHECK();
+            if (a.dbias) {
+                const dim3 blocks(static_cast<unsigned>(ceil_div(a.n, 64 * kVec<T>)),
+                                  static_cast<unsigned>(a.groups));
+                column_sums_kernel<T><<<blocks, 1024, 0, s>>>(a);
+            }
+        }
     }
     TG_LAUNCH_CHECK();
     if (!p.unit) return;
