@@ -11,8 +11,8 @@ instructions' own sums come in: 2^-12 sum|a||b|."""
 import pytest
 import torch
 
-from expert_cases import (DTYPES, U, e4m3, gen, grouped, half_step, least, offsets_of, padded, randn,
-                          wgrad, within)
+from expert_cases import (DTYPES, U, e4m3, gen, grouped, half_step, least, offsets_of, padded,
+                          randn, wgrad, within)
 
 pytestmark = pytest.mark.gpu
 

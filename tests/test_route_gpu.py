@@ -131,6 +131,18 @@ def test_route_masks(gpu, dtype, tokens, renorm):
     assert not got[0].any()
 
 
+def test_route_without_a_plan(gpu):
+    """The C entry with no plan asked for; keyword arguments of the front end."""
+    import tinygnn_amd as tg
+    x = randn(gen(2), (300, 20), torch.float32)
+    w, ids, _ = tg.route(logits=x, k=3)
+    w2, ids2 = torch.empty_like(w), torch.empty_like(ids)
+    tg.lib.check(tg.lib.tg_route(300, 20, 3, tg.TYPE_F32, x.data_ptr(), 20, 0, w2.data_ptr(),
+                                 ids2.data_ptr(), None, None, None, None, 0,
+                                 tg.stream_handle()))
+    assert torch.equal(w, w2) and torch.equal(ids, ids2)
+
+
 @pytest.mark.parametrize("n", [1, 63, 64, 65, 8192, 8193, 100_003, 1_200_000])
 @pytest.mark.parametrize("groups", [1, 2, 7, 64, 1000, 1024])
 def test_plan(gpu, n, groups):

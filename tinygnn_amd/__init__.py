@@ -422,20 +422,24 @@ def _refuse(what: str, message: str):
 def _device_call(fn):
     """The first tensor's GPU is the current device for the call."""
     import functools
+    name = fn.__code__.co_varnames[0]
 
     @functools.wraps(fn)
-    def call(first, *args, **kwargs):
+    def call(*args, **kwargs):
         global _pt
         if _pt is None:
             _pt = _Torch()
+        first = args[0] if args else kwargs.get(name)
+        if first is None:
+            return fn(*args, **kwargs)   # Python's own message
         index = getattr(first, "q", first).get_device()
         if index < 0:
             raise ValueError("tinygnn_amd expects device (cuda) tensors")
         cuda = _pt.torch.cuda
         if index != cuda.current_device():
             with cuda.device(index):
-                return fn(first, *args, **kwargs)
-        return fn(first, *args, **kwargs)
+                return fn(*args, **kwargs)
+        return fn(*args, **kwargs)
 
     return call
 
@@ -677,8 +681,8 @@ def route_combine(y, position, weights=None, out=None, stream=None):
 @_device_call
 def route_combine_backward(dout, y, position, weights=None, out=None, stream=None):
     """(dy, dweights) of route_combine (tg_route_combine_backward).  out takes
-    dy; its rows that no position names are left as they are (without out and
-    with fewer places than rows of y: zeros)."""
+    dy; rows of dy that no position names (those in no group of the plan) are
+    not written."""
     what = "route_combine_backward"
     s = _stream_of(what, stream, dout, y, position, weights, out)
     kind = _type_of(what, y)
@@ -692,8 +696,6 @@ def route_combine_backward(dout, y, position, weights=None, out=None, stream=Non
     pd, lddo = _rows_of(what, "dout", dout)
     pw = _flat(what, "weights", weights, position.shape, _pt.f32)
     dy, pdy, lddy = _out(what, "out", out, y.shape, y, y.dtype)
-    if out is None and tokens * k != rows:
-        dy.zero_()
     dw = _pt.empty((tokens, k), dtype=_pt.f32, device=y.device)
     lib.check(lib.tg_route_combine_backward(tokens, k, cols, kind, pd, lddo, py, rows, ldy, pp,
                                             pw, pdy, lddy, dw.data_ptr(), s))

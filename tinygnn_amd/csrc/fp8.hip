@@ -195,13 +195,14 @@ __device__ __forceinline__ void store_outputs(const Fp8Args& a, int p, int n, co
 template <typename T, typename S>
 __global__ __launch_bounds__(S::kThreads) void fp8_kernel(Fp8Args a) {
     constexpr int kScales = S::kM * kRowBytes;  // behind x's tile
-    __shared__ __attribute__((aligned(16))) char a0[kScales + S::kM * 4];
+    __shared__ __attribute__((aligned(16))) char a0[kScales + S::kThreads * 4];
     __shared__ __attribute__((aligned(16))) char b0[S::kN * kRowBytes];
-    __shared__ __attribute__((aligned(16))) char a1[kScales + S::kM * 4];
+    __shared__ __attribute__((aligned(16))) char a1[kScales + S::kThreads * 4];
     __shared__ __attribute__((aligned(16))) char b1[S::kN * kRowBytes];
     constexpr bool WIDE = sizeof(T) == 4;
     uint32_t mt, ntile;
-    if (!tile_of(blockIdx.x, count_tiles(a.offsets, a.groups, a.m, S::kM), a.nt, &mt, &ntile)) return;
+    if (!tile_of(blockIdx.x, count_tiles(a.offsets, a.groups, a.m, S::kM), a.nt, &mt, &ntile))
+        return;
     int g, r0, r1;
     if (!find_tile(a.offsets, a.groups, a.m, S::kM, static_cast<int>(mt), &g, &r0, &r1)) return;
     const int n0 = static_cast<int>(ntile) * S::kN;
@@ -210,7 +211,7 @@ __global__ __launch_bounds__(S::kThreads) void fp8_kernel(Fp8Args a) {
     const int wm = wave / S::kWC * S::kMI * 16, wn = wave % S::kWC * S::kNJ * 16;
     const int64_t kp = static_cast<int64_t>(a.kb) * kBlock;
     const uint8_t* w = a.wq + static_cast<int64_t>(g) * a.n * kp;
-    static_assert(S::kNJ * 16 <= kBlock && kBlock % (S::kNJ * 16) == 0, "one scale of w a wavefront");
+    static_assert(kBlock % (S::kNJ * 16) == 0, "one scale of w a wavefront");
     const int nb = (a.n + kBlock - 1) / kBlock;
     const int wblock = (n0 + wn) / kBlock < nb ? (n0 + wn) / kBlock : nb - 1;
     const float* ws = a.wscale + (static_cast<int64_t>(g) * nb + wblock) * a.kb;
@@ -233,77 +234,96 @@ __global__ __launch_bounds__(S::kThreads) void fp8_kernel(Fp8Args a) {
         chunk_place<uint8_t, S::kN, false>(t * S::kThreads + tid, &col, &c);
         bo[t] = n0 + col < a.n ? static_cast<uint32_t>(col * kp + c) : kOutside;
     }
-    // one row's scale for each thread of the first wavefronts; outside: 0
+    // one row's scale for each thread; outside, and of threads past the rows: 0
     uint32_t so = kOutside;
     if (tid < S::kM && r0 + tid < r1) {
         const int src = source_row(a, r0 + tid);
         if (src >= 0) so = static_cast<uint32_t>(src) * 4;
     }
-    auto load = [&](int kt, char* la, char* lb) {
-        const auto xbuf = buffer_of(xb + static_cast<int64_t>(kt) * kBlock, kDirectBytes);
-        const auto wbuf = buffer_of(wb + static_cast<int64_t>(kt) * kBlock, kDirectBytes);
-        if (wave * 64 < S::kM)
+    // load p of tile kt (zeros past the last tile)
+    constexpr int kLoads = 1 + S::kCA + S::kCB;
+    auto load = [&](int kt, char* la, char* lb, int p) {
+        const int64_t size = kt < a.kb ? kDirectBytes : 0;
+        const int64_t at = static_cast<int64_t>(kt) * kBlock;
+        if (p == 0) {
+            const float* xs = a.xscale + static_cast<int64_t>(kt) * a.x_rows;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                buffer_of(a.xscale + static_cast<int64_t>(kt) * a.x_rows, 4 * a.x_rows),
+                buffer_of(xs, kt < a.kb ? 4 * a.x_rows : 0),
                 (TG_LDS void*)(la + kScales + wave * 256), 4, static_cast<int>(so), 0, 0, 0);
-#pragma unroll
-        for (int t = 0; t < S::kCA; ++t)
-            load_to_lds(xbuf, la + (t * S::kThreads + wave * 64) * 16, ao[t]);
-#pragma unroll
-        for (int t = 0; t < S::kCB; ++t)
-            load_to_lds(wbuf, lb + (t * S::kThreads + wave * 64) * 16, bo[t]);
+        } else if (p <= S::kCA) {
+            load_to_lds(buffer_of(xb + at, size), la + ((p - 1) * S::kThreads + wave * 64) * 16,
+                        ao[p - 1]);
+        } else {
+            const int t = p - 1 - S::kCA;
+            load_to_lds(buffer_of(wb + at, size), lb + (t * S::kThreads + wave * 64) * 16, bo[t]);
+        }
     };
     Acc<S> acc = {};
     const Reader<uint8_t, S::kM, false, S::kMI> ra(wm, lane);
     const Reader<uint8_t, S::kN, false, S::kNJ> rb(wn, lane);
     int kt = 0;
-    auto compute = [&](const char* la, const char* lb) {
+    // the products of the tile in la and lb, the next one's loads among them
+    auto compute = [&](const char* la, const char* lb, char* na, char* nb) {
         const float scale = scalar_load(ws + kt++);
         const float* xs = reinterpret_cast<const float*>(la + kScales) + wm + r;
-        // kHalf columns' tiles at a time; while row tile i's products run, x's
-        // operands of i + 1 are read and the products of i - 1 scaled and added.
-        // No more than that may be live (registers; x's operands are read again
-        // for the other half).
-        constexpr int kHalf = S::kNJ;
+        // While row tile i's products run, x's operands of i + 1 are read, the
+        // products of i - 1 scaled and added, and a share of the next tile's loads
+        // asked for (asked for at once, they held the reads and the first products
+        // back: 8,192 x 4,096 x 8,192 330 us against 301).  No more than that may
+        // be live (registers).
         auto row_tile = [&](int i) {
             Operand x;
 #pragma unroll
             for (int s = 0; s < 2; ++s) x.c[s] = ra.read(la, i, s);
             return x;
         };
+        Operand b[S::kNJ], x[2];
 #pragma unroll
-        for (int h = 0; h < S::kNJ / kHalf; ++h) {
-            Operand b[kHalf], x[2];
+        for (int j = 0; j < S::kNJ; ++j)
 #pragma unroll
-            for (int j = 0; j < kHalf; ++j)
+            for (int s = 0; s < 2; ++s) b[j].c[s] = rb.read(lb, j, s);
+        x[0] = row_tile(0);
+        v4f part[2][S::kNJ];
 #pragma unroll
-                for (int s = 0; s < 2; ++s) b[j].c[s] = rb.read(lb, h * kHalf + j, s);
-            x[0] = row_tile(0);
-            v4f part[2][kHalf];
+        for (int i = 0; i <= S::kMI; ++i) {
+            if (i + 1 < S::kMI) x[(i + 1) & 1] = row_tile(i + 1);
+            if (i < S::kMI) {
 #pragma unroll
-            for (int i = 0; i <= S::kMI; ++i) {
-                if (i + 1 < S::kMI) x[(i + 1) & 1] = row_tile(i + 1);
-                if (i < S::kMI) {
+                for (int j = 0; j < S::kNJ; ++j)
+                    part[i & 1][j] = block_products<WIDE>(b[j], x[i & 1]);
 #pragma unroll
-                    for (int j = 0; j < kHalf; ++j)
-                        part[i & 1][j] = block_products<WIDE>(b[j], x[i & 1]);
-                }
-                if (i > 0) {
-                    const float f = xs[(i - 1) * 16] * scale;
-#pragma unroll
-                    for (int j = 0; j < kHalf; ++j) {
-                        v4f& sum = acc[i - 1][h * kHalf + j];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            sum[e] = __builtin_fmaf(part[(i - 1) & 1][j][e], f, sum[e]);
-                        asm volatile("" : "+v"(sum));  // here, not at the tile's end
-                    }
-                }
-                __builtin_amdgcn_sched_barrier(0);
+                for (int p = i * kLoads / S::kMI; p < (i + 1) * kLoads / S::kMI; ++p)
+                    load(kt, na, nb, p);
             }
+            if (i > 0) {
+                const float f = xs[(i - 1) * 16] * scale;
+#pragma unroll
+                for (int j = 0; j < S::kNJ; ++j) {
+                    v4f& sum = acc[i - 1][j];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        sum[e] = __builtin_fmaf(part[(i - 1) & 1][j][e], f, sum[e]);
+                    asm volatile("" : "+v"(sum));  // here, not at the tile's end
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
-    pipeline<true>(a.kb, a0, b0, a1, b1, load, [](char*, char*) {}, compute);
+    if (a.kb > 0) {
+#pragma unroll
+        for (int p = 0; p < kLoads; ++p) load(0, a0, b0, p);
+    }
+    while (kt + 1 < a.kb) {  // compute() counts
+        __syncthreads();
+        compute(a0, b0, a1, b1);
+        __syncthreads();
+        compute(a1, b1, a0, b0);
+    }
+    if (kt < a.kb) {
+        __syncthreads();
+        compute(a0, b0, a1, b1);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     v4f bias[S::kNJ];
 #pragma unroll
     for (int j = 0; j < S::kNJ; ++j) bias[j] = bias_of<T>(a, g, n0 + wn + j * 16 + 4 * q);
@@ -408,17 +428,18 @@ void launch_fp8(Fp8Args& a, hipStream_t s) {
         return most_tiles(a.m, a.groups, edge) * ceil_div(a.n, edge);
     };
     // Few rows: the thin form while its workgroups are few (5 rows of 4,096 x
-    // 4,096 7.6 us; 150 rows of 32 groups 46 us against 23).  Large tiles where
-    // they fill the CUs at least twice and the groups do (8,192 x 4,096 x 8,192
-    // 314 us against 389; 10,000 x 1,024 x 512 19 against 13), 128 x 128 where
-    // those do once (10,000 rows 13 against 15), else 64 x 64 (600 x 2,048 x
-    // 1,024 12 against 18).
+    // 4,096 7.6 us, 12 in 64 x 64; 150 rows of 32 groups, 2,048 x 4,096, 62 us
+    // against 41).  Large tiles where there are 160 of them of 1,024 values and the
+    // groups fill them (2,500 x 2,048 x 4,096 40 us against 47; 40,000 x 512 x 512
+    // 36 against 32), 128 x 128 where there are one for each CU (10,000 x 512 x
+    // 512 the same as 64 x 64, 10,000 x 2,048 x 4,096 126 us against 177), else 64
+    // x 64 (600 x 2,048 x 1,024 12 us against 18).
     if (!fits || tiles(16) <= 1024) {
         const unsigned grid = set_grid(a, 16, 16);
         fp8_thin_kernel<T><<<grid, 64 * kThinWaves, 0, s>>>(a);
-    } else if (tiles(256) >= 600 && a.m >= 256 * a.groups) {
+    } else if (a.kb >= 8 && tiles(256) * a.kb >= 160 * 8 && a.m >= 256 * a.groups) {
         tiled(Large{});
-    } else if (tiles(128) >= 256 && a.m >= 100 * a.groups) {
+    } else if (tiles(128) >= 300 && a.m >= 100 * a.groups) {
         tiled(Medium{});
     } else {
         tiled(Small{});

@@ -117,12 +117,13 @@ __device__ __forceinline__ void store_bias_gradient(const GroupedArgs& a, int pa
 }
 
 // ---------------------------------------------------------------------------
-// BM x BN outputs by WR x WC wavefronts, two tiles of both operands in LDS: while the matrix instructions read one, the other is loaded.
-// The wavefront's outputs are computed transposed (columns of w as the rows of
-// the instruction), so a lane holds four consecutive columns of y.
+// BM x BN outputs by WR x WC wavefronts, two tiles of both operands in LDS: while
+// the matrix instructions read one, the other is loaded.  The wavefront's outputs
+// are computed transposed (columns of w as the rows of the instruction), so a
+// lane holds four consecutive columns of y.
 //
 // DIRECT: the tiles come by loads that write to LDS; else through registers,
-// for operands that are not 16-byte aligned or reach past 2 GB.
+// for 16-bit operands of odd rows or places and those that reach past 2 GB.
 // ---------------------------------------------------------------------------
 // The products of one tile pair.
 template <typename T, typename S, typename RA, typename RB>
@@ -150,7 +151,8 @@ __global__ __launch_bounds__(S::kThreads) void grouped_kernel(GroupedArgs a) {
     __shared__ __attribute__((aligned(16))) char b1[S::kN * kRowBytes];
     constexpr int Z = sizeof(T);
     uint32_t mt, ntile;
-    if (!tile_of(blockIdx.x, count_tiles(a.offsets, a.groups, a.m, S::kM), a.nt, &mt, &ntile)) return;
+    if (!tile_of(blockIdx.x, count_tiles(a.offsets, a.groups, a.m, S::kM), a.nt, &mt, &ntile))
+        return;
     int g, r0, r1;
     if (!find_tile(a.offsets, a.groups, a.m, S::kM, static_cast<int>(mt), &g, &r0, &r1)) return;
     const int n0 = static_cast<int>(ntile) * S::kN;
@@ -666,9 +668,14 @@ void launch_ring(GroupedArgs& a, bool along, hipStream_t s) {
 // x 4,096 375 us against 459 of edge 128; 10,000 rows of 8 groups 122 against
 // 113), 64 where the groups make few tiles (40,000 x 512 x 512 52 us against
 // 69; in 8 groups 88 against 67).
+// In fp32, whose digits the result keeps, no chain is longer than kLongChain
+// rows.
+constexpr int64_t kLongChain = 16384;
+
 struct WgradPlan {
     int64_t edge, mt, nt, unit, parts;  // parts: most of them
-    size_t bytes(int64_t k, int64_t n, float** part, float** part_bias, void* ws, size_t size) const {
+    size_t bytes(int64_t k, int64_t n, float** part, float** part_bias, void* ws,
+                 size_t size) const {
         Carver c(ws, size);
         if (unit == 0) return 0;
         float* p = c.take<float>(static_cast<size_t>(parts * k * n));
@@ -695,8 +702,11 @@ WgradPlan wgrad_plan(int64_t m, int64_t k, int64_t n, int64_t groups, int type, 
     p.nt = ceil_div(n, p.edge);
     p.parts = groups;
     const int64_t tiles = p.mt * p.nt;
-    if (tiles * groups >= 512 || m < 1024) return p;
-    const int64_t unit = std::max<int64_t>(512, ceil_div(ceil_div(m * tiles, 1024), 64) * 64);
+    int64_t unit = std::max<int64_t>(512, ceil_div(ceil_div(m * tiles, 1024), 64) * 64);
+    if (tiles * groups >= 512 || m < 1024) {
+        if (type != TG_TYPE_F32 || m <= kLongChain) return p;
+        unit = kLongChain;
+    }
     if (unit >= m) return p;
     p.unit = unit;
     p.parts = most_tiles(m, groups, unit);

@@ -13,7 +13,7 @@
 // (four rows a workgroup, no barrier) to 1,024, then by 1,024 with two or four
 // loads each, up to 16,384 columns: few registers, so many wavefronts a SIMD (16
 // values a thread kept the backward pass at two of them: 16,384 x 4,096 bf16 170
-// us against RESULT).  Wider rows are walked by 1,024 threads, out of L2 after the
+// us against 105).  Wider rows are walked by 1,024 threads, out of L2 after the
 // first time.
 #include "common.hpp"
 #include "device_utils.hpp"

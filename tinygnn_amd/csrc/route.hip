@@ -8,7 +8,7 @@
 // then the lower column (32 bits for 16-bit logits, 64 for floats).  A lane sorts
 // its keys once; each of the k rounds is one maximum over the lanes' heads, whose
 // lane drops its own.  (A search by the lane that lost its largest value, in each
-// round, took 45 us of 65,536 rows of 128 and 8 places; RESULT now.)
+// round, took 46 us of 65,536 rows of 128 and 8 places; 31 now.)
 //
 // Order.  A stable counting sort of the slots by expert: workgroup b counts its
 // share of the slots (in the top-k kernel, whose rows they are), then places
@@ -400,7 +400,8 @@ __global__ __launch_bounds__(kSortThreads) void plan_count_kernel(PlanArgs p, in
     __syncthreads();
     const int64_t s0 = static_cast<int64_t>(blockIdx.x) * p.share;
     const int64_t s1 = s0 + p.share < p.slots ? s0 + p.share : p.slots;
-    for (int64_t s = s0 + threadIdx.x; s < s1; s += kSortThreads) atomicAdd(&lds[group_of(p, s)], 1);
+    for (int64_t s = s0 + threadIdx.x; s < s1; s += kSortThreads)
+        atomicAdd(&lds[group_of(p, s)], 1);
     __syncthreads();
     for (int e = threadIdx.x; e < n; e += kSortThreads)
         counts[static_cast<int64_t>(blockIdx.x) * n + e] = lds[e];
@@ -487,9 +488,9 @@ struct CombineArgs {
     int64_t ldy;
     const int32_t* position;
     const float* weights;
-    void* out;  // forward: out; backward: dout is `y`'s reader below
+    void* out;
     int64_t ldo;
-    const void* dout;
+    const void* dout;  // backward
     int64_t lddo;
     void* dy;
     int64_t lddy;
@@ -596,12 +597,12 @@ void check_route(const char* what, int64_t tokens, int64_t experts, int64_t k, i
                                                             std::to_string(type));
 }
 
-// Workgroups of a plan of n slots in units of k.
-int64_t plan_blocks(int64_t n, int64_t k, int64_t least) {
-    return std::min(kSortBlocks, ceil_div(n / k, least));
-}
+// Workgroups that n rows or slots go to, `least` each at least.
+int64_t plan_blocks(int64_t n, int64_t least) { return std::min(kSortBlocks, ceil_div(n, least)); }
 
-bool one_route(int64_t tokens, int64_t k) { return tokens <= kOneTokens && tokens * k <= kOneSlots; }
+bool one_route(int64_t tokens, int64_t k) {
+    return tokens <= kOneTokens && tokens * k <= kOneSlots;
+}
 
 size_t counts_bytes(int64_t blocks, int64_t groups) {
     Carver c(nullptr, 0);
@@ -610,7 +611,7 @@ size_t counts_bytes(int64_t blocks, int64_t groups) {
 }
 
 // Workgroups that route `tokens` rows: 64 rows each at least.
-int64_t route_blocks(int64_t tokens) { return plan_blocks(tokens, 1, 64); }
+int64_t route_blocks(int64_t tokens) { return plan_blocks(tokens, 64); }
 
 }  // namespace
 }  // namespace tg
@@ -699,7 +700,7 @@ int tg_route(int64_t tokens, int64_t experts, int64_t k, int type, const void* l
 
 size_t tg_route_plan_workspace_size(int64_t n, int64_t groups) {
     if (n <= tg::kOneSlots || groups <= 0) return 0;
-    return tg::counts_bytes(tg::plan_blocks(n, 1, 4096), groups);
+    return tg::counts_bytes(tg::plan_blocks(n, 4096), groups);
 }
 
 int tg_route_plan(int64_t n, int64_t groups, int64_t k, const int32_t* ids, int32_t* offsets,
@@ -728,7 +729,7 @@ int tg_route_plan(int64_t n, int64_t groups, int64_t k, const int32_t* ids, int3
         p.blocks = 1;
         tg::TempBuffer temp;
         if (n > tg::kOneSlots) {
-            p.share = tg::ceil_div(n, tg::plan_blocks(n, 1, 4096));
+            p.share = tg::ceil_div(n, tg::plan_blocks(n, 4096));
             p.blocks = static_cast<int>(tg::ceil_div(n, p.share));
             const size_t need = tg::counts_bytes(p.blocks, groups);
             if (!workspace) {

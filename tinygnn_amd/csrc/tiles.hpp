@@ -315,8 +315,8 @@ __device__ __forceinline__ void step_border() {
 // u + 3; also(w) sees the columns' operands.
 template <typename T, typename RA, typename RB, typename P, typename L, typename W>
 __device__ __forceinline__ void ring(int steps, RA& ra, RB& rb, P&& ahead, L&& load,
-                                     W&& also, char* a0, char* b0, char* a1, char* b1, char* a2, char* b2,
-                                     char* a3, char* b3, v4f (&acc)[8][4]) {
+                                     W&& also, char* a0, char* b0, char* a1, char* b1, char* a2,
+                                     char* b2, char* a3, char* b3, v4f (&acc)[8][4]) {
     constexpr int kLoads = 4;
     if (steps == 0) return;
     struct Operands {
