@@ -424,8 +424,8 @@ int tg_route_combine_backward(int64_t tokens, int64_t k, int64_t cols, int type,
  * bias [groups x n] or NULL; epilogue TG_EPI_*.  x, w, bias and y have `type`;
  * sums are in fp32 and rounded once.  offsets: groups + 1 int32 on the device,
  * not falling, within [0, m]; rows outside all groups are not written (of a
- * falling or outside offset, only rows within [0, m) are ever touched).  At
- * most 1,024 groups; m < 2^31.
+ * falling or outside offset, only rows within [0, m) are ever touched).  y
+ * overlaps no input.  At most 1,024 groups; m, k, n < 2^31 - 4096.
  *
  * tg_grouped_matmul_wgrad: dw_g = (rows of x of group g)^T * (those of dy),
  * [groups x k x n] contiguous, and dbias_g = sum of those rows of dy

@@ -37,7 +37,8 @@ def check_y(got, want, size, k, dt, tol=tolerance):
     within(got[inside], want[inside], tol(want, size, k, dt)[inside], "y")
 
 
-SIZES = [[1], [0, 5, 0], [3, 0, 70, 1], [64, 64, 128], [17, 33, 200, 0, 1, 0], [300], [129, 255, 257]]
+SIZES = [[1], [0, 5, 0], [3, 0, 70, 1], [64, 64, 128], [17, 33, 200, 0, 1, 0], [300],
+         [129, 255, 257]]
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
@@ -317,3 +318,38 @@ def test_matmul_fp8_empty(gpu):
     x, w = torch.empty(3, 0, device="cuda"), torch.empty(0, 7, device="cuda")
     y = tg.matmul_fp8(tg.quantize(x), tg.quantize_weight(w), bias=torch.ones(7, device="cuda"))
     assert bool((y == 1).all())
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_grouped_wgrad_whole_and_cut_groups(gpu, dtype):
+    """Groups of no row, of few and of many: some are cut to parts of rows,
+    some are one part; each group's tolerance counts its own rows."""
+    import tinygnn_amd as tg
+    dt = DTYPES[dtype]
+    sizes = [9000, 0, 1, 40, 9001, 513, 0]
+    off = offsets_of(sizes)
+    g = gen(11)
+    x, dy = randn(g, (sum(sizes), 70), dt), randn(g, (sum(sizes), 66), dt)
+    dw, db = tg.grouped_matmul_wgrad(x, dy, off, bias=True)
+    assert tg.lib.tg_grouped_matmul_wgrad_workspace_size(sum(sizes), 70, 66, len(sizes),
+                                                         tg.TYPE_F32) > 0
+    want_w, size_w, want_b, size_b = wgrad(x, dy, off)
+    n = torch.tensor(sizes, device="cuda").double()
+    within(dw, want_w, tolerance(want_w, size_w, n[:, None, None], dt), "dw")
+    within(db, want_b, tolerance(want_b, size_b, n[:, None], dt), "dbias")
+
+
+def test_grouped_wgrad_bias_only(gpu):
+    """The C entry with dw NULL, in a workspace of the size asked for."""
+    import tinygnn_amd as tg
+    m, k, n, groups = 40000, 1024, 512, 64
+    off = torch.linspace(0, m, groups + 1, device="cuda").int()
+    dy = randn(gen(3), (m, n), torch.float32)
+    size = tg.lib.tg_grouped_matmul_wgrad_workspace_size(m, k, n, groups, tg.TYPE_F32)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    db = torch.empty(groups, n, device="cuda")
+    tg.lib.check(tg.lib.tg_grouped_matmul_wgrad(
+        m, k, n, groups, tg.TYPE_F32, None, m, k, None, dy.data_ptr(), n, off.data_ptr(), None,
+        db.data_ptr(), ws.data_ptr(), size, tg.stream_handle()))
+    _, _, want, bound = wgrad(dy[:, :1], dy, off)
+    within(db, want, tolerance(want, bound, m // groups, torch.float32), "dbias")

@@ -79,8 +79,8 @@ __device__ __forceinline__ void store_outputs(const GroupedArgs& a, int g, int p
 
 // A wavefront's sums of dw from row k0, column n0 on: of group (or part) `part`.
 template <typename T, int MI, int NJ>
-__device__ __forceinline__ void store_gradient(const GroupedArgs& a, int part, int k0, int n0,
-                                               int lane, const v4f (&acc)[MI][NJ]) {
+__device__ __forceinline__ void store_gradient(const GroupedArgs& a, bool split, int part, int k0,
+                                               int n0, int lane, const v4f (&acc)[MI][NJ]) {
     const int q = lane >> 4, r = lane & 15;
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
@@ -91,7 +91,7 @@ __device__ __forceinline__ void store_gradient(const GroupedArgs& a, int part, i
         for (int j = 0; j < NJ; ++j) {
             const int n = n0 + j * 16 + 4 * q;
             const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-            if (a.unit)
+            if (split)
                 store_floats<float, 4>(a.part + row + n, a.n - n, v);
             else
                 store_floats<T, 4>(static_cast<T*>(a.dw) + row + n, a.n - n, v);
@@ -100,8 +100,8 @@ __device__ __forceinline__ void store_gradient(const GroupedArgs& a, int part, i
 }
 
 template <typename T, int NJ>
-__device__ __forceinline__ void store_bias_gradient(const GroupedArgs& a, int part, int n0,
-                                                    int lane, const v4f (&sum)[NJ]) {
+__device__ __forceinline__ void store_bias_gradient(const GroupedArgs& a, bool split, int part,
+                                                    int n0, int lane, const v4f (&sum)[NJ]) {
     const int q = lane >> 4, r = lane & 15;
     if (r != 0) return;
     const int64_t row = static_cast<int64_t>(part) * a.n;
@@ -109,7 +109,7 @@ __device__ __forceinline__ void store_bias_gradient(const GroupedArgs& a, int pa
     for (int j = 0; j < NJ; ++j) {
         const int n = n0 + j * 16 + 4 * q;
         const float v[4] = {sum[j][0], sum[j][1], sum[j][2], sum[j][3]};
-        if (a.unit)
+        if (split)
             store_floats<float, 4>(a.part_bias + row + n, a.n - n, v);
         else
             store_floats<T, 4>(static_cast<T*>(a.dbias) + row + n, a.n - n, v);
@@ -324,8 +324,7 @@ __global__ __launch_bounds__(kRingThreads) void grouped_ring_kernel(GroupedArgs 
     v4f acc[8][4] = {};
     PartReader<false, 8, true> ra(wm, lane);
     PartReader<!ALONG_W, 4, false> rb(wn, lane);
-    ring<T>((a.k + kStep - 1) / kStep, ra, rb, [](int) {}, load, [](Frag(&)[4]) {},
-            a0, b0, a1, b1, a2, b2, a3, b3, acc);
+    ring<T>((a.k + kStep - 1) / kStep, ra, rb, [](int) {}, load, a0, b0, a1, b1, a2, b2, a3, b3, acc);
     store_outputs<T>(a, g, r0 + wm, r1, n0 + wn, lane, acc);
 }
 
@@ -455,8 +454,13 @@ __global__ __launch_bounds__(S::kThreads) void wgrad_kernel(GroupedArgs a) {
         pipeline<false>(tiles, a0, b0, a1, b1, load, store, compute);
     }
 
-    if (a.dw) store_gradient<T>(a, part, k0 + wm, n0 + wn, lane, acc);
-    if (BIAS && sums) store_bias_gradient<T>(a, part, n0 + wn, lane, sum);
+    // (a group that is one part goes straight to dw)
+    int first = lo, last = hi;
+    if (a.unit) group_rows(a.offsets, g, a.m, &first, &last);
+    const bool split = lo != first || hi != last;
+    const int to = split ? part : g;
+    if (a.dw) store_gradient<T>(a, split, to, k0 + wm, n0 + wn, lane, acc);
+    if (BIAS && sums) store_bias_gradient<T>(a, split, to, n0 + wn, lane, sum);
 }
 
 constexpr int kRowParts = 64;
@@ -534,10 +538,8 @@ __global__ __launch_bounds__(kRingThreads) void wgrad_ring_kernel(GroupedArgs a)
     v4f acc[8][4] = {};
     PartReader<true, 8, true> ra(wm, lane);
     PartReader<true, 4, true> rb(wn, lane);
-    ring<T>((hi - lo + kStep - 1) / kStep, ra, rb, ahead, load,
-            [](Frag(&)[4]) {},
-            a0, b0, a1, b1, a2, b2, a3, b3, acc);
-    store_gradient<T>(a, g, k0 + wm, n0 + wn, lane, acc);
+    ring<T>((hi - lo + kStep - 1) / kStep, ra, rb, ahead, load, a0, b0, a1, b1, a2, b2, a3, b3, acc);
+    store_gradient<T>(a, false, g, k0 + wm, n0 + wn, lane, acc);
 }
 
 // dbias beside the large tiles, which have no registers left for it: the rows of
@@ -570,7 +572,8 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(GroupedArgs a) {
     store_floats<T, VEC>(static_cast<T*>(a.dbias) + static_cast<int64_t>(g) * a.n + c, a.n - c, s);
 }
 
-// out[g] = the sum of group g's parts, in order: `size` values each.
+// out[g] = the sum of group g's parts, in order: `size` values each; zeros of no
+// part.
 template <typename T>
 __global__ __launch_bounds__(256) void parts_kernel(const int32_t* __restrict__ offsets, int m,
                                                     int unit, int most,
@@ -582,13 +585,14 @@ __global__ __launch_bounds__(256) void parts_kernel(const int32_t* __restrict__ 
         int n = 0;
         if (base + lane < g) {
             group_rows(offsets, base + lane, m, &lo, &hi);
-            n = (hi - lo + unit - 1) / unit;
+            n = static_cast<int>((static_cast<int64_t>(hi) - lo + unit - 1) / unit);
         }
         first += wave_sum(n);
     }
     group_rows(offsets, g, m, &lo, &hi);
     // (falling offsets may name more parts than there are)
-    int parts = (hi - lo + unit - 1) / unit;
+    int parts = static_cast<int>((static_cast<int64_t>(hi) - lo + unit - 1) / unit);
+    if (parts == 1) return;  // it is there
     parts = parts < most - first ? parts : most - first;
     const int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
     if (at >= size) return;
@@ -836,11 +840,13 @@ int tg_grouped_matmul(int64_t m, int64_t k, int64_t n, int64_t groups, int type,
 size_t tg_grouped_matmul_wgrad_workspace_size(int64_t m, int64_t k, int64_t n, int64_t groups,
                                               int type) {
     if (m <= 0 || k < 0 || n <= 0 || groups <= 0 || groups > tg::kMaxGroups) return 0;
-    // either tile: which one depends on the operands' alignment
+    // either tile (which one depends on the operands' alignment)
+    // and k is 0 where only dbias is wanted
     size_t most = 0;
     for (const bool direct : {false, true})
-        most = std::max(most, tg::wgrad_plan(m, k, n, groups, type, direct)
-                                  .bytes(k, n, nullptr, nullptr, nullptr, 0));
+        for (const int64_t d : {k, int64_t(0)})
+            most = std::max(most, tg::wgrad_plan(m, d, n, groups, type, direct)
+                                      .bytes(d, n, nullptr, nullptr, nullptr, 0));
     return most;
 }
 

@@ -312,11 +312,11 @@ __device__ __forceinline__ void step_border() {
 
 // acc += the products of `steps` parts; load(u, la, lb) asks for part u (four
 // loads a thread; zeros from `steps` on), ahead(u) comes before the loads of u ..
-// u + 3; also(w) sees the columns' operands.
-template <typename T, typename RA, typename RB, typename P, typename L, typename W>
-__device__ __forceinline__ void ring(int steps, RA& ra, RB& rb, P&& ahead, L&& load,
-                                     W&& also, char* a0, char* b0, char* a1, char* b1, char* a2,
-                                     char* b2, char* a3, char* b3, v4f (&acc)[8][4]) {
+// u + 3.
+template <typename T, typename RA, typename RB, typename P, typename L>
+__device__ __forceinline__ void ring(int steps, RA& ra, RB& rb, P&& ahead, L&& load, char* a0,
+                                     char* b0, char* a1, char* b1, char* a2, char* b2, char* a3,
+                                     char* b3, v4f (&acc)[8][4]) {
     constexpr int kLoads = 4;
     if (steps == 0) return;
     struct Operands {
@@ -340,7 +340,6 @@ __device__ __forceinline__ void ring(int steps, RA& ra, RB& rb, P&& ahead, L&& l
         for (int i = 0; i < 8; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[i][j] = mfma<T>(now.w[j], now.x[i], acc[i][j]);
-        also(now.w);
         // An LDS read beside each of the first matrix instructions, then a load
         // beside every fourth: the reads have the rest of the step to arrive
         // (left to itself, the compiler puts them last, where the border waits
