@@ -89,6 +89,30 @@ def test_layer(gpu, dtype, share):
         within(got[name], v, share * v.abs().max(), name)
 
 
+def test_layer_gradients_by_differences(gpu):
+    """Each gradient g along its own direction against central differences of
+    the plain forward pass in 64 bits.  Steps of 1e-6: the row of equal values
+    has rstd 316, (316e-6)^2 < 1e-6 of the slope is left, and roundings of 2^-53
+    of a sum of size 1e3 over 2e-6 less.  An error of `share` of the largest
+    value in each of N places changes g's length by share * largest * sqrt(N)
+    at most."""
+    import tinygnn_amd as tg
+    p, step, share = inputs(torch.float32), 1e-6, 2e-5
+    got = forward_backward(tg, p)
+    base = {k: v.double() for k, v in p.items()}
+    for name in ("x", "gamma", "beta", "router", "w1", "b1", "w2"):
+        g = got["d" + name].double()
+
+        def loss(s):
+            moved = {k: v.clone() for k, v in base.items()}
+            moved[name] += s / g.norm() * g
+            return (reference(moved, got["experts"], got["on"])["out"] * base["dout"]).sum()
+
+        want = ((loss(step) - loss(-step)) / (2 * step)).item()
+        tol = share * g.abs().max().item() * g.numel() ** 0.5 + 1e-6 * (1 + abs(want))
+        assert abs(g.norm().item() - want) <= tol, (name, g.norm().item(), want, tol)
+
+
 def test_layer_on_another_stream(gpu):
     """Inputs are finished; results of a stream that is not the current one are
     read at once."""

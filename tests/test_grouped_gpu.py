@@ -353,3 +353,32 @@ def test_grouped_wgrad_bias_only(gpu):
         db.data_ptr(), ws.data_ptr(), size, tg.stream_handle()))
     _, _, want, bound = wgrad(dy[:, :1], dy, off)
     within(db, want, tolerance(want, bound, m // groups, torch.float32), "dbias")
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("far", [False, True])
+def test_grouped_many_wide_tiles(gpu, dtype, far):
+    """Tiles enough for the wider shapes; far: gathered from rows whose places
+    pass 2^31 bytes."""
+    import tinygnn_amd as tg
+    dt, g = DTYPES[dtype], gen(5)
+    sizes, k, n = [20000, 0, 1, 22999, 300], 38, 100
+    m, off = sum(sizes), offsets_of(sizes)
+    lead = 2 ** 34 // torch.finfo(dt).bits // m + 200 if far else 40
+    x = torch.empty(m, lead, dtype=dt, device="cuda")[:, :k]
+    x.copy_(randn(g, (m, k), dt))
+    rows = torch.randperm(m, generator=g, device="cuda").int()
+    rows[5], rows[-1] = -1, m
+    w, bias = randn(g, (len(sizes), k, n), dt, k ** -0.5), randn(g, (len(sizes), n), dt)
+    want, size = grouped(x, w, off, rows=rows, bias=bias, epi="elu")
+    got = tg.grouped_matmul(x, w, off, rows=rows, bias=bias, epilogue=tg.EPI_ELU)
+    check_y(got, want, size, k, dt)
+    wt = w.transpose(1, 2).contiguous()
+    got = tg.grouped_matmul(x, wt, off, rows=rows, bias=bias, epilogue=tg.EPI_ELU, transpose=True)
+    check_y(got, want, size, k, dt)
+    dy = randn(g, (m, n), dt)
+    dw, dw_size, db, db_size = wgrad(x, dy, off, rows=rows)
+    got, got_b = tg.grouped_matmul_wgrad(x, dy, off, rows=rows, bias=True)
+    count = torch.tensor(sizes, device="cuda").double()
+    within(got, dw, tolerance(dw, dw_size, count[:, None, None], dt), "dw")
+    within(got_b, db, tolerance(db, db_size, count[:, None], dt), "dbias")

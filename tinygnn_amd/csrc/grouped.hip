@@ -630,6 +630,7 @@ bool direct_operand(const void* p, int64_t ld, int64_t cols, int64_t stride, int
 
 using Medium = Shape<128, 128, 2, 2>;
 using Small = Shape<64, 64, 2, 2>;
+using Wide = Shape<64, 128, 2, 2>;
 using Few = Shape<32, 128, 1, 4>;
 
 unsigned grid_of(const std::string& w, int64_t tiles) {
@@ -814,9 +815,11 @@ int tg_grouped_matmul(int64_t m, int64_t k, int64_t n, int64_t groups, int type,
             // types the large tile where there are 160 of them of 1,024 values
             // (2,500 x 1,024 x 4,096 38 us against 47; 40,000 x 512 x 512 45
             // against 42) and the groups fill them, 128 x 128 where there are
-            // two for each CU (40,000 x 512 x 512 42 against 50); else, and for
-            // floats always (the matrix units' rate bounds those: 40,000 x 2,048
-            // x 1,024 1.28 ms both), 64 x 64.
+            // two for each CU (40,000 x 512 x 512 42 against 50), else 64 x 64.
+            // For floats 64 x 128 where there are as many and no column more to
+            // compute (7 groups of 232,965 x 602 x 256 704 us against 742, 40,000
+            // x 2,048 x 1,024 1.30 ms against 1.34; 3,000 x 256 x 256 22 against
+            // 18; 128 x 128 and 128 x 64 are between the two).
             const auto tiles = [&](int64_t edge) {
                 return tg::most_tiles(m, groups, edge) * tg::ceil_div(n, edge);
             };
@@ -830,6 +833,9 @@ int tg_grouped_matmul(int64_t m, int64_t k, int64_t n, int64_t groups, int type,
                     tg::launch_grouped<T, tg::Medium>(a, along, direct, s);
                 else
                     tg::launch_grouped<T, tg::Small>(a, along, direct, s);
+            } else if (tg::ceil_div(n, 64) % 2 == 0 &&
+                       tg::most_tiles(m, groups, 64) * tg::ceil_div(n, 128) >= 600) {
+                tg::launch_grouped<T, tg::Wide>(a, along, direct, s);
             } else {
                 tg::launch_grouped<T, tg::Small>(a, along, direct, s);
             }
