@@ -430,10 +430,11 @@ void launch_fp8(Fp8Args& a, hipStream_t s) {
     // Few rows: the thin form while its workgroups are few (5 rows of 4,096 x
     // 4,096 7.6 us, 12 in 64 x 64; 150 rows of 32 groups, 2,048 x 4,096, 62 us
     // against 41).  Large tiles where there are 160 of them of 1,024 values and the
-    // groups fill them (2,500 x 2,048 x 4,096 40 us against 47; 40,000 x 512 x 512
-    // 36 against 32), 128 x 128 where there are one for each CU (10,000 x 512 x
-    // 512 the same as 64 x 64, 10,000 x 2,048 x 4,096 126 us against 177), else 64
-    // x 64 (600 x 2,048 x 1,024 12 us against 18).
+    // groups fill them (2,500 x 2,048 x 4,096 46 us against 50; 40,000 x 512 x 512
+    // 36 against 32; 16,384 rows of 32 groups, 2,048 x 4,096, 220 against 300, 4,096
+    // rows of 16 groups 80 to 90 both), 128 x 128 where there are one for
+    // each CU (10,000 x 512 x 512 the same as 64 x 64, 10,000 x 2,048 x 4,096 126
+    // us against 177), else 64 x 64 (600 x 2,048 x 1,024 12 us against 18).
     if (!fits || tiles(16) <= 1024) {
         const unsigned grid = set_grid(a, 16, 16);
         fp8_thin_kernel<T><<<grid, 64 * kThinWaves, 0, s>>>(a);
