@@ -330,7 +330,7 @@ enum { TG_TYPE_F32 = 0, TG_TYPE_BF16 = 1, TG_TYPE_F16 = 2 };
  * gamma / beta: cols values of `weight_type` (TG_TYPE_F32 or `type`), NULL = 1
  * / 0.  mean / rstd: rows floats for the backward pass, or NULL.  Leading
  * dimensions are in elements, at least cols; any alignment.  y may be x (with
- * the same leading dimension).
+ * the same leading dimension).  cols < 2^28.
  *
  * tg_layer_norm_backward: from dy and the forward's x, mean, rstd
  *   t = dy * gamma, xh = (x - mean) * rstd,

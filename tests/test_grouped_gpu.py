@@ -384,22 +384,27 @@ def test_grouped_many_wide_tiles(gpu, dtype, far):
     within(got_b, db, tolerance(db, db_size, count[:, None], dt), "dbias")
 
 
-def test_matmul_fp8_far_rows(gpu):
+@pytest.mark.parametrize("count,k", [(2 ** 24 + 77, 128), (2 ** 22 + 77, 600)])
+def test_matmul_fp8_far_rows(gpu, count, k):
     """Rows gathered from places past 2^31 bytes: the same values as from a
-    copy of those rows (one block of 128: the same sums)."""
+    copy of those rows, whose products run in the same order."""
     import tinygnn_amd as tg
-    g, n, m, count = gen(9), 40, 20000, 2 ** 24 + 77
-    x = torch.zeros(count, 128, dtype=torch.bfloat16, device="cuda")
+    g, n, m = gen(9), 40, 20000
+    x = torch.zeros(count, k, dtype=torch.bfloat16, device="cuda")
     rows = torch.randint(0, count, (m,), generator=g, device="cuda").int()
     rows[0], rows[1] = count - 1, 0
-    x[rows.long()] = randn(g, (m, 128), torch.bfloat16)
-    xq, wq = tg.quantize(x), tg.quantize_weight(randn(g, (128, n), torch.bfloat16))
+    x[rows.long()] = randn(g, (m, k), torch.bfloat16)
+    xq, wq = tg.quantize(x), tg.quantize_weight(randn(g, (k, n), torch.bfloat16))
     del x
-    near = tg.BlockRows(xq.q[rows.long()].contiguous(), xq.scale[:, rows.long()].contiguous(), 128)
+    near = tg.BlockRows(xq.q[rows.long()].contiguous(), xq.scale[:, rows.long()].contiguous(), k)
+    v = near.q.double() * near.scale.double().t().repeat_interleave(128, 1)
+    wv = wq.q.double() * wq.scale.double().repeat_interleave(128, 1)
+    want, size = v @ wv.t(), v.abs() @ wv.abs().t()
+    rows[2] = count
+    want[2] = size[2] = 0
     for dt in (torch.float32, torch.bfloat16):
         got = tg.matmul_fp8(xq, wq, rows=rows, dtype=dt)
-        v = near.q.double() * near.scale[0].double()[:, None]
-        wv = wq.q.double() * wq.scale.double()
-        want, size = v @ wv.t(), v.abs() @ wv.abs().t()
-        within(got, want, tolerance_fp8(want, size, 128, dt), "y")
-        assert torch.equal(got, tg.matmul_fp8(near, wq, dtype=dt))
+        within(got, want, tolerance_fp8(want, size, k, dt), "y")
+        same = tg.matmul_fp8(near, wq, dtype=dt)
+        same[2] = 0
+        assert torch.equal(got, same)

@@ -152,3 +152,17 @@ def test_norm_gradient_by_differences(gpu):
             lo[of] = v[of] - step.view(at.shape)
             want = (loss(*hi) - loss(*lo)) / 2e-4
             assert abs(grad.flatten()[i].item() - want.item()) < 2e-5 * (1 + abs(want.item()))
+
+
+def test_norm_of_more_rows_than_a_launch_takes(gpu):
+    """2^22 rows and some, of 1,024 threads each: 2^32 threads and more."""
+    import tinygnn_amd as tg
+    rows, cols = 2 ** 22 + 300, 2052
+    x = torch.empty(rows, cols, device="cuda")
+    some = torch.tensor([0, 1, 2 ** 22 - 2, 2 ** 22 - 1, 2 ** 22, rows - 1], device="cuda")
+    values = randn(gen(4), (len(some), cols), torch.float32)
+    x[some] = values
+    y, mean, rstd = tg.layer_norm(x, with_stats=True, out=x)
+    want, want_mean, want_rstd = tg.layer_norm(values, with_stats=True)
+    assert torch.equal(y[some], want)
+    assert torch.equal(mean[some], want_mean) and torch.equal(rstd[some], want_rstd)

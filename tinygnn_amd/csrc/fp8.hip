@@ -192,7 +192,10 @@ __device__ __forceinline__ void store_outputs(const Fp8Args& a, int p, int n, co
 // to the sums (16 multiply-adds beside each 32-cycle instruction).  As in the
 // 16-bit products the outputs are computed transposed, so a lane's row of x is
 // one; x's scales of the block come to LDS with its tile.
-template <typename T, typename S>
+//
+// FAR: x and its scales come through registers, for rows gathered from places
+// past 2 GB, which the offsets of loads to LDS do not reach.
+template <typename T, typename S, bool FAR>
 __global__ __launch_bounds__(S::kThreads) void fp8_kernel(Fp8Args a) {
     constexpr int kScales = S::kM * kRowBytes;  // behind x's tile
     __shared__ __attribute__((aligned(16))) char a0[kScales + S::kThreads * 4];
@@ -220,11 +223,15 @@ __global__ __launch_bounds__(S::kThreads) void fp8_kernel(Fp8Args a) {
     const uint8_t* xb = a.rows ? a.xq : a.xq + static_cast<int64_t>(r0) * kp;
     const uint8_t* wb = w + static_cast<int64_t>(n0) * kp;
     uint32_t ao[S::kCA], bo[S::kCB];
+    const uint8_t* far[S::kCA];  // null: zeros
+    v4u held[S::kCA];            // the next tile's
+    float held_scale = 0.0f;
 #pragma unroll
     for (int t = 0; t < S::kCA; ++t) {
         int row, c;
         chunk_place<uint8_t, S::kM, false>(t * S::kThreads + tid, &row, &c);
         const int src = r0 + row < r1 ? source_row(a, r0 + row) : -1;
+        far[t] = FAR && src >= 0 ? a.xq + src * kp + c : nullptr;
         ao[t] = src < 0 ? kOutside
                         : static_cast<uint32_t>((a.rows ? src : row) * kp + c);
     }
@@ -236,16 +243,24 @@ __global__ __launch_bounds__(S::kThreads) void fp8_kernel(Fp8Args a) {
     }
     // one row's scale for each thread; outside, and of threads past the rows: 0
     uint32_t so = kOutside;
+    const float* far_scale = nullptr;
     if (tid < S::kM && r0 + tid < r1) {
         const int src = source_row(a, r0 + tid);
         if (src >= 0) so = static_cast<uint32_t>(src) * 4;
+        if (FAR && src >= 0) far_scale = a.xscale + src;
     }
     // load p of tile kt (zeros past the last tile)
     constexpr int kLoads = 1 + S::kCA + S::kCB;
     auto load = [&](int kt, char* la, char* lb, int p) {
         const int64_t size = kt < a.kb ? kDirectBytes : 0;
         const int64_t at = static_cast<int64_t>(kt) * kBlock;
-        if (p == 0) {
+        if (FAR && p == 0) {
+            held_scale = far_scale && kt < a.kb ? far_scale[kt * a.x_rows] : 0.0f;
+        } else if (FAR && p <= S::kCA) {
+            const v4u none = {0, 0, 0, 0};
+            const uint8_t* x = far[p - 1];
+            held[p - 1] = x && kt < a.kb ? *reinterpret_cast<const v4u*>(x + at) : none;
+        } else if (p == 0) {
             const float* xs = a.xscale + static_cast<int64_t>(kt) * a.x_rows;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 buffer_of(xs, kt < a.kb ? 4 * a.x_rows : 0),
@@ -257,6 +272,14 @@ __global__ __launch_bounds__(S::kThreads) void fp8_kernel(Fp8Args a) {
             const int t = p - 1 - S::kCA;
             load_to_lds(buffer_of(wb + at, size), lb + (t * S::kThreads + wave * 64) * 16, bo[t]);
         }
+    };
+    // what FAR holds, to where load() puts it otherwise
+    auto put = [&](char* la) {
+        if (!FAR) return;
+#pragma unroll
+        for (int t = 0; t < S::kCA; ++t)
+            *reinterpret_cast<v4u*>(la + (t * S::kThreads + tid) * 16) = held[t];
+        *reinterpret_cast<float*>(la + kScales + tid * 4) = held_scale;
     };
     Acc<S> acc = {};
     const Reader<uint8_t, S::kM, false, S::kMI> ra(wm, lane);
@@ -308,10 +331,12 @@ __global__ __launch_bounds__(S::kThreads) void fp8_kernel(Fp8Args a) {
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        put(na);
     };
     if (a.kb > 0) {
 #pragma unroll
         for (int p = 0; p < kLoads; ++p) load(0, a0, b0, p);
+        put(a0);
     }
     while (kt + 1 < a.kb) {  // compute() counts
         __syncthreads();
@@ -405,24 +430,22 @@ using Large = Shape<256, 256, 2, 4>;
 using Medium = Shape<128, 128, 2, 2>;
 using Small = Shape<64, 64, 2, 2>;
 
-unsigned set_grid(Fp8Args& a, int bm, int bn) {
+unsigned set_grid(Fp8Args& a, int bm, int bn, int threads) {
     a.mt = static_cast<uint32_t>(most_tiles(a.m, a.groups, bm));
     a.nt = static_cast<uint32_t>(ceil_div(a.n, bn));
     const int64_t grid = static_cast<int64_t>(a.mt) * a.nt;
-    require(grid < (int64_t(1) << 31), "matmul_fp8: too many tiles");
-    return static_cast<unsigned>(grid);
+    return grid_of("matmul_fp8", grid, threads);
 }
 
 template <typename T>
 void launch_fp8(Fp8Args& a, hipStream_t s) {
     const int64_t kp = static_cast<int64_t>(a.kb) * kBlock;
-    // tiles' offsets have 31 bits
-    const bool fits = (a.rows ? a.x_rows : 256) * kp < kDirectBytes &&
-                      256 * kp < kDirectBytes && 4 * a.x_rows < kDirectBytes;
+    // loads' offsets to LDS have 31 bits
+    const bool near = (a.rows ? a.x_rows : 256) * kp < kDirectBytes && 4 * a.x_rows < kDirectBytes;
     auto tiled = [&](auto shape) {
         using S = decltype(shape);
-        const unsigned grid = set_grid(a, S::kM, S::kN);
-        fp8_kernel<T, S><<<grid, S::kThreads, 0, s>>>(a);
+        const unsigned grid = set_grid(a, S::kM, S::kN, S::kThreads);
+        fp8_kernel<T, S, false><<<grid, S::kThreads, 0, s>>>(a);
     };
     auto tiles = [&](int64_t edge) {
         return most_tiles(a.m, a.groups, edge) * ceil_div(a.n, edge);
@@ -435,9 +458,12 @@ void launch_fp8(Fp8Args& a, hipStream_t s) {
     // rows of 16 groups 80 to 90 both), 128 x 128 where there are one for
     // each CU (10,000 x 512 x 512 the same as 64 x 64, 10,000 x 2,048 x 4,096 126
     // us against 177), else 64 x 64 (600 x 2,048 x 1,024 12 us against 18).
-    if (!fits || tiles(16) <= 1024) {
-        const unsigned grid = set_grid(a, 16, 16);
+    if (256 * kp >= kDirectBytes || tiles(16) <= 1024) {
+        const unsigned grid = set_grid(a, 16, 16, 64 * kThinWaves);
         fp8_thin_kernel<T><<<grid, 64 * kThinWaves, 0, s>>>(a);
+    } else if (!near) {
+        const unsigned grid = set_grid(a, Medium::kM, Medium::kN, Medium::kThreads);
+        fp8_kernel<T, Medium, true><<<grid, Medium::kThreads, 0, s>>>(a);
     } else if (a.kb >= 8 && tiles(256) * a.kb >= 160 * 8 && a.m >= 256 * a.groups) {
         tiled(Large{});
     } else if (tiles(128) >= 300 && a.m >= 100 * a.groups) {
@@ -467,12 +493,10 @@ int tg_quantize(int64_t rows, int64_t cols, int type, const void* x, int64_t ldx
         require(ldx >= cols, "quantize: leading dimension below cols");
         require(reinterpret_cast<uintptr_t>(q) % 16 == 0, "quantize: q must be 16-byte aligned");
         const int64_t blocks = tg::ceil_div(cols, tg::kBlock);
-        const int64_t grid = tg::ceil_div(rows * blocks, 32);
-        require(grid < (int64_t(1) << 31), "quantize: too many elements");
+        const unsigned grid = tg::grid_of("quantize", tg::ceil_div(rows * blocks, 32), 256);
         tg::with_type(type, "quantize", [&](auto t) {
             using T = decltype(t);
-            tg::quantize_kernel<T><<<static_cast<unsigned>(grid), 256, 0,
-                                     static_cast<hipStream_t>(stream)>>>(
+            tg::quantize_kernel<T><<<grid, 256, 0, static_cast<hipStream_t>(stream)>>>(
                 rows, cols, blocks, static_cast<const T*>(x), ldx, static_cast<uint8_t*>(q), scale);
         });
         TG_LAUNCH_CHECK();

@@ -633,16 +633,11 @@ using Small = Shape<64, 64, 2, 2>;
 using Wide = Shape<64, 128, 2, 2>;
 using Few = Shape<32, 128, 1, 4>;
 
-unsigned grid_of(const std::string& w, int64_t tiles) {
-    require(tiles < (int64_t(1) << 31), w + ": too many tiles");
-    return static_cast<unsigned>(tiles);
-}
-
 template <typename T, typename S>
 void launch_grouped(GroupedArgs& a, bool along, bool direct, hipStream_t s) {
     a.mt = static_cast<uint32_t>(most_tiles(a.m, a.groups, S::kM));
     a.nt = static_cast<uint32_t>(ceil_div(a.n, S::kN));
-    const unsigned grid = grid_of("grouped_matmul", static_cast<int64_t>(a.mt) * a.nt);
+    const unsigned grid = grid_of("grouped_matmul", static_cast<int64_t>(a.mt) * a.nt, S::kThreads);
     if (along)
         direct ? grouped_kernel<T, S, true, true><<<grid, S::kThreads, 0, s>>>(a)
                : grouped_kernel<T, S, true, false><<<grid, S::kThreads, 0, s>>>(a);
@@ -656,7 +651,7 @@ template <typename T>
 void launch_ring(GroupedArgs& a, bool along, hipStream_t s) {
     a.mt = static_cast<uint32_t>(most_tiles(a.m, a.groups, 256));
     a.nt = static_cast<uint32_t>(ceil_div(a.n, 256));
-    const unsigned grid = grid_of("grouped_matmul", static_cast<int64_t>(a.mt) * a.nt);
+    const unsigned grid = grid_of("grouped_matmul", static_cast<int64_t>(a.mt) * a.nt, kRingThreads);
     if (a.k % kStep == 0)
         along ? grouped_ring_kernel<T, true, true><<<grid, kRingThreads, 0, s>>>(a)
               : grouped_ring_kernel<T, false, true><<<grid, kRingThreads, 0, s>>>(a);
@@ -723,7 +718,7 @@ void launch_wgrad(GroupedArgs& a, const WgradPlan& p, bool direct, hipStream_t s
     a.mt = static_cast<uint32_t>(p.mt);
     a.nt = static_cast<uint32_t>(p.nt);
     a.unit = static_cast<int>(p.unit);
-    const unsigned grid = grid_of("grouped_matmul_wgrad", p.mt * p.nt * p.parts);
+    const unsigned grid = grid_of("grouped_matmul_wgrad", p.mt * p.nt * p.parts, kRingThreads);
     auto tiled = [&](auto shape) {
         using S = decltype(shape);
         if (a.dbias)
@@ -751,7 +746,7 @@ void launch_wgrad(GroupedArgs& a, const WgradPlan& p, bool direct, hipStream_t s
     TG_LAUNCH_CHECK();
     if (!p.unit) return;
     auto add = [&](const float* part, int64_t size, void* out) {
-        const dim3 blocks(grid_of("grouped_matmul_wgrad", ceil_div(size, 1024)),
+        const dim3 blocks(grid_of("grouped_matmul_wgrad", ceil_div(size, 1024), 256),
                           static_cast<unsigned>(a.groups));
         parts_kernel<T><<<blocks, 256, 0, s>>>(a.offsets, a.m, a.unit,
                                                static_cast<int>(p.parts), part, size,

@@ -417,8 +417,8 @@ void check_norm(const char* what, int64_t rows, int64_t cols, int type, int weig
                 bool has_weights) {
     const std::string w = what;
     require(rows >= 0 && cols >= 0, w + ": negative dimension");
-    require(rows < (int64_t(1) << 31) && cols < (int64_t(1) << 31),
-            w + ": rows and cols must be < 2^31");
+    require(rows < (int64_t(1) << 31) && cols < (int64_t(1) << 28),
+            w + ": rows must be < 2^31 and cols < 2^28");
     require(rows == 0 || cols > 0, w + ": rows of 0 columns have no mean");
     require(type >= TG_TYPE_F32 && type <= TG_TYPE_F16, w + ": unknown element type " +
                                                             std::to_string(type));
@@ -443,34 +443,37 @@ int tg_layer_norm(int64_t rows, int64_t cols, int type, const void* x, int64_t l
         require(x && y, "layer_norm: null pointer");
         require(ldx >= cols && ldy >= cols, "layer_norm: leading dimension below cols");
         tg::NormArgs a{};
-        a.rows = rows;
         a.cols = cols;
-        a.x = x;
         a.ldx = ldx;
         a.gamma = gamma;
         a.beta = beta;
         a.weight_f32 = weight_type == TG_TYPE_F32;
         a.eps = eps;
-        a.y = y;
         a.ldy = ldy;
-        a.mean = mean;
-        a.rstd = rstd;
         hipStream_t s = static_cast<hipStream_t>(stream);
-        const unsigned n = static_cast<unsigned>(rows);
-        tg::with_type(type, "layer_norm", [&](auto t) {
-            using T = decltype(t);
-            const tg::RowShape shape = tg::row_shape(cols, type);
-            if (shape.items == 0) {
-                tg::norm_wide_kernel<T><<<n, tg::kWideThreads, 0, s>>>(a);
-                return;
-            }
-            tg::with_row_shape<T>(shape, [&](auto threads, auto items) {
-                constexpr int TPR = decltype(threads)::value, RPB = TPR > 256 ? 1 : 256 / TPR;
-                tg::norm_kernel<T, TPR, decltype(items)::value>
-                    <<<(n + RPB - 1) / RPB, TPR > 256 ? TPR : 256, 0, s>>>(a);
+        const tg::RowShape shape = tg::row_shape(cols, type);
+        const int64_t z = tg::type_size(type);
+        tg::for_slices(rows, std::max(shape.threads, 64), [&](int64_t first, int64_t count) {
+            a.rows = count;
+            a.x = static_cast<const char*>(x) + first * ldx * z;
+            a.y = static_cast<char*>(y) + first * ldy * z;
+            a.mean = mean ? mean + first : nullptr;
+            a.rstd = rstd ? rstd + first : nullptr;
+            const unsigned n = static_cast<unsigned>(count);
+            tg::with_type(type, "layer_norm", [&](auto t) {
+                using T = decltype(t);
+                if (shape.items == 0) {
+                    tg::norm_wide_kernel<T><<<n, tg::kWideThreads, 0, s>>>(a);
+                    return;
+                }
+                tg::with_row_shape<T>(shape, [&](auto threads, auto items) {
+                    constexpr int TPR = decltype(threads)::value, RPB = TPR > 256 ? 1 : 256 / TPR;
+                    tg::norm_kernel<T, TPR, decltype(items)::value>
+                        <<<(n + RPB - 1) / RPB, TPR > 256 ? TPR : 256, 0, s>>>(a);
+                });
             });
+            TG_LAUNCH_CHECK();
         });
-        TG_LAUNCH_CHECK();
     });
 }
 

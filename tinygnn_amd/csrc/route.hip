@@ -768,8 +768,17 @@ int tg_route_backward(int64_t tokens, int64_t experts, int64_t k, int type, cons
             using T = decltype(t);
             tg::with_row_shape(experts, k, [&](auto lpr, auto items) {
                 constexpr int L = decltype(lpr)::value, I = decltype(items)::value;
-                const unsigned n = static_cast<unsigned>(tg::ceil_div(tokens, 256 / L));
-                tg::route_backward_kernel<T, L, I><<<n, 256, 0, s>>>(a);
+                tg::for_slices(tokens, L, [&](int64_t first, int64_t count) {
+                    tg::RouteArgs b = a;
+                    b.tokens = count;
+                    b.logits = static_cast<const T*>(logits) + first * ld;
+                    b.weights += first * k;
+                    b.ids += first * k;
+                    b.dweights += first * k;
+                    b.dlogits = static_cast<T*>(dlogits) + first * lddl;
+                    const unsigned n = static_cast<unsigned>(tg::ceil_div(count, 256 / L));
+                    tg::route_backward_kernel<T, L, I><<<n, 256, 0, s>>>(b);
+                });
             });
         });
         TG_LAUNCH_CHECK();
@@ -806,9 +815,15 @@ int tg_route_combine(int64_t tokens, int64_t k, int64_t cols, int type, const vo
             using T = decltype(t);
             const int64_t chunks = tg::ceil_div(cols, tg::kWave * tg::kVec<T>);
             a.chunks = static_cast<int>(chunks);
-            const int64_t blocks = tg::ceil_div(tokens * chunks, 4);
-            require(blocks < (int64_t(1) << 31), "route_combine: too many elements");
-            tg::combine_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
+            tg::for_slices(tokens, chunks * tg::kWave, [&](int64_t first, int64_t count) {
+                tg::CombineArgs b = a;
+                b.tokens = count;
+                b.position += first * k;
+                if (weights) b.weights += first * k;
+                b.out = static_cast<T*>(out) + first * ldo;
+                const unsigned n = static_cast<unsigned>(tg::ceil_div(count * chunks, 4));
+                tg::combine_kernel<T><<<n, 256, 0, s>>>(b);
+            });
         });
         TG_LAUNCH_CHECK();
     });
@@ -848,8 +863,16 @@ int tg_route_combine_backward(int64_t tokens, int64_t k, int64_t cols, int type,
         hipStream_t s = static_cast<hipStream_t>(stream);
         tg::with_type(type, "route_combine_backward", [&](auto t) {
             using T = decltype(t);
-            tg::combine_backward_kernel<T>
-                <<<static_cast<unsigned>(tg::ceil_div(tokens, 4)), 256, 0, s>>>(a);
+            tg::for_slices(tokens, tg::kWave, [&](int64_t first, int64_t count) {
+                tg::CombineArgs b = a;
+                b.tokens = count;
+                b.position += first * k;
+                if (weights) b.weights += first * k;
+                if (dweights) b.dweights += first * k;
+                b.dout = static_cast<const T*>(dout) + first * lddo;
+                const unsigned n = static_cast<unsigned>(tg::ceil_div(count, 4));
+                tg::combine_backward_kernel<T><<<n, 256, 0, s>>>(b);
+            });
         });
         TG_LAUNCH_CHECK();
     });

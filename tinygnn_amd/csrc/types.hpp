@@ -70,4 +70,19 @@ __device__ __forceinline__ void store_floats(T* __restrict__ p, int64_t left, co
     }
 }
 
+// Workgroups of one launch, which has fewer than 2^32 threads.
+inline unsigned grid_of(const char* what, int64_t blocks, int64_t threads) {
+    require(blocks * threads < (int64_t(1) << 32), std::string(what) + ": too many elements");
+    return static_cast<unsigned>(blocks);
+}
+
+// fn(first, count) for the slices of `rows` that one launch of `threads` threads
+// a row can take.
+template <typename F>
+void for_slices(int64_t rows, int64_t threads, F&& fn) {
+    const int64_t most = ((int64_t(1) << 32) - 1024) / threads;
+    for (int64_t first = 0; first < rows; first += most)
+        fn(first, first + most < rows ? most : rows - first);
+}
+
 }  // namespace tg
