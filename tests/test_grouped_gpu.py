@@ -408,3 +408,24 @@ def test_matmul_fp8_far_rows(gpu, count, k):
         same = tg.matmul_fp8(near, wq, dtype=dt)
         same[2] = 0
         assert torch.equal(got, same)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("m,k,n", [(3, 6, 5), (300, 512, 264)])
+def test_gathered_from_no_rows(gpu, dtype, m, k, n):
+    """Every index is outside an x of no rows: rows of zeros, plus the bias."""
+    import tinygnn_amd as tg
+    dt, off = DTYPES[dtype], offsets_of([m - 1, 1])
+    x = torch.empty(0, k, dtype=dt, device="cuda")
+    rows = torch.arange(-1, m - 1, dtype=torch.int32, device="cuda")
+    bias = torch.stack([torch.ones(n), torch.full((n,), 2.0)]).to(dt).cuda()
+    want = torch.cat([bias[:1].expand(m - 1, n), bias[1:]])
+    for t in (False, True):
+        w = torch.ones(2, *((n, k) if t else (k, n)), dtype=dt, device="cuda")
+        assert torch.equal(tg.grouped_matmul(x, w, off, rows=rows, bias=bias, transpose=t), want)
+    wq = tg.quantize_weight(w, transpose=True)
+    got = tg.matmul_fp8(tg.quantize(x), wq, offsets=off, rows=rows, bias=bias, dtype=dt)
+    assert torch.equal(got, want)
+    dw, db = tg.grouped_matmul_wgrad(x, torch.ones(m, n, dtype=dt, device="cuda"), off, rows=rows,
+                                     bias=True)
+    assert not dw.any() and torch.equal(db[:, 0], torch.tensor([m - 1, 1], device="cuda").to(dt))
