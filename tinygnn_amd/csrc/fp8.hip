@@ -339,13 +339,13 @@ __global__ __launch_bounds__(S::kThreads) void fp8_kernel(Fp8Args a) {
         put(a0);
     }
     while (kt + 1 < a.kb) {  // compute() counts
-        __syncthreads();
+        step_border<0>();
         compute(a0, b0, a1, b1);
-        __syncthreads();
+        step_border<0>();
         compute(a1, b1, a0, b0);
     }
     if (kt < a.kb) {
-        __syncthreads();
+        step_border<0>();
         compute(a0, b0, a1, b1);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
