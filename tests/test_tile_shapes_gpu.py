@@ -87,6 +87,7 @@ def check_fp8(dt, m, k, n, sizes, gather, want_shape):
     (2817, 1024, 4096, [1000, 0, 517, 1300], False),       # eight, the groups' ends ragged
     (700, 2000, 4000, [1, 1500, 0, 1100], True),           # rows twice, rows of zeros
 ])
-def test_fp8_large(gpu, dtype, m, k, n, sizes, gather):
-    """256 x 256 for 160 and more tiles of eight and more blocks."""
-    check_fp8(DTYPES[dtype], m, k, n, sizes, gather, (256, 256))
+def test_fp8_many_tiles(gpu, dtype, m, k, n, sizes, gather):
+    """256 x 256 for 160 and more tiles of eight and more blocks and 16-bit
+    results, 128 x 128 for fp32 ones."""
+    check_fp8(DTYPES[dtype], m, k, n, sizes, gather, (128, 128) if dtype == "f32" else (256, 256))

@@ -457,15 +457,20 @@ void launch_fp8(Fp8Args& a, hipStream_t s) {
     // 36 against 32; 16,384 rows of 32 groups, 2,048 x 4,096, 220 against 300, 4,096
     // rows of 16 groups 80 to 90 both), 128 x 128 where there are one for
     // each CU (10,000 x 512 x 512 the same as 64 x 64, 10,000 x 2,048 x 4,096 126
-    // us against 177), else 64 x 64 (600 x 2,048 x 1,024 12 us against 18).
+    // us against 177), else 64 x 64 (600 x 2,048 x 1,024 12 us against 18).  fp32
+    // results stay below the large tile, whose widened operands do not fit the
+    // registers beside its sums (18 spilled; 2,500 x 2,048 x 4,096 58 us against
+    // 53 of 128 x 128, 40,000 x 1,024 x 1,024 106 against 95, 8,192 x 4,096 x 8,192
+    // 477 against 499).
     if (256 * kp >= kDirectBytes || tiles(16) <= 1024) {
         const unsigned grid = set_grid(a, 16, 16, 64 * kThinWaves);
         fp8_thin_kernel<T><<<grid, 64 * kThinWaves, 0, s>>>(a);
     } else if (!near) {
         const unsigned grid = set_grid(a, Medium::kM, Medium::kN, Medium::kThreads);
         fp8_kernel<T, Medium, true><<<grid, Medium::kThreads, 0, s>>>(a);
-    } else if (a.kb >= 8 && tiles(256) * a.kb >= 160 * 8 && a.m >= 256 * a.groups) {
-        tiled(Large{});
+    } else if (sizeof(T) == 2 && a.kb >= 8 && tiles(256) * a.kb >= 160 * 8 &&
+               a.m >= 256 * a.groups) {
+        if constexpr (sizeof(T) == 2) tiled(Large{});
     } else if (tiles(128) >= 300 && a.m >= 100 * a.groups) {
         tiled(Medium{});
     } else {
