@@ -38,6 +38,38 @@ def stream_handle(stream=None) -> int:
     return int(s.cuda_stream)
 
 
+def _on(stream) -> int:
+    """The handle of the stream that a call runs on.  One that is not the
+    current one waits for what is queued there: a call's inputs may come from
+    it, and its outputs and workspaces are torch's memory of the current stream,
+    on which work of whoever held a block before may still be pending.  (Not
+    where either is being captured, and could not: there the order is the
+    caller's.)"""
+    handle = stream_handle(stream)
+    if stream is None:
+        return handle
+    cuda = _torch().cuda
+    current = cuda.current_stream()
+    if int(current.cuda_stream) == handle:
+        return handle
+    wait = getattr(stream, "wait_stream", None)
+    if wait is None:   # no torch stream: a handle alone
+        if not _capturing(None):
+            current.synchronize()
+    elif not _capturing(None) and not _capturing(stream):
+        wait(current)
+    return handle
+
+
+def _capturing(stream) -> bool:
+    """Whether `stream` (None: the current one) is being captured."""
+    cuda = _torch().cuda
+    if not cuda.is_initialized():
+        return False
+    with cuda.stream(stream):
+        return cuda.is_current_stream_capturing()
+
+
 def _finish(stream) -> None:
     """Waits for `stream` where it is not the current one.  The outputs of a
     call are torch's memory of the current stream: reading a result's size, the
@@ -102,7 +134,7 @@ class SpmmPlan:
                  stream=None, precision: int = PRECISION_EXACT):
         h = C.c_void_p()
         lib.check(lib.tg_spmm_plan_create(n_rows, nnz_bound, dptr(row_ptr), max_f, chunk_nnz,
-                                          stream_handle(stream), C.byref(h)))
+                                          _on(stream), C.byref(h)))
         self.h = h
         self.row_ptr = row_ptr
         self.n_rows = n_rows
@@ -158,7 +190,7 @@ def spmm_epilogue(a: DeviceCSR, b, plan: SpmmPlan, bias=None, epilogue: int = EP
     lib.check(lib.tg_spmm_execute_epilogue(plan.h, a.n_cols, f, dptr(a.row_ptr),
                                            dptr(a.col_ind), dptr(a.val), dptr(b), b.stride(0),
                                            dptr(out), out.stride(0), dptr(bias), epilogue,
-                                           stream_handle(stream)))
+                                           _on(stream)))
     return out
 
 
@@ -174,7 +206,7 @@ def spmm(a: DeviceCSR, b, plan: SpmmPlan | None = None, out=None, stream=None,
     f = b.shape[1]
     if out is None:
         out = torch.empty((a.n_rows, f), dtype=torch.float32, device=b.device)
-    s = stream_handle(stream)
+    s = _on(stream)
     if plan is None:
         lib.check(lib.tg_spmm_ex(a.n_rows, a.n_cols, f, a.nnz, dptr(a.row_ptr), dptr(a.col_ind),
                                  dptr(a.val), dptr(b), b.stride(0), dptr(out), out.stride(0),
@@ -200,7 +232,7 @@ def edge_list_to_csr(src, dst, n_nodes: int, stream=None) -> DeviceCSR:
     v = torch.empty(max(e, 1), dtype=torch.float32, device=dev)[:e]
     lib.check(lib.tg_edge_list_to_csr(n_nodes, e, dptr(src, torch.int32), dptr(dst, torch.int32),
                                       dptr(rp), ci.data_ptr(), v.data_ptr(), None, 0,
-                                      stream_handle(stream)))
+                                      _on(stream)))
     _finish(stream)
     return DeviceCSR(n_nodes, n_nodes, rp, ci, v)
 
@@ -208,7 +240,7 @@ def edge_list_to_csr(src, dst, n_nodes: int, stream=None) -> DeviceCSR:
 def csr_validate(a: DeviceCSR, stream=None) -> None:
     """The checks of Tensor::sparse_csr (tensor.cpp:46-86); raises InvalidArgument."""
     lib.check(lib.tg_csr_validate(a.n_rows, a.n_cols, a.nnz, dptr(a.row_ptr),
-                                  a.col_ind.data_ptr() if a.nnz else None, stream_handle(stream)))
+                                  a.col_ind.data_ptr() if a.nnz else None, _on(stream)))
 
 
 def _require_square(a: DeviceCSR, fn: str):
@@ -238,7 +270,7 @@ def add_self_loops(a: DeviceCSR, stream=None) -> DeviceCSR:
     rp, ci, v = _self_loop_outputs(a)
     lib.check(lib.tg_add_self_loops(a.n_rows, a.nnz, dptr(a.row_ptr), a.col_ind.data_ptr(),
                                     a.val.data_ptr(), dptr(rp), dptr(ci), dptr(v), None, 0,
-                                    stream_handle(stream)))
+                                    _on(stream)))
     return _trim(a, rp, ci, v, stream)
 
 
@@ -252,7 +284,7 @@ def gcn_norm(a: DeviceCSR, with_degrees: bool = False, stream=None):
     dis = torch.empty_like(deg)
     lib.check(lib.tg_gcn_norm(a.n_rows, a.nnz, dptr(a.row_ptr), a.col_ind.data_ptr(),
                               a.val.data_ptr(), dptr(rp), dptr(ci), dptr(v), dptr(deg), dptr(dis),
-                              None, 0, stream_handle(stream)))
+                              None, 0, _on(stream)))
     out = _trim(a, rp, ci, v, stream)
     return (out, deg[:a.n_rows], dis[:a.n_rows]) if with_degrees else out
 
@@ -262,7 +294,7 @@ def edge_softmax(a: DeviceCSR, stream=None) -> DeviceCSR:
     torch = _torch()
     v = torch.zeros_like(a.val)
     lib.check(lib.tg_edge_softmax(a.n_rows, dptr(a.row_ptr), a.val.data_ptr(), v.data_ptr(),
-                                  stream_handle(stream)))
+                                  _on(stream)))
     return DeviceCSR(a.n_rows, a.n_cols, a.row_ptr, a.col_ind, v)
 
 
@@ -283,12 +315,12 @@ def matmul(a, b, bias=None, epilogue: int = EPI_NONE, algo: int = GEMM_AUTO, out
     if out is None:
         out = torch.empty((m, n), dtype=torch.float32, device=a.device)
     lib.check(lib.tg_matmul(m, k, n, dptr(a), a.stride(0), dptr(b), b.stride(0), dptr(out),
-                            out.stride(0), dptr(bias), epilogue, algo, stream_handle(stream)))
+                            out.stride(0), dptr(bias), epilogue, algo, _on(stream)))
     return out
 
 
 def _unary(name, x, *extra, stream=None):
-    lib.check(getattr(lib, name)(x.numel(), dptr(x), *extra, stream_handle(stream)))
+    lib.check(getattr(lib, name)(x.numel(), dptr(x), *extra, _on(stream)))
     return x
 
 
@@ -317,12 +349,12 @@ def gelu_(x, stream=None):
 
 
 def softmax_(x, stream=None):
-    lib.check(lib.tg_softmax(x.shape[0], x.shape[1], dptr(x), stream_handle(stream)))
+    lib.check(lib.tg_softmax(x.shape[0], x.shape[1], dptr(x), _on(stream)))
     return x
 
 
 def log_softmax_(x, stream=None):
-    lib.check(lib.tg_log_softmax(x.shape[0], x.shape[1], dptr(x), stream_handle(stream)))
+    lib.check(lib.tg_log_softmax(x.shape[0], x.shape[1], dptr(x), _on(stream)))
     return x
 
 
@@ -332,7 +364,7 @@ def add_bias_(x, bias, stream=None):
         shp = tuple(bias.shape) if bias.dim() == 2 else (1, bias.numel())
         raise InvalidArgument(1, f"add_bias: bias must be shape (1×{n}) to match X columns, "
                                  f"but got ({shp[0]}×{shp[1]}).")
-    lib.check(lib.tg_add_bias(x.shape[0], n, dptr(x), dptr(bias), stream_handle(stream)))
+    lib.check(lib.tg_add_bias(x.shape[0], n, dptr(x), dptr(bias), _on(stream)))
     return x
 
 
@@ -344,7 +376,7 @@ def sage_aggregate(plan: SpmmPlan, a: DeviceCSR, h, agg: int = AGG_MEAN, stream=
     out = torch.empty((a.n_rows, h.shape[1]), dtype=torch.float32, device=h.device)
     lib.check(lib.tg_sage_aggregate(plan.h, a.n_rows, h.shape[1], agg, dptr(a.row_ptr),
                                     a.col_ind.data_ptr(), dptr(h), h.stride(0), dptr(out),
-                                    out.stride(0), stream_handle(stream)))
+                                    out.stride(0), _on(stream)))
     return out
 
 
@@ -359,7 +391,7 @@ def sage_forward(plan: SpmmPlan, a: DeviceCSR, h, w_neigh, w_self, bias=None,
     lib.check(lib.tg_sage_forward(plan.h, a.n_rows, f_in, f_out, agg, dptr(a.row_ptr),
                                   a.col_ind.data_ptr(), dptr(h), dptr(w_neigh), dptr(w_self),
                                   dptr(bias), act, post, dataflow, dptr(out), None, 0,
-                                  stream_handle(stream)))
+                                  _on(stream)))
     _finish(stream)
     return out
 
@@ -370,7 +402,7 @@ def gat_scores(wh, heads: int, f: int, att_l, att_r, stream=None):
     src = torch.empty((n, heads), dtype=torch.float32, device=wh.device)
     dst = torch.empty_like(src)
     lib.check(lib.tg_gat_scores(n, heads, f, dptr(wh), wh.stride(0), dptr(att_l), dptr(att_r),
-                                dptr(src), dptr(dst), stream_handle(stream)))
+                                dptr(src), dptr(dst), _on(stream)))
     return src, dst
 
 
@@ -385,7 +417,7 @@ def gat_aggregate(plan: SpmmPlan, a_sl: DeviceCSR, wh, heads: int, f: int, src, 
     lib.check(lib.tg_gat_aggregate(plan.h, a_sl.n_rows, heads, f, dptr(a_sl.row_ptr),
                                    a_sl.col_ind.data_ptr(), dptr(wh), wh.stride(0), dptr(src),
                                    dptr(dst), slope, dptr(bias), act, post, int(concat),
-                                   dptr(out), out.stride(0), None, 0, stream_handle(stream)))
+                                   dptr(out), out.stride(0), None, 0, _on(stream)))
     _finish(stream)
     return out
 
@@ -394,7 +426,8 @@ def gat_aggregate(plan: SpmmPlan, a_sl: DeviceCSR, wh, heads: int, f: int, src, 
 # Expert layers: norm, routing, grouped and 8-bit products.  Tensors are
 # float32, bfloat16 or float16 on one device, rows contiguous (any row stride).
 # A call runs on `stream`, or on the current stream of its tensors' device;
-# given a `stream` that is not the current one, it returns finished results.
+# given a `stream` that is not the current one, it runs after what is queued on
+# the current one and returns finished results.
 # Outputs and workspaces are torch memory, so the calls can be captured.
 # (Small calls are bound by this code: messages are made when they are needed.)
 # ---------------------------------------------------------------------------
@@ -453,7 +486,7 @@ def _stream_of(what: str, stream, first, *others) -> int:
                 raise ValueError("tinygnn_amd expects device (cuda) tensors")
             _refuse(what, f"tensors on {first.device} and {t.device}.")
     if stream is not None or _pt.raw_stream is None:
-        return stream_handle(stream)
+        return _on(stream)
     return _pt.raw_stream(index)
 
 
@@ -1035,7 +1068,7 @@ class Model:
         self._adj_key = None
         lib.check(lib.tg_model_forward(self.h, adj.n_rows, adj.nnz, dptr(adj.row_ptr),
                                        adj.col_ind.data_ptr(), adj.val.data_ptr(), x.shape[1],
-                                       dptr(x), dptr(out), mode, stream_handle(stream)))
+                                       dptr(x), dptr(out), mode, _on(stream)))
         self._adj_key = key
         return out
 
@@ -1094,7 +1127,7 @@ class CsvText:
     @classmethod
     def open(cls, path, stream=None) -> "CsvText":
         h = C.c_void_p()
-        lib.check(lib.tg_csv_open(os.fsencode(path), C.byref(h), stream_handle(stream)))
+        lib.check(lib.tg_csv_open(os.fsencode(path), C.byref(h), _on(stream)))
         return cls(h)
 
     @classmethod
@@ -1104,7 +1137,7 @@ class CsvText:
             raise ValueError("CsvText.from_device expects a contiguous uint8 device tensor")
         h = C.c_void_p()
         lib.check(lib.tg_csv_index(dptr(text), text.numel(), name.encode(), C.byref(h),
-                                   stream_handle(stream)))
+                                   _on(stream)))
         return cls(h, keep=text)
 
     @property
@@ -1121,13 +1154,13 @@ class CsvText:
         dst = torch.empty(max(n, 1), dtype=torch.int32, device=device)[:n]
         mx = C.c_int64()
         lib.check(lib.tg_csv_parse_edges(self.h, src.data_ptr(), dst.data_ptr(), C.byref(mx),
-                                         stream_handle(stream)))
+                                         _on(stream)))
         return src, dst, int(mx.value)
 
     def feature_shape(self, stream=None):
         rows, cols = C.c_int64(), C.c_int64()
         lib.check(lib.tg_csv_feature_shape(self.h, C.byref(rows), C.byref(cols),
-                                           stream_handle(stream)))
+                                           _on(stream)))
         return int(rows.value), int(cols.value)
 
     def parse_features(self, n_rows: int | None = None, device=None, stream=None):
@@ -1139,7 +1172,7 @@ class CsvText:
         n_rows = rows if n_rows is None else int(n_rows)
         out = torch.empty((n_rows, cols), dtype=torch.float32, device=device)
         lib.check(lib.tg_csv_parse_features(self.h, out.data_ptr() if out.numel() else None,
-                                            n_rows, cols, stream_handle(stream)))
+                                            n_rows, cols, _on(stream)))
         return out
 
     def close(self):
@@ -1290,7 +1323,7 @@ def load_cora_binary(path, stream=None) -> CoraData:
         ci = torch.empty(max(e, 1), dtype=torch.int32, device=dev)[:e]
         v = torch.empty(max(e, 1), dtype=torch.float32, device=dev)[:e]
         lib.check(lib.tg_cora_upload(h, x.data_ptr() if x.numel() else None, rp.data_ptr(),
-                                     ci.data_ptr(), v.data_ptr(), stream_handle(stream)))
+                                     ci.data_ptr(), v.data_ptr(), _on(stream)))
         ptrs = [C.c_void_p() for _ in range(4)]
         lib.check(lib.tg_cora_host(h, *[C.byref(p) for p in ptrs]))
         labels = np.empty(n, np.int32)
