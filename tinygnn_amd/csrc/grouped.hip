@@ -143,6 +143,42 @@ __device__ __forceinline__ void multiply(const RA& ra, const RB& rb, const char*
     }
 }
 
+// Sums of floats keep their digits: kSumTiles tiles (256 values) are one chain in
+// `now`, and the chains' sums another in `all`.  (One chain of n values is off by up
+// to n 2^-24 of the sum of sizes: a training step of 233K rows of 7 types, 602 x
+// 256, was 8.9e-7 off with it and is 3.1e-7; 2.38 -> 2.40 ms.)  A 16-bit result's
+// own rounding, 2^-9 and 2^-12, is far above a chain's: one chain.
+constexpr int kSumTiles = 8;
+
+template <typename T, int N, int M>
+struct Sums {
+    v4f now[N][M] = {}, all[sizeof(T) == 4 ? N : 1][sizeof(T) == 4 ? M : 1] = {};
+    int tiles = 0;
+    __device__ __forceinline__ void tile() {
+        if constexpr (sizeof(T) == 4)
+            if (++tiles == kSumTiles) join();
+    }
+    __device__ __forceinline__ void join() {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+#pragma unroll
+                for (int j = 0; j < M; ++j) {
+                    all[i][j] += now[i][j];
+                    now[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                }
+            tiles = 0;
+        }
+    }
+    __device__ __forceinline__ auto& result() {
+        join();
+        if constexpr (sizeof(T) == 4)
+            return all;
+        else
+            return now;
+    }
+};
+
 template <typename T, typename S, bool ALONG_W, bool DIRECT>
 __global__ __launch_bounds__(S::kThreads) void grouped_kernel(GroupedArgs a) {
     __shared__ __attribute__((aligned(16))) char a0[S::kM * kRowBytes];
@@ -176,10 +212,13 @@ __global__ __launch_bounds__(S::kThreads) void grouped_kernel(GroupedArgs a) {
     for (int t = 0; t < S::kCB; ++t)
         chunk_place<T, S::kN, !ALONG_W>(t * S::kThreads + tid, &bmaj[t], &bmin[t]);
 
-    Acc<S> acc = {};
+    Sums<T, S::kMI, S::kNJ> acc;
     const Reader<T, S::kM, false, S::kMI> ra(wm, lane);
     const Reader<T, S::kN, !ALONG_W, S::kNJ> rb(wn, lane);
-    auto compute = [&](const char* la, const char* lb) { multiply<T, S>(ra, rb, la, lb, acc); };
+    auto compute = [&](const char* la, const char* lb) {
+        multiply<T, S>(ra, rb, la, lb, acc.now);
+        acc.tile();
+    };
     if constexpr (DIRECT) {
         // offsets from the tile's first row (gathered: x's) and w's tile
         const T* xb = a.rows ? x : x + static_cast<int64_t>(r0) * a.ldx;
@@ -268,7 +307,7 @@ __global__ __launch_bounds__(S::kThreads) void grouped_kernel(GroupedArgs a) {
         pipeline<false>(tiles, a0, b0, a1, b1, load, store, compute);
     }
 
-    store_outputs<T>(a, g, r0 + wm, r1, n0 + wn, lane, acc);
+    store_outputs<T>(a, g, r0 + wm, r1, n0 + wn, lane, acc.result());
 }
 
 // The large tile (tiles.hpp): 16-bit operands that can be loaded directly, in
@@ -334,7 +373,7 @@ __global__ __launch_bounds__(kRingThreads) void grouped_ring_kernel(GroupedArgs 
 // the groups' own tiles are too few for the CUs (233K rows of 7 types, 602 x 256:
 // 70 tiles), and the chains over 33K rows too long for fp32's digits.
 template <typename T, typename S, bool DIRECT, bool BIAS>
-__global__ __launch_bounds__(S::kThreads) void wgrad_kernel(GroupedArgs a) {
+__global__ __launch_bounds__(S::kThreads, DIRECT ? 2 : 1) void wgrad_kernel(GroupedArgs a) {
     __shared__ __attribute__((aligned(16))) char a0[S::kM * kRowBytes];
     __shared__ __attribute__((aligned(16))) char b0[S::kN * kRowBytes];
     __shared__ __attribute__((aligned(16))) char a1[S::kM * kRowBytes];
@@ -365,20 +404,22 @@ __global__ __launch_bounds__(S::kThreads) void wgrad_kernel(GroupedArgs a) {
     for (int t = 0; t < S::kCB; ++t)
         chunk_place<T, S::kN, true>(t * S::kThreads + tid, &bp[t], &bc[t]);
 
-    Acc<S> acc = {};
-    v4f sum[BIAS ? S::kNJ : 1] = {};
+    Sums<T, S::kMI, S::kNJ> acc;
+    Sums<T, 1, BIAS ? S::kNJ : 1> sum;
     const bool sums = BIAS && mt == 0 && wm == 0;  // uniform
     const Frag one = ones<T>();
     const Reader<T, S::kM, true, S::kMI> ra(wm, lane);
     const Reader<T, S::kN, true, S::kNJ> rb(wn, lane);
     auto compute = [&](const char* la, const char* lb) {
-        multiply<T, S>(ra, rb, la, lb, acc);
+        multiply<T, S>(ra, rb, la, lb, acc.now);
+        acc.tile();
         if (BIAS && sums) {
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int j = 0; j < S::kNJ; ++j)
-                    sum[j] = mfma<T>(rb.read(lb, j, s), one, sum[j]);
+                    sum.now[0][j] = mfma<T>(rb.read(lb, j, s), one, sum.now[0][j]);
+            sum.tile();
         }
     };
     if constexpr (DIRECT) {
@@ -459,8 +500,8 @@ __global__ __launch_bounds__(S::kThreads) void wgrad_kernel(GroupedArgs a) {
     if (a.unit) group_rows(a.offsets, g, a.m, &first, &last);
     const bool split = lo != first || hi != last;
     const int to = split ? part : g;
-    if (a.dw) store_gradient<T>(a, split, to, k0 + wm, n0 + wn, lane, acc);
-    if (BIAS && sums) store_bias_gradient<T>(a, split, to, n0 + wn, lane, sum);
+    if (a.dw) store_gradient<T>(a, split, to, k0 + wm, n0 + wn, lane, acc.result());
+    if (BIAS && sums) store_bias_gradient<T>(a, split, to, n0 + wn, lane, sum.result()[0]);
 }
 
 constexpr int kRowParts = 64;
@@ -668,8 +709,8 @@ void launch_ring(GroupedArgs& a, bool along, hipStream_t s) {
 // x 4,096 375 us against 459 of edge 128; 10,000 rows of 8 groups 122 against
 // 113), 64 where the groups make few tiles (40,000 x 512 x 512 52 us against
 // 69; in 8 groups 88 against 67).
-// In fp32, whose digits the result keeps, no chain is longer than kLongChain
-// rows.
+// In fp32, whose digits the result keeps, no part has more than kLongChain rows
+// (64 chains of kSumTiles tiles).
 constexpr int64_t kLongChain = 16384;
 
 struct WgradPlan {
@@ -703,10 +744,8 @@ WgradPlan wgrad_plan(int64_t m, int64_t k, int64_t n, int64_t groups, int type, 
     p.parts = groups;
     const int64_t tiles = p.mt * p.nt;
     int64_t unit = std::max<int64_t>(512, ceil_div(ceil_div(m * tiles, 1024), 64) * 64);
-    if (tiles * groups >= 512 || m < 1024) {
-        if (type != TG_TYPE_F32 || m <= kLongChain) return p;
-        unit = kLongChain;
-    }
+    if (tiles * groups >= 512 || m < 1024) unit = m;
+    if (type == TG_TYPE_F32) unit = std::min(unit, kLongChain);
     if (unit >= m) return p;
     p.unit = unit;
     p.parts = most_tiles(m, groups, unit);
