@@ -32,7 +32,8 @@ struct GroupedArgs {
     void* dw;
     void* dbias;
     int unit;    // rows of a part of a group, 0: whole groups
-    float* part;  // [parts][k][n] sums of the parts, [parts][n] of dy's
+    int slots;   // most parts of groups of several
+    float* part;  // [slots][k][n] sums of those parts, [slots][n] of dy's
     float* part_bias;
 };
 
@@ -383,10 +384,10 @@ __global__ __launch_bounds__(S::kThreads, DIRECT ? 2 : 1) void wgrad_kernel(Grou
     const int part = static_cast<int>(blockIdx.x / per);
     uint32_t mt, ntile;
     tile_of(blockIdx.x % per, a.mt, a.nt, &mt, &ntile);
-    int g = part, lo, hi;
+    int g = part, lo, hi, slot = 0;
     if (a.unit == 0)
         group_rows(a.offsets, g, a.m, &lo, &hi);
-    else if (!find_tile(a.offsets, a.groups, a.m, a.unit, part, &g, &lo, &hi))
+    else if (!find_tile(a.offsets, a.groups, a.m, a.unit, part, &g, &lo, &hi, &slot))
         return;
     const int k0 = static_cast<int>(mt) * S::kM, n0 = static_cast<int>(ntile) * S::kN;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -499,7 +500,8 @@ __global__ __launch_bounds__(S::kThreads, DIRECT ? 2 : 1) void wgrad_kernel(Grou
     int first = lo, last = hi;
     if (a.unit) group_rows(a.offsets, g, a.m, &first, &last);
     const bool split = lo != first || hi != last;
-    const int to = split ? part : g;
+    if (split && slot >= a.slots) return;  // falling offsets name more than there are
+    const int to = split ? slot : g;
     if (a.dw) store_gradient<T>(a, split, to, k0 + wm, n0 + wn, lane, acc.result());
     if (BIAS && sums) store_bias_gradient<T>(a, split, to, n0 + wn, lane, sum.result()[0]);
 }
@@ -614,10 +616,10 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(GroupedArgs a) {
 }
 
 // out[g] = the sum of group g's parts, in order: `size` values each; zeros of no
-// part.
+// part.  A group of one part has none here: its sum is in out.
 template <typename T>
 __global__ __launch_bounds__(256) void parts_kernel(const int32_t* __restrict__ offsets, int m,
-                                                    int unit, int most,
+                                                    int unit, int slots,
                                                     const float* __restrict__ part, int64_t size,
                                                     T* __restrict__ out) {
     const int g = blockIdx.y, lane = threadIdx.x & (kWave - 1);
@@ -628,13 +630,13 @@ __global__ __launch_bounds__(256) void parts_kernel(const int32_t* __restrict__ 
             group_rows(offsets, base + lane, m, &lo, &hi);
             n = static_cast<int>((static_cast<int64_t>(hi) - lo + unit - 1) / unit);
         }
-        first += wave_sum(n);
+        first += wave_sum(n > 1 ? n : 0);
     }
     group_rows(offsets, g, m, &lo, &hi);
     // (falling offsets may name more parts than there are)
     int parts = static_cast<int>((static_cast<int64_t>(hi) - lo + unit - 1) / unit);
-    if (parts == 1) return;  // it is there
-    parts = parts < most - first ? parts : most - first;
+    if (parts == 1) return;
+    parts = parts < slots - first ? parts : slots - first;
     const int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
     if (at >= size) return;
     const float* p = part + first * size + at;
@@ -714,13 +716,13 @@ void launch_ring(GroupedArgs& a, bool along, hipStream_t s) {
 constexpr int64_t kLongChain = 16384;
 
 struct WgradPlan {
-    int64_t edge, mt, nt, unit, parts;  // parts: most of them
+    int64_t edge, mt, nt, unit, parts, slots;  // most parts, most of groups of several
     size_t bytes(int64_t k, int64_t n, float** part, float** part_bias, void* ws,
                  size_t size) const {
         Carver c(ws, size);
         if (unit == 0) return 0;
-        float* p = c.take<float>(static_cast<size_t>(parts * k * n));
-        float* b = c.take<float>(static_cast<size_t>(parts * n));
+        float* p = c.take<float>(static_cast<size_t>(slots * k * n));
+        float* b = c.take<float>(static_cast<size_t>(slots * n));
         if (part) *part = p;
         if (part_bias) *part_bias = b;
         return c.bytes();
@@ -749,6 +751,8 @@ WgradPlan wgrad_plan(int64_t m, int64_t k, int64_t n, int64_t groups, int type, 
     if (unit >= m) return p;
     p.unit = unit;
     p.parts = most_tiles(m, groups, unit);
+    // a group of several has more than `unit` rows: m / unit such groups at most
+    p.slots = m / unit + std::min(groups, m / unit);
     return p;
 }
 
@@ -757,6 +761,7 @@ void launch_wgrad(GroupedArgs& a, const WgradPlan& p, bool direct, hipStream_t s
     a.mt = static_cast<uint32_t>(p.mt);
     a.nt = static_cast<uint32_t>(p.nt);
     a.unit = static_cast<int>(p.unit);
+    a.slots = static_cast<int>(p.slots);
     const unsigned grid = grid_of("grouped_matmul_wgrad", p.mt * p.nt * p.parts, kRingThreads);
     auto tiled = [&](auto shape) {
         using S = decltype(shape);
@@ -788,7 +793,7 @@ void launch_wgrad(GroupedArgs& a, const WgradPlan& p, bool direct, hipStream_t s
         const dim3 blocks(grid_of("grouped_matmul_wgrad", ceil_div(size, 1024), 256),
                           static_cast<unsigned>(a.groups));
         parts_kernel<T><<<blocks, 256, 0, s>>>(a.offsets, a.m, a.unit,
-                                               static_cast<int>(p.parts), part, size,
+                                               a.slots, part, size,
                                                static_cast<T*>(out));
         TG_LAUNCH_CHECK();
     };

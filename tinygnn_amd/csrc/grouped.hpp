@@ -25,9 +25,11 @@ __device__ __forceinline__ void group_rows(const int32_t* __restrict__ offsets, 
 // The tile of `unit` rows with number t over all groups, each cut from its own
 // first row: its group and rows [*r0, *r1); false past the last.  Every
 // wavefront finds it by itself, 64 groups at a time (offsets come from L2).
-// offsets null: one group of all m rows.
+// offsets null: one group of all m rows.  `slot` (or null): the tile's number among
+// those of groups of several.
 __device__ __forceinline__ bool find_tile(const int32_t* __restrict__ offsets, int groups, int m,
-                                          int unit, int t, int* g, int* r0, int* r1) {
+                                          int unit, int t, int* g, int* r0, int* r1,
+                                          int* slot = nullptr) {
     if (offsets == nullptr) {
         *g = 0;
         *r0 = t * unit;
@@ -35,11 +37,14 @@ __device__ __forceinline__ bool find_tile(const int32_t* __restrict__ offsets, i
         return *r0 < m;
     }
     const int lane = threadIdx.x & (kWave - 1);
+    int slots = 0;
     for (int base = 0; base < groups; base += kWave) {
         int lo = 0, hi = 0;
         if (base + lane < groups) group_rows(offsets, base + lane, m, &lo, &hi);
         const int n = static_cast<int>((static_cast<int64_t>(hi) - lo + unit - 1) / unit);
         const int upto = wave_inclusive_scan(n);
+        const int several = n > 1 ? n : 0;
+        const int mine = slot ? wave_inclusive_scan(several) : 0;
         const uint64_t past = __ballot(upto > t);
         if (past) {
             const int w = __ffsll(static_cast<unsigned long long>(past)) - 1;
@@ -48,8 +53,10 @@ __device__ __forceinline__ bool find_tile(const int32_t* __restrict__ offsets, i
             *g = base + w;
             *r0 = a + (t - first) * unit;
             *r1 = b - *r0 > unit ? *r0 + unit : b;
+            if (slot) *slot = slots + __builtin_amdgcn_readlane(mine - several, w) + t - first;
             return true;
         }
+        if (slot) slots += __builtin_amdgcn_readlane(mine, kWave - 1);
         t -= __builtin_amdgcn_readlane(upto, kWave - 1);
     }
     return false;
