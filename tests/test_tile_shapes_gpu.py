@@ -3,13 +3,15 @@ at sizes from both sides of the rules that choose it, against 64 bits.
 
 Tolerances (u = 2^-24) as in test_grouped_gpu: a float32 sum of k products is
 off by (k + 8) u sum|a||b| at most, bias and epilogue among it, the result
-rounded to its type; e4m3 products of 16-bit results by 2^-12 sum|a||b| more."""
+rounded to its type; e4m3 products of 16-bit results by 2^-12 sum|a||b| more.
+Where operands are -1, 0 and 1 the sums are exact, and results equal."""
 import re
 
 import pytest
 import torch
 
-from expert_cases import DTYPES, U, e4m3, gen, grouped, half_step, least, offsets_of, randn, within
+from expert_cases import (DTYPES, U, e4m3, gen, grouped, half_step, least, offsets_of, randn,
+                          wgrad, within)
 
 pytestmark = pytest.mark.gpu
 
@@ -24,12 +26,13 @@ def kernels(fn):
 
 
 def shape_of(names, kernel):
-    """(rows, columns) of the tile of the one kernel of a name, which is mangled
-    or not, as the profiler can."""
+    """(rows, columns, flags) of the tile of the one kernel of a name, which is
+    mangled or not, as the profiler can."""
     found = [n for n in names if re.search(rf"(\b|\d){kernel}(<|I)", n)]
     assert len(found) == 1, (kernel, names)
-    shape = re.search(r"Shape(?:<|ILi)(\d+)(?:, |ELi)(\d+)", found[0])
-    return int(shape[1]), int(shape[2])
+    shape = re.search(r"Shape(?:<|ILi)(\d+)(?:, |ELi)(\d+)(.*)", found[0])
+    flags = re.findall(r"true|false|Lb[01]E", shape[3])
+    return int(shape[1]), int(shape[2]), [f in ("true", "Lb1E") for f in flags]
 
 
 def tolerance(want, size, k, dt, own=0.0):
@@ -71,7 +74,7 @@ def check_fp8(dt, m, k, n, sizes, gather, want_shape):
                              out=out)
 
     got, names = kernels(run)
-    assert shape_of(names, "fp8_kernel") == want_shape
+    assert shape_of(names, "fp8_kernel")[:2] == want_shape
     inside = ~torch.isnan(want[:, 0])
     own = 0.0 if dt == torch.float32 else 2.0 ** -12
     within(got[inside], want[inside], tolerance(want, size, k, dt, own)[inside], "y")
@@ -91,3 +94,134 @@ def test_fp8_many_tiles(gpu, dtype, m, k, n, sizes, gather):
     """256 x 256 for 160 and more tiles of eight and more blocks and 16-bit
     results, 128 x 128 for fp32 ones."""
     check_fp8(DTYPES[dtype], m, k, n, sizes, gather, (128, 128) if dtype == "f32" else (256, 256))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("m,k,n,sizes,gather", [
+    (1500, 300, 200, [700, 0, 1, 799], False),
+    (500, 900, 136, [3, 1200, 64, 0, 65, 700], True),
+])
+def test_fp8_small(gpu, dtype, m, k, n, sizes, gather):
+    """64 x 64 for more than 1,024 tiles of 16 x 16 and fewer than 300 of 128 x
+    128, in several groups."""
+    check_fp8(DTYPES[dtype], m, k, n, sizes, gather, (64, 64))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("m,k,n,sizes,gather", [
+    (10_000, 400, 520, [5000, 0, 129, 4871], False),
+    (3000, 130, 648, [1, 6000, 0, 3999], True),
+])
+def test_fp8_medium(gpu, dtype, m, k, n, sizes, gather):
+    """128 x 128 for 300 and more tiles, of fewer than eight blocks."""
+    check_fp8(DTYPES[dtype], m, k, n, sizes, gather, (128, 128))
+
+
+def integers(g, shape, dt):
+    """-1, 0 and 1: sums of up to 2^24 products are exact in fp32 in any order,
+    so results equal the 64-bit sum rounded to their type."""
+    return torch.randint(-1, 2, shape, generator=g, device="cuda").to(dt)
+
+
+def gathered(g, m, x_rows):
+    rows = torch.randint(0, x_rows, (m,), generator=g, device="cuda", dtype=torch.int32)
+    rows[[0, m // 2]] = torch.tensor([x_rows, -1], dtype=torch.int32, device="cuda")
+    return rows
+
+
+HALF, FLOAT = ["bf16", "f16"], ["f32"]
+RING = None
+
+
+@pytest.mark.parametrize("transpose", [False, True])
+@pytest.mark.parametrize("gather", [False, True])
+@pytest.mark.parametrize("dtypes,sizes,k,n,shape,direct", [
+    (HALF, [3, 0, 40, 1, 0], 72, 130, (32, 128), True),
+    (HALF, [3, 0, 40, 1, 0], 71, 131, (32, 128), False),
+    (HALF, [200, 0, 55], 64, 200, (64, 64), True),
+    (HALF, [200, 0, 55], 65, 201, (64, 64), False),
+    (HALF, [20000, 0, 1, 19999], 64, 130, (128, 128), True),
+    (HALF, [20000, 0, 1, 19999], 33, 131, (128, 128), False),    # odd rows: by registers
+    (HALF, [30000, 129, 9000], 257, 129, (128, 128), False),
+    (HALF, [2000, 0, 3001], 1024, 2048, RING, True),
+    (HALF, [2000, 0, 3001], 1160, 2056, RING, True),             # ends inside a part, a tile
+    (FLOAT, [3, 0, 40, 1, 0], 71, 131, (32, 128), True),
+    (FLOAT, [200, 0, 55], 65, 201, (64, 64), True),
+    (FLOAT, [20000, 0, 1, 19999], 301, 100, (64, 128), True),
+])
+def test_grouped_forward(gpu, dtypes, sizes, k, n, shape, direct, gather, transpose):
+    import tinygnn_amd as tg
+    m, off = sum(sizes), offsets_of(sizes)
+    for dt in (DTYPES[d] for d in dtypes):
+        g = gen(m + k)
+        x = integers(g, (m // 2 + 1 if gather else m, k), dt)
+        rows = gathered(g, m, x.shape[0]) if gather else None
+        w = integers(g, (len(sizes), n, k) if transpose else (len(sizes), k, n), dt)
+        got, names = kernels(lambda: tg.grouped_matmul(x, w, off, rows=rows,
+                                                       transpose=transpose))
+        if shape is RING:
+            assert any("grouped_ring_kernel" in v for v in names), names
+        else:
+            assert shape_of(names, "grouped_kernel") == (*shape, [transpose, direct])
+        want, _ = grouped(x, w, off, rows=rows, transpose=transpose)
+        assert torch.equal(got, want.to(dt))
+
+
+@pytest.mark.parametrize("gather", [False, True])
+@pytest.mark.parametrize("dtypes,sizes,k,n,shape,direct", [
+    (HALF, [900, 0, 1, 355], 130, 200, (64, 64), True),
+    (HALF, [900, 0, 1, 355], 131, 201, (64, 64), False),
+    (HALF, [1537, 0, 1, 3462], 1030, 1032, (128, 128), True),     # parts of 512 rows
+    (HALF, [1537, 0, 1, 3462], 1031, 1033, (128, 128), False),    # odd rows: by registers
+    (HALF, [200 + 7 * (i % 23) for i in range(62)] + [5003, 0], 512, 2048, RING, True),
+    (FLOAT, [900, 0, 1, 355], 131, 201, (64, 64), True),
+    (FLOAT, [1537, 0, 1, 3462], 1031, 1033, (128, 128), True),
+    (FLOAT + HALF, [0, 9000, 1, 40, 9001, 513], 70, 66, (64, 64), True),
+    (FLOAT + HALF, [1_100_000, 3, 0, 700], 16, 16, (64, 64), True),
+])
+def test_grouped_gradient(gpu, dtypes, sizes, k, n, shape, direct, gather):
+    """dw and dbias; the oracle without the last row of the largest group, or of
+    one of its parts, differs."""
+    import tinygnn_amd as tg
+    m, off = sum(sizes), offsets_of(sizes)
+    for dt in (DTYPES[d] for d in dtypes):
+        g = gen(m + k)
+        x = integers(g, (m // 2 + 1 if gather else m, k), dt)
+        rows = gathered(g, m, x.shape[0]) if gather else None
+        dy = integers(g, (m, n), dt)
+        got, names = kernels(lambda: tg.grouped_matmul_wgrad(x, dy, off, rows=rows, bias=True))
+        if shape is RING:
+            assert any("wgrad_ring_kernel" in v for v in names), names
+        else:
+            assert shape_of(names, "wgrad_kernel") == (*shape, [direct, True])
+        dw, _, db, _ = wgrad(x, dy, off, rows=rows)
+        assert torch.equal(got[0], dw.to(dt)) and torch.equal(got[1], db.to(dt))
+        most = max(range(len(sizes)), key=lambda i: sizes[i])
+        for p in (int(off[most + 1]) - 1, int(off[most]) + 511):
+            r = p if rows is None else int(rows[p])
+            row = x[r].double() if 0 <= r < x.shape[0] else x[0].double() * 0
+            assert bool(row.any()) and bool(dy[p].any())
+            less = dw[most] - row[:, None] * dy[p].double()[None]
+            assert not torch.equal(got[0][most], less.to(dt))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_grouped_far_rows(gpu, dtype):
+    """Rows gathered from places past 2^31 bytes: by registers, whatever the
+    alignment."""
+    import tinygnn_amd as tg
+    dt, g = DTYPES[dtype], gen(5)
+    sizes, k, n = [20000, 0, 1, 22999, 300], 38, 100
+    m, off = sum(sizes), offsets_of(sizes)
+    lead = 2 ** 34 // torch.finfo(dt).bits // m + 200
+    x = torch.empty(m, lead, dtype=dt, device="cuda")[:, :k]
+    x.copy_(integers(g, (m, k), dt))
+    rows = gathered(g, m, m)
+    w, dy = integers(g, (len(sizes), k, n), dt), integers(g, (m, n), dt)
+    got, names = kernels(lambda: tg.grouped_matmul(x, w, off, rows=rows))
+    assert shape_of(names, "grouped_kernel")[2] == [False, False]
+    assert torch.equal(got, grouped(x, w, off, rows=rows)[0].to(dt))
+    got, names = kernels(lambda: tg.grouped_matmul_wgrad(x, dy, off, rows=rows, bias=True))
+    assert shape_of(names, "wgrad_kernel")[2] == [False, True]
+    dw, _, db, _ = wgrad(x, dy, off, rows=rows)
+    assert torch.equal(got[0], dw.to(dt)) and torch.equal(got[1], db.to(dt))
