@@ -458,9 +458,10 @@ int tg_grouped_matmul_wgrad(int64_t m, int64_t k, int64_t n, int64_t groups, int
  *   q [groups][n x kp] and scale [groups][ceil(n/128) x kp/128].
  * tg_matmul_fp8: y[p] = epilogue(sum over b of xscale_b[p] * wscale_b[n/128] *
  *   (the products of block b), + bias), sums in fp32, y and bias of `type`.
- *   With a 16-bit `type` the products of a block go through the e4m3 matrix
- *   instructions, whose sum is within 2^-12 of the sum of the products' sizes
- *   (normal operands: 2^-16); with TG_TYPE_F32 it is that of an fp32 sum;
+ *   With a 16-bit `type` and many rows the products of a block go through the
+ *   e4m3 matrix instructions, whose sum is within 2^-12 of the sum of the products'
+ *   sizes (normal operands: 2^-16); with few rows (1,024 tiles of 16 x 16 results
+ *   at most) or TG_TYPE_F32 it is that of an fp32 sum;
  *   offsets NULL: one matrix for all m rows (groups = 1), else groups as for
  *   tg_grouped_matmul; rows as there, over x_rows quantised rows.  xq and wq
  *   are 16-byte aligned (as allocated).

@@ -117,6 +117,23 @@ def test_fp8_medium(gpu, dtype, m, k, n, sizes, gather):
     check_fp8(DTYPES[dtype], m, k, n, sizes, gather, (128, 128))
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("m,kb,n", [(1, 1, 16), (5, 3, 40), (33, 9, 130)])
+def test_fp8_few_rows_keep_small_products(gpu, dtype, m, kb, n):
+    """Large products that cancel leave the small ones beside them: each block
+    sums to 240 * 240 - 240 * 240 + 126 / 8."""
+    import tinygnn_amd as tg
+    x, w = torch.full((m, kb, 128), 0.5), torch.full((n, kb, 128), 0.25)
+    x[:, :, [3, 90]], w[:, :, 3], w[:, :, 90] = 240, 240, -240
+    f8 = torch.float8_e4m3fn
+    xq = tg.BlockRows(x.flatten(1).to("cuda", f8), torch.ones(kb, m, device="cuda"), kb * 128)
+    wq = tg.BlockWeight(w.flatten(1).to("cuda", f8),
+                        torch.ones(-(-n // 128), kb, device="cuda"), kb * 128)
+    got, names = kernels(lambda: tg.matmul_fp8(xq, wq, dtype=DTYPES[dtype]))
+    assert any("fp8_thin_kernel" in v for v in names), names
+    assert torch.equal(got, torch.full((m, n), 15.75 * kb).to(DTYPES[dtype]).cuda())
+
+
 def integers(g, shape, dt):
     """-1, 0 and 1: sums of up to 2^24 products are exact in fp32 in any order,
     so results equal the 64-bit sum rounded to their type."""

@@ -131,12 +131,15 @@ __device__ __forceinline__ v8h to_f16(uint32_t lo, uint32_t hi) {
     return v;
 }
 
-// The sum of a block's products, 16 x 16.  The e4m3 matrix instructions line
-// the products up with the largest of them and drop what lies far below it:
-// against 64 bits a block's sum is off by up to 2^-12.8 of the sum of its
-// products' sizes for operands of random bits, 2^-16.3 (2^-18.9 in the mean) for
-// normal ones.  That is below a 16-bit result's own rounding; for fp32 results
-// (WIDE) the operands are widened to fp16, exactly, at half the rate.
+// The sum of a block's products, 16 x 16.  The e4m3 matrix instructions (of any
+// shape) line the products up with the largest of them and drop what lies far
+// below it: against 64 bits a block's sum is off by up to 2^-12.5 of the sum of its
+// products' sizes for operands of random bits, 2^-16.1 (2^-19.6 in the mean) for
+// normal ones.  A 16-bit result of many rows takes that for twice the rate: it is
+// far below the operands' own rounding to e4m3 (2^-4 of each product), though where
+// a sum cancels it can be far above the result's to 2^-9 or 2^-12.
+// Where the rate does not count (few rows) and for fp32 results the operands
+// are widened to fp16, exactly (WIDE).
 template <bool WIDE>
 __device__ __forceinline__ v4f block_products(const Operand& a, const Operand& b) {
     v4f p = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -367,13 +370,13 @@ __global__ __launch_bounds__(S::kThreads) void fp8_kernel(Fp8Args a) {
 
 // Few rows: 16 rows x 16 columns, each of four wavefronts a quarter of the
 // blocks straight from memory (w is read once, and that is what counts), four
-// blocks in flight; their sums are joined in LDS, in order.
+// blocks in flight; their sums are joined in LDS, in order.  The products are exact
+// (5 rows of 4,096 x 4,096 7.0 us against 6.6 of the e4m3 instructions).
 constexpr int kThinWaves = 4, kThinAhead = 4;
 
 template <typename T>
 __global__ __launch_bounds__(64 * kThinWaves) void fp8_thin_kernel(Fp8Args a) {
     __shared__ v4f join[kThinWaves - 1][64];
-    constexpr bool WIDE = sizeof(T) == 4;
     uint32_t mt, ntile;
     if (!tile_of(blockIdx.x, count_tiles(a.offsets, a.groups, a.m, 16), a.nt, &mt, &ntile)) return;
     int g, r0, r1;
@@ -408,7 +411,7 @@ __global__ __launch_bounds__(64 * kThinWaves) void fp8_thin_kernel(Fp8Args a) {
         }
 #pragma unroll
         for (int u = 0; u < kThinAhead; ++u) {
-            const v4f p = block_products<WIDE>(w[u], x[u]);
+            const v4f p = block_products<true>(w[u], x[u]);
             if (base + u >= b1) break;
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(p[e], s[u], acc[e]);
@@ -451,7 +454,7 @@ void launch_fp8(Fp8Args& a, hipStream_t s) {
         return most_tiles(a.m, a.groups, edge) * ceil_div(a.n, edge);
     };
     // Few rows: the thin form while its workgroups are few (5 rows of 4,096 x
-    // 4,096 7.6 us, 12 in 64 x 64; 150 rows of 32 groups, 2,048 x 4,096, 62 us
+    // 4,096 7.0 us, 12 in 64 x 64; 150 rows of 32 groups, 2,048 x 4,096, 62 us
     // against 41).  Large tiles where there are 160 of them of 1,024 values and the
     // groups fill them (2,500 x 2,048 x 4,096 46 us against 50; 40,000 x 512 x 512
     // 36 against 32; 16,384 rows of 32 groups, 2,048 x 4,096, 220 against 300, 4,096
