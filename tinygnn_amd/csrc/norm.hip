@@ -11,10 +11,10 @@
 //
 // A row is taken by as many threads as one 16-byte load of x each covers, 64
 // (four rows a workgroup, no barrier) to 1,024, then by 1,024 with two or four
-// loads each, up to 16,384 columns: few registers, so many wavefronts a SIMD (16
-// values a thread kept the backward pass at two of them: 16,384 x 4,096 bf16 170
-// us against 105).  Wider rows are walked by 1,024 threads, out of L2 after the
-// first time.
+// loads each: forward up to 16,384 columns, backward up to 8,192.  Few registers, so
+// many wavefronts a SIMD (16 values a thread kept the backward pass at two of
+// them: 16,384 x 4,096 bf16 170 us against 105).  Wider rows are walked by 1,024
+// threads, out of L2 after the first time.
 #include "common.hpp"
 #include "device_utils.hpp"
 #include "types.hpp"
@@ -337,7 +337,7 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(const float* __restri
                                                            void* dgamma, void* dbeta, int f32) {
     __shared__ float lds[16][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+    const int64_t c = (static_cast<int64_t>(blockIdx.z) * gridDim.x + blockIdx.x) * 64 + lane;
     const int which = blockIdx.y;
     const int64_t share = (parts + 15) / 16;
     const int64_t lo = w * share, hi = lo + share < parts ? lo + share : parts;
@@ -546,7 +546,10 @@ int tg_layer_norm_backward(int64_t rows, int64_t cols, int type, const void* dy,
                 TG_LAUNCH_CHECK();
             }
             if (sums) {
-                const dim3 grid(static_cast<unsigned>(tg::ceil_div(cols, 64)), 2);
+                // (2^22 workgroups of 1,024 threads are more than a grid's x takes)
+                const int64_t b = tg::ceil_div(cols, 64), z = tg::ceil_div(b, 1 << 21);
+                const dim3 grid(static_cast<unsigned>(tg::ceil_div(b, z)), 2,
+                                static_cast<unsigned>(z));
                 tg::norm_reduce_kernel<T><<<grid, 1024, 0, s>>>(a.part, rows > 0 ? blocks : 0, cols,
                                                                 dgamma, dbeta,
                                                                 weight_type == TG_TYPE_F32);
