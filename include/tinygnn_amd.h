@@ -425,7 +425,8 @@ int tg_route_combine_backward(int64_t tokens, int64_t k, int64_t cols, int type,
  * sums are in fp32 and rounded once.  offsets: groups + 1 int32 on the device,
  * not falling, within [0, m]; rows outside all groups are not written (of a
  * falling or outside offset, only rows within [0, m) are ever touched).  y
- * overlaps no input.  At most 1,024 groups; m, k, n < 2^31 - 4096.
+ * overlaps no input.  At most 1,024 groups; m, k, n < 2^31 - 4096, and fewer than
+ * 2^24 tiles of 64 x 64 results.
  *
  * tg_grouped_matmul_wgrad: dw_g = (rows of x of group g)^T * (those of dy),
  * [groups x k x n] contiguous, and dbias_g = sum of those rows of dy
@@ -453,7 +454,8 @@ int tg_grouped_matmul_wgrad(int64_t m, int64_t k, int64_t n, int64_t groups, int
  * value e4m3(x / scale), product and quotient rounded to fp32, the quotient then
  * to nearest even; a NaN stays NaN, and an infinity makes its block NaN.
  * tg_quantize: x [rows x cols] to q [rows x kp], kp = cols rounded up to whole
- *   128 (zeros there), and scale [kp/128 x rows]: row r, block b at b*rows + r.
+ *   128 (zeros there), and scale [kp/128 x rows]: row r, block b at b*rows + r;
+ *   rows * kp < 2^36.
  * tg_quantize_weight: w [groups][k x n] (ldw, w_stride; transposed: [n x k]) to
  *   q [groups][n x kp] and scale [groups][ceil(n/128) x kp/128].
  * tg_matmul_fp8: y[p] = epilogue(sum over b of xscale_b[p] * wscale_b[n/128] *

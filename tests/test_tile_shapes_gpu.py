@@ -242,3 +242,18 @@ def test_grouped_far_rows(gpu, dtype):
     assert shape_of(names, "wgrad_kernel")[2] == [False, True]
     dw, _, db, _ = wgrad(x, dy, off, rows=rows)
     assert torch.equal(got[0], dw.to(dt)) and torch.equal(got[1], db.to(dt))
+
+
+def test_falling_offsets_of_many_rows(gpu):
+    """Offsets that fall 512 times from m to 0 name 2^31 tiles and more of 64
+    rows: rows of x and y alone are touched."""
+    import tinygnn_amd as tg
+    m, groups, guard = 3 << 27, 1024, 1 << 20
+    off = torch.tensor([0, m] * 512 + [0], dtype=torch.int32, device="cuda")
+    x = torch.full((m, 1), 2.0, device="cuda")
+    out = torch.full((guard + m + guard, 1), 7.0, device="cuda")
+    w = torch.full((groups, 1, 1), 3.0, device="cuda")
+    tg.grouped_matmul(x, w, off, out=out[guard:guard + m])
+    assert bool((out[:guard] == 7).all()) and bool((out[guard + m:] == 7).all())
+    inside = out[guard:guard + m]
+    assert bool(((inside == 6) | (inside == 7)).all()) and bool((inside == 6).any())

@@ -64,7 +64,9 @@ __device__ __forceinline__ bool find_tile(const int32_t* __restrict__ offsets, i
 
 // Row tiles of `unit` rows of all groups.  (Their number decides which tiles an
 // XCD takes: with the most that there can be instead, the last XCDs had only
-// tiles that do not exist, and 256 tiles took two rounds of the 256 CUs.)
+// tiles that do not exist, and 256 tiles took two rounds of the 256 CUs.)  Falling
+// offsets can name more rows than m, 512 times at most: the lanes' counts stop at
+// 2^24, below which a launch's tiles are, and their sum is a whole number.
 __device__ __forceinline__ int count_tiles(const int32_t* __restrict__ offsets, int groups, int m,
                                            int unit) {
     if (offsets == nullptr) return static_cast<int>((static_cast<int64_t>(m) + unit - 1) / unit);
@@ -75,7 +77,7 @@ __device__ __forceinline__ int count_tiles(const int32_t* __restrict__ offsets, 
         if (base + lane < groups) group_rows(offsets, base + lane, m, &lo, &hi);
         n += static_cast<int>((static_cast<int64_t>(hi) - lo + unit - 1) / unit);
     }
-    return __builtin_amdgcn_readfirstlane(wave_sum(n));
+    return __builtin_amdgcn_readfirstlane(wave_sum(std::min(n, 1 << 24)));
 }
 
 // Most tiles of `unit` rows that m rows in `groups` groups can make.
