@@ -257,3 +257,27 @@ def test_falling_offsets_of_many_rows(gpu):
     assert bool((out[:guard] == 7).all()) and bool((out[guard + m:] == 7).all())
     inside = out[guard:guard + m]
     assert bool(((inside == 6) | (inside == 7)).all()) and bool((inside == 6).any())
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("m,k,n", [(20, 300, 40), (1500, 300, 200), (10_000, 400, 520),
+                                   (2600, 1100, 4104)])
+@pytest.mark.parametrize("x_rows", [0, 50])
+def test_fp8_rows_of_zeros_times_nan(gpu, dtype, m, k, n, x_rows):
+    """An index outside x is a row of zeros in every tile shape, as in
+    grouped_matmul: 0 times a NaN, in a weight or in a scale, is NaN."""
+    import tinygnn_amd as tg
+    dt, g = DTYPES[dtype], gen(m)
+    w = randn(g, (k, n), torch.float32)
+    w[k // 2, 5] = float("nan")
+    x = randn(g, (x_rows, k), torch.float32)
+    rows = torch.full((m,), x_rows, dtype=torch.int32, device="cuda")
+    if x_rows:
+        rows[::2] = torch.randint(0, x_rows, (len(rows[::2]),), generator=g, device="cuda").int()
+    got = tg.matmul_fp8(tg.quantize(x), tg.quantize_weight(w), rows=rows, dtype=dt)
+    outside = rows == x_rows
+    other = [i for i in range(n) if i != 5]
+    assert torch.isnan(got[:, 5]).all() and not got[outside][:, other].any()
+    assert torch.isfinite(got[:, other]).all()
+    y = tg.grouped_matmul(x, w[None], offsets_of([m]), rows=rows)
+    assert torch.equal(torch.isnan(y), torch.isnan(got))

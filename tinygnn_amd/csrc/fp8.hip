@@ -371,7 +371,8 @@ __global__ __launch_bounds__(S::kThreads) void fp8_kernel(Fp8Args a) {
 // Few rows: 16 rows x 16 columns, each of four wavefronts a quarter of the
 // blocks straight from memory (w is read once, and that is what counts), four
 // blocks in flight; their sums are joined in LDS, in order.  The products are exact
-// (5 rows of 4,096 x 4,096 7.0 us against 6.6 of the e4m3 instructions).
+// (5 rows of 4,096 x 4,096 6.0 us, 64 x 2,048 x 4,096 10.6; with the e4m3
+// instructions' dropped bits 6.6 and 10.6).
 constexpr int kThinWaves = 4, kThinAhead = 4;
 
 template <typename T>
@@ -388,16 +389,18 @@ __global__ __launch_bounds__(64 * kThinWaves) void fp8_thin_kernel(Fp8Args a) {
     const int src = r0 + r < r1 ? source_row(a, r0 + r) : -1;
     const int col = n0 + r < a.n ? n0 + r : a.n - 1;  // past the last: computed, not stored
     const int nb = (a.n + kBlock - 1) / kBlock;
-    const uint8_t* px = a.xq + (src < 0 ? 0 : src) * kp + 16 * q;
+    const uint8_t* px = a.xq + (src < 0 ? 0 : src) * kp + 16 * q;  // (any: not used)
     const uint8_t* pw = a.wq + (static_cast<int64_t>(g) * a.n + col) * kp + 16 * q;
     const float* xs = a.xscale + (src < 0 ? 0 : src);
     const float* ws = a.wscale + (static_cast<int64_t>(g) * nb + n0 / kBlock) * a.kb;
     const int share = (a.kb + kThinWaves - 1) / kThinWaves;
     const int b0 = wave * share, b1 = b0 + share < a.kb ? b0 + share : a.kb;
+    const uint32_t keep = src < 0 ? 0 : ~0u;
+    const v4u kept = {keep, keep, keep, keep};
     v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int base = b0; base < b1; base += kThinAhead) {
         Operand x[kThinAhead], w[kThinAhead];
-        float s[kThinAhead];
+        float sx[kThinAhead], sw[kThinAhead];
 #pragma unroll
         for (int u = 0; u < kThinAhead; ++u) {
             const int b = base + u < b1 ? base + u : b1 - 1;  // again, for nothing
@@ -407,14 +410,24 @@ __global__ __launch_bounds__(64 * kThinWaves) void fp8_thin_kernel(Fp8Args a) {
                 w[u].c[h].u = *reinterpret_cast<const v4u*>(pw + at + 64 * h);
                 x[u].c[h].u = *reinterpret_cast<const v4u*>(px + at + 64 * h);
             }
-            s[u] = xs[static_cast<int64_t>(b) * a.x_rows] * ws[b];
+            sx[u] = xs[static_cast<int64_t>(b) * a.x_rows];
+            sw[u] = ws[b];
+        }
+        if (a.rows) {  // an index outside x is a row of zeros
+#pragma unroll
+            for (int u = 0; u < kThinAhead; ++u) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) x[u].c[h].u &= kept;
+                if (src < 0) sx[u] = 0.0f;
+            }
         }
 #pragma unroll
         for (int u = 0; u < kThinAhead; ++u) {
             const v4f p = block_products<true>(w[u], x[u]);
             if (base + u >= b1) break;
+            const float s = sx[u] * sw[u];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(p[e], s[u], acc[e]);
+            for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(p[e], s, acc[e]);
         }
     }
     if (wave > 0) join[wave - 1][lane] = acc;
@@ -422,7 +435,6 @@ __global__ __launch_bounds__(64 * kThinWaves) void fp8_thin_kernel(Fp8Args a) {
     if (wave > 0 || r0 + r >= r1) return;
 #pragma unroll
     for (int u = 0; u < kThinWaves - 1; ++u) acc += join[u][lane];
-    if (src < 0) acc = v4f{0.0f, 0.0f, 0.0f, 0.0f};  // a row of zeros
     const v4f bias = bias_of<T>(a, g, n0 + 4 * q);
     with_epilogue(a.epi, [&](auto epi) {
         store_outputs<T, decltype(epi)::value>(a, r0 + r, n0 + 4 * q, acc, bias);
@@ -454,7 +466,7 @@ void launch_fp8(Fp8Args& a, hipStream_t s) {
         return most_tiles(a.m, a.groups, edge) * ceil_div(a.n, edge);
     };
     // Few rows: the thin form while its workgroups are few (5 rows of 4,096 x
-    // 4,096 7.0 us, 12 in 64 x 64; 150 rows of 32 groups, 2,048 x 4,096, 62 us
+    // 4,096 6.0 us, 12 in 64 x 64; 150 rows of 32 groups, 2,048 x 4,096, 62 us
     // against 41).  Large tiles where there are 160 of them of 1,024 values and the
     // groups fill them (2,500 x 2,048 x 4,096 46 us against 50; 40,000 x 512 x 512
     // 36 against 32; 16,384 rows of 32 groups, 2,048 x 4,096, 220 against 300, 4,096
@@ -579,7 +591,10 @@ int tg_matmul_fp8(int64_t m, int64_t k, int64_t n, int64_t groups, const void* x
         a.epi = epilogue;
         a.y = y;
         a.ldy = ldy;
-        if (x_rows == 0) a.kb = 0;  // every row is one of zeros
+        if (x_rows == 0) {  // every row is one of zeros: read, and not used
+            a.xq = a.wq;
+            a.xscale = a.wscale;
+        }
         tg::with_type(type, "matmul_fp8", [&](auto t) {
             tg::launch_fp8<decltype(t)>(a, static_cast<hipStream_t>(stream));
         });
