@@ -147,8 +147,10 @@ __device__ __forceinline__ void multiply(const RA& ra, const RB& rb, const char*
 // Sums of floats keep their digits: kSumTiles tiles (256 values) are one chain in
 // `now`, and the chains' sums another in `all`.  (One chain of n values is off by up
 // to n 2^-24 of the sum of sizes: a training step of 233K rows of 7 types, 602 x
-// 256, was 8.9e-7 off with it and is 3.1e-7; 2.38 -> 2.40 ms.)  A 16-bit result's
-// own rounding, 2^-9 and 2^-12, is far above a chain's: one chain.
+// 256, was 8.9e-7 off with it and is 3.1e-7; 2.38 -> 2.40 ms.)  16-bit products
+// are one chain, to which the instructions add eight at a time: n of one sign are
+// off by n 2^-27 of their sum at most, n^(1/2) 2^-25 or so of random ones; the
+// result's own rounding is 2^-9 or 2^-12.
 constexpr int kSumTiles = 8;
 
 template <typename T, int N, int M>
