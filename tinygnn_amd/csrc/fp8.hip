@@ -342,13 +342,13 @@ __global__ __launch_bounds__(S::kThreads) void fp8_kernel(Fp8Args a) {
         put(a0);
     }
     while (kt + 1 < a.kb) {  // compute() counts
-        step_border<0>();
+        loads_border();
         compute(a0, b0, a1, b1);
-        step_border<0>();
+        loads_border();
         compute(a1, b1, a0, b0);
     }
     if (kt < a.kb) {
-        step_border<0>();
+        loads_border();
         compute(a0, b0, a1, b1);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");

@@ -147,20 +147,13 @@ __device__ __forceinline__ void multiply(const RA& ra, const RB& rb, const char*
 // Sums of floats keep their digits: kSumTiles tiles (256 values) are one chain in
 // `now`, and the chains' sums another in `all`.  (One chain of n values is off by up
 // to n 2^-24 of the sum of sizes: a training step of 233K rows of 7 types, 602 x
-// 256, was 8.9e-7 off with it and is 3.1e-7; 2.38 -> 2.40 ms.)  16-bit products
+// 256, was 8.9e-7 off with it and is 3.1e-7; 2.27 -> 2.31 ms.)  16-bit products
 // are one chain, to which the instructions add eight at a time: n of one sign are
 // off by n 2^-27 of their sum at most, n^(1/2) 2^-25 or so of random ones; the
 // result's own rounding is 2^-9 or 2^-12.
-constexpr int kSumTiles = 8;
-
 template <typename T, int N, int M>
 struct Sums {
     v4f now[N][M] = {}, all[sizeof(T) == 4 ? N : 1][sizeof(T) == 4 ? M : 1] = {};
-    int tiles = 0;
-    __device__ __forceinline__ void tile() {
-        if constexpr (sizeof(T) == 4)
-            if (++tiles == kSumTiles) join();
-    }
     __device__ __forceinline__ void join() {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -170,7 +163,6 @@ struct Sums {
                     all[i][j] += now[i][j];
                     now[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
                 }
-            tiles = 0;
         }
     }
     __device__ __forceinline__ auto& result() {
@@ -218,10 +210,8 @@ __global__ __launch_bounds__(S::kThreads) void grouped_kernel(GroupedArgs a) {
     Sums<T, S::kMI, S::kNJ> acc;
     const Reader<T, S::kM, false, S::kMI> ra(wm, lane);
     const Reader<T, S::kN, !ALONG_W, S::kNJ> rb(wn, lane);
-    auto compute = [&](const char* la, const char* lb) {
-        multiply<T, S>(ra, rb, la, lb, acc.now);
-        acc.tile();
-    };
+    auto compute = [&](const char* la, const char* lb) { multiply<T, S>(ra, rb, la, lb, acc.now); };
+    auto join = [&] { acc.join(); };
     if constexpr (DIRECT) {
         // offsets from the tile's first row (gathered: x's) and w's tile
         const T* xb = a.rows ? x : x + static_cast<int64_t>(r0) * a.ldx;
@@ -278,7 +268,7 @@ __global__ __launch_bounds__(S::kThreads) void grouped_kernel(GroupedArgs a) {
                                                                                  : bo[t]);
             }
         };
-        pipeline<true>(tiles, a0, b0, a1, b1, load, [](char*, char*) {}, compute);
+        pipeline<true>(tiles, a0, b0, a1, b1, load, [](char*, char*) {}, compute, join);
     } else {
         v4u av[S::kCA], bv[S::kCB];
         auto load = [&](int kt, char*, char*) {
@@ -307,7 +297,7 @@ __global__ __launch_bounds__(S::kThreads) void grouped_kernel(GroupedArgs a) {
             for (int t = 0; t < S::kCB; ++t)
                 *reinterpret_cast<v4u*>(lb + (t * S::kThreads + tid) * 16) = bv[t];
         };
-        pipeline<false>(tiles, a0, b0, a1, b1, load, store, compute);
+        pipeline<false>(tiles, a0, b0, a1, b1, load, store, compute, join);
     }
 
     store_outputs<T>(a, g, r0 + wm, r1, n0 + wn, lane, acc.result());
@@ -415,15 +405,17 @@ __global__ __launch_bounds__(S::kThreads, DIRECT ? 2 : 1) void wgrad_kernel(Grou
     const Reader<T, S::kN, true, S::kNJ> rb(wn, lane);
     auto compute = [&](const char* la, const char* lb) {
         multiply<T, S>(ra, rb, la, lb, acc.now);
-        acc.tile();
         if (BIAS && sums) {
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int j = 0; j < S::kNJ; ++j)
                     sum.now[0][j] = mfma<T>(rb.read(lb, j, s), one, sum.now[0][j]);
-            sum.tile();
         }
+    };
+    auto join = [&] {
+        acc.join();
+        sum.join();
     };
     if constexpr (DIRECT) {
         uint32_t ao[S::kCA], bo[S::kCB];
@@ -470,7 +462,7 @@ __global__ __launch_bounds__(S::kThreads, DIRECT ? 2 : 1) void wgrad_kernel(Grou
             for (int t = 0; t < S::kCB; ++t)
                 load_to_lds(dbuf, lb + (t * S::kThreads + wave * 64) * 16, bo[t]);
         };
-        pipeline<true>(tiles, a0, b0, a1, b1, load, [](char*, char*) {}, compute);
+        pipeline<true>(tiles, a0, b0, a1, b1, load, [](char*, char*) {}, compute, join);
     } else {
         v4u av[S::kCA], bv[S::kCB];
         auto load = [&](int kt, char*, char*) {
@@ -495,7 +487,7 @@ __global__ __launch_bounds__(S::kThreads, DIRECT ? 2 : 1) void wgrad_kernel(Grou
             for (int t = 0; t < S::kCB; ++t)
                 *reinterpret_cast<v4u*>(lb + (t * S::kThreads + tid) * 16) = bv[t];
         };
-        pipeline<false>(tiles, a0, b0, a1, b1, load, store, compute);
+        pipeline<false>(tiles, a0, b0, a1, b1, load, store, compute, join);
     }
 
     // (a group that is one part goes straight to dw)

@@ -212,46 +212,51 @@ struct Shape {
 template <typename S>
 using Acc = v4f[S::kMI][S::kNJ];
 
-// A step's border: what this wavefront asked of LDS is there, and all but
-// LOADS of its loads; then the same of every wavefront.  Loads that write
-// straight to LDS need it in place of __syncthreads(), which orders a
-// wavefront's reads and writes of memory, not these: before a loop's barrier the
-// compiler may wait for the loop's first entry alone, and did where registers
-// were spilled.
-template <int LOADS>
-__device__ __forceinline__ void step_border() {
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
+// The barrier of a loop over tiles that loads write straight to LDS: what this
+// wavefront asked for is there, then the same of every wavefront.
+// __syncthreads() alone orders reads and writes, not these loads: the compiler may
+// wait for a loop's first entry alone, and did where registers were spilled.  (The
+// wait is the builtin, which the compiler counts: written as inline assembly it cost
+// fp32 233K x 602 x 256 700 us against 615.)
+__device__ __forceinline__ void loads_border() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
 }
 
 // The loop over `tiles` tiles: load(kt, la, lb) brings tile kt.  With DIRECT
 // the loads are in flight until the barrier; else load keeps them in registers
-// and store(la, lb) writes them.
-template <bool DIRECT, typename L, typename W, typename C>
+// and store(la, lb) writes them.  join() comes after every kSumTiles tiles: in a
+// loop around theirs, for a branch among them was made into selects, which read
+// the sums in every tile.
+constexpr int kSumTiles = 8;
+template <bool DIRECT, typename L, typename W, typename C, typename J>
 __device__ __forceinline__ void pipeline(int tiles, char* a0, char* b0, char* a1, char* b1,
-                                         L&& load, W&& store, C&& compute) {
+                                         L&& load, W&& store, C&& compute, J&& join) {
     if (tiles == 0) return;
     auto border = [] {
         if constexpr (DIRECT)
-            step_border<0>();
+            loads_border();
         else
             __syncthreads();
     };
     load(0, a0, b0);
     if (!DIRECT) store(a0, b0);
     int kt = 0;
-    for (; kt + 1 < tiles; kt += 2) {
-        border();
-        load(kt + 1, a1, b1);
-        compute(a0, b0);
-        if (!DIRECT) store(a1, b1);
-        border();
-        if (kt + 2 < tiles) load(kt + 2, a0, b0);
-        compute(a1, b1);
-        if (!DIRECT && kt + 2 < tiles) store(a0, b0);
+    while (kt + 1 < tiles) {
+        const int stop = tiles - kt > kSumTiles ? kt + kSumTiles : tiles;
+        for (; kt + 1 < stop; kt += 2) {
+            border();
+            load(kt + 1, a1, b1);
+            compute(a0, b0);
+            if (!DIRECT) store(a1, b1);
+            border();
+            if (kt + 2 < tiles) load(kt + 2, a0, b0);
+            compute(a1, b1);
+            if (!DIRECT && kt + 2 < tiles) store(a0, b0);
+        }
+        join();
     }
     if (kt < tiles) {
         border();
@@ -319,6 +324,17 @@ struct PartReader {
         return f;
     }
 };
+
+// A step's border: what this wavefront asked of LDS is there, and all but
+// LOADS of its loads; then the same of every wavefront.
+template <int LOADS>
+__device__ __forceinline__ void step_border() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
 
 // acc += the products of `steps` parts; load(u, la, lb) asks for part u (four
 // loads a thread; zeros from `steps` on), ahead(u) comes before the loads of u ..
