@@ -402,7 +402,8 @@ int tg_route_backward(int64_t tokens, int64_t experts, int64_t k, int type, cons
  * Backward: dy[position[t*k + j]] = weights[t*k + j] * dout[t]; rows of dy that
  * no position names are left as they are; dweights[t*k + j] = dot of dout[t]
  * and y[position[t*k + j]] in fp32, 0 without a position.  dy or dweights may
- * be NULL (y is read for dweights only).  No position may occur twice.
+ * be NULL (y is read for dweights only).  No position may occur twice.  Outputs
+ * overlap no input.
  * ------------------------------------------------------------------------ */
 int tg_route_combine(int64_t tokens, int64_t k, int64_t cols, int type, const void* y,
                      int64_t y_rows, int64_t ldy, const int32_t* position,
