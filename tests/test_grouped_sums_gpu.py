@@ -50,3 +50,16 @@ def test_gradient_of_weights(gpu, m, k, n, groups):
     tol = (256 + min(rows, 16384) / 256 + parts + 2) * U * rows * v
     assert float((dw.double() - rows * v).abs().max()) <= tol
     assert float((db.double() - rows * v).abs().max()) <= tol
+
+
+def test_bias_beside_large_tiles(gpu):
+    """dbias of 2^20 rows in fp16, 65,536 to each of 16 wavefronts: a chain of
+    them from 2^14 on drops 2^-10 of every v = 1 + 2^-10, 7e-4 in all, where the
+    result's own rounding is 4.9e-4."""
+    import tinygnn_amd as tg
+    m, k, n = 1 << 20, 4096, 8192
+    v = (1 + 2.0 ** -10) / 256      # the sum is 4,100
+    x = torch.ones(m, k, dtype=torch.float16, device="cuda")
+    dy = torch.full((m, n), v, dtype=torch.float16, device="cuda")
+    _, db = tg.grouped_matmul_wgrad(x, dy, offsets_of([m]), bias=True)
+    assert bool((db == 4100).all())

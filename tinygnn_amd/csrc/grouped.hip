@@ -591,12 +591,18 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(GroupedArgs a) {
     const int64_t c = (static_cast<int64_t>(blockIdx.x) * 64 + lane) * VEC;
     const T* dy = static_cast<const T*>(a.dy) + c;
     float s[VEC] = {};
+    for (int p = lo + wave; p < hi;) {  // chains of 64 rows (a row an add, unlike the products)
+        const int stop = hi - p > 1024 ? p + 1024 : hi;
+        float now[VEC] = {};
 #pragma unroll 8
-    for (int p = lo + wave; p < hi; p += 16) {
-        float v[VEC];
-        load_floats<T, VEC>(dy + p * a.lddy, a.n - c, v);
+        for (; p < stop; p += 16) {
+            float v[VEC];
+            load_floats<T, VEC>(dy + p * a.lddy, a.n - c, v);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) s[e] += v[e];
+            for (int e = 0; e < VEC; ++e) now[e] += v[e];
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s[e] += now[e];
     }
 #pragma unroll
     for (int e = 0; e < VEC; ++e) join[wave][lane][e] = s[e];
