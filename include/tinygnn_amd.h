@@ -480,6 +480,88 @@ int tg_matmul_fp8(int64_t m, int64_t k, int64_t n, int64_t groups, const void* x
                   const void* bias, int epilogue, void* y, int64_t ldy, tg_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Dense layers with an epilogue (no counterpart in the reference, whose matmul
+ * is fp32 with separate passes): y = residual + act(x * w + bias).
+ *
+ * tg_linear: x [m x k] times w [k x n] (leading dimension ldw) or, transposed,
+ * w [n x k]; bias [n] or NULL; act = TG_EPI_NONE / RELU / ELU / GELU / SILU,
+ * GELU in tg_gelu's form (0.5 v (1 + tanh(0.79788456 (v + 0.044715 v^3)))), SILU
+ * v / (1 + exp(-v)); residual [m x n] or NULL.  pre (or NULL) receives
+ * x * w + bias, for the backward pass.  All of `type`; sums in fp32, y and pre
+ * rounded once.  y may be the residual (same leading dimension) and overlaps
+ * nothing else.  m, k, n < 2^31 - 4096.
+ *
+ * tg_linear_backward: from dy and the forward's x, w and pre
+ *   d = dy * act'(pre), rounded to `type` (act NONE: d = dy, pre is not read),
+ *   dx = d * w^T, dw = x^T * d (transposed: d^T * x) in w's layout, contiguous,
+ *   dbias = the sum of d's rows before that rounding
+ * (any of the three may be NULL; the residual's gradient is dy).  Sums in fp32,
+ * equal calls give equal bits.  With m = 0 dw and dbias are zeros, with n = 0 dx.
+ * workspace: the size function's bytes (for dx, dw and dbias, whichever are
+ * asked for), or NULL.
+ * ------------------------------------------------------------------------ */
+enum { TG_EPI_GELU = 3, TG_EPI_SILU = 4 }; /* tg_linear's alone */
+size_t tg_linear_workspace_size(int64_t m, int64_t k, int64_t n, int type);
+int tg_linear(int64_t m, int64_t k, int64_t n, int type, const void* x, int64_t ldx,
+              const void* w, int64_t ldw, int transposed, const void* bias, int act,
+              const void* residual, int64_t ldr, void* y, int64_t ldy, void* pre, int64_t ldp,
+              void* workspace, size_t workspace_bytes, tg_stream_t stream);
+size_t tg_linear_backward_workspace_size(int64_t m, int64_t k, int64_t n, int type);
+int tg_linear_backward(int64_t m, int64_t k, int64_t n, int type, const void* dy, int64_t lddy,
+                       const void* x, int64_t ldx, const void* w, int64_t ldw, int transposed,
+                       const void* pre, int64_t ldp, int act, void* dx, int64_t lddx, void* dw,
+                       void* dbias, void* workspace, size_t workspace_bytes, tg_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * What a classifier answers and learns from (no counterpart in the reference).
+ * logits [rows x classes] of `type`; z = logits / temperature (1e-4 to 1e4),
+ * p = softmax of a row of z, in fp32.  A logit of -inf is a masked class (p = 0).
+ *
+ * tg_log_probs: value[r] = log p of class labels[r]; 0 where the label lies
+ * outside [0, classes) (no label).  entropy[r] = -sum of p log p.  The `top`
+ * largest logits of a row (at most 64), in falling order, the lower class first
+ * among equals: top_ids[r*top + j] and top_values = their log p; places past the
+ * unmasked classes hold -1 and -inf.  stats [rows x 2] (largest logit, log of the
+ * sum of exp(z - its z)), for the backward pass.  labels with value, entropy and
+ * stats may be NULL.  A row of -inf alone has value -inf, entropy 0 and stats
+ * (-inf, 0).  A NaN is no top class; it, and a logit of +inf, make the row's
+ * results NaN.
+ * workspace: the size function's bytes, or NULL.
+ *
+ * tg_log_probs_backward: dlogits from dvalue (with labels) and dentropy (with
+ * entropy), either pair NULL:
+ *   1/T * (dvalue * ([i = label] - p_i) - dentropy * p_i * (log p_i + entropy)),
+ * dvalue of rows without a label not used; zeros in a row whose dvalue and
+ * dentropy are 0 (whatever its logits hold) and in a row of -inf alone.
+ * dlogits may be logits (same leading dimension).
+ *
+ * tg_distill: a teacher's k logits (of teacher_type, contiguous [rows x k]; its
+ * log probabilities do as well) of the classes ids [rows x k]: q = softmax of
+ * them / temperature over the places whose id lies in [0, classes), and
+ *   loss[r] = sum over the places of q_j (log q_j - log p of class ids_j),
+ *   dlogits = dloss / T * (p_i - sum of q_j with ids_j = i)
+ * (dloss and dlogits NULL: the loss alone; dlogits may be logits, with the same
+ * leading dimension).  Terms of q_j = 0 are 0.  A row without places has loss 0
+ * and gradient 0; a row of dloss 0 gradient 0; a row of -inf logits alone gradient
+ * 0 and, as where a class of q_j > 0 is masked, loss inf.  k at most 256; a class
+ * may come up several times.
+ * ------------------------------------------------------------------------ */
+size_t tg_log_probs_workspace_size(int64_t rows, int64_t classes, int64_t top, int type);
+int tg_log_probs(int64_t rows, int64_t classes, int type, const void* logits, int64_t ld,
+                 const int32_t* labels, float temperature, int64_t top, float* value,
+                 float* entropy, float* top_values, int32_t* top_ids, float* stats,
+                 void* workspace, size_t workspace_bytes, tg_stream_t stream);
+int tg_log_probs_backward(int64_t rows, int64_t classes, int type, const void* logits, int64_t ld,
+                          const int32_t* labels, float temperature, const float* stats,
+                          const float* entropy, const float* dvalue, const float* dentropy,
+                          void* dlogits, int64_t lddl, tg_stream_t stream);
+size_t tg_distill_workspace_size(int64_t rows, int64_t classes, int64_t k, int type);
+int tg_distill(int64_t rows, int64_t classes, int64_t k, int type, const void* logits, int64_t ld,
+               int teacher_type, const void* teacher, const int32_t* ids, float temperature,
+               float* loss, const float* dloss, void* dlogits, int64_t lddl, void* workspace,
+               size_t workspace_bytes, tg_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * Model -- replaces tinygnn::Model (include/tinygnn/model.hpp:89-164,
  * src/model.cpp:191-439): a sequential GCN / SAGE / GAT layer graph with
  * device-resident weights.

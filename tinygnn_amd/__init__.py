@@ -21,6 +21,7 @@ POST_NONE, POST_RELU, POST_ELU = 0, 1, 2
 AGG_MEAN, AGG_MAX = 0, 1
 GEMM_AUTO, GEMM_INORDER, GEMM_MFMA = 0, 1, 2
 EPI_NONE, EPI_RELU, EPI_ELU = 0, 1, 2
+EPI_GELU, EPI_SILU = 3, 4   # linear's alone
 SAGE_AUTO, SAGE_CONCAT, SAGE_TRANSFORM_FIRST = 0, 1, 2
 FORWARD_REFERENCE, FORWARD_CACHED = 0, 1
 PRECISION_FAST, PRECISION_EXACT = 0, 1
@@ -453,7 +454,8 @@ def _refuse(what: str, message: str):
 
 
 def _device_call(fn):
-    """The first tensor's GPU is the current device for the call."""
+    """The GPU of the first argument, or of the first tensor where that is None,
+    is the current device for the call."""
     import functools
     name = fn.__code__.co_varnames[0]
 
@@ -464,7 +466,11 @@ def _device_call(fn):
             _pt = _Torch()
         first = args[0] if args else kwargs.get(name)
         if first is None:
-            return fn(*args, **kwargs)   # Python's own message
+            for first in (*args, *kwargs.values()):
+                if hasattr(first, "get_device"):
+                    break
+            else:
+                return fn(*args, **kwargs)   # Python's own message
         index = getattr(first, "q", first).get_device()
         if index < 0:
             raise ValueError("tinygnn_amd expects device (cuda) tensors")
@@ -918,6 +924,198 @@ def matmul_fp8(x: BlockRows, w: BlockWeight, offsets=None, rows=None, bias=None,
                                 epilogue, py, ldy, s))
     _finish(stream)
     return y
+
+
+# ---------------------------------------------------------------------------
+# Dense layers, and what a classifier answers and learns from: the conventions
+# of the expert layers' calls above.
+# ---------------------------------------------------------------------------
+def _linear_weight(what: str, x, w, transpose: bool):
+    """(n, k, pointer, leading dimension) of linear's w."""
+    if w.dim() != 2 or w.dtype is not x.dtype:
+        _refuse(what, f"w must be a {x.dtype} matrix, got {tuple(w.shape)} {w.dtype}.")
+    n, k = w.shape if transpose else w.shape[::-1]
+    if x.dim() != 2 or x.shape[1] != k:
+        _refuse(what, f"dimension mismatch: x is {tuple(x.shape)}, w has {k} rows of x's columns.")
+    return n, k, *_rows_of(what, "w", w)
+
+
+def _like(what: str, name: str, t, shape, dtype):
+    """Pointer and leading dimension of an input matrix of a given shape and
+    type; None's."""
+    if t is None:
+        return None, 0
+    if t.shape != shape or t.dtype is not dtype:
+        _refuse(what, f"{name} must be {tuple(shape)} {dtype}, got {tuple(t.shape)} {t.dtype}.")
+    return _rows_of(what, name, t)
+
+
+@_device_call
+def linear(x, w, bias=None, epilogue: int = EPI_NONE, residual=None, transpose: bool = False,
+           with_pre: bool = False, out=None, stream=None):
+    """y = residual + epilogue(x @ w + bias) (tg_linear).  w: [k, n], or [n, k]
+    with transpose; bias: [n]; residual: [rows, n]; epilogue: EPI_NONE, EPI_RELU,
+    EPI_ELU, EPI_GELU or EPI_SILU.  All of x's type; rounded once.  with_pre:
+    (y, pre), pre = x @ w + bias for linear_backward.  out may be the residual."""
+    what = "linear"
+    s = _stream_of(what, stream, x, w, bias, residual, out)
+    kind = _type_of(what, x)
+    n, k, pw, ldw = _linear_weight(what, x, w, transpose)
+    px, ldx = _rows_of(what, "x", x)
+    m = x.shape[0]
+    pb = _flat(what, "bias", bias, (n,), x.dtype)
+    pr, ldr = _like(what, "residual", residual, (m, n), x.dtype)
+    y, py, ldy = _out(what, "out", out, (m, n), x, x.dtype)
+    pre, pp, ldp = _out(what, "pre", None, (m, n), x, x.dtype) if with_pre else (None, None, 0)
+    size = lib.tg_linear_workspace_size(m, k, n, kind)
+    ws, pws = _workspace(size, x)
+    lib.check(lib.tg_linear(m, k, n, kind, px, ldx, pw, ldw, 1 if transpose else 0, pb, epilogue,
+                            pr, ldr, py, ldy, pp, ldp, pws, size, s))
+    _finish(stream)
+    return (y, pre) if with_pre else y
+
+
+@_device_call
+def linear_backward(dy, x, w, pre=None, epilogue: int = EPI_NONE, bias: bool = False,
+                    transpose: bool = False, stream=None):
+    """(dx, dw, dbias) of linear from dy, its x, w and, with an epilogue, pre
+    (tg_linear_backward); dw in w's layout, dbias None unless bias.  The
+    residual's gradient is dy."""
+    what = "linear_backward"
+    s = _stream_of(what, stream, dy, x, w, pre)
+    kind = _type_of(what, x)
+    n, k, pw, ldw = _linear_weight(what, x, w, transpose)
+    px, ldx = _rows_of(what, "x", x)
+    m = x.shape[0]
+    pd, lddy = _like(what, "dy", dy, (m, n), x.dtype)
+    if epilogue != EPI_NONE and pre is None:
+        _refuse(what, "an epilogue's gradient needs pre (linear's with_pre).")
+    pp, ldp = _like(what, "pre", pre, (m, n), x.dtype)
+    dx = _pt.empty((m, k), dtype=x.dtype, device=x.device)
+    dw = _pt.empty(w.shape, dtype=x.dtype, device=x.device)
+    db = _pt.empty(n, dtype=x.dtype, device=x.device) if bias else None
+    size = lib.tg_linear_backward_workspace_size(m, k, n, kind)
+    ws, pws = _workspace(size, x)
+    lib.check(lib.tg_linear_backward(m, k, n, kind, pd, lddy, px, ldx, pw, ldw,
+                                     1 if transpose else 0, pp, ldp, epilogue, dx.data_ptr(),
+                                     max(k, 1), dw.data_ptr(), db.data_ptr() if bias else None,
+                                     pws, size, s))
+    _finish(stream)
+    return dx, dw, db
+
+
+@dataclass
+class LogProbs:
+    """What log_probs returns: value float32 [rows] (None without labels),
+    entropy float32 [rows] or None, top_values float32 and top_ids int32 [rows,
+    top] or None, and for log_probs_backward stats float32 [rows, 2] and the
+    temperature."""
+    value: object
+    entropy: object
+    top_values: object
+    top_ids: object
+    stats: object
+    temperature: float
+
+
+@_device_call
+def log_probs(logits, labels=None, top: int = 0, entropy: bool = False, temperature: float = 1.0,
+              stream=None) -> LogProbs:
+    """Log probabilities of the classes labels (int32 [rows]; outside [0,
+    classes): none, 0) under softmax(logits / temperature), the rows' entropy
+    and their `top` likeliest classes (tg_log_probs)."""
+    what = "log_probs"
+    s = _stream_of(what, stream, logits, labels)
+    kind = _type_of(what, logits)
+    pl, ld = _rows_of(what, "logits", logits)
+    rows, classes = logits.shape
+    if not 0 <= top <= min(64, classes):
+        _refuse(what, f"top must be between 0 and min(64, classes), got {top} of {classes}.")
+    dev = logits.device
+    py = _flat(what, "labels", labels, (rows,), _pt.i32)
+    value = ent = top_values = top_ids = None
+    pv = pe = ptv = pti = None
+    if labels is not None:
+        value = _pt.empty(rows, dtype=_pt.f32, device=dev)
+        pv = value.data_ptr()
+    if entropy:
+        ent = _pt.empty(rows, dtype=_pt.f32, device=dev)
+        pe = ent.data_ptr()
+    if top:
+        top_values = _pt.empty((rows, top), dtype=_pt.f32, device=dev)
+        top_ids = _pt.empty((rows, top), dtype=_pt.i32, device=dev)
+        ptv, pti = top_values.data_ptr(), top_ids.data_ptr()
+    stats = _pt.empty((rows, 2), dtype=_pt.f32, device=dev)
+    size = lib.tg_log_probs_workspace_size(rows, classes, top, kind)
+    ws, pws = _workspace(size, logits)
+    lib.check(lib.tg_log_probs(rows, classes, kind, pl, ld, py, temperature, top, pv, pe, ptv, pti,
+                               stats.data_ptr(), pws, size, s))
+    _finish(stream)
+    return LogProbs(value, ent, top_values, top_ids, stats, temperature)
+
+
+@_device_call
+def log_probs_backward(dvalue, logits, labels, result: LogProbs, dentropy=None,
+                       temperature: float | None = None, out=None, stream=None):
+    """dlogits of log_probs from the gradients of its value (float32 [rows]; None:
+    of none, labels None too) and of its entropy (tg_log_probs_backward).  out takes
+    dlogits (it may be logits)."""
+    what = "log_probs_backward"
+    first = logits if dvalue is None else dvalue
+    s = _stream_of(what, stream, first, logits, labels, result.stats, result.entropy, dentropy, out)
+    kind = _type_of(what, logits)
+    pl, ld = _rows_of(what, "logits", logits)
+    rows, classes = logits.shape
+    if temperature is not None and temperature != result.temperature:
+        _refuse(what, f"temperature {temperature} is not log_probs' {result.temperature}.")
+    if (dvalue is None) != (labels is None):
+        _refuse(what, "dvalue and labels go together.")
+    pd = _flat(what, "dvalue", dvalue, (rows,), _pt.f32)
+    py = _flat(what, "labels", labels, (rows,), _pt.i32)
+    pst = _flat(what, "stats", result.stats, (rows, 2), _pt.f32)
+    ph = _flat(what, "dentropy", dentropy, (rows,), _pt.f32)
+    if ph is not None and result.entropy is None:
+        _refuse(what, "dentropy needs log_probs' entropy.")
+    pe = _flat(what, "entropy", result.entropy, (rows,), _pt.f32) if ph is not None else None
+    d, po, ldo = _out(what, "out", out, logits.shape, logits, logits.dtype)
+    lib.check(lib.tg_log_probs_backward(rows, classes, kind, pl, ld, py, result.temperature, pst,
+                                        pe, pd, ph, po, ldo, s))
+    _finish(stream)
+    return d
+
+
+@_device_call
+def distill(logits, teacher, ids, temperature: float = 1.0, dloss=None, out=None, stream=None):
+    """The divergence of softmax(logits / temperature) from a teacher's k top
+    logits [rows, k] of the classes ids (int32; outside [0, classes): no place),
+    softmax(teacher / temperature) over them: loss float32 [rows] (tg_distill).
+    With dloss (float32 [rows], the gradient of each row's loss): (loss,
+    dlogits); out takes dlogits (it may be logits)."""
+    what = "distill"
+    s = _stream_of(what, stream, logits, teacher, ids, dloss, out)
+    kind = _type_of(what, logits)
+    pl, ld = _rows_of(what, "logits", logits)
+    rows, classes = logits.shape
+    tk = _type_of(what, teacher)
+    if teacher.dim() != 2 or teacher.shape[0] != rows or not 1 <= teacher.shape[1] <= 256:
+        _refuse(what, f"teacher must be [{rows}, k] with k between 1 and 256, got "
+                      f"{tuple(teacher.shape)}.")
+    pt = _flat(what, "teacher", teacher, teacher.shape, teacher.dtype)
+    pi = _flat(what, "ids", ids, teacher.shape, _pt.i32)
+    pd = _flat(what, "dloss", dloss, (rows,), _pt.f32)
+    loss = _pt.empty(rows, dtype=_pt.f32, device=logits.device)
+    d, po, ldo = None, None, 0
+    if dloss is not None:
+        d, po, ldo = _out(what, "out", out, logits.shape, logits, logits.dtype)
+    elif out is not None:
+        _refuse(what, "out takes the gradient, which needs dloss.")
+    k = teacher.shape[1]
+    size = lib.tg_distill_workspace_size(rows, classes, k, kind)
+    ws, pws = _workspace(size, logits)
+    lib.check(lib.tg_distill(rows, classes, k, kind, pl, ld, tk, pt, pi, temperature,
+                             loss.data_ptr(), pd, po, ldo, pws, size, s))
+    _finish(stream)
+    return loss if dloss is None else (loss, d)
 
 
 # ---------------------------------------------------------------------------

@@ -116,6 +116,18 @@ SIGNATURES = {
     "tg_quantize_weight": (i32, [i64, i64, i64, i32, vp, i64, i64, i32, vp, vp, vp]),
     "tg_matmul_fp8": (i32, [i64, i64, i64, i64, vp, vp, i64, vp, vp, vp, vp, i32, vp, i32, vp,
                             i64, vp]),
+    "tg_linear_workspace_size": (sz, [i64, i64, i64, i32]),
+    "tg_linear": (i32, [i64, i64, i64, i32, vp, i64, vp, i64, i32, vp, i32, vp, i64, vp, i64, vp,
+                        i64, vp, sz, vp]),
+    "tg_linear_backward_workspace_size": (sz, [i64, i64, i64, i32]),
+    "tg_linear_backward": (i32, [i64, i64, i64, i32, vp, i64, vp, i64, vp, i64, i32, vp, i64, i32,
+                                 vp, i64, vp, vp, vp, sz, vp]),
+    "tg_log_probs_workspace_size": (sz, [i64, i64, i64, i32]),
+    "tg_log_probs": (i32, [i64, i64, i32, vp, i64, vp, f32, i64, vp, vp, vp, vp, vp, vp, sz, vp]),
+    "tg_log_probs_backward": (i32, [i64, i64, i32, vp, i64, vp, f32, vp, vp, vp, vp, vp, i64, vp]),
+    "tg_distill_workspace_size": (sz, [i64, i64, i64, i32]),
+    "tg_distill": (i32, [i64, i64, i64, i32, vp, i64, i32, vp, vp, f32, vp, vp, vp, i64, vp, sz,
+                         vp]),
     "tg_model_create": (i32, [C.POINTER(vp)]),
     "tg_model_destroy": (i32, [vp]),
     "tg_model_add_gcn_layer": (i32, [vp, i64, i64, i32, i32, i32, pi64]),

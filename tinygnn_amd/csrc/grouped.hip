@@ -126,54 +126,6 @@ __device__ __forceinline__ void store_bias_gradient(const GroupedArgs& a, bool s
 // DIRECT: the tiles come by loads that write to LDS; else through registers,
 // for 16-bit operands of odd rows or places and those that reach past 2 GB.
 // ---------------------------------------------------------------------------
-// The products of one tile pair.
-template <typename T, typename S, typename RA, typename RB>
-__device__ __forceinline__ void multiply(const RA& ra, const RB& rb, const char* la, const char* lb,
-                                         Acc<S>& acc) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        Frag b[S::kNJ];
-#pragma unroll
-        for (int j = 0; j < S::kNJ; ++j) b[j] = rb.read(lb, j, s);
-#pragma unroll
-        for (int i = 0; i < S::kMI; ++i) {
-            const Frag a = ra.read(la, i, s);
-#pragma unroll
-            for (int j = 0; j < S::kNJ; ++j) acc[i][j] = mfma<T>(b[j], a, acc[i][j]);
-        }
-    }
-}
-
-// Sums of floats keep their digits: kSumTiles tiles (256 values) are one chain in
-// `now`, and the chains' sums another in `all`.  (One chain of n values is off by up
-// to n 2^-24 of the sum of sizes: a training step of 233K rows of 7 types, 602 x
-// 256, was 8.9e-7 off with it and is 3.1e-7; 2.27 -> 2.31 ms.)  16-bit products
-// are one chain, to which the instructions add eight at a time: n of one sign are
-// off by n 2^-27 of their sum at most, n^(1/2) 2^-25 or so of random ones; the
-// result's own rounding is 2^-9 or 2^-12.
-template <typename T, int N, int M>
-struct Sums {
-    v4f now[N][M] = {}, all[sizeof(T) == 4 ? N : 1][sizeof(T) == 4 ? M : 1] = {};
-    __device__ __forceinline__ void join() {
-        if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-#pragma unroll
-                for (int j = 0; j < M; ++j) {
-                    all[i][j] += now[i][j];
-                    now[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-                }
-        }
-    }
-    __device__ __forceinline__ auto& result() {
-        join();
-        if constexpr (sizeof(T) == 4)
-            return all;
-        else
-            return now;
-    }
-};
-
 template <typename T, typename S, bool ALONG_W, bool DIRECT>
 __global__ __launch_bounds__(S::kThreads) void grouped_kernel(GroupedArgs a) {
     __shared__ __attribute__((aligned(16))) char a0[S::kM * kRowBytes];

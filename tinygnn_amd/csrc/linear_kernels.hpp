@@ -1,0 +1,454 @@
+// linear_kernels.hpp -- the kernels of the dense layers, compiled for one element
+// type by each of linear_f32.hip, linear_bf16.hip and linear_f16.hip.
+//
+// All three products (x w; d w^T; x^T d) are one kernel, out [m x n] = the sum
+// over the contraction of X's row and W's column, whose operands run along or
+// across the contraction (tiles.hpp): x w has x along and w across (or along, if
+// transposed), d w^T the other of the two for w, x^T d both across.  16-bit types go
+// through v_mfma_f32_16x16x32, floats through v_mfma_f32_16x16x4f32; sums are
+// fp32.  Where the tiles are too few for the CUs, or a chain of floats too long,
+// the contraction is cut in parts whose fp32 sums a second kernel adds in order,
+// with the epilogue.
+#pragma once
+
+#include "grouped.hpp"
+#include "linear.hpp"
+#include "tiles.hpp"
+#include "types.hpp"
+
+namespace tg {
+namespace {
+
+constexpr float kGeluScale = 1.5957691216f;  // 2 sqrt(2 / pi)
+constexpr float kGeluCube = 0.044715f;
+
+// 1 / (1 + exp(-s)): GELU's (1 + tanh(s / 2)) / 2, too.  (The reciprocal
+// instruction is within one unit in the last place.)
+__device__ __forceinline__ float sigmoid(float s) {
+    return __builtin_amdgcn_rcpf(1.0f + __expf(-s));
+}
+
+template <int ACT>
+__device__ __forceinline__ float act_of(float v) {
+    if constexpr (ACT == TG_EPI_RELU) return 0.0f < v ? v : 0.0f;
+    if constexpr (ACT == TG_EPI_ELU) return v < 0.0f ? expm1_negative(v) : v;
+    if constexpr (ACT == TG_EPI_GELU)
+        return v * sigmoid(kGeluScale * __builtin_fmaf(kGeluCube * v * v, v, v));
+    if constexpr (ACT == TG_EPI_SILU) return v * sigmoid(v);
+    return v;
+}
+
+// act'(v).  Where p (1 - p) is 0, so is its term, however large v's powers are.
+template <int ACT>
+__device__ __forceinline__ float slope_of(float v) {
+    if constexpr (ACT == TG_EPI_RELU) return 0.0f < v ? 1.0f : 0.0f;
+    if constexpr (ACT == TG_EPI_ELU) return v < 0.0f ? __expf(v) : 1.0f;
+    if constexpr (ACT == TG_EPI_GELU || ACT == TG_EPI_SILU) {
+        const float c = kGeluCube * v * v;
+        const float s = ACT == TG_EPI_GELU ? kGeluScale * __builtin_fmaf(c, v, v) : v;
+        const float ds = ACT == TG_EPI_GELU ? kGeluScale * __builtin_fmaf(3.0f, c, 1.0f) : 1.0f;
+        const float p = sigmoid(s), t = p * (1.0f - p);
+        return t == 0.0f ? p : __builtin_fmaf(t * v, ds, p);
+    }
+    return 1.0f;
+}
+
+template <typename F>
+__device__ __forceinline__ void with_act(int act, F&& fn) {
+    switch (act) {
+        case TG_EPI_RELU: return fn(std::integral_constant<int, TG_EPI_RELU>{});
+        case TG_EPI_ELU: return fn(std::integral_constant<int, TG_EPI_ELU>{});
+        case TG_EPI_GELU: return fn(std::integral_constant<int, TG_EPI_GELU>{});
+        case TG_EPI_SILU: return fn(std::integral_constant<int, TG_EPI_SILU>{});
+        default: return fn(std::integral_constant<int, TG_EPI_NONE>{});
+    }
+}
+
+// Four consecutive results of a row: bias, the value before the activation, the
+// activation, the residual.
+template <typename T, int ACT>
+__device__ __forceinline__ void finish(const LinearArgs& a, int64_t row, int n,
+                                       const float (&sum)[4], const float (&bias)[4]) {
+    float v[4], r[4] = {};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = sum[e] + bias[e];
+    if (a.pre) store_floats<T, 4>(static_cast<T*>(a.pre) + row * a.ldp + n, a.n - n, v);
+    if (a.residual)
+        load_floats<T, 4>(static_cast<const T*>(a.residual) + row * a.ldr + n, a.n - n, r);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = act_of<ACT>(v[e]) + r[e];
+    store_floats<T, 4>(static_cast<T*>(a.y) + row * a.ldy + n, a.n - n, v);
+}
+
+// A wavefront's sums from row m0, column n0 on.  Lane (q, r) holds row r of a
+// tile, columns 4 q .. 4 q + 3.
+template <typename T, int MI, int NJ>
+__device__ __forceinline__ void store_sums(const LinearArgs& a, int part, int m0, int n0, int lane,
+                                           const v4f (&acc)[MI][NJ]) {
+    const int q = lane >> 4, r = lane & 15;
+    if (a.part) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const int m = m0 + i * 16 + r;
+            if (m >= a.m) continue;
+            float* to = a.part + (static_cast<int64_t>(part) * a.m + m) * a.n;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int n = n0 + j * 16 + 4 * q;
+                const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                store_floats<float, 4>(to + n, a.n - n, v);
+            }
+        }
+        return;
+    }
+    float bias[NJ][4] = {};
+    if (a.bias) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int n = n0 + j * 16 + 4 * q;
+            load_floats<T, 4>(static_cast<const T*>(a.bias) + n, a.n - n, bias[j]);
+        }
+    }
+    with_act(a.act, [&](auto act) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const int m = m0 + i * 16 + r;
+            if (m >= a.m) continue;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                finish<T, decltype(act)::value>(a, m, n0 + j * 16 + 4 * q, v, bias[j]);
+            }
+        }
+    });
+}
+
+// y = the epilogue of the parts' sums, in order.
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(LinearArgs a) {
+    const uint32_t chunks = (static_cast<uint32_t>(a.n) + 3) / 4;
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t row = t / chunks;
+    if (row >= a.m) return;
+    const int n = static_cast<int>(t - row * chunks) * 4;
+    const int64_t size = static_cast<int64_t>(a.m) * a.n;
+    const float* p = a.part + row * a.n + n;
+    float s[4] = {};
+#pragma unroll 4
+    for (int i = 0; i < a.parts; ++i) {
+        float v[4];
+        load_floats<float, 4>(p + i * size, a.n - n, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += v[e];
+    }
+    float bias[4] = {};
+    if (a.bias) load_floats<T, 4>(static_cast<const T*>(a.bias) + n, a.n - n, bias);
+    with_act(a.act, [&](auto act) { finish<T, decltype(act)::value>(a, row, n, s, bias); });
+}
+
+// ---------------------------------------------------------------------------
+// One operand's side of the tiles: R rows (of X) or columns (of W) from `first`
+// on of `count`, the contraction from k0 to k1.
+// ---------------------------------------------------------------------------
+template <typename T, int R, bool ACROSS, int CHUNKS, int THREADS>
+struct Side {
+    static constexpr int Z = sizeof(T);
+    const T* base;
+    int64_t ld;
+    int left;          // of count
+    int k1;
+    int maj[CHUNKS], min[CHUNKS];
+    uint32_t offset[CHUNKS];
+    v4u held[CHUNKS];
+    __device__ __forceinline__ Side(const void* p, int64_t ld_, int first, int count, int k1_)
+        : ld(ld_), left(count - first), k1(k1_) {
+        base = static_cast<const T*>(p) + (ACROSS ? first : first * ld);
+#pragma unroll
+        for (int t = 0; t < CHUNKS; ++t) {
+            chunk_place<T, R, ACROSS>(t * THREADS + static_cast<int>(threadIdx.x), &maj[t],
+                                      &min[t]);
+            const bool in = (ACROSS ? min[t] : maj[t]) < left;
+            offset[t] = in ? static_cast<uint32_t>(Z * (maj[t] * ld + min[t])) : kOutside;
+        }
+    }
+    // The tile from contraction value k0 on, straight to LDS.  What lies past k1
+    // is 0: across, past the buffer (which ends with its last row's columns) or
+    // past k1; along, whole chunks past it, and the one that k1 ends in by registers.
+    __device__ __forceinline__ void direct(int k0, char* lds, int wave) {
+        const auto buf =
+            ACROSS ? buffer_of(base + k0 * ld, Z * ((k1 - k0 - 1) * ld + left))
+                   : buffer_of(base + k0, kDirectBytes);
+        const bool part = k0 + kDepth<T> > k1;
+        const bool split = !ACROSS && part && (k1 - k0) % kVec<T> != 0;
+#pragma unroll
+        for (int t = 0; t < CHUNKS; ++t) {
+            const int k = k0 + (ACROSS ? maj[t] : min[t]);
+            if (split) {
+                const bool out = offset[t] == kOutside;
+                const T* p = reinterpret_cast<const T*>(
+                    reinterpret_cast<const char*>(base + k0) + (out ? 0 : offset[t]));
+                *reinterpret_cast<v4u*>(lds + (t * THREADS + threadIdx.x) * 16) =
+                    load_chunk(p, out ? 0 : k1 - k);
+            } else {
+                load_to_lds(buf, lds + (t * THREADS + wave * 64) * 16,
+                            part && k >= k1 ? kOutside : offset[t]);
+            }
+        }
+    }
+    // The same through registers.
+    __device__ __forceinline__ void fetch(int k0) {
+#pragma unroll
+        for (int t = 0; t < CHUNKS; ++t) {
+            const int k = k0 + (ACROSS ? maj[t] : min[t]);
+            const int at = ACROSS ? min[t] : maj[t];
+            const int64_t most = ACROSS ? (k < k1 ? left - at : 0) : (at < left ? k1 - k : 0);
+            const int64_t from = most <= 0 ? 0 : ACROSS ? k * ld + at : at * ld + k;
+            held[t] = load_chunk(base + from, most);
+        }
+    }
+    __device__ __forceinline__ void put(char* lds) const {
+#pragma unroll
+        for (int t = 0; t < CHUNKS; ++t)
+            *reinterpret_cast<v4u*>(lds + (t * THREADS + threadIdx.x) * 16) = held[t];
+    }
+};
+
+// Part, row tile and column tile of this workgroup; false past the last.
+__device__ __forceinline__ bool place_of(const LinearArgs& a, int* part, uint32_t* mt,
+                                         uint32_t* nt) {
+    const uint32_t per = 8 * ((a.mt * a.nt + 7) / 8);
+    *part = static_cast<int>(blockIdx.x / per);
+    return tile_of(blockIdx.x % per, a.mt, a.nt, mt, nt);
+}
+
+template <typename T, typename S, bool AX, bool AW, bool DIRECT>
+__global__ __launch_bounds__(S::kThreads) void linear_kernel(LinearArgs a) {
+    __shared__ __attribute__((aligned(16))) char a0[S::kM * kRowBytes];
+    __shared__ __attribute__((aligned(16))) char b0[S::kN * kRowBytes];
+    __shared__ __attribute__((aligned(16))) char a1[S::kM * kRowBytes];
+    __shared__ __attribute__((aligned(16))) char b1[S::kN * kRowBytes];
+    int part;
+    uint32_t mt, nt;
+    if (!place_of(a, &part, &mt, &nt)) return;
+    const int m0 = static_cast<int>(mt) * S::kM, n0 = static_cast<int>(nt) * S::kN;
+    const int k0 = part * a.unit, k1 = a.k - k0 > a.unit ? k0 + a.unit : a.k;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / S::kWC * S::kMI * 16, wn = wave % S::kWC * S::kNJ * 16;
+    const int tiles = (k1 - k0 + kDepth<T> - 1) / kDepth<T>;
+    Side<T, S::kM, AX, S::kCA, S::kThreads> xs(a.x, a.ldx, m0, a.m, k1);
+    Side<T, S::kN, AW, S::kCB, S::kThreads> ws(a.w, a.ldw, n0, a.n, k1);
+    Sums<T, S::kMI, S::kNJ> acc;
+    const Reader<T, S::kM, AX, S::kMI> ra(wm, lane);
+    const Reader<T, S::kN, AW, S::kNJ> rb(wn, lane);
+    auto compute = [&](const char* la, const char* lb) { multiply<T, S>(ra, rb, la, lb, acc.now); };
+    auto join = [&] { acc.join(); };
+    auto load = [&](int kt, char* la, char* lb) {
+        const int k = k0 + kt * kDepth<T>;
+        if constexpr (DIRECT) {
+            xs.direct(k, la, wave);
+            ws.direct(k, lb, wave);
+        } else {
+            xs.fetch(k);
+            ws.fetch(k);
+        }
+    };
+    auto store = [&](char* la, char* lb) {
+        xs.put(la);
+        ws.put(lb);
+    };
+    pipeline<DIRECT>(tiles, a0, b0, a1, b1, load, store, compute, join);
+    store_sums<T>(a, part, m0 + wm, n0 + wn, lane, acc.result());
+}
+
+// The large tile (tiles.hpp): 16-bit operands that can be loaded directly, in
+// whole chunks (along the contraction, its length % 8 = 0; across it, the rows or
+// columns % 8 = 0).
+template <typename T, bool AX, bool AW>
+__global__ __launch_bounds__(kRingThreads) void linear_ring_kernel(LinearArgs a) {
+    TG_RING_LDS;
+    int part;
+    uint32_t mt, nt;
+    if (!place_of(a, &part, &mt, &nt)) return;
+    const int m0 = static_cast<int>(mt) * 256, n0 = static_cast<int>(nt) * 256;
+    const int kb = part * a.unit, k1 = a.k - kb > a.unit ? kb + a.unit : a.k;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / 4 * 128, wn = wave % 4 * 64;
+    const T* xb = static_cast<const T*>(a.x) + (AX ? m0 : m0 * a.ldx);
+    const T* wb = static_cast<const T*>(a.w) + (AW ? n0 : n0 * a.ldw);
+    uint32_t ao[2], bo[2];
+    int ak[2], bk[2];  // the chunks' places along the contraction
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        int major, minor;
+        part_place<AX>(t * kRingThreads + tid, &major, &minor);
+        ak[t] = AX ? major : minor;
+        ao[t] = m0 + (AX ? minor : major) < a.m ? static_cast<uint32_t>(2 * (major * a.ldx + minor))
+                                                : kOutside;
+        part_place<AW>(t * kRingThreads + tid, &major, &minor);
+        bk[t] = AW ? major : minor;
+        bo[t] = n0 + (AW ? minor : major) < a.n ? static_cast<uint32_t>(2 * (major * a.ldw + minor))
+                                                : kOutside;
+    }
+    auto load = [&](int u, char* la, char* lb) {
+        const int k0 = kb + u * kStep;
+        // What lies behind k1 is 0: where both operands run across, past buffers
+        // that end with it (no registers for the chunks' places; 11 were spilled).
+        constexpr bool kEnds = AX && AW;
+        const int64_t rows = k1 - k0, most = rows > 0 ? kDirectBytes : 0;
+        const auto xbuf = buffer_of(AX ? xb + k0 * a.ldx : xb + k0,
+                                    kEnds && rows > 0 ? 2 * ((rows - 1) * a.ldx + a.m - m0) : most);
+        const auto wbuf = buffer_of(AW ? wb + k0 * a.ldw : wb + k0,
+                                    kEnds && rows > 0 ? 2 * ((rows - 1) * a.ldw + a.n - n0) : most);
+        const bool part = !kEnds && k0 + kStep > k1;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+            load_to_lds(xbuf, la + (t * kRingThreads + wave * 64) * 16,
+                        part && k0 + ak[t] >= k1 ? kOutside : ao[t]);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+            load_to_lds(wbuf, lb + (t * kRingThreads + wave * 64) * 16,
+                        part && k0 + bk[t] >= k1 ? kOutside : bo[t]);
+    };
+    v4f acc[8][4] = {};
+    PartReader<AX, 8, true> ra(wm, lane);
+    PartReader<AW, 4, AX> rb(wn, lane);
+    ring<T>((k1 - kb + kStep - 1) / kStep, ra, rb, [](int) {}, load, a0, b0, a1, b1, a2, b2, a3, b3,
+            acc);
+    store_sums<T>(a, part, m0 + wm, n0 + wn, lane, acc);
+}
+
+using Medium = Shape<128, 128, 2, 2>;
+using Small = Shape<64, 64, 2, 2>;
+using Few = Shape<32, 128, 1, 4>;
+
+template <typename T, bool AX, bool AW>
+void launch_product(LinearArgs& a, const LinearPlan& p, bool direct, hipStream_t s) {
+    a.mt = static_cast<uint32_t>(p.mt);
+    a.nt = static_cast<uint32_t>(p.nt);
+    a.unit = static_cast<int>(p.unit);
+    a.parts = static_cast<int>(p.parts);
+    const int64_t per = 8 * ceil_div(p.mt * p.nt, 8);
+    const unsigned grid = grid_of("linear", per * p.parts, kRingThreads);
+    auto tiled = [&](auto shape) {
+        using S = decltype(shape);
+        direct ? linear_kernel<T, S, AX, AW, true><<<grid, S::kThreads, 0, s>>>(a)
+               : linear_kernel<T, S, AX, AW, false><<<grid, S::kThreads, 0, s>>>(a);
+    };
+    if (p.em == 32) {
+        tiled(Few{});
+    } else if (p.em == 64) {
+        tiled(Small{});
+    } else if (p.em == 128) {
+        tiled(Medium{});
+    } else if constexpr (sizeof(T) == 2) {
+        linear_ring_kernel<T, AX, AW><<<grid, kRingThreads, 0, s>>>(a);
+    }
+    TG_LAUNCH_CHECK();
+    if (p.parts > 1) {
+        const int64_t threads = static_cast<int64_t>(a.m) * ceil_div(a.n, 4);
+        join_kernel<T><<<grid_of("linear", ceil_div(threads, 256), 256), 256, 0, s>>>(a);
+        TG_LAUNCH_CHECK();
+    }
+}
+
+// ---------------------------------------------------------------------------
+// d = dy act'(pre) and its columns' sums: a workgroup takes kActRows rows of 32
+// VEC columns, 8 rows at a time; the parts' sums are added in order by
+// columns_kernel.  ACT NONE: the sums alone.
+// ---------------------------------------------------------------------------
+template <typename T, int ACT>
+__global__ __launch_bounds__(256) void act_backward_kernel(ActArgs a) {
+    constexpr int VEC = kVec<T>;
+    __shared__ float join[8][32 * VEC];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const int64_t c = (static_cast<int64_t>(blockIdx.x) * 32 + x) * VEC;
+    const int64_t r0 = static_cast<int64_t>(blockIdx.y) * a.rows;
+    const int64_t r1 = a.m - r0 > a.rows ? r0 + a.rows : a.m;
+    float s[VEC] = {};
+    for (int64_t r = r0 + y; r < r1; r += 8) {
+        float v[VEC], p[VEC];
+        load_floats<T, VEC>(static_cast<const T*>(a.dy) + r * a.lddy + c, a.n - c, v);
+        if constexpr (ACT != TG_EPI_NONE) {
+            load_floats<T, VEC>(static_cast<const T*>(a.pre) + r * a.ldp + c, a.n - c, p);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[e] *= slope_of<ACT>(p[e]);
+            if (a.d) store_floats<T, VEC>(static_cast<T*>(a.d) + r * a.ldd + c, a.n - c, v);
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s[e] += v[e];
+    }
+    if (!a.part) return;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) join[y][x * VEC + e] = s[e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * VEC; i += 256) {
+        const int64_t at = static_cast<int64_t>(blockIdx.x) * 32 * VEC + i;
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) v += join[w][i];
+        if (at < a.n) a.part[static_cast<int64_t>(blockIdx.y) * a.n + at] = v;
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void columns_kernel(const float* __restrict__ part, int64_t n,
+                                                      int64_t parts, T* __restrict__ out) {
+    __shared__ float join[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+    float s = 0.0f;
+    if (c < n)
+        for (int64_t p = wave; p < parts; p += 4) s += part[p * n + c];
+    join[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && c < n)
+        out[c] = static_cast<T>(join[0][lane] + join[1][lane] + (join[2][lane] + join[3][lane]));
+}
+
+template <typename T>
+void launch_act(const ActArgs& a, int act, hipStream_t s) {
+    const int64_t cols = ceil_div(a.n, 32 * kVec<T>), parts = ceil_div(a.m, a.rows);
+    require(cols * 256 < (int64_t(1) << 32) && parts < 65536, "linear_backward: too many elements");
+    const dim3 grid(static_cast<unsigned>(cols), static_cast<unsigned>(parts));
+    if (act == TG_EPI_NONE) act_backward_kernel<T, TG_EPI_NONE><<<grid, 256, 0, s>>>(a);
+    if (act == TG_EPI_RELU) act_backward_kernel<T, TG_EPI_RELU><<<grid, 256, 0, s>>>(a);
+    if (act == TG_EPI_ELU) act_backward_kernel<T, TG_EPI_ELU><<<grid, 256, 0, s>>>(a);
+    if (act == TG_EPI_GELU) act_backward_kernel<T, TG_EPI_GELU><<<grid, 256, 0, s>>>(a);
+    if (act == TG_EPI_SILU) act_backward_kernel<T, TG_EPI_SILU><<<grid, 256, 0, s>>>(a);
+    TG_LAUNCH_CHECK();
+}
+
+template <typename T>
+void launch_columns(const float* part, int64_t n, int64_t parts, void* out, hipStream_t s) {
+    columns_kernel<T><<<grid_of("linear_backward", ceil_div(n, 64), 256), 256, 0, s>>>(
+        part, n, parts, static_cast<T*>(out));
+    TG_LAUNCH_CHECK();
+}
+
+}  // namespace
+
+// What one of the .hip files compiles.
+#define TG_LINEAR_OF(T)                                                                          \
+    template <>                                                                                  \
+    void linear_product<T>(LinearArgs & a, const LinearPlan& p, bool ax, bool aw, bool direct,    \
+                           hipStream_t s) {                                                      \
+        if (ax)                                                                                  \
+            launch_product<T, true, true>(a, p, direct, s);                                      \
+        else if (aw)                                                                             \
+            launch_product<T, false, true>(a, p, direct, s);                                     \
+        else                                                                                     \
+            launch_product<T, false, false>(a, p, direct, s);                                    \
+    }                                                                                            \
+    template <>                                                                                  \
+    void linear_act<T>(const ActArgs& a, int act, hipStream_t s) {                               \
+        launch_act<T>(a, act, s);                                                                \
+    }                                                                                            \
+    template <>                                                                                  \
+    void linear_columns<T>(const float* part, int64_t n, int64_t parts, void* out,               \
+                           hipStream_t s) {                                                      \
+        launch_columns<T>(part, n, parts, out, s);                                               \
+    }
+
+}  // namespace tg
