@@ -13,7 +13,8 @@ I32 = torch.int32
 SIZES = [(1, 1), (3, 2), (700, 7), (65, 41), (64, 47), (1, 41), (7, 64), (9, 65), (200, 100),
          (33, 257), (5, 511), (3, 1000), (4, 1025), (2, 2048), (3, 2049), (2, 4097), (2, 8200),
          (300, 5000), (1, 16384), (2, 32000), (1, 32769), (3, 65537), (1, 131072), (2, 131079),
-         (1, 200003), (1, 1100001), (20011, 41), (600, 9001)]
+         (1, 200003), (1, 1100001), (20011, 41), (600, 9001), (1030, 3000), (1030, 12000),
+         (1030, 30000), (1030, 60000)]
 
 
 def make(rows, classes, dt, seed):
