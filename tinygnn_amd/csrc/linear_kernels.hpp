@@ -123,24 +123,42 @@ __device__ __forceinline__ void store_sums(const LinearArgs& a, int part, int m0
     });
 }
 
-// y = the epilogue of the parts' sums, in order.
-template <typename T>
+// y = the epilogue of the parts' sums: Y threads take every Y-th part of four
+// results, whose sums are added in order.
+template <typename T, int Y>
 __global__ __launch_bounds__(256) void join_kernel(LinearArgs a) {
+    constexpr int X = 256 / Y;
+    __shared__ float sums[Y > 1 ? Y - 1 : 1][X][4];
+    const int x = threadIdx.x % X, y = threadIdx.x / X;
     const uint32_t chunks = (static_cast<uint32_t>(a.n) + 3) / 4;
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * X + x;
     const int64_t row = t / chunks;
-    if (row >= a.m) return;
     const int n = static_cast<int>(t - row * chunks) * 4;
     const int64_t size = static_cast<int64_t>(a.m) * a.n;
     const float* p = a.part + row * a.n + n;
     float s[4] = {};
-#pragma unroll 4
-    for (int i = 0; i < a.parts; ++i) {
-        float v[4];
-        load_floats<float, 4>(p + i * size, a.n - n, v);
+    if (row < a.m) {
+#pragma unroll 8
+        for (int i = y; i < a.parts; i += Y) {
+            float v[4];
+            load_floats<float, 4>(p + i * size, a.n - n, v);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] += v[e];
+            for (int e = 0; e < 4; ++e) s[e] += v[e];
+        }
     }
+    if constexpr (Y > 1) {
+        if (y > 0) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sums[y - 1][x][e] = s[e];
+        }
+        __syncthreads();
+        if (y > 0) return;
+#pragma unroll
+        for (int i = 0; i < Y - 1; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] += sums[i][x][e];
+    }
+    if (row >= a.m) return;
     float bias[4] = {};
     if (a.bias) load_floats<T, 4>(static_cast<const T*>(a.bias) + n, a.n - n, bias);
     with_act(a.act, [&](auto act) { finish<T, decltype(act)::value>(a, row, n, s, bias); });
@@ -348,7 +366,8 @@ void launch_product(LinearArgs& a, const LinearPlan& p, bool direct, hipStream_t
     TG_LAUNCH_CHECK();
     if (p.parts > 1) {
         const int64_t threads = static_cast<int64_t>(a.m) * ceil_div(a.n, 4);
-        join_kernel<T><<<grid_of("linear", ceil_div(threads, 256), 256), 256, 0, s>>>(a);
+        p.parts > 8 ? join_kernel<T, 8><<<grid_of("linear", ceil_div(threads, 32), 256), 256, 0, s>>>(a)
+                    : join_kernel<T, 1><<<grid_of("linear", ceil_div(threads, 256), 256), 256, 0, s>>>(a);
         TG_LAUNCH_CHECK();
     }
 }
@@ -393,18 +412,22 @@ __global__ __launch_bounds__(256) void act_backward_kernel(ActArgs a) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void columns_kernel(const float* __restrict__ part, int64_t n,
-                                                      int64_t parts, T* __restrict__ out) {
-    __shared__ float join[4][64];
+__global__ __launch_bounds__(1024) void columns_kernel(const float* __restrict__ part, int64_t n,
+                                                       int64_t parts, T* __restrict__ out) {
+    __shared__ float join[16][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + lane;
     float s = 0.0f;
-    if (c < n)
-        for (int64_t p = wave; p < parts; p += 4) s += part[p * n + c];
+    if (c < n) {
+#pragma unroll 8
+        for (int64_t p = wave; p < parts; p += 16) s += part[p * n + c];
+    }
     join[wave][lane] = s;
     __syncthreads();
-    if (wave == 0 && c < n)
-        out[c] = static_cast<T>(join[0][lane] + join[1][lane] + (join[2][lane] + join[3][lane]));
+    if (wave > 0 || c >= n) return;
+#pragma unroll
+    for (int w = 1; w < 16; ++w) s += join[w][lane];
+    out[c] = static_cast<T>(s);
 }
 
 template <typename T>
@@ -422,7 +445,7 @@ void launch_act(const ActArgs& a, int act, hipStream_t s) {
 
 template <typename T>
 void launch_columns(const float* part, int64_t n, int64_t parts, void* out, hipStream_t s) {
-    columns_kernel<T><<<grid_of("linear_backward", ceil_div(n, 64), 256), 256, 0, s>>>(
+    columns_kernel<T><<<grid_of("linear_backward", ceil_div(n, 64), 1024), 1024, 0, s>>>(
         part, n, parts, static_cast<T*>(out));
     TG_LAUNCH_CHECK();
 }

@@ -193,11 +193,25 @@ __device__ __forceinline__ int key_class(Key k) {
     return static_cast<int>(~static_cast<uint32_t>(k));
 }
 
-// A step of a bitonic sort of the wavefront's keys: the partner is lane ^ J (a
-// mirrored one for 8 and 4: see sort_falling).
+// The value of lane ^ J, for every lane.
+template <int J>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+    const int x = static_cast<int>(v);
+    if constexpr (J == 4) {  // banks 0, 2 from four lanes up, 1, 3 from four down
+        const int up = __builtin_amdgcn_update_dpp(x, x, 0x104, 0xF, 0x5, false);
+        return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(up, x, 0x114, 0xF, 0xA, false));
+    } else if constexpr (J == 8) {
+        return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, x, 0x128, 0xF, 0xF, false));
+    } else {
+        return lane_flip<J>(v);
+    }
+}
+
+// A step of a bitonic sort of the wavefront's keys.
 template <int J>
 __device__ __forceinline__ Key sort_step(Key v, bool high) {
-    const Key o = static_cast<Key>(__shfl_xor(v, J, kWave));
+    const Key o = static_cast<Key>(lane_xor<J>(static_cast<uint32_t>(v >> 32))) << 32 |
+                  lane_xor<J>(static_cast<uint32_t>(v));
     return (v > o) == high ? v : o;
 }
 
@@ -512,6 +526,13 @@ __device__ __forceinline__ float distill_factor(const LossArgs& a, int64_t row, 
     return g == 0.0f || total == 0.0f || st.empty() ? 0.0f : g * a.inv * (total / total);
 }
 
+// d[at] -= v.
+template <int VEC>
+__device__ __forceinline__ void subtract(int at, float v, float (&d)[VEC]) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) d[e] -= at == e ? v : 0.0f;
+}
+
 enum { kLogProbs = 0, kDistill = 1, kSegment = 2 };
 
 // One row (kSegment: one segment) for each NT threads.
@@ -557,6 +578,8 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void row_kernel(LossArgs a) {
     } else {
         __shared__ float q[kRows][kMaxTeacher];
         __shared__ int id[kRows][kMaxTeacher];
+        // places among a thread's classes: their count << 16, and the sum of their
+        // numbers, which is the number of a single one
         __shared__ uint32_t hits[kRows][NT];
         __shared__ float factor[kRows];
         const RowStats st(r);
@@ -572,13 +595,15 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void row_kernel(LossArgs a) {
         }
         if (!a.dlogits) return;
         x.group_sync();
-        // the chunks with a class of the teacher's, by their owners
         for (int j = x.tid; j < a.k; j += NT) {
             const int c = id[sub][j];
-            if (c >= 0) atomicOr(&hits[sub][c / VEC % NT], 1u << (c / VEC / NT));
+            if (c >= 0) atomicAdd(&hits[sub][c / VEC % NT], 1u << 16 | static_cast<uint32_t>(j));
         }
         x.group_sync();
         const uint32_t hit = hits[sub][x.tid];
+        const bool several = hit >> 16 > 1;
+        const int only = hit >> 16 == 1 ? id[sub][hit & 0xFFFF] : -1;
+        const float only_q = hit >> 16 == 1 ? q[sub][hit & 0xFFFF] : 0.0f;
         const float g = factor[sub];
         const RowGradient grad{st.m, st.log_s * kLog2e, g, 0.0f};
         T* out = static_cast<T*>(a.dlogits) + row * a.lddl;
@@ -588,11 +613,11 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void row_kernel(LossArgs a) {
             x.values(i, v);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) d[e] = grad(v[e], a.c);
-            if (hit >> i & 1) {
+            if (static_cast<uint32_t>(only - x.at(i)) < VEC) subtract(only - x.at(i), only_q * g, d);
+            if (several) {
                 for (int j = 0; j < a.k; ++j) {
                     const int at = id[sub][j] - x.at(i);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) d[e] -= at == e ? q[sub][j] * g : 0.0f;
+                    if (static_cast<uint32_t>(at) < VEC) subtract(at, q[sub][j] * g, d);
                 }
             }
             if (g == 0.0f) {
@@ -606,15 +631,16 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void row_kernel(LossArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// The segments of a row joined, by one wavefront: the sums, and the top classes
-// by k rounds over the segments' lists, which are in falling order.
+// The segments of a row joined: the sums by the first wavefront, the top classes by
+// all NT / 64: each merges its share of the segments' lists (in falling order, 64
+// at most), then pairs of wavefronts theirs.
 // ---------------------------------------------------------------------------
-template <typename T, int MODE>
-__global__ __launch_bounds__(kWave) void join_kernel(LossArgs a) {
-    extern __shared__ __attribute__((aligned(16))) uint8_t heads[];  // [segments]: places taken
+template <typename T, int MODE, int NT>
+__global__ __launch_bounds__(NT) void join_kernel(LossArgs a) {
     const int64_t row = a.row0 + blockIdx.x;
-    const int lane = threadIdx.x;
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const float* part = a.part + 4 * row * a.segments;
+    // (every wavefront needs the sums: the values of the top classes are by wave 0)
     float m = -INFINITY;
     for (int i = lane; i < a.segments; i += kWave) m = __builtin_fmaxf(m, part[4 * i]);
     m = wave_all(m, Max{});
@@ -631,23 +657,28 @@ __global__ __launch_bounds__(kWave) void join_kernel(LossArgs a) {
     const RowSums r{m, wave_all(s, Add{}), wave_all(u, Add{})};
     const RowStats st(r);
     if constexpr (MODE == kLogProbs) {
-        if (lane == 0) put_row<T>(a, row, r, st);
-        if (!a.top) return;
-        const Key* keys = a.part_keys + row * a.segments * a.top;
-        for (int i = lane; i < a.segments; i += kWave) heads[i] = 0;
-        for (int j = 0; j < a.top; ++j) {
-            Key best = 0;
-            int from = -1;
-            for (int i = lane; i < a.segments; i += kWave) {
-                const Key k = heads[i] < a.top ? keys[static_cast<int64_t>(i) * a.top + heads[i]] : 0;
-                if (k > best) {
-                    best = k;
-                    from = i;
-                }
+        if (threadIdx.x == 0) put_row<T>(a, row, r, st);
+        if constexpr (NT > kWave) {  // top classes
+            __shared__ Key lists[NT];
+            const Key* keys = a.part_keys + row * a.segments * a.top;
+            auto list = [&](int i, int at) {
+                return i < a.segments && at < a.top ? keys[static_cast<int64_t>(i) * a.top + at]
+                                                    : Key(0);
+            };
+            constexpr int kStride = NT / kWave;
+            Key v = list(wave, lane), next = list(wave + kStride, 63 - lane);
+            for (int i = wave + kStride; i < a.segments; i += kStride) {
+                const Key o = next;
+                next = list(i + kStride, 63 - lane);
+                v = merge_falling(v, o);
             }
-            const Key most = wave_all(best, Max{});
-            if (best == most && from >= 0) heads[from] += 1;
-            if (lane == 0) put_top(a, row, j, most, st);
+#pragma unroll
+            for (int half = NT / kWave / 2; half >= 1; half /= 2) {
+                if (wave >= half && wave < 2 * half) lists[threadIdx.x] = v;
+                __syncthreads();
+                if (wave < half) v = merge_falling(v, lists[(wave + half) * kWave + 63 - lane]);
+            }
+            if (wave == 0 && lane < a.top) put_top(a, row, lane, v, st);
         }
     } else {
         const Teacher t = teach<T>(
@@ -755,10 +786,9 @@ __global__ __launch_bounds__(256) void gradient_kernel(LossArgs a, int64_t spans
         } else {
             if (hit >> i & 1) {
                 for (int j = 0; j < a.k; ++j) {
-                    const int64_t c = a.ids[row * a.k + j];
-                    const float q = a.q[row * a.k + j] * g;
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) d[e] -= c == first + at + e ? q : 0.0f;
+                    const int64_t c = a.ids[row * a.k + j] - first - at;
+                    if (static_cast<uint64_t>(c) < VEC)
+                        subtract(static_cast<int>(c), a.q[row * a.k + j] * g, d);
                 }
             }
         }
@@ -776,39 +806,50 @@ __device__ __forceinline__ int row_of(int e, uint32_t magic) {
     return magic == 0 ? e : static_cast<int>(__umulhi(static_cast<uint32_t>(e), magic));
 }
 
-template <typename T, typename F>
-__device__ __forceinline__ void each_chunk(int rows, int classes, uint32_t magic, F&& fn) {
-    constexpr int VEC = kVec<T>;
-    const int all = rows * classes;
-#pragma unroll 4
-    for (int e = threadIdx.x * VEC; e < all; e += kWave * VEC) {
-        const int row = row_of(e, magic);
-        fn(e, all - e, row, e - row * classes);
+// fn(i-th value, its place in LDS) for the VEC values from e on of rows that lie
+// one behind the other.
+template <int VEC, typename F>
+__device__ __forceinline__ void each_value(int e, int left, int classes, uint32_t magic, F&& fn) {
+    const int stride = classes | 1;
+    int row = row_of(e, magic), c = e - row * classes, at = row * stride + c;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+        if (i < left) fn(i, at);
+        const bool next = ++c == classes;
+        c = next ? 0 : c;
+        at += next ? stride - classes + 1 : 1;
     }
 }
 
 template <typename T, int MODE, bool ENTROPY, bool GRADIENT>
 __global__ __launch_bounds__(kWave) void tiny_kernel(LossArgs a, uint32_t magic) {
     constexpr int VEC = kVec<T>;
-    __shared__ float lds[kWave * (kTinyClasses + 1)];
+    extern __shared__ __attribute__((aligned(16))) float lds[];  // [64][classes | 1]
     const int classes = static_cast<int>(a.classes), stride = classes | 1;
     const int64_t r0 = a.row0 + static_cast<int64_t>(blockIdx.x) * kWave, row = r0 + threadIdx.x;
     const int rows = static_cast<int>(a.rows - r0 < kWave ? a.rows - r0 : kWave);
     const T* p = static_cast<const T*>(a.logits) + r0 * a.ld;
+    const int all = rows * classes;
     if (a.ld == classes) {
-        each_chunk<T>(rows, classes, magic, [&](int e, int left, int r, int c) {
-            float v[VEC];
-            floats_of<T>(load_classes<T>(p + e, left), v);
+        constexpr int kBatch = 8;  // loads in flight
+        for (int base = 0; base < all; base += kBatch * kWave * VEC) {
+            v4u v[kBatch];
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                if (i < left) lds[r * stride + c] = v[i];
-                const bool next = ++c == classes;
-                c = next ? 0 : c;
-                r += next ? 1 : 0;
+            for (int b = 0; b < kBatch; ++b) {
+                const int e = base + (b * kWave + threadIdx.x) * VEC;
+                v[b] = load_classes<T>(p + e, all - e);
             }
-        });
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const int e = base + (b * kWave + threadIdx.x) * VEC;
+                if (e >= all) continue;
+                float f[VEC];
+                floats_of<T>(v[b], f);
+                each_value<VEC>(e, all - e, classes, magic, [&](int i, int at) { lds[at] = f[i]; });
+            }
+        }
     } else {
-        for (int e = threadIdx.x; e < rows * classes; e += kWave) {
+        for (int e = threadIdx.x; e < all; e += kWave) {
             const int r = row_of(e, magic);
             lds[e + r * (stride - classes)] = static_cast<float>(p[r * a.ld + e - r * classes]);
         }
@@ -875,40 +916,53 @@ __global__ __launch_bounds__(kWave) void tiny_kernel(LossArgs a, uint32_t magic)
             }
             if (in && !zero) x[y] += g;
         } else {
+            // the teacher's places, kPlaces at a time; with no more they are read once
             const RowStats st(r);
-            const int64_t at = row * a.k;
-            float tm = -INFINITY, total = 0.0f, loss = 0.0f;
-            auto place = [&](int j, int* c) {
-                *c = a.ids[at + j];
-                return *c >= 0 && *c < classes ? teacher_at(a, at + j) : -INFINITY;
-            };
-            int c;
-            for (int j = 0; j < a.k; ++j) tm = __builtin_fmaxf(tm, place(j, &c));
-            for (int j = 0; j < a.k; ++j) {
-                const float t = place(j, &c);
-                total += t == -INFINITY ? 0.0f : exp2_of((t - tm) * a.c);
-            }
-            const float log_total = logf(total), per = total == 0.0f ? 0.0f : 1.0f / total;
-            for (int j = 0; j < a.k; ++j) {
-                const float t = place(j, &c);
-                const float q = t == -INFINITY ? 0.0f * per : exp2_of((t - tm) * a.c) * per;
-                if (q != 0.0f && t != -INFINITY) {
-                    const float logp = st.empty() ? -INFINITY : st.logp(x[c], a.inv);
-                    loss += q * ((t - tm) * a.inv - log_total - logp);
+            constexpr int kPlaces = 8;
+            float t[kPlaces];
+            int c[kPlaces];
+            auto places = [&](int j0) {
+#pragma unroll
+                for (int j = 0; j < kPlaces; ++j) {
+                    const bool there = j0 + j < a.k;
+                    const int64_t at = row * a.k + (there ? j0 + j : 0);
+                    c[j] = a.ids[at];
+                    t[j] = teacher_at(a, at);
+                    if (!there || c[j] < 0 || c[j] >= classes) {
+                        t[j] = -INFINITY;
+                        c[j] = 0;
+                    }
                 }
-            }
+            };
+            auto each = [&](auto&& fn) {
+                for (int j0 = 0; j0 < a.k; j0 += kPlaces) {
+                    if (a.k > kPlaces) places(j0);
+#pragma unroll
+                    for (int j = 0; j < kPlaces; ++j) fn(t[j], c[j]);
+                }
+            };
+            if (a.k <= kPlaces) places(0);
+            float tm = -INFINITY, total = 0.0f, loss = 0.0f;
+            each([&](float tj, int) { tm = __builtin_fmaxf(tm, tj); });
+            each([&](float tj, int) {
+                total += tj == -INFINITY ? 0.0f : exp2_of((tj - tm) * a.c);
+            });
+            const float log_total = logf(total), per = total == 0.0f ? 0.0f : 1.0f / total;
+            each([&](float tj, int cj) {
+                const float q = tj == -INFINITY ? 0.0f : exp2_of((tj - tm) * a.c) * per;
+                const float logp = st.empty() ? -INFINITY : st.logp(x[cj], a.inv);
+                if (q != 0.0f) loss += q * ((tj - tm) * a.inv - log_total - logp);
+            });
             a.loss[row] = loss;
             if (GRADIENT) {
                 const float g = distill_factor(a, row, total, st);
                 const RowGradient grad{st.m, st.log_s * kLog2e, g, 0.0f};
 #pragma unroll 8
                 for (int i = 0; i < classes; ++i) x[i] = g == 0.0f ? 0.0f : grad(x[i], a.c);
-                if (g != 0.0f) {
-                    for (int j = 0; j < a.k; ++j) {
-                        const float t = place(j, &c);
-                        if (t != -INFINITY) x[c] -= g * (exp2_of((t - tm) * a.c) * per);
-                    }
-                }
+                if (g != 0.0f)
+                    each([&](float tj, int cj) {
+                        if (tj != -INFINITY) x[cj] -= g * (exp2_of((tj - tm) * a.c) * per);
+                    });
             }
         }
     }
@@ -916,19 +970,13 @@ __global__ __launch_bounds__(kWave) void tiny_kernel(LossArgs a, uint32_t magic)
         __syncthreads();
         T* out = static_cast<T*>(a.dlogits) + r0 * a.lddl;
         if (a.lddl == classes) {
-            each_chunk<T>(rows, classes, magic, [&](int e, int left, int r, int c) {
-                float v[VEC];
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    v[i] = i < left ? lds[r * stride + c] : 0.0f;
-                    const bool next = ++c == classes;
-                    c = next ? 0 : c;
-                    r += next ? 1 : 0;
-                }
-                store_classes<T>(out + e, left, v);
-            });
+            for (int e = threadIdx.x * VEC; e < all; e += kWave * VEC) {
+                float v[VEC] = {};
+                each_value<VEC>(e, all - e, classes, magic, [&](int i, int at) { v[i] = lds[at]; });
+                store_classes<T>(out + e, all - e, v);
+            }
         } else {
-            for (int e = threadIdx.x; e < rows * classes; e += kWave) {
+            for (int e = threadIdx.x; e < all; e += kWave) {
                 const int r = row_of(e, magic);
                 out[r * a.lddl + e - r * classes] = static_cast<T>(lds[e + r * (stride - classes)]);
             }
@@ -976,8 +1024,8 @@ bool with_shape(int64_t n, int vec, F&& fn) {
         fn(integral_constant<int, 64>{}, integral_constant<int, 4>{});
     else if (chunks <= 256 * 4)
         fn(integral_constant<int, 256>{}, integral_constant<int, 4>{});
-    else if (chunks <= 1024 * 4)
-        fn(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
+    else if (chunks <= 256 * 16)
+        fn(integral_constant<int, 256>{}, integral_constant<int, 16>{});
     else if (chunks <= 1024 * 8)
         fn(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
     else if (chunks <= kMostChunks)
@@ -1066,7 +1114,8 @@ void launch_tiny(const char* what, const LossArgs& a, hipStream_t s) {
     const unsigned grid = grid_of(what, ceil_div(a.rows, kWave), kWave);
     const uint32_t magic =
         static_cast<uint32_t>(((uint64_t(1) << 32) + a.classes - 1) / a.classes);
-    tiny_kernel<T, MODE, ENTROPY, GRADIENT><<<grid, kWave, 0, s>>>(a, magic);
+    const size_t lds = sizeof(float) * kWave * (a.classes | 1);
+    tiny_kernel<T, MODE, ENTROPY, GRADIENT><<<grid, kWave, lds, s>>>(a, magic);
     TG_LAUNCH_CHECK();
 }
 
@@ -1083,9 +1132,15 @@ void launch_gradient(const char* what, const LossArgs& all, hipStream_t s) {
 // Joins the rows' segments.
 template <typename T, int MODE>
 void launch_join(const char* what, const LossArgs& all, hipStream_t s) {
-    const size_t lds = MODE == kLogProbs && all.top ? (all.segments + 15) / 16 * 16 : 0;
-    sliced(all, kWave, [&](const LossArgs& a, int64_t rows) {
-        join_kernel<T, MODE><<<grid_of(what, rows, kWave), kWave, lds, s>>>(a);
+    constexpr int kTop = 1024;
+    const int threads = all.top ? kTop : kWave;
+    sliced(all, threads, [&](const LossArgs& a, int64_t rows) {
+        const unsigned grid = grid_of(what, rows, threads);
+        if constexpr (MODE == kLogProbs)
+            a.top ? join_kernel<T, MODE, kTop><<<grid, kTop, 0, s>>>(a)
+                  : join_kernel<T, MODE, kWave><<<grid, kWave, 0, s>>>(a);
+        else
+            join_kernel<T, MODE, kWave><<<grid, kWave, 0, s>>>(a);
         TG_LAUNCH_CHECK();
     });
 }
