@@ -12,30 +12,79 @@ namespace {
 
 constexpr int64_t kLongChain = 16384;  // of floats: 64 chains of kSumTiles tiles
 
-// How an out [m x n] with contraction k is cut.
-LinearPlan linear_plan(int64_t m, int64_t n, int64_t k, int type, bool ring) {
-    LinearPlan p{};
+// The time of a product in us by tile, as measured: a tile of `m` x `n` results
+// alone on a CU takes `alone` for each value of the contraction, one of many `busy`
+// of the CU's time, and `fixed` beside that (lookup, first loads, results).
+struct TileCost {
+    int64_t m, n;
+    double alone, busy, fixed;
+};
+constexpr TileCost kTiles16[] = {
+    {32, 128, 0.0082, 0.0035, 0.6},  {64, 64, 0.0078, 0.0031, 0.6},
+    {64, 128, 0.0105, 0.0051, 1.4},  {128, 64, 0.0105, 0.0051, 1.4},
+    {128, 128, 0.0126, 0.0084, 2.5}, {256, 256, 0.0183, 0.0268, 8.0},
+};
+constexpr TileCost kTiles32[] = {
+    {32, 128, 0.0290, 0.0170, 0.7},
+    {64, 64, 0.0262, 0.0172, 0.7},
+    {64, 128, 0.0420, 0.0325, 1.3},
+    {128, 64, 0.0420, 0.0325, 1.3},
+};
+
+// How an out [m x n] with contraction k is cut: the tile and the parts of the
+// contraction that the costs above and the parts' join (2.5 us, its bytes at 9 TB/s,
+// past 200 MB at 5.3) make cheapest.  What it takes is within 10% of the best of 30
+// measured tiles and parts for 19 of 22 products, and within 17% for the others:
+// bf16 4,000 x 2,048, contraction 8,192: 256 x 256 in 2 parts 125 us (128 x 128 in
+// one 134); 512 x 4,096 x 4,096: 64 x 128 in 2 parts 35 (128 x 128 in 4 32); 2,048^3:
+// 64 x 128 29 (128 x 128 32, 256 x 256 51); fp32 232,965 x 256 x 256: 64 x 128 281
+// (64 x 64 311, 128 x 128, which leaves one wavefront a SIMD, 362).
+// Operands that come through registers (kRegisters) take 64 x 64 or, of 16 bits,
+// 128 x 128.
+enum Loads { kRegisters, kDirect, kRing };
+
+LinearPlan linear_plan(int64_t m, int64_t n, int64_t k, int type, Loads loads) {
     const int64_t z = type_size(type), depth = kRowBytes / z;
-    const auto tiles = [&](int64_t a, int64_t b) { return ceil_div(m, a) * ceil_div(n, b); };
-    if (ring && tiles(256, 256) >= 160) {
-        p.em = p.en = 256;
-    } else if (m <= 32) {
-        p.em = 32;
-        p.en = 128;
-    } else if (tiles(128, 128) >= 400) {
-        p.em = p.en = 128;
-    } else {
-        p.em = p.en = 64;
-    }
-    p.mt = ceil_div(m, p.em);
-    p.nt = ceil_div(n, p.en);
-    const int64_t all = p.mt * p.nt;
-    // parts of 4 tiles of the contraction at least, for about 512 workgroups
-    int64_t parts = all >= 256 ? 1 : std::min(ceil_div(512, all), ceil_div(k, 4 * depth));
-    if (type == TG_TYPE_F32) parts = std::max(parts, ceil_div(k, kLongChain));
-    p.unit = std::max(depth, ceil_div(ceil_div(k, std::max<int64_t>(parts, 1)), depth) * depth);
-    p.parts = std::max<int64_t>(1, ceil_div(k, p.unit));
-    return p;
+    LinearPlan best{};
+    double least = 0.0;
+    auto consider = [&](const TileCost& t) {
+        const int64_t mt = ceil_div(m, t.m), nt = ceil_div(n, t.n), tiles = mt * nt;
+        for (int64_t parts = 1; parts <= 256; parts *= 2) {
+            if (parts > 1 && (k < 4 * depth * parts || tiles * parts > 2048)) break;
+            int64_t unit = ceil_div(ceil_div(k, parts), depth) * depth;
+            // (the digits of long chains of floats)
+            if (type == TG_TYPE_F32) unit = std::min(unit, kLongChain);
+            unit = std::max(unit, depth);
+            const int64_t real = std::max<int64_t>(1, ceil_div(k, unit)), groups = tiles * real;
+            const double load = groups < 256 ? static_cast<double>(groups) / 256
+                                             : static_cast<double>(ceil_div(groups, 256));
+            const double u = static_cast<double>(unit);
+            double us = std::max(t.alone * u + t.fixed, load * (t.busy * u + t.fixed));
+            if (real > 1) {
+                const double bytes = 8.0 * static_cast<double>(real) * static_cast<double>(m) *
+                                     static_cast<double>(n);
+                us += 2.5 + bytes / (bytes < 2e8 ? 9e6 : 5.3e6);
+            }
+            if (best.em == 0 || us < least) {
+                least = us;
+                best = {t.m, t.n, mt, nt, unit, real};
+            }
+        }
+    };
+    auto all = [&](const auto& tiles) {
+        for (const TileCost& t : tiles) {
+            const bool square = t.m == t.n;
+            if (loads == kRing || (loads == kDirect ? t.m < 256 : square && t.m < 256)) consider(t);
+        }
+    };
+    type == TG_TYPE_F32 ? all(kTiles32) : all(kTiles16);
+    return best;
+}
+
+// Few rows of x with w's rows along the contraction (few_kernel): no parts.
+// (bf16 1 x 4,096 x 4,096: ...)
+bool few_rows(const LinearArgs& a, bool ax, bool aw) {
+    return !ax && !aw && a.m <= 32 && a.k <= 32768 && (a.n >= 1024 || a.k <= 4096);
 }
 
 // Whether an operand's tiles of up to 256 of its rows or columns can come by
@@ -46,15 +95,20 @@ bool direct_side(const void* p, int64_t ld, int64_t cols, int64_t z, bool across
            (!across || cols * z % 4 == 0) && (256 * ld + cols) * z < kDirectBytes;
 }
 
-// One product with the operands' layouts; part: room for its parts.
-void product(LinearArgs& a, int type, bool ax, bool aw, float* part, hipStream_t s) {
+// One product with the operands' layouts; `room` floats in `part` for its parts.
+void product(LinearArgs& a, int type, bool ax, bool aw, void* part, size_t room, hipStream_t s) {
     const int64_t z = type_size(type);
     const bool direct = direct_side(a.x, a.ldx, ax ? a.m : a.k, z, ax) &&
                         direct_side(a.w, a.ldw, aw ? a.n : a.k, z, aw);
     const bool ring = direct && z == 2 && ((ax && aw) || a.k % 8 == 0) && (!ax || a.m % 8 == 0) &&
                       (!aw || a.n % 8 == 0);
-    const LinearPlan p = linear_plan(a.m, a.n, a.k, type, ring);
-    a.part = p.parts > 1 ? part : nullptr;
+    LinearPlan p{};
+    if (!few_rows(a, ax, aw)) {
+        p = linear_plan(a.m, a.n, a.k, type, ring ? kRing : direct ? kDirect : kRegisters);
+        Carver c(part, room);
+        a.part = reinterpret_cast<float*>(c.take<char>(p.bytes(a.m, a.n)));
+        if (p.parts == 1) a.part = nullptr;
+    }
     with_type(type, "linear", [&](auto t) {
         linear_product<decltype(t)>(a, p, ax, aw, direct, s);
     });
@@ -63,8 +117,10 @@ void product(LinearArgs& a, int type, bool ax, bool aw, float* part, hipStream_t
 // Bytes for the parts of a product, whichever tiles its operands allow.
 size_t parts_bytes(int64_t m, int64_t n, int64_t k, int type) {
     if (m <= 0 || n <= 0) return 0;
-    return std::max(linear_plan(m, n, k, type, false).bytes(m, n),
-                    linear_plan(m, n, k, type, true).bytes(m, n));
+    size_t most = 0;
+    for (const Loads loads : {kRegisters, kDirect, kRing})
+        most = std::max(most, linear_plan(m, n, k, type, loads).bytes(m, n));
+    return most;
 }
 
 constexpr int64_t kActRows = 256;
@@ -72,7 +128,8 @@ constexpr int64_t kActRows = 256;
 struct BackwardPlace {
     void* d;
     float* columns;
-    float* part;
+    void* part;
+    size_t room;
     size_t bytes;
 };
 
@@ -82,9 +139,9 @@ BackwardPlace backward_place(int64_t m, int64_t k, int64_t n, int type, void* ws
     p.d = c.take<char>(static_cast<size_t>(m) * n * type_size(type));
     p.columns = c.take<float>(static_cast<size_t>(ceil_div(m, kActRows)) * n);
     // dx's parts, then dw's, in the same place
-    const size_t part = std::max(parts_bytes(m, k, n, type),
-                                 std::max(parts_bytes(k, n, m, type), parts_bytes(n, k, m, type)));
-    p.part = reinterpret_cast<float*>(c.take<char>(part));
+    p.room = std::max(parts_bytes(m, k, n, type),
+                      std::max(parts_bytes(k, n, m, type), parts_bytes(n, k, m, type)));
+    p.part = c.take<char>(p.room);
     p.bytes = c.bytes();
     return p;
 }
@@ -141,16 +198,15 @@ int tg_linear(int64_t m, int64_t k, int64_t n, int type, const void* x, int64_t 
         a.pre = pre;
         a.ldp = ldp;
         hipStream_t s = static_cast<hipStream_t>(stream);
-        const size_t need = tg::parts_bytes(m, n, k, type);
         tg::TempBuffer temp;
-        if (need && !workspace) {
-            temp.allocate(need, s);
-            workspace = temp.get();
-            workspace_bytes = need;
+        if (!workspace) {
+            workspace_bytes = tg::parts_bytes(m, n, k, type);
+            if (workspace_bytes) {
+                temp.allocate(workspace_bytes, s);
+                workspace = temp.get();
+            }
         }
-        tg::Carver c(workspace, workspace_bytes);
-        float* part = reinterpret_cast<float*>(c.take<char>(need));
-        tg::product(a, type, false, !transposed, part, s);
+        tg::product(a, type, false, !transposed, workspace, workspace_bytes, s);
     });
 }
 
@@ -220,7 +276,7 @@ int tg_linear_backward(int64_t m, int64_t k, int64_t n, int type, const void* dy
             g.ldw = ldw;
             g.y = dx;
             g.ldy = lddx;
-            tg::product(g, type, false, transposed != 0, at.part, s);
+            tg::product(g, type, false, transposed != 0, at.part, at.room, s);
         }
         if (dw) {
             g = tg::LinearArgs{};
@@ -233,7 +289,7 @@ int tg_linear_backward(int64_t m, int64_t k, int64_t n, int type, const void* dy
             g.ldw = transposed ? ldx : ldd;
             g.y = dw;
             g.ldy = g.n;
-            tg::product(g, type, true, true, at.part, s);
+            tg::product(g, type, true, true, at.part, at.room, s);
         }
     });
 }

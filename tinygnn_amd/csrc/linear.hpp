@@ -49,7 +49,8 @@ struct LinearPlan {
     }
 };
 
-// The launches of one element type: a product whose operands run across the
+// The launches of one element type: a product (p.em 0: of few rows, both operands
+// along) whose operands run across the
 // contraction (ax, aw) or along it, d and its columns' sums by parts of rows, and
 // the join of those.
 template <typename T>

@@ -82,7 +82,8 @@ __device__ __forceinline__ void finish(const LinearArgs& a, int64_t row, int n,
 
 // A wavefront's sums from row m0, column n0 on.  Lane (q, r) holds row r of a
 // tile, columns 4 q .. 4 q + 3.
-template <typename T, int MI, int NJ>
+// PLAIN: a product without an epilogue.
+template <typename T, bool PLAIN, int MI, int NJ>
 __device__ __forceinline__ void store_sums(const LinearArgs& a, int part, int m0, int n0, int lane,
                                            const v4f (&acc)[MI][NJ]) {
     const int q = lane >> 4, r = lane & 15;
@@ -97,6 +98,21 @@ __device__ __forceinline__ void store_sums(const LinearArgs& a, int part, int m0
                 const int n = n0 + j * 16 + 4 * q;
                 const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
                 store_floats<float, 4>(to + n, a.n - n, v);
+            }
+        }
+        return;
+    }
+    if constexpr (PLAIN) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const int m = m0 + i * 16 + r;
+            if (m >= a.m) continue;
+            T* to = static_cast<T*>(a.y) + m * a.ldy;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int n = n0 + j * 16 + 4 * q;
+                const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                store_floats<T, 4>(to + n, a.n - n, v);
             }
         }
         return;
@@ -276,7 +292,8 @@ __global__ __launch_bounds__(S::kThreads) void linear_kernel(LinearArgs a) {
         ws.put(lb);
     };
     pipeline<DIRECT>(tiles, a0, b0, a1, b1, load, store, compute, join);
-    store_sums<T>(a, part, m0 + wm, n0 + wn, lane, acc.result());
+    // (both across: the weights' gradient)
+    store_sums<T, AX>(a, part, m0 + wm, n0 + wn, lane, acc.result());
 }
 
 // The large tile (tiles.hpp): 16-bit operands that can be loaded directly, in
@@ -334,12 +351,90 @@ __global__ __launch_bounds__(kRingThreads) void linear_ring_kernel(LinearArgs a)
     PartReader<AW, 4, AX> rb(wn, lane);
     ring<T>((k1 - kb + kStep - 1) / kStep, ra, rb, [](int) {}, load, a0, b0, a1, b1, a2, b2, a3, b3,
             acc);
-    store_sums<T>(a, part, m0 + wm, n0 + wn, lane, acc);
+    store_sums<T, AX>(a, part, m0 + wm, n0 + wn, lane, acc);
 }
 
 using Medium = Shape<128, 128, 2, 2>;
 using Small = Shape<64, 64, 2, 2>;
 using Few = Shape<32, 128, 1, 4>;
+using Wide = Shape<64, 128, 2, 2>;
+using Tall = Shape<128, 64, 2, 2>;
+
+// ---------------------------------------------------------------------------
+// Few rows of x, w's rows along the contraction: 16 columns by the 16 wavefronts of
+// a workgroup, which take turns of 128 bytes of the contraction, loaded straight to
+// the matrix instructions' operands; their sums are added in order.  Bound by
+// reading w once.
+// ---------------------------------------------------------------------------
+constexpr int kFewWaves = 16;
+
+template <typename T, int MI>
+__global__ __launch_bounds__(kFewWaves * 64) void few_kernel(LinearArgs a) {
+    constexpr int VEC = kVec<T>, kTurn = 8 * VEC;
+    __shared__ v4f sums[kFewWaves][MI][64];
+    const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = static_cast<int>(blockIdx.x) * 16;
+    // rows and columns past the last: the last one again, and not stored
+    const int col = n0 + r < a.n ? n0 + r : a.n - 1;
+    const T* w = static_cast<const T*>(a.w) + col * a.ldw + q * VEC;
+    const T* x[MI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+        const int row = i * 16 + r < a.m ? i * 16 + r : a.m - 1;
+        x[i] = static_cast<const T*>(a.x) + row * a.ldx + q * VEC;
+    }
+    v4f acc[MI] = {};
+    auto turns = [&](int k, auto count, auto whole) {
+        constexpr int N = decltype(count)::value;
+        Frag fw[N][2], fx[N][MI][2];
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int at = k + u * kFewWaves * kTurn + h * 4 * VEC;
+                const int64_t left = decltype(whole)::value ? VEC : a.k - at - q * VEC;
+                fw[u][h].u = load_chunk(w + (left > 0 ? at : 0), left);
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+                    fx[u][i][h].u = load_chunk(x[i] + (left > 0 ? at : 0), left);
+            }
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < MI; ++i) acc[i] = mfma<T>(fw[u][h], fx[u][i][h], acc[i]);
+    };
+    constexpr int kMany = MI == 1 ? 4 : 2;
+    using std::integral_constant;
+    int k = wave * kTurn;
+    for (; k + (kMany - 1) * kFewWaves * kTurn + kTurn <= a.k; k += kMany * kFewWaves * kTurn)
+        turns(k, integral_constant<int, kMany>{}, std::true_type{});
+    for (; k < a.k; k += kFewWaves * kTurn)
+        turns(k, integral_constant<int, 1>{}, std::false_type{});
+#pragma unroll
+    for (int i = 0; i < MI; ++i) sums[wave][i][lane] = acc[i];
+    __syncthreads();
+    if (wave >= MI) return;
+    v4f s = sums[0][wave][lane];
+#pragma unroll
+    for (int v = 1; v < kFewWaves; ++v) s += sums[v][wave][lane];
+    const int m = wave * 16 + r, n = n0 + 4 * q;
+    if (m >= a.m) return;
+    float bias[4] = {};
+    if (a.bias) load_floats<T, 4>(static_cast<const T*>(a.bias) + n, a.n - n, bias);
+    const float v[4] = {s[0], s[1], s[2], s[3]};
+    with_act(a.act, [&](auto act) { finish<T, decltype(act)::value>(a, m, n, v, bias); });
+}
+
+template <typename T>
+void launch_few(const LinearArgs& a, hipStream_t s) {
+    const unsigned grid = grid_of("linear", ceil_div(a.n, 16), kFewWaves * 64);
+    a.m <= 16 ? few_kernel<T, 1><<<grid, kFewWaves * 64, 0, s>>>(a)
+              : few_kernel<T, 2><<<grid, kFewWaves * 64, 0, s>>>(a);
+    TG_LAUNCH_CHECK();
+}
 
 template <typename T, bool AX, bool AW>
 void launch_product(LinearArgs& a, const LinearPlan& p, bool direct, hipStream_t s) {
@@ -351,17 +446,29 @@ void launch_product(LinearArgs& a, const LinearPlan& p, bool direct, hipStream_t
     const unsigned grid = grid_of("linear", per * p.parts, kRingThreads);
     auto tiled = [&](auto shape) {
         using S = decltype(shape);
-        direct ? linear_kernel<T, S, AX, AW, true><<<grid, S::kThreads, 0, s>>>(a)
-               : linear_kernel<T, S, AX, AW, false><<<grid, S::kThreads, 0, s>>>(a);
+        linear_kernel<T, S, AX, AW, true><<<grid, S::kThreads, 0, s>>>(a);
     };
-    if (p.em == 32) {
+    auto by_registers = [&](auto shape) {
+        using S = decltype(shape);
+        linear_kernel<T, S, AX, AW, false><<<grid, S::kThreads, 0, s>>>(a);
+    };
+    constexpr bool kHalf = sizeof(T) == 2;
+    if (!direct) {
+        if (p.em == 64)
+            by_registers(Small{});
+        else if constexpr (kHalf)
+            by_registers(Medium{});
+    } else if (p.em == 32) {
         tiled(Few{});
     } else if (p.em == 64) {
-        tiled(Small{});
-    } else if (p.em == 128) {
-        tiled(Medium{});
-    } else if constexpr (sizeof(T) == 2) {
-        linear_ring_kernel<T, AX, AW><<<grid, kRingThreads, 0, s>>>(a);
+        p.en == 64 ? tiled(Small{}) : tiled(Wide{});
+    } else if (p.en == 64) {
+        tiled(Tall{});
+    } else if constexpr (kHalf) {
+        if (p.em == 128)
+            tiled(Medium{});
+        else
+            linear_ring_kernel<T, AX, AW><<<grid, kRingThreads, 0, s>>>(a);
     }
     TG_LAUNCH_CHECK();
     if (p.parts > 1) {
@@ -457,7 +564,9 @@ void launch_columns(const float* part, int64_t n, int64_t parts, void* out, hipS
     template <>                                                                                  \
     void linear_product<T>(LinearArgs & a, const LinearPlan& p, bool ax, bool aw, bool direct,    \
                            hipStream_t s) {                                                      \
-        if (ax)                                                                                  \
+        if (p.em == 0)                                                                           \
+            launch_few<T>(a, s);                                                                 \
+        else if (ax)                                                                             \
             launch_product<T, true, true>(a, p, direct, s);                                      \
         else if (aw)                                                                             \
             launch_product<T, false, true>(a, p, direct, s);                                     \
