@@ -50,7 +50,7 @@ LinearPlan linear_plan(int64_t m, int64_t n, int64_t k, int type, Loads loads) {
     auto consider = [&](const TileCost& t) {
         const int64_t mt = ceil_div(m, t.m), nt = ceil_div(n, t.n), tiles = mt * nt;
         for (int64_t parts = 1; parts <= 256; parts *= 2) {
-            if (parts > 1 && (k < 4 * depth * parts || tiles * parts > 2048)) break;
+            if (parts > 1 && (k < 2 * depth * parts || tiles * parts > 2048)) break;
             int64_t unit = ceil_div(ceil_div(k, parts), depth) * depth;
             // (the digits of long chains of floats)
             if (type == TG_TYPE_F32) unit = std::min(unit, kLongChain);
@@ -123,7 +123,12 @@ size_t parts_bytes(int64_t m, int64_t n, int64_t k, int type) {
     return most;
 }
 
-constexpr int64_t kActRows = 256;
+// Rows of a workgroup of act_backward_kernel: for about 1,024 workgroups.
+int64_t act_rows(int64_t m, int64_t n, int type) {
+    const int64_t cols = std::max<int64_t>(1, ceil_div(n, 32 * 16 / type_size(type)));
+    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(1024 / cols, 4096));
+    return std::max<int64_t>(8, ceil_div(ceil_div(m, parts), 8) * 8);
+}
 
 struct BackwardPlace {
     void* d;
@@ -137,7 +142,7 @@ BackwardPlace backward_place(int64_t m, int64_t k, int64_t n, int type, void* ws
     Carver c(ws, size);
     BackwardPlace p{};
     p.d = c.take<char>(static_cast<size_t>(m) * n * type_size(type));
-    p.columns = c.take<float>(static_cast<size_t>(ceil_div(m, kActRows)) * n);
+    p.columns = c.take<float>(static_cast<size_t>(ceil_div(m, act_rows(m, n, type))) * n);
     // dx's parts, then dw's, in the same place
     p.room = std::max(parts_bytes(m, k, n, type),
                       std::max(parts_bytes(k, n, m, type), parts_bytes(n, k, m, type)));
@@ -251,7 +256,7 @@ int tg_linear_backward(int64_t m, int64_t k, int64_t n, int type, const void* dy
             tg::ActArgs a{};
             a.m = m;
             a.n = n;
-            a.rows = tg::kActRows;
+            a.rows = tg::act_rows(m, n, type);
             a.dy = dy;
             a.lddy = lddy;
             a.pre = pre;
@@ -259,7 +264,7 @@ int tg_linear_backward(int64_t m, int64_t k, int64_t n, int type, const void* dy
             a.d = dx || dw ? at.d : nullptr;
             a.ldd = n;
             a.part = dbias ? at.columns : nullptr;
-            const int64_t parts = given ? tg::ceil_div(m, tg::kActRows) : 0;
+            const int64_t parts = given ? tg::ceil_div(m, a.rows) : 0;
             if (given && (slopes || dbias)) tg::linear_act<T>(a, act, s);
             if (dbias) tg::linear_columns<T>(at.columns, n, parts, dbias, s);
         });

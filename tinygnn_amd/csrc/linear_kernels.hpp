@@ -480,7 +480,7 @@ void launch_product(LinearArgs& a, const LinearPlan& p, bool direct, hipStream_t
 }
 
 // ---------------------------------------------------------------------------
-// d = dy act'(pre) and its columns' sums: a workgroup takes kActRows rows of 32
+// d = dy act'(pre) and its columns' sums: a workgroup takes a.rows rows of 32
 // VEC columns, 8 rows at a time; the parts' sums are added in order by
 // columns_kernel.  ACT NONE: the sums alone.
 // ---------------------------------------------------------------------------
@@ -493,6 +493,7 @@ __global__ __launch_bounds__(256) void act_backward_kernel(ActArgs a) {
     const int64_t r0 = static_cast<int64_t>(blockIdx.y) * a.rows;
     const int64_t r1 = a.m - r0 > a.rows ? r0 + a.rows : a.m;
     float s[VEC] = {};
+#pragma unroll 4
     for (int64_t r = r0 + y; r < r1; r += 8) {
         float v[VEC], p[VEC];
         load_floats<T, VEC>(static_cast<const T*>(a.dy) + r * a.lddy + c, a.n - c, v);

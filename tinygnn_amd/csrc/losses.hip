@@ -19,7 +19,7 @@ namespace tg {
 namespace {
 
 constexpr int64_t kMaxTop = 64, kMaxTeacher = 256;
-constexpr int kTinyClasses = 64;
+constexpr int kTinyClasses = 128, kTinyPlaces = 64;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
@@ -161,6 +161,12 @@ __device__ __forceinline__ V wave_all(V v, O op) {
 // between two barriers.
 template <int NT, typename V, typename O>
 __device__ __forceinline__ V group_all(V v, O op, V* lds) {
+    if constexpr (NT == 16) {
+        v = op(v, lane_flip<8>(v));
+        v = op(v, lane_flip<4>(v));
+        v = op(v, lane_flip<2>(v));
+        return op(v, lane_flip<1>(v));
+    }
     v = wave_all(v, op);
     if constexpr (NT > kWave) {
         constexpr int NW = NT / kWave;
@@ -287,6 +293,50 @@ __device__ __forceinline__ v4u load_classes(const T* p, int left) {
     return v;
 }
 
+// v without its first s values, -inf behind the others.
+template <typename T>
+__device__ __forceinline__ v4u shifted(v4u v, int s) {
+    const uint32_t fill = kMasked<T>;
+    const int words = sizeof(T) == 4 ? s : s >> 1;
+    const bool two = words & 2, one = words & 1;
+    v4u a = {two ? v[2] : v[0], two ? v[3] : v[1], two ? fill : v[2], two ? fill : v[3]};
+    v4u b = {one ? a[1] : a[0], one ? a[2] : a[1], one ? a[3] : a[2], one ? fill : a[3]};
+    if constexpr (sizeof(T) == 2) {
+        if (s & 1)
+            b = v4u{__builtin_amdgcn_alignbit(b[1], b[0], 16), __builtin_amdgcn_alignbit(b[2], b[1], 16),
+                    __builtin_amdgcn_alignbit(b[3], b[2], 16), __builtin_amdgcn_alignbit(fill, b[3], 16)};
+    }
+    return s >= kVec<T> ? v4u{fill, fill, fill, fill} : b;
+}
+
+// Chunks [at, at + VEC), at = at0 + i * step, of the n values at p, -inf behind them;
+// `before`: as many values in front of p may be read.  A chunk that n ends in comes
+// from the last VEC values, and all loads are asked for before the first is looked
+// at (a branch for cut chunks among them had each wait for the one before).
+template <typename T, int N>
+__device__ __forceinline__ void load_chunks(const T* p, int at0, int step, int n, int64_t before,
+                                            v4u (&x)[N]) {
+    constexpr int VEC = kVec<T>;
+    typedef T Whole __attribute__((ext_vector_type(VEC)));
+    if (n + before < VEC) {  // (uniform, and fewer than one chunk)
+        x[0] = load_classes<T>(p + at0, n - at0);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int at = at0 + i * step, from = at < n - VEC ? at : n - VEC;
+        if (i == 0 || i * step < n)
+            x[i] = __builtin_bit_cast(v4u, static_cast<Whole>(
+                *reinterpret_cast<const typename Pack<T, VEC>::V*>(p + from)));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int past = at0 + i * step - (n - VEC);
+        if ((i == 0 || i * step < n) && past > 0) x[i] = shifted<T>(x[i], past);
+    }
+}
+
 template <typename T>
 __device__ __forceinline__ void floats_of(v4u v, float (&x)[kVec<T>]) {
     typedef T Whole __attribute__((ext_vector_type(kVec<T>)));
@@ -303,14 +353,16 @@ constexpr size_t top_lds(int top) {
 
 template <typename T, int NT, int NV>
 struct Held {
-    static constexpr int VEC = kVec<T>, NW = NT / kWave;
+    static constexpr int VEC = kVec<T>, NW = NT < kWave ? 1 : NT / kWave;
     v4u x[NV];
     int n, tid;
-    __device__ __forceinline__ Held(const T* p, int n_) : n(n_), tid(threadIdx.x % NT) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) x[i] = load_classes<T>(p + at(i), n - at(i));
+    __device__ __forceinline__ Held(const T* p, int n_, int64_t before)
+        : n(n_), tid(threadIdx.x % NT) {
+        load_chunks<T>(p, at(0), NT * VEC, n, before, x);
     }
     __device__ __forceinline__ int at(int i) const { return (i * NT + tid) * VEC; }
+    // Whether any thread has a chunk i (n is the same in all).
+    __device__ __forceinline__ bool used(int i) const { return i == 0 || i * NT * VEC < n; }
     // Chunk i's values.  (Each pass makes them again: kept from one to the next,
     // by the compiler, they took twice the registers that there are.)
     __device__ __forceinline__ void values(int i, float (&v)[VEC]) {
@@ -330,13 +382,15 @@ struct Held {
     __device__ __forceinline__ RowSums sums(float c, float* lds) {
         float m = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) m = __builtin_fmaxf(m, largest(i));
+        for (int i = 0; i < NV; ++i)
+            if (used(i)) m = __builtin_fmaxf(m, largest(i));
         m = group_all<NT>(m, Max{}, lds);
         // (a row of -inf alone: its z are -inf, not NaN; a NaN stays one)
         const float base = m == -INFINITY ? 0.0f : m;
         float s = 0.0f, u = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
+            if (!used(i)) continue;
             float v[VEC], si = 0.0f, ui = 0.0f;
             values(i, v);
 #pragma unroll
@@ -365,23 +419,31 @@ struct Held {
     __device__ __forceinline__ void tops(int top, uint32_t first, Key* lds, int* count, P&& put) {
         float best = -INFINITY;
         int which = 0;
+        v4u w = x[0];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
+            if (!used(i)) continue;
             const float m = largest(i);
             const bool more = m > best;
             best = more ? m : best;
             which = more ? i : which;
-        }
-        v4u w = x[0];
+            // (words of a copy: else the compiler indexes x, and keeps it in memory)
+            v4u xi = x[i];
+            asm volatile("" : "+v"(xi));
 #pragma unroll
-        for (int i = 1; i < NV; ++i)
-            if (which == i) w = x[i];
+            for (int d = 0; d < 4; ++d) w[d] = more ? xi[d] : w[d];
+        }
         float v[VEC];
         floats_of<T>(w, v);
         int e0 = 0;
 #pragma unroll
         for (int e = VEC - 1; e >= 0; --e) e0 = v[e] == best ? e : e0;
         const Key mine = key_of(best, first + static_cast<uint32_t>(at(which) + e0));
+        if (top == 1) {
+            const Key k = group_all<NT>(mine, Max{}, lds);
+            if (tid == 0) put(0, k);
+            return;
+        }
         if (tid == 0) *count = 0;
         const Key limit = kth_of<NT>(mine, top, lds);
         if constexpr (NT == kWave) {
@@ -392,12 +454,14 @@ struct Held {
         const float floor = limit ? key_value(limit) : -INFINITY;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if (largest(i) >= floor) {
+            if (used(i) && largest(i) >= floor) {
                 values(i, v);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
-                    const Key k = key_of(v[e], first + static_cast<uint32_t>(at(i) + e));
-                    if (k != 0 && k >= limit) cand[atomicAdd(count, 1)] = k;
+                    if (v[e] >= floor) {
+                        const Key k = key_of(v[e], first + static_cast<uint32_t>(at(i) + e));
+                        if (k != 0 && k >= limit) cand[atomicAdd(count, 1)] = k;
+                    }
                 }
             }
         }
@@ -540,9 +604,11 @@ template <typename T, int NT, int NV, int MODE, bool ENTROPY>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void row_kernel(LossArgs a) {
     constexpr int kBlock = NT < 256 ? 256 : NT, kRows = kBlock / NT, VEC = kVec<T>;
     extern __shared__ __attribute__((aligned(16))) Key top_keys[];
-    __shared__ float reduce[kRows][3 * (NT / kWave)];
+    __shared__ float reduce[kRows][3 * (NT < kWave ? 1 : NT / kWave)];
     __shared__ int count[kRows];
-    const int sub = kRows == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
+    const int sub = NT < kWave   ? threadIdx.x / NT
+                    : kRows == 1 ? 0
+                                 : __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
     int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + sub;
     int seg = 0;
     if constexpr (MODE == kSegment) {
@@ -551,13 +617,13 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void row_kernel(LossArgs a) {
         seg = static_cast<int>(all - row * a.segments);
     }
     row += a.row0;
-    if (row >= a.rows) return;  // (whole wavefronts; no barriers where rows share a workgroup)
+    if (row >= a.rows) return;  // (all of a row's lanes; no barriers where rows share a workgroup)
     const int64_t first = MODE == kSegment ? seg * a.segment : 0;
     const int n = static_cast<int>(MODE == kSegment && a.classes - first > a.segment
                                        ? a.segment
                                        : a.classes - first);
     const T* p = static_cast<const T*>(a.logits) + row * a.ld + first;
-    Held<T, NT, NV> x(p, n);
+    Held<T, NT, NV> x(p, n, first);
     const RowSums r = x.template sums<ENTROPY>(a.c, reduce[sub]);
     Key* lds = top_keys + (a.top == 0 ? 0 : sub * (NT + a.top * NV * VEC));
     if constexpr (MODE == kSegment) {
@@ -573,8 +639,11 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void row_kernel(LossArgs a) {
     } else if constexpr (MODE == kLogProbs) {
         const RowStats st(r);
         if (x.tid == 0) put_row<T>(a, row, r, st);
-        if (a.top)
-            x.tops(a.top, 0, lds, &count[sub], [&](int j, Key k) { put_top(a, row, j, k, st); });
+        if constexpr (NT >= kWave) {
+            if (a.top)
+                x.tops(a.top, 0, lds, &count[sub],
+                       [&](int j, Key k) { put_top(a, row, j, k, st); });
+        }
     } else {
         __shared__ float q[kRows][kMaxTeacher];
         __shared__ int id[kRows][kMaxTeacher];
@@ -609,6 +678,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void row_kernel(LossArgs a) {
         T* out = static_cast<T*>(a.dlogits) + row * a.lddl;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
+            if (!x.used(i)) continue;
             float v[VEC], d[VEC];
             x.values(i, v);
 #pragma unroll
@@ -760,19 +830,16 @@ __global__ __launch_bounds__(256) void gradient_kernel(LossArgs a, int64_t spans
 #pragma unroll
         for (int i = 0; i < kSpan; ++i) {
             const int at = (i * kWave + lane) * VEC;
-            store_classes<T>(out + at, n - at, d);
+            if (i * kWave * VEC < n) store_classes<T>(out + at, n - at, d);
         }
         return;
     }
     v4u x[kSpan];
+    load_chunks<T>(p, lane * VEC, kWave * VEC, n, first, x);
 #pragma unroll
     for (int i = 0; i < kSpan; ++i) {
         const int at = (i * kWave + lane) * VEC;
-        x[i] = load_classes<T>(p + at, n - at);
-    }
-#pragma unroll
-    for (int i = 0; i < kSpan; ++i) {
-        const int at = (i * kWave + lane) * VEC;
+        if (i * kWave * VEC >= n) continue;
         float v[VEC];
         floats_of<T>(x[i], v);
 #pragma unroll
@@ -822,9 +889,10 @@ __device__ __forceinline__ void each_value(int e, int left, int classes, uint32_
 }
 
 template <typename T, int MODE, bool ENTROPY, bool GRADIENT>
-__global__ __launch_bounds__(kWave) void tiny_kernel(LossArgs a, uint32_t magic) {
+__global__ __launch_bounds__(kWave) void tiny_kernel(LossArgs a, uint32_t magic, uint32_t magic_k) {
     constexpr int VEC = kVec<T>;
-    extern __shared__ __attribute__((aligned(16))) float lds[];  // [64][classes | 1]
+    // [64][classes | 1], and of the teacher [64][k | 1] values and classes
+    extern __shared__ __attribute__((aligned(16))) float lds[];
     const int classes = static_cast<int>(a.classes), stride = classes | 1;
     const int64_t r0 = a.row0 + static_cast<int64_t>(blockIdx.x) * kWave, row = r0 + threadIdx.x;
     const int rows = static_cast<int>(a.rows - r0 < kWave ? a.rows - r0 : kWave);
@@ -852,6 +920,20 @@ __global__ __launch_bounds__(kWave) void tiny_kernel(LossArgs a, uint32_t magic)
         for (int e = threadIdx.x; e < all; e += kWave) {
             const int r = row_of(e, magic);
             lds[e + r * (stride - classes)] = static_cast<float>(p[r * a.ld + e - r * classes]);
+        }
+    }
+    float* const taught = lds + kWave * stride;
+    const int stride_k = a.k | 1;
+    if constexpr (MODE == kDistill) {
+        const int places = rows * a.k;
+#pragma unroll 4
+        for (int e = threadIdx.x; e < places; e += kWave) {
+            const int c = a.ids[r0 * a.k + e];
+            const float t = teacher_at(a, r0 * a.k + e);
+            const int to = e + row_of(e, magic_k) * (stride_k - a.k);
+            const bool in = c >= 0 && c < classes;
+            taught[to] = in ? t : -INFINITY;
+            taught[kWave * stride_k + to] = __int_as_float(in ? c : 0);
         }
     }
     __syncthreads();
@@ -916,32 +998,13 @@ __global__ __launch_bounds__(kWave) void tiny_kernel(LossArgs a, uint32_t magic)
             }
             if (in && !zero) x[y] += g;
         } else {
-            // the teacher's places, kPlaces at a time; with no more they are read once
             const RowStats st(r);
-            constexpr int kPlaces = 8;
-            float t[kPlaces];
-            int c[kPlaces];
-            auto places = [&](int j0) {
-#pragma unroll
-                for (int j = 0; j < kPlaces; ++j) {
-                    const bool there = j0 + j < a.k;
-                    const int64_t at = row * a.k + (there ? j0 + j : 0);
-                    c[j] = a.ids[at];
-                    t[j] = teacher_at(a, at);
-                    if (!there || c[j] < 0 || c[j] >= classes) {
-                        t[j] = -INFINITY;
-                        c[j] = 0;
-                    }
-                }
-            };
+            const float* t = taught + threadIdx.x * stride_k;
+            const float* c = t + kWave * stride_k;
             auto each = [&](auto&& fn) {
-                for (int j0 = 0; j0 < a.k; j0 += kPlaces) {
-                    if (a.k > kPlaces) places(j0);
-#pragma unroll
-                    for (int j = 0; j < kPlaces; ++j) fn(t[j], c[j]);
-                }
+#pragma unroll 4
+                for (int j = 0; j < a.k; ++j) fn(t[j], __float_as_int(c[j]));
             };
-            if (a.k <= kPlaces) places(0);
             float tm = -INFINITY, total = 0.0f, loss = 0.0f;
             each([&](float tj, int) { tm = __builtin_fmaxf(tm, tj); });
             each([&](float tj, int) {
@@ -1011,41 +1074,53 @@ LossArgs loss_args(int64_t rows, int64_t classes, const void* logits, int64_t ld
     return a;
 }
 
-// fn with NT threads and NV chunks a thread for rows (or segments) of n classes;
-// false: too long.
+// fn with NT threads and NV chunks a thread for rows (or segments) of n classes.
+// Many rows: few threads a row, so that several rows' loads, sums and stores run
+// beside each other on a CU; where rows are few, more threads for each.  LANES16:
+// 16 lanes may take a row (227,701 x 470 bf16...).
 constexpr int64_t kMostChunks = 1024 * 16;
-template <typename F>
-bool with_shape(int64_t n, int vec, F&& fn) {
+template <bool LANES16, typename F>
+void with_shape(int64_t rows, int64_t n, int vec, F&& fn) {
     const int64_t chunks = ceil_div(n, vec);
+    const bool few = rows < 512;
     using std::integral_constant;
-    if (chunks <= 64)
-        fn(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-    else if (chunks <= 64 * 4)
-        fn(integral_constant<int, 64>{}, integral_constant<int, 4>{});
-    else if (chunks <= 256 * 4)
-        fn(integral_constant<int, 256>{}, integral_constant<int, 4>{});
-    else if (chunks <= 256 * 16)
-        fn(integral_constant<int, 256>{}, integral_constant<int, 16>{});
-    else if (chunks <= 1024 * 8)
-        fn(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
-    else if (chunks <= kMostChunks)
-        fn(integral_constant<int, 1024>{}, integral_constant<int, 16>{});
-    else
-        return false;
-    return true;
+    auto shape = [&](auto nt, auto nv) {
+        if (chunks > decltype(nt)::value * decltype(nv)::value) return false;
+        fn(nt, nv);
+        return true;
+    };
+    constexpr integral_constant<int, 64> t64{};
+    constexpr integral_constant<int, 256> t256{};
+    constexpr integral_constant<int, 1024> t1024{};
+    constexpr integral_constant<int, 1> v1{};
+    constexpr integral_constant<int, 4> v4{};
+    constexpr integral_constant<int, 8> v8{};
+    constexpr integral_constant<int, 16> v16{};
+    if constexpr (LANES16) {
+        constexpr integral_constant<int, 16> t16{};
+        if (!few && (shape(t16, v4) || shape(t16, v8))) return;
+    }
+    if (few) {
+        shape(t64, v1) || shape(t256, v4) || shape(t1024, v4) || shape(t1024, v8) ||
+            shape(t1024, v16);
+    } else {
+        shape(t64, v1) || shape(t64, v4) || shape(t256, v4) || shape(t256, v16) ||
+            shape(t1024, v8) || shape(t1024, v16);
+    }
 }
 
-// How rows are cut: one segment, or as many as give 1,024 workgroups of 4,096
-// classes at least, 64 at most unless a row is longer than 64 workgroups hold.
+// How rows are cut: one segment, but where there are few of more than 16,384
+// classes (as many as give 1,024 workgroups of 4,096 classes at least, 64 at most),
+// and longer ones than a workgroup holds.  (A distillation with its gradient reads
+// cut rows twice, the others once.)
 struct Cut {
     int64_t segment, segments;
 };
 
 Cut cut_of(int64_t rows, int64_t classes, int type) {
     const int64_t vec = 16 / type_size(type), most = kMostChunks * vec;
-    if (classes <= kTinyClasses) return {classes, 1};
     int64_t segments = 1;
-    if (rows < 1024)
+    if (rows < 1024 && classes > 16384)
         segments = std::min<int64_t>({ceil_div(1024, rows), ceil_div(classes, 4096), 64});
     segments = std::max(segments, ceil_div(classes, most));
     const int64_t segment = ceil_div(ceil_div(classes, segments), vec) * vec;
@@ -1092,10 +1167,10 @@ void sliced(LossArgs a, int64_t threads, F&& fn) {
 template <typename T, int MODE, bool ENTROPY>
 void launch_rows(const char* what, const LossArgs& all, hipStream_t s) {
     const int64_t each = MODE == kSegment ? all.segments : 1;
-    with_shape(MODE == kSegment ? all.segment : all.classes, kVec<T>, [&](auto nt, auto nv) {
+    auto launch = [&](auto nt, auto nv) {
         constexpr int NT = decltype(nt)::value, NV = decltype(nv)::value;
         constexpr int kBlock = NT < 256 ? 256 : NT, kRows = kBlock / NT;
-        const size_t lds = kRows * top_lds<T, NT, NV>(all.top);
+        const size_t lds = NT < kWave ? 0 : kRows * top_lds<T, NT, NV>(all.top);
         auto kernel = row_kernel<T, NT, NV, MODE, ENTROPY>;
         if (lds > 48 * 1024)
             TG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
@@ -1106,7 +1181,12 @@ void launch_rows(const char* what, const LossArgs& all, hipStream_t s) {
             kernel<<<grid, kBlock, lds, s>>>(a);
             TG_LAUNCH_CHECK();
         });
-    });
+    };
+    const int64_t length = MODE == kSegment ? all.segment : all.classes;
+    if (MODE == kLogProbs && all.top == 0)
+        with_shape<MODE == kLogProbs>(all.rows * each, length, kVec<T>, launch);
+    else
+        with_shape<false>(all.rows * each, length, kVec<T>, launch);
 }
 
 template <typename T, int MODE, bool ENTROPY, bool GRADIENT>
@@ -1114,8 +1194,15 @@ void launch_tiny(const char* what, const LossArgs& a, hipStream_t s) {
     const unsigned grid = grid_of(what, ceil_div(a.rows, kWave), kWave);
     const uint32_t magic =
         static_cast<uint32_t>(((uint64_t(1) << 32) + a.classes - 1) / a.classes);
-    const size_t lds = sizeof(float) * kWave * (a.classes | 1);
-    tiny_kernel<T, MODE, ENTROPY, GRADIENT><<<grid, kWave, lds, s>>>(a, magic);
+    const uint32_t magic_k =
+        a.k ? static_cast<uint32_t>(((uint64_t(1) << 32) + a.k - 1) / a.k) : 0;
+    const size_t lds = sizeof(float) * kWave * ((a.classes | 1) + (a.k ? 2 * (a.k | 1) : 0));
+    auto kernel = tiny_kernel<T, MODE, ENTROPY, GRADIENT>;
+    if (lds > 48 * 1024)
+        TG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                   hipFuncAttributeMaxDynamicSharedMemorySize,
+                                   static_cast<int>(lds)));
+    kernel<<<grid, kWave, lds, s>>>(a, magic, magic_k);
     TG_LAUNCH_CHECK();
 }
 
@@ -1143,6 +1230,15 @@ void launch_join(const char* what, const LossArgs& all, hipStream_t s) {
             join_kernel<T, MODE, kWave><<<grid, kWave, 0, s>>>(a);
         TG_LAUNCH_CHECK();
     });
+}
+
+// Whether a thread takes a row: up to 64 classes, but where it would look for many
+// top classes of few rows; up to 128 where many rows have top classes or a teacher
+// (a wavefront's work on a row is the same for 65 as for 256).
+bool tiny_rows(const LossArgs& a) {
+    if (a.k > kTinyPlaces || a.classes > kTinyClasses) return false;
+    if (a.rows < 8192) return a.classes <= 64 && a.top * a.classes <= 512;
+    return a.classes <= 64 || a.top > 0 || a.k > 0;
 }
 
 template <typename F>
@@ -1217,7 +1313,7 @@ int tg_log_probs(int64_t rows, int64_t classes, int type, const void* logits, in
             using T = decltype(t);
             tg::with_bool(entropy != nullptr, [&](auto ent) {
                 constexpr bool E = decltype(ent)::value;
-                if (classes <= tg::kTinyClasses) {
+                if (tg::tiny_rows(a)) {
                     tg::launch_tiny<T, tg::kLogProbs, E, false>("log_probs", a, s);
                 } else if (cut) {
                     tg::launch_rows<T, tg::kSegment, E>("log_probs", a, s);
@@ -1256,7 +1352,7 @@ int tg_log_probs_backward(int64_t rows, int64_t classes, int type, const void* l
             using T = decltype(t);
             tg::with_bool(dentropy != nullptr, [&](auto ent) {
                 constexpr bool E = decltype(ent)::value;
-                if (classes <= tg::kTinyClasses)
+                if (classes <= 64)
                     tg::launch_tiny<T, tg::kLogProbs, E, true>("log_probs_backward", a, s);
                 else
                     tg::launch_gradient<T, tg::kLogProbs, E>("log_probs_backward", a, s);
@@ -1300,7 +1396,7 @@ int tg_distill(int64_t rows, int64_t classes, int64_t k, int type, const void* l
         const bool cut = tg::place_segments(a, type, workspace, workspace_bytes, &temp, s);
         tg::with_type(type, "distill", [&](auto t) {
             using T = decltype(t);
-            if (classes <= tg::kTinyClasses) {
+            if (tg::tiny_rows(a)) {
                 tg::with_bool(dlogits != nullptr, [&](auto grad) {
                     tg::launch_tiny<T, tg::kDistill, false, decltype(grad)::value>("distill", a, s);
                 });
