@@ -158,9 +158,18 @@ def test_falling_and_equal_rows(gpu, classes, dtype):
     comes from one part of the row."""
     dt = DTYPES[dtype]
     ramp = torch.linspace(-4, 4, classes, device="cuda")
-    x = torch.stack([ramp, -ramp, 0 * ramp, ramp.abs(), -ramp.abs()] * 3).to(dt)
-    labels = torch.arange(15, device="cuda").to(I32) % classes
-    check_log_probs(x, labels, min(64, classes), 1.0)
+    rows = [ramp, -ramp, 0 * ramp, ramp.abs(), -ramp.abs()]
+    # large values on few of the threads that may share a row
+    at = torch.arange(classes, device="cuda")
+    for period in (8 * 16, 8 * 64, 8 * 256, 8 * 1024, 4 * 64, 4 * 1024):
+        rows.append((at % period).float() / period + (at % 7) / 70)
+        rows.append((at % period >= period // 2).float() + ramp / 10)
+    x = torch.stack(rows).to(dt)
+    labels = torch.arange(len(rows), device="cuda").to(I32) % classes
+    many = x.repeat(1 + 600 // len(rows), 1)   # as many rows, too
+    for top in (2, 31, 64):
+        check_log_probs(x, labels, min(top, classes), 1.0)
+        check_log_probs(many, labels.repeat(1 + 600 // len(rows)), min(top, classes), 1.0)
 
 
 @pytest.mark.parametrize("rows,classes", [(50, 30), (30, 700), (9, 9000), (2, 150000)])
