@@ -120,6 +120,17 @@ __device__ __forceinline__ V wave_all(V v, O op) {
     return op(v, lane_flip<32>(v));
 }
 
+// What a row's threads wrote to LDS is there for all of them.
+template <int NT>
+__device__ __forceinline__ void group_sync() {
+    if constexpr (NT > kWave) {
+        __syncthreads();
+    } else {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
 // Over the NT threads of a row.  `lds`: NT / 64 values of its own for each call
 // between two barriers.
 template <int NT, typename V, typename O>
@@ -309,7 +320,7 @@ __device__ __forceinline__ void floats_of(v4u v, float (&x)[kVec<T>]) {
 }
 
 // Keys of LDS that a row's top classes need: its threads' and its candidates'.
-__host__ __device__ constexpr int candidates(int top) { return 8 * top + 64; }
+__host__ __device__ constexpr int candidates(int top) { return 12 * top + 64; }
 __host__ __device__ constexpr int top_keys(int nt, int top) {
     return top == 0 ? 0 : nt + candidates(top);
 }
@@ -408,6 +419,12 @@ struct Held {
             if (tid == 0) put(0, k);
             return;
         }
+        if constexpr (NT >= kWave) many_tops(top, first, mine, lds, count, put);
+    }
+    template <typename P>
+    __device__ __forceinline__ void many_tops(int top, uint32_t first, Key mine, Key* lds,
+                                              int* count, P&& put) {
+        float v[VEC];
         if (tid == 0) *count = 0;
         const Key limit = kth_of<NT>(mine, top, lds);
         if constexpr (NT == kWave) {
@@ -437,7 +454,7 @@ struct Held {
                 }
             }
         }
-        group_sync();
+        group_sync<NT>();
         const int many = *count;
         if (many > candidates(top)) {
             Key last = ~Key(0);
@@ -457,8 +474,18 @@ struct Held {
                 }
                 last = group_all<NT>(next, Max{}, lds);
                 if (tid == 0) put(j, last);
-                group_sync();
+                group_sync<NT>();
             }
+            return;
+        }
+        if (many > 2 * kWave && NT <= 256) {  // 64 at a time
+            if (tid >= kWave) return;
+            Key best = sort_falling(cand[tid]);
+            for (int base = kWave; base < many; base += kWave) {
+                const Key k = sort_falling(base + tid < many ? cand[base + tid] : Key(0));
+                best = merge_falling(best, static_cast<Key>(__shfl(k, 63 - tid, kWave)));
+            }
+            if (tid < top) put(tid, best);
             return;
         }
         for (int i = tid; i < many; i += NT) {
@@ -469,14 +496,6 @@ struct Held {
             if (rank < top) put(rank, k);
         }
         for (int j = many + tid; j < top; j += NT) put(j, Key(0));
-    }
-    __device__ __forceinline__ static void group_sync() {
-        if constexpr (NT > kWave) {
-            __syncthreads();
-        } else {
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-            __builtin_amdgcn_wave_barrier();
-        }
     }
 };
 
@@ -544,12 +563,11 @@ struct Teacher {
     float loss, total;
 };
 
-template <typename T, typename Q, typename I>
-__device__ __forceinline__ Teacher teach(const LossArgs& a, int64_t row, const RowStats& st,
+template <typename T, int N, typename Q, typename I>
+__device__ __forceinline__ Teacher teach_of(const LossArgs& a, int64_t row, const RowStats& st,
                                          Q&& put_q, I&& put_id) {
     const int lane = threadIdx.x & (kWave - 1);
     const T* x = static_cast<const T*>(a.logits) + row * a.ld;
-    constexpr int N = kMaxTeacher / kWave;
     float t[N], xs[N];
     float tm = -INFINITY;
 #pragma unroll
@@ -593,6 +611,13 @@ __device__ __forceinline__ Teacher teach(const LossArgs& a, int64_t row, const R
     return {wave_all(loss, Add{}), total};
 }
 
+template <typename T, typename Q, typename I>
+__device__ __forceinline__ Teacher teach(const LossArgs& a, int64_t row, const RowStats& st,
+                                         Q&& put_q, I&& put_id) {
+    return a.k <= kWave ? teach_of<T, 1>(a, row, st, put_q, put_id)
+                        : teach_of<T, kMaxTeacher / kWave>(a, row, st, put_q, put_id);
+}
+
 // The factor of a row's distillation gradient; 0: the row's gradient is 0.  A NaN
 // among the teacher's values is one in the whole row.
 __device__ __forceinline__ float distill_factor(const LossArgs& a, int64_t row, float total,
@@ -608,6 +633,82 @@ __device__ __forceinline__ void subtract(int at, float v, float (&d)[VEC]) {
     for (int e = 0; e < VEC; ++e) d[e] -= at == e ? v : 0.0f;
 }
 
+
+// A teacher's places by the thread that holds their class: id and q of each (id -1:
+// none, or its class in a place before, whose q has its own, added in order) and lists
+// of a thread's places, whose order therefore changes nothing.
+template <int NT>
+struct Places {
+    float q[kMaxTeacher];
+    int id[kMaxTeacher];
+    int before[kMaxTeacher];  // the place before in its list, -1: none
+    int last[NT];
+    // id and q are there, last is -1; of `k` places.  NT threads.
+    template <int VEC>
+    __device__ __forceinline__ void build(int tid, int k) {
+        constexpr int N = kMaxTeacher / kWave;
+        float sum[N];
+        group_sync<NT>();
+        if (tid < kWave) {
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                const int j = u * kWave + tid;
+                sum[u] = -1.0f;
+                if (j >= k || id[j] < 0) continue;
+                const int c = id[j];
+                bool other = false;
+                float s = 0.0f;
+                for (int w = 0; w < k; ++w) {
+                    const bool same = id[w] == c;
+                    other |= same && w < j;
+                    s += same ? q[w] : 0.0f;
+                }
+                sum[u] = other ? -1.0f : s;
+            }
+        }
+        group_sync<NT>();
+        if (tid < kWave) {
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                const int j = u * kWave + tid;
+                if (j >= k) continue;
+                if (sum[u] == -1.0f) {
+                    id[j] = -1;
+                } else {
+                    q[j] = sum[u];
+                    before[j] = atomicExch(&last[id[j] / VEC % NT], j);
+                }
+            }
+        }
+        group_sync<NT>();
+    }
+};
+
+// A thread's places: two in registers, the others looked up.
+template <int NT, int VEC>
+struct MyPlaces {
+    int c0 = -1, c1 = -1, more = -1;
+    float q0 = 0.0f, q1 = 0.0f;
+    __device__ __forceinline__ MyPlaces(const Places<NT>& p, int tid) {
+        const int j0 = p.last[tid];
+        if (j0 < 0) return;
+        c0 = p.id[j0];
+        q0 = p.q[j0];
+        const int j1 = p.before[j0];
+        if (j1 < 0) return;
+        c1 = p.id[j1];
+        q1 = p.q[j1];
+        more = p.before[j1];
+    }
+    // d -= g q of the places of the chunk at `at`.
+    __device__ __forceinline__ void subtract_from(const Places<NT>& p, int at, float g,
+                                                  float (&d)[VEC]) const {
+        if (static_cast<uint32_t>(c0 - at) < VEC) subtract(c0 - at, q0 * g, d);
+        if (static_cast<uint32_t>(c1 - at) < VEC) subtract(c1 - at, q1 * g, d);
+        for (int j = more; j >= 0; j = p.before[j])
+            if (static_cast<uint32_t>(p.id[j] - at) < VEC) subtract(p.id[j] - at, p.q[j] * g, d);
+    }
+};
 
 // One row (kSegment: one segment) for each NT threads.
 template <typename T, int NT, int NV, int MODE, bool ENTROPY>
@@ -649,40 +750,26 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void row_kernel(LossArgs a) {
     } else if constexpr (MODE == kLogProbs) {
         const RowStats st(r);
         if (x.tid == 0) put_row<T>(a, row, r, st);
-        if constexpr (NT >= kWave) {
-            if (a.top)
-                x.tops(a.top, 0, lds, &count[sub],
-                       [&](int j, Key k) { put_top(a, row, j, k, st); });
-        }
+        if (a.top)
+            x.tops(a.top, 0, lds, &count[sub], [&](int j, Key k) { put_top(a, row, j, k, st); });
     } else {
-        __shared__ float q[kRows][kMaxTeacher];
-        __shared__ int id[kRows][kMaxTeacher];
-        // places among a thread's classes: their count << 16, and the sum of their
-        // numbers, which is the number of a single one
-        __shared__ uint32_t hits[kRows][NT];
+        __shared__ Places<NT> places[kRows];
         __shared__ float factor[kRows];
         const RowStats st(r);
-        hits[sub][x.tid] = 0;
+        Places<NT>& pl = places[sub];
+        pl.last[x.tid] = -1;
         if (NT == kWave || threadIdx.x < kWave) {
             const Teacher t = teach<T>(
-                a, row, st, [&](int j, float v) { q[sub][j] = v; },
-                [&](int j, int v) { id[sub][j] = v; });
+                a, row, st, [&](int j, float v) { pl.q[j] = v; },
+                [&](int j, int v) { pl.id[j] = v; });
             if (x.tid == 0) {
                 a.loss[row] = t.loss;
                 if (a.dlogits) factor[sub] = distill_factor(a, row, t.total, st);
             }
         }
         if (!a.dlogits) return;
-        x.group_sync();
-        for (int j = x.tid; j < a.k; j += NT) {
-            const int c = id[sub][j];
-            if (c >= 0) atomicAdd(&hits[sub][c / VEC % NT], 1u << 16 | static_cast<uint32_t>(j));
-        }
-        x.group_sync();
-        const uint32_t hit = hits[sub][x.tid];
-        const bool several = hit >> 16 > 1;
-        const int only = hit >> 16 == 1 ? id[sub][hit & 0xFFFF] : -1;
-        const float only_q = hit >> 16 == 1 ? q[sub][hit & 0xFFFF] : 0.0f;
+        pl.template build<VEC>(x.tid, a.k);
+        const MyPlaces<NT, VEC> mine(pl, x.tid);
         const float g = factor[sub];
         const RowGradient grad{st.m, st.log_s * kLog2e, g, 0.0f};
         T* out = static_cast<T*>(a.dlogits) + row * a.lddl;
@@ -693,13 +780,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void row_kernel(LossArgs a) {
             x.values(i, v);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) d[e] = grad(v[e], a.c);
-            if (static_cast<uint32_t>(only - x.at(i)) < VEC) subtract(only - x.at(i), only_q * g, d);
-            if (several) {
-                for (int j = 0; j < a.k; ++j) {
-                    const int at = id[sub][j] - x.at(i);
-                    if (static_cast<uint32_t>(at) < VEC) subtract(at, q[sub][j] * g, d);
-                }
-            }
+            mine.subtract_from(pl, x.at(i), g, d);
             if (g == 0.0f) {
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) d[e] = 0.0f;
@@ -784,7 +865,7 @@ constexpr int kSpan = 4;
 template <typename T, int MODE, bool ENTROPY>
 __global__ __launch_bounds__(256) void gradient_kernel(LossArgs a, int64_t spans) {
     constexpr int VEC = kVec<T>;
-    __shared__ uint32_t hits[4][kWave];
+    __shared__ Places<kWave> places[MODE == kDistill ? 4 : 1];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
     const int64_t w = static_cast<int64_t>(blockIdx.x) * 4 + wave;
     const int64_t row = a.row0 + w / spans;
@@ -798,7 +879,7 @@ __global__ __launch_bounds__(256) void gradient_kernel(LossArgs a, int64_t spans
     float g = 0.0f;
     int64_t y = -1;  // the label's place
     bool zero;
-    uint32_t hit = 0;
+    Places<kWave>& pl = places[MODE == kDistill ? wave : 0];
     if constexpr (MODE == kLogProbs) {
         const RowStats st(a.stats[2 * row], a.stats[2 * row + 1]);
         if (a.labels) {
@@ -820,18 +901,14 @@ __global__ __launch_bounds__(256) void gradient_kernel(LossArgs a, int64_t spans
         g = o[2];
         grad = {o[0], o[1] * kLog2e, g, 0.0f};
         zero = g == 0.0f;
-        hits[wave][lane] = 0;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        pl.last[lane] = -1;
         for (int j = lane; j < a.k; j += kWave) {
             const int c = a.ids[row * a.k + j];
             const int64_t at = c - first;
-            if (c >= 0 && c < a.classes && at >= 0 && at < n)
-                atomicOr(&hits[wave][at / VEC % kWave], 1u << (at / VEC / kWave));
+            pl.id[j] = c >= 0 && c < a.classes && at >= 0 && at < n ? static_cast<int>(at) : -1;
+            pl.q[j] = a.q[row * a.k + j];
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        hit = hits[wave][lane];
+        pl.template build<VEC>(lane, a.k);
     }
     float d[VEC];
     if (zero) {  // whatever the logits hold
@@ -846,6 +923,10 @@ __global__ __launch_bounds__(256) void gradient_kernel(LossArgs a, int64_t spans
     }
     v4u x[kSpan];
     load_chunks<T>(p, lane * VEC, kWave * VEC, n, first, x);
+    struct None {
+        __device__ None(const Places<kWave>&, int) {}
+    };
+    const std::conditional_t<MODE == kDistill, MyPlaces<kWave, VEC>, None> mine(pl, lane);
 #pragma unroll
     for (int i = 0; i < kSpan; ++i) {
         const int at = (i * kWave + lane) * VEC;
@@ -861,13 +942,7 @@ __global__ __launch_bounds__(256) void gradient_kernel(LossArgs a, int64_t spans
                 for (int e = 0; e < VEC; ++e) d[e] += y - at == e ? g : 0.0f;
             }
         } else {
-            if (hit >> i & 1) {
-                for (int j = 0; j < a.k; ++j) {
-                    const int64_t c = a.ids[row * a.k + j] - first - at;
-                    if (static_cast<uint64_t>(c) < VEC)
-                        subtract(static_cast<int>(c), a.q[row * a.k + j] * g, d);
-                }
-            }
+            mine.subtract_from(pl, at, g, d);
         }
         store_classes<T>(out + at, n - at, d);
     }
@@ -1151,7 +1226,7 @@ void launch_rows(const char* what, const LossArgs& all, hipStream_t s) {
     auto launch = [&](auto nt, auto nv) {
         constexpr int NT = decltype(nt)::value, NV = decltype(nv)::value;
         constexpr int kBlock = NT < 256 ? 256 : NT, kRows = kBlock / NT;
-        const size_t lds = NT < kWave ? 0 : sizeof(Key) * kRows * top_keys(NT, all.top);
+        const size_t lds = sizeof(Key) * kRows * top_keys(NT, all.top);
         auto kernel = row_kernel<T, NT, NV, MODE, ENTROPY>;
         sliced(all, each * NT, [&](const LossArgs& a, int64_t rows) {
             const unsigned grid = grid_of(what, ceil_div(rows * each, kRows), kBlock);
@@ -1160,7 +1235,7 @@ void launch_rows(const char* what, const LossArgs& all, hipStream_t s) {
         });
     };
     const int64_t length = MODE == kSegment ? all.segment : all.classes;
-    if (MODE == kLogProbs && all.top == 0)
+    if (MODE == kLogProbs && all.top <= 1)
         with_shape<MODE == kLogProbs>(all.rows * each, length, kVec<T>, launch);
     else
         with_shape<false>(all.rows * each, length, kVec<T>, launch);
