@@ -43,12 +43,17 @@ constexpr TileCost kTiles32[] = {
 // 128 x 128.
 enum Loads { kRegisters, kDirect, kRing };
 
-LinearPlan linear_plan(int64_t m, int64_t n, int64_t k, int type, Loads loads) {
+struct LinearPlans {
+    LinearPlan of[3];  // by Loads
+};
+
+LinearPlans linear_plans(int64_t m, int64_t n, int64_t k, int type) {
     const int64_t z = type_size(type), depth = kRowBytes / z;
-    LinearPlan best{};
-    double least = 0.0;
+    LinearPlans best{};
+    double least[3] = {1e300, 1e300, 1e300};
     auto consider = [&](const TileCost& t) {
         const int64_t mt = ceil_div(m, t.m), nt = ceil_div(n, t.n), tiles = mt * nt;
+        const bool square = t.m == t.n, large = t.m == 256;
         for (int64_t parts = 1; parts <= 256; parts *= 2) {
             if (parts > 1 && (k < 2 * depth * parts || tiles * parts > 2048)) break;
             int64_t unit = ceil_div(ceil_div(k, parts), depth) * depth;
@@ -56,28 +61,27 @@ LinearPlan linear_plan(int64_t m, int64_t n, int64_t k, int type, Loads loads) {
             if (type == TG_TYPE_F32) unit = std::min(unit, kLongChain);
             unit = std::max(unit, depth);
             const int64_t real = std::max<int64_t>(1, ceil_div(k, unit)), groups = tiles * real;
-            const double load = groups < 256 ? static_cast<double>(groups) / 256
-                                             : static_cast<double>(ceil_div(groups, 256));
+            const double load = groups < 256 ? static_cast<double>(groups) * (1.0 / 256)
+                                             : static_cast<double>((groups + 255) / 256);
             const double u = static_cast<double>(unit);
             double us = std::max(t.alone * u + t.fixed, load * (t.busy * u + t.fixed));
             if (real > 1) {
                 const double bytes = 8.0 * static_cast<double>(real) * static_cast<double>(m) *
                                      static_cast<double>(n);
-                us += 2.5 + bytes / (bytes < 2e8 ? 9e6 : 5.3e6);
+                us += 2.5 + bytes * (bytes < 2e8 ? 1 / 9e6 : 1 / 5.3e6);
             }
-            if (best.em == 0 || us < least) {
-                least = us;
-                best = {t.m, t.n, mt, nt, unit, real};
+            for (const Loads l : {kRegisters, kDirect, kRing}) {
+                if ((l == kRegisters && !square) || (l != kRing && large) || us >= least[l])
+                    continue;
+                least[l] = us;
+                best.of[l] = {t.m, t.n, mt, nt, unit, real};
             }
         }
     };
-    auto all = [&](const auto& tiles) {
-        for (const TileCost& t : tiles) {
-            const bool square = t.m == t.n;
-            if (loads == kRing || (loads == kDirect ? t.m < 256 : square && t.m < 256)) consider(t);
-        }
-    };
-    type == TG_TYPE_F32 ? all(kTiles32) : all(kTiles16);
+    if (type == TG_TYPE_F32)
+        for (const TileCost& t : kTiles32) consider(t);
+    else
+        for (const TileCost& t : kTiles16) consider(t);
     return best;
 }
 
@@ -104,10 +108,11 @@ void product(LinearArgs& a, int type, bool ax, bool aw, void* part, size_t room,
                       (!aw || a.n % 8 == 0);
     LinearPlan p{};
     if (!few_rows(a, ax, aw)) {
-        p = linear_plan(a.m, a.n, a.k, type, ring ? kRing : direct ? kDirect : kRegisters);
-        Carver c(part, room);
-        a.part = reinterpret_cast<float*>(c.take<char>(p.bytes(a.m, a.n)));
-        if (p.parts == 1) a.part = nullptr;
+        p = linear_plans(a.m, a.n, a.k, type).of[ring ? kRing : direct ? kDirect : kRegisters];
+        if (p.parts > 1) {
+            Carver c(part, room);
+            a.part = reinterpret_cast<float*>(c.take<char>(p.bytes(a.m, a.n)));
+        }
     }
     with_type(type, "linear", [&](auto t) {
         linear_product<decltype(t)>(a, p, ax, aw, direct, s);
@@ -117,38 +122,53 @@ void product(LinearArgs& a, int type, bool ax, bool aw, void* part, size_t room,
 // Bytes for the parts of a product, whichever tiles its operands allow.
 size_t parts_bytes(int64_t m, int64_t n, int64_t k, int type) {
     if (m <= 0 || n <= 0) return 0;
+    const LinearPlans plans = linear_plans(m, n, k, type);
     size_t most = 0;
-    for (const Loads loads : {kRegisters, kDirect, kRing})
-        most = std::max(most, linear_plan(m, n, k, type, loads).bytes(m, n));
+    for (const LinearPlan& p : plans.of) most = std::max(most, p.bytes(m, n));
     return most;
 }
 
-// Rows of a workgroup of act_backward_kernel: for about 1,024 workgroups.
+// Chunks of columns of a workgroup of act_backward_kernel, as a power of two, and
+// its rows: for about 1,024 workgroups.
+int act_log_wide(int64_t n, int type) {
+    const int64_t chunks = ceil_div(n, 16 / type_size(type));
+    int log = 0;
+    while (log < 5 && (int64_t(1) << log) < chunks) ++log;
+    return log;
+}
+
 int64_t act_rows(int64_t m, int64_t n, int type) {
-    const int64_t cols = std::max<int64_t>(1, ceil_div(n, 32 * 16 / type_size(type)));
-    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(1024 / cols, 4096));
-    return std::max<int64_t>(8, ceil_div(ceil_div(m, parts), 8) * 8);
+    const int64_t chunks = std::max<int64_t>(1, ceil_div(n, 16 / type_size(type)));
+    const int log = act_log_wide(n, type);
+    const int64_t cols = ceil_div(chunks, int64_t(1) << log), high = 256 >> log;
+    const int64_t parts = std::max<int64_t>(1, 1024 / cols);
+    return std::max(high, ceil_div(ceil_div(m, parts), high) * high);
 }
 
 struct BackwardPlace {
     void* d;
     float* columns;
-    void* part;
+    void* part;  // dx's parts, then dw's: what is left of the workspace
     size_t room;
-    size_t bytes;
+    size_t bytes;  // without the parts
 };
 
-BackwardPlace backward_place(int64_t m, int64_t k, int64_t n, int type, void* ws, size_t size) {
+BackwardPlace backward_place(int64_t m, int64_t n, int type, int act, bool dbias, void* ws,
+                             size_t size) {
     Carver c(ws, size);
     BackwardPlace p{};
-    p.d = c.take<char>(static_cast<size_t>(m) * n * type_size(type));
-    p.columns = c.take<float>(static_cast<size_t>(ceil_div(m, act_rows(m, n, type))) * n);
-    // dx's parts, then dw's, in the same place
-    p.room = std::max(parts_bytes(m, k, n, type),
-                      std::max(parts_bytes(k, n, m, type), parts_bytes(n, k, m, type)));
-    p.part = c.take<char>(p.room);
+    if (act != TG_EPI_NONE) p.d = c.take<char>(static_cast<size_t>(m) * n * type_size(type));
+    if (dbias) p.columns = c.take<float>(static_cast<size_t>(ceil_div(m, act_rows(m, n, type))) * n);
     p.bytes = c.bytes();
+    p.part = ws ? static_cast<char*>(ws) + p.bytes : nullptr;
+    p.room = size > p.bytes ? size - p.bytes : 0;
     return p;
+}
+
+size_t backward_bytes(int64_t m, int64_t k, int64_t n, int type, int act, bool dbias) {
+    return backward_place(m, n, type, act, dbias, nullptr, 0).bytes +
+           std::max(parts_bytes(m, k, n, type),
+                    std::max(parts_bytes(k, n, m, type), parts_bytes(n, k, m, type)));
 }
 
 void check_linear(const std::string& w, int64_t m, int64_t k, int64_t n, int type, int act) {
@@ -217,7 +237,7 @@ int tg_linear(int64_t m, int64_t k, int64_t n, int type, const void* x, int64_t 
 
 size_t tg_linear_backward_workspace_size(int64_t m, int64_t k, int64_t n, int type) {
     if (m <= 0 || k < 0 || n <= 0 || type < TG_TYPE_F32 || type > TG_TYPE_F16) return 0;
-    return tg::backward_place(m, k, n, type, nullptr, 0).bytes;
+    return tg::backward_bytes(m, k, n, type, TG_EPI_SILU, true);
 }
 
 int tg_linear_backward(int64_t m, int64_t k, int64_t n, int type, const void* dy, int64_t lddy,
@@ -243,13 +263,14 @@ int tg_linear_backward(int64_t m, int64_t k, int64_t n, int type, const void* dy
         tg::BackwardPlace at{};
         tg::TempBuffer temp;
         if (given) {
-            const size_t need = tg::backward_place(m, k, n, type, nullptr, 0).bytes;
             if (!workspace) {
-                temp.allocate(need, s);
-                workspace = temp.get();
-                workspace_bytes = need;
+                workspace_bytes = tg::backward_bytes(m, k, n, type, act, dbias != nullptr);
+                if (workspace_bytes) {
+                    temp.allocate(workspace_bytes, s);
+                    workspace = temp.get();
+                }
             }
-            at = tg::backward_place(m, k, n, type, workspace, workspace_bytes);
+            at = tg::backward_place(m, n, type, act, dbias != nullptr, workspace, workspace_bytes);
         }
         tg::with_type(type, "linear_backward", [&](auto t) {
             using T = decltype(t);
@@ -257,6 +278,7 @@ int tg_linear_backward(int64_t m, int64_t k, int64_t n, int type, const void* dy
             a.m = m;
             a.n = n;
             a.rows = tg::act_rows(m, n, type);
+            a.log_wide = tg::act_log_wide(n, type);
             a.dy = dy;
             a.lddy = lddy;
             a.pre = pre;

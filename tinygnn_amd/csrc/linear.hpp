@@ -32,6 +32,7 @@ struct LinearArgs {
 
 struct ActArgs {
     int64_t m, n, rows;  // rows of a workgroup
+    int log_wide;        // ... and 16-byte chunks of columns
     const void* dy;
     int64_t lddy;
     const void* pre;

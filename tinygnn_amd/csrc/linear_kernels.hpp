@@ -64,78 +64,110 @@ __device__ __forceinline__ void with_act(int act, F&& fn) {
     }
 }
 
-// Four consecutive results of a row: bias, the value before the activation, the
-// activation, the residual.
-template <typename T, int ACT>
-__device__ __forceinline__ void finish(const LinearArgs& a, int64_t row, int n,
-                                       const float (&sum)[4], const float (&bias)[4]) {
-    float v[4], r[4] = {};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = sum[e] + bias[e];
-    if (a.pre) store_floats<T, 4>(static_cast<T*>(a.pre) + row * a.ldp + n, a.n - n, v);
-    if (a.residual)
-        load_floats<T, 4>(static_cast<const T*>(a.residual) + row * a.ldr + n, a.n - n, r);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = act_of<ACT>(v[e]) + r[e];
-    store_floats<T, 4>(static_cast<T*>(a.y) + row * a.ldy + n, a.n - n, v);
+// The residual's W values of a row from column n on (zeros without one).
+template <typename T, int W>
+__device__ __forceinline__ void residual_of(const LinearArgs& a, int64_t row, int n, float (&r)[W]) {
+    const bool in = a.residual && row < a.m;
+    load_floats<T, W>(static_cast<const T*>(a.residual) + (in ? row * a.ldr + n : 0),
+                      in ? a.n - n : 0, r);
 }
 
-// A wavefront's sums from row m0, column n0 on.  Lane (q, r) holds row r of a
-// tile, columns 4 q .. 4 q + 3.
-// PLAIN: a product without an epilogue.
+// W consecutive results of a row: bias, the value before the activation, the
+// activation, the residual.
+template <typename T, int ACT, int W>
+__device__ __forceinline__ void finish(const LinearArgs& a, int64_t row, int n,
+                                       const float (&sum)[W], const float (&bias)[W],
+                                       const float (&r)[W]) {
+    float v[W];
+#pragma unroll
+    for (int e = 0; e < W; ++e) v[e] = sum[e] + bias[e];
+    if (a.pre) store_floats<T, W>(static_cast<T*>(a.pre) + row * a.ldp + n, a.n - n, v);
+#pragma unroll
+    for (int e = 0; e < W; ++e) v[e] = act_of<ACT>(v[e]) + r[e];
+    store_floats<T, W>(static_cast<T*>(a.y) + row * a.ldy + n, a.n - n, v);
+}
+
+// fn(row, column, W sums, W values) for a wavefront's sums from row m0, column n0
+// on.  Lane (q, r) holds row r of a tile, columns 4 q .. 4 q + 3; 16 rows at a time
+// go through `lds` (16 (16 NJ + 4) floats of the wavefront's own), so that memory is
+// reached 16 bytes a lane and whole lines a row.  ahead(row, column, values) loads
+// the values, 16 rows before they are used.
+template <int W, int MI, int NJ, typename P, typename F>
+__device__ __forceinline__ void each_sums(const LinearArgs& a, int m0, int n0, int lane,
+                                          const v4f (&acc)[MI][NJ], float* lds, P&& ahead,
+                                          F&& fn) {
+    constexpr int kStride = NJ * 16 + 4, L = NJ * 16 / W, R = 64 / L, N = 16 / R;
+    static_assert(L <= 64 && 16 % R == 0, "lanes of a row");
+    const int q = lane >> 4, r = lane & 15, row = lane / L, col = lane % L * W;
+    float next[N][W];
+#pragma unroll
+    for (int p = 0; p < N; ++p) ahead(m0 + p * R + row, n0 + col, next[p]);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+            *reinterpret_cast<v4f*>(lds + r * kStride + j * 16 + 4 * q) = acc[i][j];
+        float now[N][W];
+#pragma unroll
+        for (int p = 0; p < N; ++p) {
+#pragma unroll
+            for (int e = 0; e < W; ++e) now[p][e] = next[p][e];
+            if (i + 1 < MI) ahead(m0 + (i + 1) * 16 + p * R + row, n0 + col, next[p]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int p = 0; p < N; ++p) {
+            float v[W];
+#pragma unroll
+            for (int c = 0; c < W; c += 4) {
+                const v4f f = *reinterpret_cast<const v4f*>(lds + (p * R + row) * kStride + col + c);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[c + e] = f[e];
+            }
+            const int m = m0 + i * 16 + p * R + row;
+            if (m < a.m) fn(m, n0 + col, v, now[p]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// PLAIN: a product without an epilogue.  Every wavefront is past its reads of the
+// tiles, whose place lds is.
 template <typename T, bool PLAIN, int MI, int NJ>
 __device__ __forceinline__ void store_sums(const LinearArgs& a, int part, int m0, int n0, int lane,
-                                           const v4f (&acc)[MI][NJ]) {
-    const int q = lane >> 4, r = lane & 15;
+                                           const v4f (&acc)[MI][NJ], float* lds) {
+    constexpr int W = kVec<T>;
     if (a.part) {
-#pragma unroll
-        for (int i = 0; i < MI; ++i) {
-            const int m = m0 + i * 16 + r;
-            if (m >= a.m) continue;
+        auto none = [](int, int, float(&)[4]) {};
+        each_sums<4>(a, m0, n0, lane, acc, lds, none,
+                     [&](int m, int n, const float (&v)[4], const float(&)[4]) {
             float* to = a.part + (static_cast<int64_t>(part) * a.m + m) * a.n;
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                const int n = n0 + j * 16 + 4 * q;
-                const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-                store_floats<float, 4>(to + n, a.n - n, v);
-            }
-        }
+            store_floats<float, 4>(to + n, a.n - n, v);
+        });
         return;
     }
-    if constexpr (PLAIN) {
-#pragma unroll
-        for (int i = 0; i < MI; ++i) {
-            const int m = m0 + i * 16 + r;
-            if (m >= a.m) continue;
-            T* to = static_cast<T*>(a.y) + m * a.ldy;
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                const int n = n0 + j * 16 + 4 * q;
-                const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-                store_floats<T, 4>(to + n, a.n - n, v);
-            }
-        }
+    if (PLAIN || (a.act == TG_EPI_NONE && !a.bias && !a.residual && !a.pre)) {
+        auto none = [](int, int, float(&)[W]) {};
+        each_sums<W>(a, m0, n0, lane, acc, lds, none,
+                     [&](int m, int n, const float (&v)[W], const float(&)[W]) {
+            store_floats<T, W>(static_cast<T*>(a.y) + m * a.ldy + n, a.n - n, v);
+        });
         return;
     }
-    float bias[NJ][4] = {};
+    if constexpr (PLAIN) return;
+    float bias[W] = {};
     if (a.bias) {
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const int n = n0 + j * 16 + 4 * q;
-            load_floats<T, 4>(static_cast<const T*>(a.bias) + n, a.n - n, bias[j]);
-        }
+        const int n = n0 + lane % (NJ * 16 / W) * W;
+        load_floats<T, W>(static_cast<const T*>(a.bias) + n, a.n - n, bias);
     }
+    auto residual = [&](int m, int n, float (&r)[W]) { residual_of<T, W>(a, m, n, r); };
     with_act(a.act, [&](auto act) {
-#pragma unroll
-        for (int i = 0; i < MI; ++i) {
-            const int m = m0 + i * 16 + r;
-            if (m >= a.m) continue;
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-                finish<T, decltype(act)::value>(a, m, n0 + j * 16 + 4 * q, v, bias[j]);
-            }
-        }
+        each_sums<W>(a, m0, n0, lane, acc, lds, residual,
+                     [&](int m, int n, const float (&v)[W], const float (&r)[W]) {
+            finish<T, decltype(act)::value>(a, m, n, v, bias, r);
+        });
     });
 }
 
@@ -152,8 +184,9 @@ __global__ __launch_bounds__(256) void join_kernel(LinearArgs a) {
     const int n = static_cast<int>(t - row * chunks) * 4;
     const int64_t size = static_cast<int64_t>(a.m) * a.n;
     const float* p = a.part + row * a.n + n;
-    float s[4] = {};
+    float s[4] = {}, r[4] = {};
     if (row < a.m) {
+        if (y == 0) residual_of<T, 4>(a, row, n, r);
 #pragma unroll 8
         for (int i = y; i < a.parts; i += Y) {
             float v[4];
@@ -177,7 +210,7 @@ __global__ __launch_bounds__(256) void join_kernel(LinearArgs a) {
     if (row >= a.m) return;
     float bias[4] = {};
     if (a.bias) load_floats<T, 4>(static_cast<const T*>(a.bias) + n, a.n - n, bias);
-    with_act(a.act, [&](auto act) { finish<T, decltype(act)::value>(a, row, n, s, bias); });
+    with_act(a.act, [&](auto act) { finish<T, decltype(act)::value>(a, row, n, s, bias, r); });
 }
 
 // ---------------------------------------------------------------------------
@@ -255,8 +288,13 @@ __device__ __forceinline__ bool place_of(const LinearArgs& a, int* part, uint32_
     return tile_of(blockIdx.x % per, a.mt, a.nt, mt, nt);
 }
 
+// (Wavefronts a SIMD that floats' tiles of 64 x 128 are compiled for: one register
+// more left two, 232,965 x 256 x 256 347 us against 332.)
+template <typename T, typename S>
+constexpr int kMinWaves = sizeof(T) == 4 && S::kM * S::kN == 8192 ? 3 : 1;
+
 template <typename T, typename S, bool AX, bool AW, bool DIRECT>
-__global__ __launch_bounds__(S::kThreads) void linear_kernel(LinearArgs a) {
+__global__ __launch_bounds__(S::kThreads, (kMinWaves<T, S>)) void linear_kernel(LinearArgs a) {
     __shared__ __attribute__((aligned(16))) char a0[S::kM * kRowBytes];
     __shared__ __attribute__((aligned(16))) char b0[S::kN * kRowBytes];
     __shared__ __attribute__((aligned(16))) char a1[S::kM * kRowBytes];
@@ -292,8 +330,12 @@ __global__ __launch_bounds__(S::kThreads) void linear_kernel(LinearArgs a) {
         ws.put(lb);
     };
     pipeline<DIRECT>(tiles, a0, b0, a1, b1, load, store, compute, join);
+    __syncthreads();
+    static_assert(S::kThreads == 256, "a place for each wavefront");
+    char* const own = wave == 0 ? a0 : wave == 1 ? b0 : wave == 2 ? a1 : b1;
     // (both across: the weights' gradient)
-    store_sums<T, AX>(a, part, m0 + wm, n0 + wn, lane, acc.result());
+    store_sums<T, AX>(a, part, m0 + wm, n0 + wn, lane, acc.result(),
+                      reinterpret_cast<float*>(own));
 }
 
 // The large tile (tiles.hpp): 16-bit operands that can be loaded directly, in
@@ -351,7 +393,10 @@ __global__ __launch_bounds__(kRingThreads) void linear_ring_kernel(LinearArgs a)
     PartReader<AW, 4, AX> rb(wn, lane);
     ring<T>((k1 - kb + kStep - 1) / kStep, ra, rb, [](int) {}, load, a0, b0, a1, b1, a2, b2, a3, b3,
             acc);
-    store_sums<T, AX>(a, part, m0 + wm, n0 + wn, lane, acc);
+    __syncthreads();
+    char* const own = wave < 4 ? (wave == 0 ? a0 : wave == 1 ? b0 : wave == 2 ? a1 : b1)
+                               : (wave == 4 ? a2 : wave == 5 ? b2 : wave == 6 ? a3 : b3);
+    store_sums<T, AX>(a, part, m0 + wm, n0 + wn, lane, acc, reinterpret_cast<float*>(own));
 }
 
 using Medium = Shape<128, 128, 2, 2>;
@@ -425,7 +470,9 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_kernel(LinearArgs a) {
     float bias[4] = {};
     if (a.bias) load_floats<T, 4>(static_cast<const T*>(a.bias) + n, a.n - n, bias);
     const float v[4] = {s[0], s[1], s[2], s[3]};
-    with_act(a.act, [&](auto act) { finish<T, decltype(act)::value>(a, m, n, v, bias); });
+    float res[4];
+    residual_of<T, 4>(a, m, n, res);
+    with_act(a.act, [&](auto act) { finish<T, decltype(act)::value>(a, m, n, v, bias, res); });
 }
 
 template <typename T>
@@ -473,28 +520,33 @@ void launch_product(LinearArgs& a, const LinearPlan& p, bool direct, hipStream_t
     TG_LAUNCH_CHECK();
     if (p.parts > 1) {
         const int64_t threads = static_cast<int64_t>(a.m) * ceil_div(a.n, 4);
-        p.parts > 8 ? join_kernel<T, 8><<<grid_of("linear", ceil_div(threads, 32), 256), 256, 0, s>>>(a)
-                    : join_kernel<T, 1><<<grid_of("linear", ceil_div(threads, 256), 256), 256, 0, s>>>(a);
+        auto join = [&](auto kernel, int64_t results) {
+            kernel<<<grid_of("linear", ceil_div(threads, results), 256), 256, 0, s>>>(a);
+        };
+        p.parts > 48  ? join(join_kernel<T, 32>, 8)
+        : p.parts > 8 ? join(join_kernel<T, 8>, 32)
+                      : join(join_kernel<T, 1>, 256);
         TG_LAUNCH_CHECK();
     }
 }
 
 // ---------------------------------------------------------------------------
-// d = dy act'(pre) and its columns' sums: a workgroup takes a.rows rows of 32
-// VEC columns, 8 rows at a time; the parts' sums are added in order by
+// d = dy act'(pre) and its columns' sums: a workgroup takes a.rows rows of up
+// to 32 VEC columns, 8 rows or more at a time; the parts' sums are added in order by
 // columns_kernel.  ACT NONE: the sums alone.
 // ---------------------------------------------------------------------------
 template <typename T, int ACT>
 __global__ __launch_bounds__(256) void act_backward_kernel(ActArgs a) {
     constexpr int VEC = kVec<T>;
-    __shared__ float join[8][32 * VEC];
-    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-    const int64_t c = (static_cast<int64_t>(blockIdx.x) * 32 + x) * VEC;
+    __shared__ float join[256 * VEC];
+    const int wide = 1 << a.log_wide, high = 256 >> a.log_wide;
+    const int x = threadIdx.x & (wide - 1), y = threadIdx.x >> a.log_wide;
+    const int64_t c = (static_cast<int64_t>(blockIdx.x) * wide + x) * VEC;
     const int64_t r0 = static_cast<int64_t>(blockIdx.y) * a.rows;
     const int64_t r1 = a.m - r0 > a.rows ? r0 + a.rows : a.m;
     float s[VEC] = {};
 #pragma unroll 4
-    for (int64_t r = r0 + y; r < r1; r += 8) {
+    for (int64_t r = r0 + y; r < r1; r += high) {
         float v[VEC], p[VEC];
         load_floats<T, VEC>(static_cast<const T*>(a.dy) + r * a.lddy + c, a.n - c, v);
         if constexpr (ACT != TG_EPI_NONE) {
@@ -508,13 +560,12 @@ __global__ __launch_bounds__(256) void act_backward_kernel(ActArgs a) {
     }
     if (!a.part) return;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) join[y][x * VEC + e] = s[e];
+    for (int e = 0; e < VEC; ++e) join[(y * wide + x) * VEC + e] = s[e];
     __syncthreads();
-    for (int i = threadIdx.x; i < 32 * VEC; i += 256) {
-        const int64_t at = static_cast<int64_t>(blockIdx.x) * 32 * VEC + i;
+    for (int i = threadIdx.x; i < wide * VEC; i += 256) {
+        const int64_t at = static_cast<int64_t>(blockIdx.x) * wide * VEC + i;
         float v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) v += join[w][i];
+        for (int w = 0; w < high; ++w) v += join[w * wide * VEC + i];
         if (at < a.n) a.part[static_cast<int64_t>(blockIdx.y) * a.n + at] = v;
     }
 }
@@ -540,7 +591,7 @@ __global__ __launch_bounds__(1024) void columns_kernel(const float* __restrict__
 
 template <typename T>
 void launch_act(const ActArgs& a, int act, hipStream_t s) {
-    const int64_t cols = ceil_div(a.n, 32 * kVec<T>), parts = ceil_div(a.m, a.rows);
+    const int64_t cols = ceil_div(a.n, kVec<T> << a.log_wide), parts = ceil_div(a.m, a.rows);
     require(cols * 256 < (int64_t(1) << 32) && parts < 65536, "linear_backward: too many elements");
     const dim3 grid(static_cast<unsigned>(cols), static_cast<unsigned>(parts));
     if (act == TG_EPI_NONE) act_backward_kernel<T, TG_EPI_NONE><<<grid, 256, 0, s>>>(a);
