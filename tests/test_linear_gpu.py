@@ -13,7 +13,8 @@ SIZES = [(1, 1, 1), (1, 4096, 512), (1, 37, 1000), (2, 8, 3), (3, 602, 41), (5, 
          (8, 1024, 4096), (16, 512, 640), (17, 300, 130), (31, 8192, 256), (33, 64, 64),
          (64, 1000, 70), (130, 257, 129), (200, 96, 1024), (500, 33, 7), (1000, 256, 256),
          (1031, 602, 256), (700, 8, 2000), (2000, 40, 41), (4096, 64, 16), (3000, 512, 520),
-         (260, 4096, 264), (2048, 2048, 2048), (5000, 1024, 1280), (40000, 128, 24)]
+         (260, 4096, 264), (2048, 2048, 2048), (5000, 1024, 1280), (40000, 128, 24),
+         (4096, 1024, 4096), (8200, 520, 4104), (20, 1500, 900), (32, 40000, 16), (70, 6000, 8)]
 
 
 def code(tg, name):

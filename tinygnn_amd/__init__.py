@@ -1103,12 +1103,12 @@ def distill(logits, teacher, ids, temperature: float = 1.0, dloss=None, out=None
     pt = _flat(what, "teacher", teacher, teacher.shape, teacher.dtype)
     pi = _flat(what, "ids", ids, teacher.shape, _pt.i32)
     pd = _flat(what, "dloss", dloss, (rows,), _pt.f32)
-    loss = _pt.empty(rows, dtype=_pt.f32, device=logits.device)
     d, po, ldo = None, None, 0
     if dloss is not None:
         d, po, ldo = _out(what, "out", out, logits.shape, logits, logits.dtype)
     elif out is not None:
         _refuse(what, "out takes the gradient, which needs dloss.")
+    loss = _pt.empty(rows, dtype=_pt.f32, device=logits.device)
     k = teacher.shape[1]
     size = lib.tg_distill_workspace_size(rows, classes, k, kind)
     ws, pws = _workspace(size, logits)
