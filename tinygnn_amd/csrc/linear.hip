@@ -85,10 +85,15 @@ LinearPlans linear_plans(int64_t m, int64_t n, int64_t k, int type) {
     return best;
 }
 
-// Few rows of x with w's rows along the contraction (few_kernel): no parts.
-// (bf16 1 x 4,096 x 4,096: ...)
-bool few_rows(const LinearArgs& a, bool ax, bool aw) {
-    return !ax && !aw && a.m <= 32 && a.k <= 32768 && (a.n >= 1024 || a.k <= 4096);
+// Few rows of x with w's rows along the contraction (few_kernel): one launch, no
+// parts.  Measured against the tiles with theirs (bf16, 1 row: 4,096 x 4,096 7.2 us
+// against 8.5, 512 x 8,192 4.2 against 6.0, 2,048 x 128 4.5 against 5.6; but 8,192 x
+// 1,024 11.5 against 7.1, 4,096 x 64 6.6 against 5.3, 1,024 x 32,000 17.3 against 14.8;
+// 32 rows of 4,096 x 4,096 14.6 against 13.2; fp32, 16 rows of 2,048 x 128 10.9 against
+// 8.0).
+bool few_rows(const LinearArgs& a, int64_t z, bool ax, bool aw) {
+    return !ax && !aw && a.m <= 16 && a.k <= 4096 && a.n <= 16384 &&
+           (a.n >= 1024 || (a.k <= 2048 && a.m * z <= 32));
 }
 
 // Whether an operand's tiles of up to 256 of its rows or columns can come by
@@ -107,7 +112,7 @@ void product(LinearArgs& a, int type, bool ax, bool aw, void* part, size_t room,
     const bool ring = direct && z == 2 && ((ax && aw) || a.k % 8 == 0) && (!ax || a.m % 8 == 0) &&
                       (!aw || a.n % 8 == 0);
     LinearPlan p{};
-    if (!few_rows(a, ax, aw)) {
+    if (!few_rows(a, z, ax, aw)) {
         p = linear_plans(a.m, a.n, a.k, type).of[ring ? kRing : direct ? kDirect : kRegisters];
         if (p.parts > 1) {
             Carver c(part, room);

@@ -406,33 +406,27 @@ using Wide = Shape<64, 128, 2, 2>;
 using Tall = Shape<128, 64, 2, 2>;
 
 // ---------------------------------------------------------------------------
-// Few rows of x, w's rows along the contraction: 16 columns by the 16 wavefronts of
+// Up to 16 rows of x, w's rows along the contraction: 16 columns by the 16 wavefronts of
 // a workgroup, which take turns of 128 bytes of the contraction, loaded straight to
 // the matrix instructions' operands; their sums are added in order.  Bound by
 // reading w once.
 // ---------------------------------------------------------------------------
 constexpr int kFewWaves = 16;
 
-template <typename T, int MI>
+template <typename T>
 __global__ __launch_bounds__(kFewWaves * 64) void few_kernel(LinearArgs a) {
     constexpr int VEC = kVec<T>, kTurn = 8 * VEC;
-    __shared__ v4f sums[kFewWaves][MI][64];
+    __shared__ v4f sums[kFewWaves][64];
     const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n0 = static_cast<int>(blockIdx.x) * 16;
     // rows and columns past the last: the last one again, and not stored
-    const int col = n0 + r < a.n ? n0 + r : a.n - 1;
-    const T* w = static_cast<const T*>(a.w) + col * a.ldw + q * VEC;
-    const T* x[MI];
-#pragma unroll
-    for (int i = 0; i < MI; ++i) {
-        const int row = i * 16 + r < a.m ? i * 16 + r : a.m - 1;
-        x[i] = static_cast<const T*>(a.x) + row * a.ldx + q * VEC;
-    }
-    v4f acc[MI] = {};
+    const T* w = static_cast<const T*>(a.w) + (n0 + r < a.n ? n0 + r : a.n - 1) * a.ldw + q * VEC;
+    const T* x = static_cast<const T*>(a.x) + (r < a.m ? r : a.m - 1) * a.ldx + q * VEC;
+    v4f acc = {};
     auto turns = [&](int k, auto count, auto whole) {
         constexpr int N = decltype(count)::value;
-        Frag fw[N][2], fx[N][MI][2];
+        Frag fw[N][2], fx[N][2];
 #pragma unroll
         for (int u = 0; u < N; ++u)
 #pragma unroll
@@ -440,46 +434,39 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_kernel(LinearArgs a) {
                 const int at = k + u * kFewWaves * kTurn + h * 4 * VEC;
                 const int64_t left = decltype(whole)::value ? VEC : a.k - at - q * VEC;
                 fw[u][h].u = load_chunk(w + (left > 0 ? at : 0), left);
-#pragma unroll
-                for (int i = 0; i < MI; ++i)
-                    fx[u][i][h].u = load_chunk(x[i] + (left > 0 ? at : 0), left);
+                fx[u][h].u = load_chunk(x + (left > 0 ? at : 0), left);
             }
 #pragma unroll
         for (int u = 0; u < N; ++u)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < MI; ++i) acc[i] = mfma<T>(fw[u][h], fx[u][i][h], acc[i]);
+            for (int h = 0; h < 2; ++h) acc = mfma<T>(fw[u][h], fx[u][h], acc);
     };
-    constexpr int kMany = MI == 1 ? 4 : 2;
+    constexpr int kMany = 4;
     using std::integral_constant;
     int k = wave * kTurn;
     for (; k + (kMany - 1) * kFewWaves * kTurn + kTurn <= a.k; k += kMany * kFewWaves * kTurn)
         turns(k, integral_constant<int, kMany>{}, std::true_type{});
     for (; k < a.k; k += kFewWaves * kTurn)
         turns(k, integral_constant<int, 1>{}, std::false_type{});
-#pragma unroll
-    for (int i = 0; i < MI; ++i) sums[wave][i][lane] = acc[i];
+    sums[wave][lane] = acc;
     __syncthreads();
-    if (wave >= MI) return;
-    v4f s = sums[0][wave][lane];
+    if (wave > 0) return;
+    v4f s = sums[0][lane];
 #pragma unroll
-    for (int v = 1; v < kFewWaves; ++v) s += sums[v][wave][lane];
-    const int m = wave * 16 + r, n = n0 + 4 * q;
-    if (m >= a.m) return;
-    float bias[4] = {};
+    for (int v = 1; v < kFewWaves; ++v) s += sums[v][lane];
+    const int n = n0 + 4 * q;
+    if (r >= a.m) return;
+    float bias[4] = {}, res[4];
     if (a.bias) load_floats<T, 4>(static_cast<const T*>(a.bias) + n, a.n - n, bias);
+    residual_of<T, 4>(a, r, n, res);
     const float v[4] = {s[0], s[1], s[2], s[3]};
-    float res[4];
-    residual_of<T, 4>(a, m, n, res);
-    with_act(a.act, [&](auto act) { finish<T, decltype(act)::value>(a, m, n, v, bias, res); });
+    with_act(a.act, [&](auto act) { finish<T, decltype(act)::value>(a, r, n, v, bias, res); });
 }
 
 template <typename T>
 void launch_few(const LinearArgs& a, hipStream_t s) {
     const unsigned grid = grid_of("linear", ceil_div(a.n, 16), kFewWaves * 64);
-    a.m <= 16 ? few_kernel<T, 1><<<grid, kFewWaves * 64, 0, s>>>(a)
-              : few_kernel<T, 2><<<grid, kFewWaves * 64, 0, s>>>(a);
+    few_kernel<T><<<grid, kFewWaves * 64, 0, s>>>(a);
     TG_LAUNCH_CHECK();
 }
 
@@ -545,18 +532,24 @@ __global__ __launch_bounds__(256) void act_backward_kernel(ActArgs a) {
     const int64_t r0 = static_cast<int64_t>(blockIdx.y) * a.rows;
     const int64_t r1 = a.m - r0 > a.rows ? r0 + a.rows : a.m;
     float s[VEC] = {};
+    for (int64_t r = r0 + y; r < r1;) {  // chains of 64 rows
+        const int64_t stop = r1 - r > 64 * high ? r + 64 * high : r1;
+        float now[VEC] = {};
 #pragma unroll 4
-    for (int64_t r = r0 + y; r < r1; r += high) {
-        float v[VEC], p[VEC];
-        load_floats<T, VEC>(static_cast<const T*>(a.dy) + r * a.lddy + c, a.n - c, v);
-        if constexpr (ACT != TG_EPI_NONE) {
-            load_floats<T, VEC>(static_cast<const T*>(a.pre) + r * a.ldp + c, a.n - c, p);
+        for (; r < stop; r += high) {
+            float v[VEC], p[VEC];
+            load_floats<T, VEC>(static_cast<const T*>(a.dy) + r * a.lddy + c, a.n - c, v);
+            if constexpr (ACT != TG_EPI_NONE) {
+                load_floats<T, VEC>(static_cast<const T*>(a.pre) + r * a.ldp + c, a.n - c, p);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[e] *= slope_of<ACT>(p[e]);
-            if (a.d) store_floats<T, VEC>(static_cast<T*>(a.d) + r * a.ldd + c, a.n - c, v);
+                for (int e = 0; e < VEC; ++e) v[e] *= slope_of<ACT>(p[e]);
+                if (a.d) store_floats<T, VEC>(static_cast<T*>(a.d) + r * a.ldd + c, a.n - c, v);
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) now[e] += v[e];
         }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) s[e] += v[e];
+        for (int e = 0; e < VEC; ++e) s[e] += now[e];
     }
     if (!a.part) return;
 #pragma unroll
