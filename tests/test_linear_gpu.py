@@ -91,6 +91,41 @@ def test_onto_the_residual(gpu, m, k, n, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("m,k,n", [(1, 1, 1024), (15, 127, 1031), (16, 4096, 1024), (16, 4095, 1040),
+                                   (7, 2000, 16384), (16, 4100, 1024), (3, 64, 16400)])
+def test_few_rows(gpu, m, k, n, dtype):
+    """w's rows along the contraction, at the ends of where one launch takes them."""
+    p = make(m, k, n, DTYPES[dtype], True)
+    check(p, "silu", True)
+    check(p, "none", True, bias=False, residual=False, pad=(8, 8, 0, 0, 0))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("m,n", [(300000, 41), (40000, 4096), (1000, 3)])
+def test_long_sums_of_the_bias_gradient(gpu, m, n, dtype):
+    """Values of one sign: chains of 64 rows, of 64 such, and trees of as many parts
+    leave 256 roundings of the sum at most."""
+    import tinygnn_amd as tg
+    dt = DTYPES[dtype]
+    dy = ((1 + torch.rand(m, n, generator=gen(m), device="cuda")) / 32).to(dt)
+    one = torch.ones(m, 1, dtype=dt, device="cuda")
+    _, _, db = tg.linear_backward(dy, one, torch.ones(1, n, dtype=dt, device="cuda"), bias=True)
+    want = dy.double().sum(0)
+    within(db, want, hc.rounded(want, 256 * hc.U * want, dt), "db")
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_nothing_to_contract(gpu, dtype):
+    """k = 0: the epilogue of zeros, by tiles."""
+    import tinygnn_amd as tg
+    dt = DTYPES[dtype]
+    p = make(100, 1, 70, dt, False)
+    y = tg.linear(p["x"][:, :0], p["w"][:0], bias=p["bias"], residual=p["residual"])
+    want = p["residual"].double() + p["bias"].double()
+    within(y, want, hc.rounded(want, 2 * hc.U * want.abs(), dt), "y")
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
 def test_empty(gpu, dtype):
     import tinygnn_amd as tg
     dt = DTYPES[dtype]

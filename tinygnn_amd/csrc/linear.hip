@@ -31,6 +31,14 @@ constexpr TileCost kTiles32[] = {
     {128, 64, 0.0420, 0.0325, 1.3},
 };
 
+// How both operands come: through registers, straight to LDS, or to the ring of the
+// large tile.
+enum Loads { kRegisters, kDirect, kRing };
+
+struct LinearPlans {
+    LinearPlan of[3];  // by Loads
+};
+
 // How an out [m x n] with contraction k is cut: the tile and the parts of the
 // contraction that the costs above and the parts' join (2.5 us, its bytes at 9 TB/s,
 // past 200 MB at 5.3) make cheapest.  What it takes is within 10% of the best of 30
@@ -41,12 +49,6 @@ constexpr TileCost kTiles32[] = {
 // (64 x 64 311, 128 x 128, which leaves one wavefront a SIMD, 362).
 // Operands that come through registers (kRegisters) take 64 x 64 or, of 16 bits,
 // 128 x 128.
-enum Loads { kRegisters, kDirect, kRing };
-
-struct LinearPlans {
-    LinearPlan of[3];  // by Loads
-};
-
 LinearPlans linear_plans(int64_t m, int64_t n, int64_t k, int type) {
     const int64_t z = type_size(type), depth = kRowBytes / z;
     LinearPlans best{};
@@ -104,7 +106,7 @@ bool direct_side(const void* p, int64_t ld, int64_t cols, int64_t z, bool across
            (!across || cols * z % 4 == 0) && (256 * ld + cols) * z < kDirectBytes;
 }
 
-// One product with the operands' layouts; `room` floats in `part` for its parts.
+// One product with the operands' layouts; `room` bytes at `part` for its parts.
 void product(LinearArgs& a, int type, bool ax, bool aw, void* part, size_t room, hipStream_t s) {
     const int64_t z = type_size(type);
     const bool direct = direct_side(a.x, a.ldx, ax ? a.m : a.k, z, ax) &&

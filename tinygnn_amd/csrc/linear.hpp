@@ -50,10 +50,9 @@ struct LinearPlan {
     }
 };
 
-// The launches of one element type: a product (p.em 0: of few rows, both operands
-// along) whose operands run across the
-// contraction (ax, aw) or along it, d and its columns' sums by parts of rows, and
-// the join of those.
+// The launches of one element type: a product whose operands run across the
+// contraction (ax, aw) or along it (p.em 0: of few rows, both along), d and its
+// columns' sums by parts of rows, and the join of those.
 template <typename T>
 void linear_product(LinearArgs& a, const LinearPlan& p, bool ax, bool aw, bool direct,
                     hipStream_t s);

@@ -8,7 +8,10 @@
 // through v_mfma_f32_16x16x32, floats through v_mfma_f32_16x16x4f32; sums are
 // fp32.  Where the tiles are too few for the CUs, or a chain of floats too long,
 // the contraction is cut in parts whose fp32 sums a second kernel adds in order,
-// with the epilogue.
+// with the epilogue.  The epilogue is in float, one rounding for each stored value:
+//   pre = sum + bias,  y = residual + act(pre),  d = dy act'(pre), dbias = sum of d;
+// d is rounded to the element type before d w^T and x^T d read it (the operands of the
+// matrix instructions; dbias sums the values before that).
 #pragma once
 
 #include "grouped.hpp"
@@ -21,11 +24,16 @@ namespace {
 
 constexpr float kGeluScale = 1.5957691216f;  // 2 sqrt(2 / pi)
 constexpr float kGeluCube = 0.044715f;
+constexpr float kLog2e = 1.4426950409f;
 
-// 1 / (1 + exp(-s)): GELU's (1 + tanh(s / 2)) / 2, too.  (The reciprocal
-// instruction is within one unit in the last place.)
-__device__ __forceinline__ float sigmoid(float s) {
-    return __builtin_amdgcn_rcpf(1.0f + __expf(-s));
+// 1 / (1 + 2^e), e = -s log2(e): the sigmoid of s, and GELU's (1 + tanh(s / 2)) / 2,
+// whose constants take the logarithm.  (The reciprocal instruction is within one unit
+// in the last place.)
+__device__ __forceinline__ float sigmoid_of_log2(float e) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(e));
+}
+__device__ __forceinline__ float gelu_log2(float v) {
+    return v * __builtin_fmaf(v * v, -kGeluScale * kGeluCube * kLog2e, -kGeluScale * kLog2e);
 }
 
 template <int ACT>
@@ -33,8 +41,8 @@ __device__ __forceinline__ float act_of(float v) {
     if constexpr (ACT == TG_EPI_RELU) return 0.0f < v ? v : 0.0f;
     if constexpr (ACT == TG_EPI_ELU) return v < 0.0f ? expm1_negative(v) : v;
     if constexpr (ACT == TG_EPI_GELU)
-        return v * sigmoid(kGeluScale * __builtin_fmaf(kGeluCube * v * v, v, v));
-    if constexpr (ACT == TG_EPI_SILU) return v * sigmoid(v);
+        return v * sigmoid_of_log2(gelu_log2(v));
+    if constexpr (ACT == TG_EPI_SILU) return v * sigmoid_of_log2(-kLog2e * v);
     return v;
 }
 
@@ -44,10 +52,12 @@ __device__ __forceinline__ float slope_of(float v) {
     if constexpr (ACT == TG_EPI_RELU) return 0.0f < v ? 1.0f : 0.0f;
     if constexpr (ACT == TG_EPI_ELU) return v < 0.0f ? __expf(v) : 1.0f;
     if constexpr (ACT == TG_EPI_GELU || ACT == TG_EPI_SILU) {
-        const float c = kGeluCube * v * v;
-        const float s = ACT == TG_EPI_GELU ? kGeluScale * __builtin_fmaf(c, v, v) : v;
-        const float ds = ACT == TG_EPI_GELU ? kGeluScale * __builtin_fmaf(3.0f, c, 1.0f) : 1.0f;
-        const float p = sigmoid(s), t = p * (1.0f - p);
+        const float ds =
+            ACT == TG_EPI_GELU
+                ? __builtin_fmaf(v * v, 3.0f * kGeluScale * kGeluCube, kGeluScale)
+                : 1.0f;
+        const float p = sigmoid_of_log2(ACT == TG_EPI_GELU ? gelu_log2(v) : -kLog2e * v);
+        const float t = p * (1.0f - p);
         return t == 0.0f ? p : __builtin_fmaf(t * v, ds, p);
     }
     return 1.0f;
@@ -172,7 +182,8 @@ __device__ __forceinline__ void store_sums(const LinearArgs& a, int part, int m0
 }
 
 // y = the epilogue of the parts' sums: Y threads take every Y-th part of four
-// results, whose sums are added in order.
+// results, whose sums are added in order.  Bound by reading the parts: 4,000 x 2,048
+// in two 18.7 us.
 template <typename T, int Y>
 __global__ __launch_bounds__(256) void join_kernel(LinearArgs a) {
     constexpr int X = 256 / Y;
@@ -293,6 +304,10 @@ __device__ __forceinline__ bool place_of(const LinearArgs& a, int* part, uint32_
 template <typename T, typename S>
 constexpr int kMinWaves = sizeof(T) == 4 && S::kM * S::kN == 8192 ? 3 : 1;
 
+// A tile of S::kM x S::kN results in the registers of 256 threads, its operands by two
+// tiles of LDS in turn.  Bound by the matrix instructions: floats, whose instruction
+// has an eighth of the rate: 232,965 x 256 x 256 forward 367 us with the store of pre
+// and y (83 TFLOP/s; 281 without pre, 109), its d w^T 318 (96), its x^T d 300 (102).
 template <typename T, typename S, bool AX, bool AW, bool DIRECT>
 __global__ __launch_bounds__(S::kThreads, (kMinWaves<T, S>)) void linear_kernel(LinearArgs a) {
     __shared__ __attribute__((aligned(16))) char a0[S::kM * kRowBytes];
@@ -340,7 +355,9 @@ __global__ __launch_bounds__(S::kThreads, (kMinWaves<T, S>)) void linear_kernel(
 
 // The large tile (tiles.hpp): 16-bit operands that can be loaded directly, in
 // whole chunks (along the contraction, its length % 8 = 0; across it, the rows or
-// columns % 8 = 0).
+// columns % 8 = 0).  One workgroup a CU, so that nothing runs beside its first loads
+// and its results: bf16 16,384 rows, 2,048 to 8,192, with GELU, pre and y 605 us (909
+// TFLOP/s), its d w^T 466 (1,180), its x^T d 490 (1,122).
 template <typename T, bool AX, bool AW>
 __global__ __launch_bounds__(kRingThreads) void linear_ring_kernel(LinearArgs a) {
     TG_RING_LDS;
@@ -409,7 +426,7 @@ using Tall = Shape<128, 64, 2, 2>;
 // Up to 16 rows of x, w's rows along the contraction: 16 columns by the 16 wavefronts of
 // a workgroup, which take turns of 128 bytes of the contraction, loaded straight to
 // the matrix instructions' operands; their sums are added in order.  Bound by
-// reading w once.
+// reading w once: 1 x 4,096 x 4,096 bf16 7.2 us (4.7 TB/s).
 // ---------------------------------------------------------------------------
 constexpr int kFewWaves = 16;
 
@@ -520,7 +537,8 @@ void launch_product(LinearArgs& a, const LinearPlan& p, bool direct, hipStream_t
 // ---------------------------------------------------------------------------
 // d = dy act'(pre) and its columns' sums: a workgroup takes a.rows rows of up
 // to 32 VEC columns, 8 rows or more at a time; the parts' sums are added in order by
-// columns_kernel.  ACT NONE: the sums alone.
+// columns_kernel.  ACT NONE: the sums alone.  Bound by its two reads and one write:
+// 232,965 x 256 fp32 135 us (5.3 TB/s), 16,384 x 8,192 bf16 with GELU 180 (4.5).
 // ---------------------------------------------------------------------------
 template <typename T, int ACT>
 __global__ __launch_bounds__(256) void act_backward_kernel(ActArgs a) {

@@ -33,7 +33,8 @@ LossArgs loss_args(int64_t rows, int64_t classes, const void* logits, int64_t ld
 }
 
 // How rows are cut: one segment, but where there are few of more than 16,384
-// classes (as many as give 1,024 workgroups of 4,096 classes at least, 64 at most),
+// classes (as many as give 512 workgroups of 4,096 classes at least, 64 at most;
+// 1 x 102,400 bf16 in one 20 us, in 25 with the join 11.4),
 // and longer ones than a workgroup holds.  (A distillation with its gradient reads
 // cut rows twice, the others once.)
 struct Cut {
