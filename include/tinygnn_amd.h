@@ -489,7 +489,9 @@ int tg_matmul_fp8(int64_t m, int64_t k, int64_t n, int64_t groups, const void* x
  * v / (1 + exp(-v)); residual [m x n] or NULL.  pre (or NULL) receives
  * x * w + bias, for the backward pass.  All of `type`; sums in fp32, y and pre
  * rounded once.  y may be the residual (same leading dimension) and overlaps
- * nothing else.  m, k, n < 2^31 - 4096.
+ * nothing else; nor does pre.  m, k, n < 2^31 - 4096, and the products' results
+ * within 2^23 tiles (of 32 x 128 or 64 x 64 at the least), else
+ * TG_ERR_INVALID_ARGUMENT.
  *
  * tg_linear_backward: from dy and the forward's x, w and pre
  *   d = dy * act'(pre), rounded to `type` (act NONE: d = dy, pre is not read),

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import head_cases as hc
-from expert_cases import gen, randn, within
+from expert_cases import DTYPES, gen, randn, within
 
 pytestmark = pytest.mark.gpu
 T, D, H, C, K = 300, 40, 72, 50, 6
@@ -271,6 +271,55 @@ def test_written_inside_only(gpu):
                 dy.data_ptr(), n, 4, dx.data_ptr(), k, dw.data_ptr(), db.data_ptr(), ws.data_ptr(),
                 size, tg.stream_handle()))
             assert ok() and dx_ok() and dw_ok() and db_ok()
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("lead", [1, 2, 3, 5])
+def test_any_alignment(gpu, dtype, lead):
+    """Every operand and result `lead` elements into its memory: the bits of whole ones."""
+    import tinygnn_amd as tg
+    dt = DTYPES[dtype]
+
+    def moved(t):
+        wide = torch.full((t.numel() + lead + 8,), float("nan") if t.is_floating_point() else -7,
+                          dtype=t.dtype, device="cuda")
+        wide[lead:lead + t.numel()] = t.flatten()
+        return wide[lead:lead + t.numel()].view(t.shape)
+
+    def place(*shape):
+        return moved(torch.zeros(shape, dtype=dt, device="cuda"))
+
+    for m, k, n in ((3, 700, 1100), (33, 100, 41), (600, 520, 264)):
+        g = gen(m + lead)
+        for transpose in (False, True):
+            x, w = randn(g, (m, k), dt), randn(g, (n, k) if transpose else (k, n), dt, k ** -0.5)
+            b, r, dy = randn(g, n, dt), randn(g, (m, n), dt), randn(g, (m, n), dt)
+            y = tg.linear(moved(x), moved(w), bias=moved(b), epilogue=tg.EPI_SILU,
+                          residual=moved(r), transpose=transpose, out=place(m, n))
+            want, tol, _, _ = hc.linear(x, w, b, "silu", r, transpose)
+            within(y, want, hc.rounded(want, tol, dt), "y")
+            got = tg.linear_backward(moved(dy), moved(x), moved(w), pre=moved(r),
+                                     epilogue=tg.EPI_SILU, bias=True, transpose=transpose)
+            ref = hc.linear_backward(dy, x, w, r, "silu", transpose, dt)
+            for t, key in zip(got, ("dx", "dw", "db")):
+                within(t, ref[key][0], hc.rounded(*ref[key], dt), key)
+    for rows, classes in ((70, 41), (50, 300), (5, 20_003)):
+        g = gen(classes + lead)
+        z, dv = randn(g, (rows, classes), dt), randn(g, rows, torch.float32)
+        labels = torch.randint(0, classes, (rows,), generator=g, device="cuda").to(I32)
+        t, ids = randn(g, (rows, 5), dt), torch.randint(0, classes, (rows, 5), generator=g,
+                                                        device="cuda").to(I32)
+        a, c = (tg.log_probs(u, v, top=7, entropy=True) for u, v in
+                ((z, labels), (moved(z), moved(labels))))
+        for name in ("value", "entropy", "top_values", "top_ids"):
+            assert torch.equal(getattr(a, name), getattr(c, name)), name
+        assert torch.equal(tg.log_probs_backward(dv, z, labels, a),
+                           tg.log_probs_backward(moved(dv), moved(z), moved(labels), c,
+                                                 out=place(rows, classes)))
+        for u, v in zip(tg.distill(z, t, ids, dloss=dv),
+                        tg.distill(moved(z), moved(t), moved(ids), dloss=moved(dv),
+                                   out=place(rows, classes))):
+            assert torch.equal(u, v)
 
 
 def test_far_rows(gpu):

@@ -70,6 +70,18 @@ def test_log_probs(gpu, rows, classes, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,classes", [(1, 20_001), (1, 40_003), (127, 20_003), (127, 40_005),
+                                          (128, 48_001), (130, 151_001), (1023, 95_005),
+                                          (1024, 95_001)])
+def test_rows_whole_and_cut(gpu, rows, classes, dtype):
+    """At both sides of where rows are cut."""
+    g, x, labels = make(rows, classes, DTYPES[dtype], rows + classes)
+    dvalue, dentropy = (torch.randn(rows, generator=g, device="cuda") for _ in range(2))
+    for top in (0, 20):
+        check_log_probs(x, labels, top, 0.9, dvalue, dentropy)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("rows,classes", SIZES)
 def test_distill(gpu, rows, classes, dtype):
     import tinygnn_amd as tg

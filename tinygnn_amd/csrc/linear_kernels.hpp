@@ -183,7 +183,7 @@ __device__ __forceinline__ void store_sums(const LinearArgs& a, int part, int m0
 
 // y = the epilogue of the parts' sums: Y threads take every Y-th part of four
 // results, whose sums are added in order.  Bound by reading the parts: 4,000 x 2,048
-// in two 18.7 us.
+// in two 19.4 us.
 template <typename T, int Y>
 __global__ __launch_bounds__(256) void join_kernel(LinearArgs a) {
     constexpr int X = 256 / Y;
@@ -306,8 +306,10 @@ constexpr int kMinWaves = sizeof(T) == 4 && S::kM * S::kN == 8192 ? 3 : 1;
 
 // A tile of S::kM x S::kN results in the registers of 256 threads, its operands by two
 // tiles of LDS in turn.  Bound by the matrix instructions: floats, whose instruction
-// has an eighth of the rate: 232,965 x 256 x 256 forward 367 us with the store of pre
-// and y (83 TFLOP/s; 281 without pre, 109), its d w^T 318 (96), its x^T d 300 (102).
+// has an eighth of the rate, and beside them by the results: 232,965 x 256 x 256 forward
+// 380 us with residual, pre and y, 0.95 GB (80 TFLOP/s; 289 with bias alone, 106), its
+// d w^T 322 (95), its x^T d 317 (96).  They are busy for 77% of the cycles, at the 2.1
+// GHz that their power leaves.
 template <typename T, typename S, bool AX, bool AW, bool DIRECT>
 __global__ __launch_bounds__(S::kThreads, (kMinWaves<T, S>)) void linear_kernel(LinearArgs a) {
     __shared__ __attribute__((aligned(16))) char a0[S::kM * kRowBytes];

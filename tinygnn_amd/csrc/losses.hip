@@ -32,20 +32,26 @@ LossArgs loss_args(int64_t rows, int64_t classes, const void* logits, int64_t ld
     return a;
 }
 
-// How rows are cut: one segment, but where there are few of more than 16,384
-// classes (as many as give 512 workgroups of 4,096 classes at least, 64 at most;
-// 1 x 102,400 bf16 in one 20 us, in 25 with the join 11.4),
-// and longer ones than a workgroup holds.  (A distillation with its gradient reads
-// cut rows twice, the others once.)
+// How rows are cut: one segment, but few long rows: of more than 80,000 bytes where
+// there are fewer than 128 (as many as give 256 workgroups), of 190,000, with top
+// classes 300,000, where fewer than 1,024 (1,024 workgroups), each of 4,096 classes at
+// least, 64 at most; and rows longer than a workgroup holds.  Over 1 to 1,500 rows of
+// 20,000 to 250,000 fp32 and bf16 within 3% in the mean of the best of 1, 256, 512
+// and 1,024 workgroups: 1 x 131,072 fp32 with 20 top classes 18.0 us in two, 10.5 in
+// 32; 200 x 131,072 fp32 28.0 in 400, 21.3 in 1,200; but 1 x 20,000 fp32 4.3 in one, 5.2
+// in five, 200 x 100,003 bf16 15.9 in 200, 20.6 in 400.  (A distillation with its
+// gradient reads cut rows twice, the others once.)
 struct Cut {
     int64_t segment, segments;
 };
 
-Cut cut_of(int64_t rows, int64_t classes, int type) {
+Cut cut_of(int64_t rows, int64_t classes, int type, bool tops) {
     const int64_t vec = 16 / type_size(type), most = kMostChunks * vec;
+    const bool some = rows < 128;
     int64_t segments = 1;
-    if (rows < 1024 && classes > 16384)
-        segments = std::min<int64_t>({ceil_div(512, rows), ceil_div(classes, 4096), 64});
+    if (rows < 1024 && classes * type_size(type) > (some ? 80000 : tops ? 300000 : 190000))
+        segments =
+            std::min<int64_t>({ceil_div(some ? 256 : 1024, rows), ceil_div(classes, 4096), 64});
     segments = std::max(segments, ceil_div(classes, most));
     const int64_t segment = ceil_div(ceil_div(classes, segments), vec) * vec;
     return {segment, ceil_div(classes, segment)};
@@ -62,7 +68,7 @@ struct LossPlace {
 LossPlace loss_place(int64_t rows, int64_t classes, int64_t top, int64_t k, int type, void* ws,
                      size_t size) {
     LossPlace p{};
-    const Cut cut = cut_of(rows, classes, type);
+    const Cut cut = cut_of(rows, classes, type, top > 0);
     if (cut.segments == 1) return p;
     Carver c(ws, size);
     const size_t parts = static_cast<size_t>(rows) * cut.segments;
@@ -79,7 +85,7 @@ LossPlace loss_place(int64_t rows, int64_t classes, int64_t top, int64_t k, int 
 // The workspace's pieces into a; whether the rows are cut.
 bool place_segments(LossArgs& a, int type, void* workspace, size_t bytes, TempBuffer* temp,
                     hipStream_t s) {
-    const Cut cut = cut_of(a.rows, a.classes, type);
+    const Cut cut = cut_of(a.rows, a.classes, type, a.top > 0);
     a.segment = cut.segment;
     a.segments = static_cast<int>(cut.segments);
     if (cut.segments == 1) return false;

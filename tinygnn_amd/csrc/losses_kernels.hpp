@@ -717,10 +717,11 @@ struct MyPlaces {
 
 // One row (kSegment: one segment) for each NT threads: one read of the logits, and
 // for distillation one write of the gradient.  8,192 x 32,000 bf16: log probabilities
-// 130 us (4.0 TB/s); 4,096 x 64,000 bf16 with 32 places and gradient 224 us (4.7).  Top
+// 128 us (4.1 TB/s); 4,096 x 65,536 bf16 with 32 places and gradient 224 (4.8).  Top
 // classes cost beside it the largest of each thread, one sort of those and the few
-// candidates: 64 x 32,000 bf16 with 64 of them and the join 18 us.
-template <typename T, int NT, int NV, int MODE, bool ENTROPY>
+// candidates: 64 x 32,000 bf16 with 64 of them 12.7 us.  (TOPS apart: their registers,
+// 77 of 42, leave one workgroup of 1,024 a CU; 4,096 x 65,536 bf16 134 us -> 95.)
+template <typename T, int NT, int NV, int MODE, bool ENTROPY, bool TOPS>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void row_kernel(LossArgs a) {
     constexpr int kBlock = NT < 256 ? 256 : NT, kRows = kBlock / NT, VEC = kVec<T>;
     extern __shared__ __attribute__((aligned(16))) Key top_lds[];
@@ -753,13 +754,13 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void row_kernel(LossArgs a) {
             a.part[4 * at + 1] = r.s;
             a.part[4 * at + 2] = r.u;
         }
-        if (a.top)
+        if constexpr (TOPS)
             x.tops(a.top, static_cast<uint32_t>(first), lds, &count[sub],
                    [&](int j, Key k) { a.part_keys[at * a.top + j] = k; });
     } else if constexpr (MODE == kLogProbs) {
         const RowStats st(r);
         if (x.tid == 0) put_row<T>(a, row, r, st);
-        if (a.top)
+        if constexpr (TOPS)
             x.tops(a.top, 0, lds, &count[sub], [&](int j, Key k) { put_top(a, row, j, k, st); });
     } else {
         __shared__ Places<NT> places[kRows];
@@ -867,7 +868,7 @@ __global__ __launch_bounds__(NT) void join_kernel(LossArgs a) {
 
 // ---------------------------------------------------------------------------
 // The gradient of rows whose statistics are known: a wavefront takes kSpan chunks
-// a lane of one row, one read and one write; 8,192 x 32,000 bf16 178 us (5.9 TB/s,
+// a lane of one row, one read and one write; 8,192 x 32,000 bf16 174 us (6.0 TB/s,
 // the end of what log_probs read still in the caches).
 // ---------------------------------------------------------------------------
 constexpr int kSpan = 4;
@@ -964,8 +965,8 @@ __global__ __launch_bounds__(256) void gradient_kernel(LossArgs a, int64_t spans
 // Few classes: a thread takes a row.  64 rows come through LDS (so that memory is
 // read and written in whole lines), their rows an odd number of floats apart.  A
 // workgroup is one wavefront, so that many stand at different points of load, sums and
-// store; 232,965 x 41 fp32 from memory: log probabilities 14.6 us (2.6 TB/s), their
-// gradient 23.6 (3.2), distillation with its gradient 33.3.  What it waits for is the
+// store; 232,965 x 41 fp32: log probabilities 14.4 us (2.8 TB/s), their gradient 22.9
+// (3.5), distillation with its gradient 34.  What it waits for is the
 // turns of the three in a wavefront; the next rows' loads ahead of the sums spilled.
 // ---------------------------------------------------------------------------
 // e / classes: magic = 2^32 / classes rounded up (0 for one class); exact below
@@ -1244,21 +1245,26 @@ void sliced(LossArgs a, int64_t threads, F&& fn) {
     });
 }
 
-template <typename T, int MODE, bool ENTROPY>
+template <typename T, int MODE, bool ENTROPY, bool TOPS>
 void launch_rows(const char* what, const LossArgs& all, hipStream_t s) {
     const int64_t each = MODE == kSegment ? all.segments : 1;
+    const int64_t length = MODE == kSegment ? all.segment : all.classes;
     auto launch = [&](auto nt, auto nv) {
         constexpr int NT = decltype(nt)::value, NV = decltype(nv)::value;
         constexpr int kBlock = NT < 256 ? 256 : NT, kRows = kBlock / NT;
-        const size_t lds = sizeof(Key) * kRows * top_keys(NT, all.top);
-        auto kernel = row_kernel<T, NT, NV, MODE, ENTROPY>;
+        // (rows that fill the registers, read alone: LDS for four workgroups a CU.  Six
+        // have more loads in flight than the memory likes: 8,192 x 32,000 bf16 95 us ->
+        // 90, with its gradient 303 -> 296; 8,192 x 16,000 fp32 87 -> 85; but 20,000 x
+        // 10,000 bf16, which leaves most registers empty, 71 -> 86)
+        const bool four = NT == 256 && !TOPS && MODE != kDistill && length > 12 * NT * kVec<T>;
+        const size_t lds = four ? 36 * 1024 : sizeof(Key) * kRows * top_keys(NT, all.top);
+        auto kernel = row_kernel<T, NT, NV, MODE, ENTROPY, TOPS>;
         sliced(all, each * NT, [&](const LossArgs& a, int64_t rows) {
             const unsigned grid = grid_of(what, ceil_div(rows * each, kRows), kBlock);
             kernel<<<grid, kBlock, lds, s>>>(a);
             TG_LAUNCH_CHECK();
         });
     };
-    const int64_t length = MODE == kSegment ? all.segment : all.classes;
     if (MODE == kLogProbs && all.top <= 1)
         with_shape<MODE == kLogProbs>(all.rows * each, length, kVec<T>, launch);
     else
@@ -1328,12 +1334,17 @@ void launch_log_probs(const LossArgs& a, bool cut, hipStream_t s) {
         constexpr bool E = decltype(ent)::value;
         if (tiny_rows(a)) {
             launch_tiny<T, kLogProbs, E, false>("log_probs", a, s);
-        } else if (cut) {
-            launch_rows<T, kSegment, E>("log_probs", a, s);
-            launch_join<T, kLogProbs>("log_probs", a, s);
-        } else {
-            launch_rows<T, kLogProbs, E>("log_probs", a, s);
+            return;
         }
+        with_bool(a.top > 0, [&](auto tops) {
+            constexpr bool K = decltype(tops)::value;
+            if (cut) {
+                launch_rows<T, kSegment, E, K>("log_probs", a, s);
+                launch_join<T, kLogProbs>("log_probs", a, s);
+            } else {
+                launch_rows<T, kLogProbs, E, K>("log_probs", a, s);
+            }
+        });
     });
 }
 
@@ -1355,11 +1366,11 @@ void launch_distill(const LossArgs& a, bool cut, hipStream_t s) {
             launch_tiny<T, kDistill, false, decltype(grad)::value>("distill", a, s);
         });
     } else if (cut) {
-        launch_rows<T, kSegment, false>("distill", a, s);
+        launch_rows<T, kSegment, false, false>("distill", a, s);
         launch_join<T, kDistill>("distill", a, s);
         if (a.dlogits) launch_gradient<T, kDistill, false>("distill", a, s);
     } else {
-        launch_rows<T, kDistill, false>("distill", a, s);
+        launch_rows<T, kDistill, false, false>("distill", a, s);
     }
 }
 
