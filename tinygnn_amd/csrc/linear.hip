@@ -10,7 +10,15 @@
 namespace tg {
 namespace {
 
-constexpr int64_t kLongChain = 16384;  // of floats: 64 chains of kSumTiles tiles
+// The longest contraction of one part.  Floats: 64 chains of kSumTiles tiles.  16-bit
+// operands, whose sums are one chain that the instructions add eight products at a
+// time to: n values of one sign are off by n 2^-27 of their sum at most, here
+// half the result's own rounding (2^-11, 2^-8).  (In one chain, fp16 4,096 x 4,096 of
+// constant columns, contraction 262,144, was 9.8e-4 off; one rounding is 4.9e-4.  In
+// eight parts the product takes 7.51 ms, in one 7.50.)
+int64_t long_chain(int type) {
+    return type == TG_TYPE_F32 ? 16384 : type == TG_TYPE_F16 ? 32768 : 262144;
+}
 
 // The time of a product in us by tile, as measured: a tile of `m` x `n` results
 // alone on a CU takes `alone` for each value of the contraction, one of many `busy`
@@ -59,9 +67,7 @@ LinearPlans linear_plans(int64_t m, int64_t n, int64_t k, int type) {
         for (int64_t parts = 1; parts <= 256; parts *= 2) {
             if (parts > 1 && (k < 2 * depth * parts || tiles * parts > 2048)) break;
             int64_t unit = ceil_div(ceil_div(k, parts), depth) * depth;
-            // (the digits of long chains of floats)
-            if (type == TG_TYPE_F32) unit = std::min(unit, kLongChain);
-            unit = std::max(unit, depth);
+            unit = std::max(std::min(unit, long_chain(type)), depth);
             const int64_t real = std::max<int64_t>(1, ceil_div(k, unit)), groups = tiles * real;
             const double load = groups < 256 ? static_cast<double>(groups) * (1.0 / 256)
                                              : static_cast<double>((groups + 255) / 256);
