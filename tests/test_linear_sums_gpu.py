@@ -33,3 +33,44 @@ def test_one_sign_of_16_bits(gpu, dtype, k, layout):
                         transpose=layout == "transposed")
     own = (half_step(dt) / 2 + 66 * U) * want
     within(got, want, own + half_step(dt) * (want + own), layout)
+
+
+def integers(g, shape, dt):
+    """-1, 0 and 1: sums of up to 2^24 products are exact in float32 in any order."""
+    return torch.randint(-1, 2, shape, generator=g, device="cuda").to(dt)
+
+
+def exact(x, w):
+    """x @ w of integers: sums of 4,096 products, exact in float32, in 64 bits."""
+    out = torch.zeros(x.shape[0], w.shape[1], dtype=torch.float64, device="cuda")
+    for at in range(0, x.shape[1], 4096):
+        out += x[:, at:at + 4096].float() @ w[at:at + 4096].float()
+    return out
+
+
+@pytest.mark.parametrize("layout", ["dw", "y", "transposed"])
+@pytest.mark.parametrize("dtype,m,k,n", [
+    ("f32", 8192, 100_001, 8000),    # 7 parts, 4 at a time
+    ("f16", 8192, 200_004, 8000),    # in whole chunks: 7 parts of the large tile
+    ("f16", 8191, 200_001, 8001),    # through registers
+    ("f32", 12_000, 40_000, 12_004),  # 3 parts, 2 at a time
+    ("f32", 2056, 300_000, 1032),    # 19 parts at once
+])
+def test_parts_at_a_time(gpu, dtype, m, k, n, layout):
+    import tinygnn_amd as tg
+    dt, g = DTYPES[dtype], gen(m)
+    x, w = integers(g, (m, k), dt), integers(g, (k, n), dt)
+    want = exact(x, w)
+    if layout == "dw":
+        x = x.t().contiguous()
+        got = tg.linear_backward(w, x, torch.ones(m, n, dtype=dt, device="cuda"))[1]
+    else:
+        bias, residual = integers(g, (n,), dt), integers(g, (m, n), dt)
+        if layout == "transposed":
+            w = w.t().contiguous()
+        got, pre = tg.linear(x, w, bias=bias, residual=residual, epilogue=tg.EPI_RELU,
+                             transpose=layout == "transposed", with_pre=True)
+        want += bias
+        assert torch.equal(pre, want.to(dt))
+        want = want.clamp_min(0) + residual
+    assert torch.equal(got, want.to(dt))

@@ -20,6 +20,10 @@ int64_t long_chain(int type) {
     return type == TG_TYPE_F32 ? 16384 : type == TG_TYPE_F16 ? 32768 : 262144;
 }
 
+// Bytes of the parts' sums that a product keeps at a time, where it can: two of
+// them, one of which is the sum of those before, at the least.
+constexpr int64_t kKeptBytes = int64_t(1) << 30;
+
 // The time of a product in us by tile, as measured: a tile of `m` x `n` results
 // alone on a CU takes `alone` for each value of the contraction, one of many `busy`
 // of the CU's time, and `fixed` beside that (lookup, first loads, results).
@@ -46,6 +50,11 @@ enum Loads { kRegisters, kDirect, kRing };
 struct LinearPlans {
     LinearPlan of[3];  // by Loads
 };
+
+int64_t kept_parts(int64_t m, int64_t n, int64_t parts) {
+    const int64_t fit = m > 0 && n > 0 ? kKeptBytes / 4 / m / n : parts;
+    return std::min(parts, std::max<int64_t>(2, fit));
+}
 
 // How an out [m x n] with contraction k is cut: the tile and the parts of the
 // contraction that the costs above and the parts' join (2.5 us, its bytes at 9 TB/s,
@@ -82,7 +91,7 @@ LinearPlans linear_plans(int64_t m, int64_t n, int64_t k, int type) {
                 if ((l == kRegisters && !square) || (l != kRing && large) || us >= least[l])
                     continue;
                 least[l] = us;
-                best.of[l] = {t.m, t.n, mt, nt, unit, real};
+                best.of[l] = {t.m, t.n, mt, nt, unit, real, kept_parts(m, n, real)};
             }
         }
     };

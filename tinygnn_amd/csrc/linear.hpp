@@ -26,8 +26,9 @@ struct LinearArgs {
     int64_t ldp;
     uint32_t mt, nt;
     int unit;     // contraction of a part
-    int parts;
-    float* part;  // [parts][m][n], or null: one part, straight to y
+    int parts;    // (join) whose sums stand at part
+    bool more;    // (join) and others come: no results yet
+    float* part;  // [kept parts][m][n], or null: one part, straight to y
 };
 
 struct ActArgs {
@@ -45,8 +46,9 @@ struct ActArgs {
 struct LinearPlan {
     int64_t em, en;  // the tile
     int64_t mt, nt, unit, parts;
+    int64_t kept;  // parts whose sums stand in the workspace at a time
     size_t bytes(int64_t m, int64_t n) const {
-        return parts > 1 ? static_cast<size_t>(parts) * m * n * 4 : 0;
+        return parts > 1 ? static_cast<size_t>(kept) * m * n * 4 : 0;
     }
 };
 
