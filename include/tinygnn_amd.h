@@ -499,8 +499,8 @@ int tg_matmul_fp8(int64_t m, int64_t k, int64_t n, int64_t groups, const void* x
  *   dbias = the sum of d's rows before that rounding
  * (any of the three may be NULL; the residual's gradient is dy).  Sums in fp32,
  * equal calls give equal bits.  With m = 0 dw and dbias are zeros, with n = 0 dx.
- * workspace: the size function's bytes (for dx, dw and dbias, whichever are
- * asked for), or NULL.
+ * workspace: the size function's bytes, or NULL: those of a call with this act and
+ * (dbias != 0) with dbias, or of any call of these sizes.
  * ------------------------------------------------------------------------ */
 enum { TG_EPI_GELU = 3, TG_EPI_SILU = 4 }; /* tg_linear's alone */
 size_t tg_linear_workspace_size(int64_t m, int64_t k, int64_t n, int type);
@@ -509,6 +509,8 @@ int tg_linear(int64_t m, int64_t k, int64_t n, int type, const void* x, int64_t 
               const void* residual, int64_t ldr, void* y, int64_t ldy, void* pre, int64_t ldp,
               void* workspace, size_t workspace_bytes, tg_stream_t stream);
 size_t tg_linear_backward_workspace_size(int64_t m, int64_t k, int64_t n, int type);
+size_t tg_linear_backward_call_workspace_size(int64_t m, int64_t k, int64_t n, int type, int act,
+                                              int dbias);
 int tg_linear_backward(int64_t m, int64_t k, int64_t n, int type, const void* dy, int64_t lddy,
                        const void* x, int64_t ldx, const void* w, int64_t ldw, int transposed,
                        const void* pre, int64_t ldp, int act, void* dx, int64_t lddx, void* dw,

@@ -31,3 +31,18 @@ def test_parts_of_large_results(kind):
     m = n = 40_000
     assert L.tg_linear_workspace_size(m, 1_000_000, n, kind) == 2 * 4 * m * n
     assert L.tg_linear_workspace_size(m, 1000, n, kind) == 0
+
+
+def test_backward_asks_for_what_it_uses():
+    """d is there with an epilogue alone, parts of dbias with dbias alone."""
+    L = _lib.lib.load()
+    m, k, n = 16_384, 32_000, 2048
+    size = L.tg_linear_backward_call_workspace_size
+    for kind, z in ((F32, 4), (BF16, 2), (F16, 2)):
+        assert L.tg_linear_workspace_size(m, n, k, kind) == 0      # (dx, dw: of one part)
+        plain, bias = size(m, k, n, kind, 0, 0), size(m, k, n, kind, 0, 1)
+        assert plain == 0 and 0 < bias < m * n
+        assert size(m, k, n, kind, 3, 0) == m * n * z
+        assert size(m, k, n, kind, 3, 1) == m * n * z + bias \
+            == L.tg_linear_backward_workspace_size(m, k, n, kind)
+    assert size(m, k, n, F32, 9, 0) == size(m, k, n, 7, 0, 0) == size(0, k, n, F32, 0, 0) == 0

@@ -74,3 +74,23 @@ def test_parts_at_a_time(gpu, dtype, m, k, n, layout):
         assert torch.equal(pre, want.to(dt))
         want = want.clamp_min(0) + residual
     assert torch.equal(got, want.to(dt))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_memory_of_a_plain_backward(gpu, dtype):
+    """A product without an epilogue: dx, dw and dbias with its few parts, no d."""
+    import tinygnn_amd as tg
+    dt = DTYPES[dtype]
+    m, k, n = 16_384, 1024, 8192
+    x, w, dy = (torch.zeros(s, dtype=dt, device="cuda") for s in ((m, k), (k, n), (m, n)))
+    for _ in range(2):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        out = tg.linear_backward(dy, x, w, bias=True)
+        used = torch.cuda.max_memory_allocated() - before
+        parts = tg.lib.tg_linear_workspace_size(k, m, n, tg.TYPE_F32 if dt == torch.float32 else
+                                                tg.TYPE_BF16)
+        results = sum(t.numel() * t.element_size() for t in out)
+        assert used <= results + parts + 16 * 2 ** 20, (used, results, parts)
+        del out

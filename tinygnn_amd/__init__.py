@@ -994,7 +994,7 @@ def linear_backward(dy, x, w, pre=None, epilogue: int = EPI_NONE, bias: bool = F
     dx = _pt.empty((m, k), dtype=x.dtype, device=x.device)
     dw = _pt.empty(w.shape, dtype=x.dtype, device=x.device)
     db = _pt.empty(n, dtype=x.dtype, device=x.device) if bias else None
-    size = lib.tg_linear_backward_workspace_size(m, k, n, kind)
+    size = lib.tg_linear_backward_call_workspace_size(m, k, n, kind, epilogue, 1 if bias else 0)
     ws, pws = _workspace(size, x)
     lib.check(lib.tg_linear_backward(m, k, n, kind, pd, lddy, px, ldx, pw, ldw,
                                      1 if transpose else 0, pp, ldp, epilogue, dx.data_ptr(),

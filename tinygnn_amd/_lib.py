@@ -120,6 +120,7 @@ SIGNATURES = {
     "tg_linear": (i32, [i64, i64, i64, i32, vp, i64, vp, i64, i32, vp, i32, vp, i64, vp, i64, vp,
                         i64, vp, sz, vp]),
     "tg_linear_backward_workspace_size": (sz, [i64, i64, i64, i32]),
+    "tg_linear_backward_call_workspace_size": (sz, [i64, i64, i64, i32, i32, i32]),
     "tg_linear_backward": (i32, [i64, i64, i64, i32, vp, i64, vp, i64, vp, i64, i32, vp, i64, i32,
                                  vp, i64, vp, vp, vp, sz, vp]),
     "tg_log_probs_workspace_size": (sz, [i64, i64, i64, i32]),

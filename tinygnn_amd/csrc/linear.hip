@@ -258,8 +258,14 @@ int tg_linear(int64_t m, int64_t k, int64_t n, int type, const void* x, int64_t 
 }
 
 size_t tg_linear_backward_workspace_size(int64_t m, int64_t k, int64_t n, int type) {
+    return tg_linear_backward_call_workspace_size(m, k, n, type, TG_EPI_SILU, 1);
+}
+
+size_t tg_linear_backward_call_workspace_size(int64_t m, int64_t k, int64_t n, int type, int act,
+                                              int dbias) {
     if (m <= 0 || k < 0 || n <= 0 || type < TG_TYPE_F32 || type > TG_TYPE_F16) return 0;
-    return tg::backward_bytes(m, k, n, type, TG_EPI_SILU, true);
+    if (act < TG_EPI_NONE || act > TG_EPI_SILU) return 0;
+    return tg::backward_bytes(m, k, n, type, act, dbias != 0);
 }
 
 int tg_linear_backward(int64_t m, int64_t k, int64_t n, int type, const void* dy, int64_t lddy,
