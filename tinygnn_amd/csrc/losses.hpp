@@ -45,7 +45,7 @@ struct LossArgs {
     int segments;
     float* part;      // [rows][segments][4]: m, s, u
     Key* part_keys;   // [rows][segments][top]
-    float* row_part;  // distillation: [rows][4]: m, log2 s, factor
+    float* row_part;  // distillation: [rows][4]: m, factor / s, factor
     float* q;         // [rows][k]
 };
 
