@@ -44,8 +44,18 @@ struct RowStats {
         : m(r.m), log_s(r.s == 0.0f ? 0.0f : logf(r.s)) {}
     __device__ __forceinline__ RowStats(float m_, float log_s_) : m(m_), log_s(log_s_) {}
     __device__ __forceinline__ bool empty() const { return m == -INFINITY && log_s == 0.0f; }
+    // Half of x - m, which may lie past the largest float where both are finite and
+    // their log probability is.
+    __device__ __forceinline__ float half_gap(float x) const {
+        return __builtin_fmaf(0.5f, x, -0.5f * m);
+    }
     __device__ __forceinline__ float logp(float x, float inv) const {
-        return (x - m) * inv - log_s;
+        return half_gap(x) * (2.0f * inv) - log_s;
+    }
+    // q (log_q - log p), q > 0: infinite only where that is.
+    __device__ __forceinline__ float divergence(float q, float log_q, float x, float inv) const {
+        if (empty()) return q * INFINITY;
+        return __builtin_fmaf(q, log_q + log_s, -(q * half_gap(x)) * (2.0f * inv));
     }
     __device__ __forceinline__ float entropy(const RowSums& r) const {
         return r.s == 0.0f ? 0.0f : log_s - kLn2 * r.u / r.s;
@@ -621,10 +631,8 @@ __device__ __forceinline__ Teacher teach_of(const LossArgs& a, int64_t row, cons
         const int j = i * kWave + lane;
         const float q = total == 0.0f ? 0.0f : e[i] / total;
         if (j < a.k) put_q(j, q);
-        if (j < a.k && q != 0.0f) {
-            const float logp = st.empty() ? -INFINITY : st.logp(xs[i], a.inv);
-            loss += q * ((t[i] - tm) * a.inv - log_total - logp);
-        }
+        if (j < a.k && q != 0.0f)
+            loss += st.divergence(q, (t[i] - tm) * a.inv - log_total, xs[i], a.inv);
     }
     return {wave_all(loss, Add{}), total};
 }
@@ -1159,12 +1167,11 @@ __global__ __launch_bounds__(kWave) void tiny_kernel(LossArgs a, uint32_t magic,
             // loss = sum of q (log q - logp), log q = z - log total
             each([&](float tj, int cj) {
                 const float e = tj == -INFINITY ? 0.0f : exp2_of((tj - tm) * a.c);
-                const float logp = st.empty() ? -INFINITY : st.logp(x[cj], a.inv);
                 total += e;
                 // (a 64th of each: of 64 places at most, so that the sum of terms near
                 // the largest float is one)
                 if (e != 0.0f)
-                    loss = __builtin_fmaf(e * (1.0f / kTinyPlaces), (tj - tm) * a.inv - logp, loss);
+                    loss += st.divergence(e * (1.0f / kTinyPlaces), (tj - tm) * a.inv, x[cj], a.inv);
             });
             const float per = total == 0.0f ? 0.0f : 1.0f / total;
             loss = total == 0.0f ? 0.0f : loss * per * kTinyPlaces - logf(total);
