@@ -94,3 +94,22 @@ def test_memory_of_a_plain_backward(gpu, dtype):
         results = sum(t.numel() * t.element_size() for t in out)
         assert used <= results + parts + 16 * 2 ** 20, (used, results, parts)
         del out
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 300_000, 41), (512, 300_001, 520), (2056, 300_001, 1032),
+                                   (128, 40_000, 24)])
+def test_one_sign_of_floats(gpu, m, k, n):
+    """Chains of 256 values, 64 of those at most in a part, 512 parts at most in a
+    chain of their own: that many steps of 2^-24, of sums that only grow."""
+    import tinygnn_amd as tg
+    g = gen(k)
+    x, dy = (1 + torch.rand((k, c), generator=g, device="cuda") for c in (m, n))
+    want = torch.zeros(m, n, dtype=torch.float64, device="cuda")
+    for at in range(0, k, 50_000):
+        want += x[at:at + 50_000].double().t().contiguous() @ dy[at:at + 50_000].double()
+    parts = tg.lib.tg_linear_workspace_size(m, k, n, tg.TYPE_F32) // (4 * m * n)
+    assert 0 < parts <= 512
+    for got in (tg.linear_backward(dy, x, torch.ones(m, n, device="cuda"))[1],
+                tg.linear(x.t().contiguous(), dy),
+                tg.linear(x.t().contiguous(), dy.t().contiguous(), transpose=True)):
+        within(got, want, (256 + 64 + parts + 2) * U * want, "sums")
