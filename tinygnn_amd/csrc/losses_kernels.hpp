@@ -62,14 +62,6 @@ struct RowStats {
     }
 };
 
-// e and e z of one logit.  A masked one's z is kept finite: its e is 0.
-__device__ __forceinline__ void add_class(float x, float m, float c, float* s, float* u) {
-    const float z = (x - m) * c;
-    const float e = exp2_of(z);
-    *s += e;
-    *u = __builtin_fmaf(e, __builtin_fmaxf(z, -1000.0f), *u);
-}
-
 // What a row's gradient needs: e = exp2(z), z = (x - m) c, and
 //   d = e (f + h z), f and h of the row, 1 / s among them.
 // (With log2 s in the exponent its rounding, of numbers up to 17, was one of every p:
@@ -400,6 +392,7 @@ struct Held {
                 const float z = (v[e] - base) * c;
                 const float ex = exp2_of(z);
                 si += ex;
+                // (a masked one's z is kept finite: its exponential is 0)
                 if (ENTROPY) ui = __builtin_fmaf(ex, __builtin_fmaxf(z, -1000.0f), ui);
             }
             s += si;
