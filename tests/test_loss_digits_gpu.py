@@ -44,3 +44,41 @@ def test_log_probs(gpu, rows, classes):
     want = want.clone()
     want[:, 0] += g[:, 0]
     within(d, want, 5 * U * want.abs(), "dlogits")
+
+
+@pytest.mark.parametrize("rows,classes", [(500, 2), (500, 7), (500, 41), (500, 53), (9000, 64),
+                                          (9, 65), (700, 201), (40, 256)])
+def test_the_same_distribution(gpu, rows, classes):
+    """A teacher of all classes' logits, all equal: both logarithms are those of the same
+    whole number, and every place's difference is 0."""
+    import tinygnn_amd as tg
+    x = torch.full((rows, classes), 0.75, device="cuda")
+    ids = torch.arange(classes, device="cuda").to(I32).repeat(rows, 1)
+    teacher = torch.full((rows, classes), -2.0, device="cuda")
+    for temperature in (1.0, 3.0):
+        loss = tg.distill(x, teacher, ids, temperature=temperature)
+        assert not loss.any(), loss.abs().max()
+        loss, d = tg.distill(x, teacher, ids, temperature=temperature,
+                             dloss=torch.ones(rows, device="cuda"))
+        assert not loss.any()
+        # (p, q and their products by 1 / T: a few roundings of 1 / classes)
+        within(d, torch.zeros_like(d), 10 * U / classes, "dlogits")
+
+
+def test_loss_of_random_rows(gpu):
+    """Losses of 41 classes in the 2-norm: no more than half as far again from 64
+    bits as place by place in float32."""
+    import head_cases as hc
+    import tinygnn_amd as tg
+    from expert_cases import gen, randn
+    g, rows, classes, k = gen(3), 20_000, 41, 8
+    x = randn(g, (rows, classes), torch.float32, 2.0)
+    teacher, ids = torch.topk(x + 0.7 * randn(g, (rows, classes), torch.float32), k, 1)
+    ids = ids.to(I32)
+    want, _ = hc.distill(hc.Row(x, 2.0), teacher, ids, 2.0)
+    z = (x - x.max(1, keepdim=True)[0]) * 0.5
+    t = (teacher - teacher.max(1, keepdim=True)[0]) * 0.5
+    q, log_q = torch.softmax(t, 1), torch.log_softmax(t, 1)
+    plain = (q * (log_q - torch.gather(torch.log_softmax(z, 1), 1, ids.long()))).sum(1)
+    off = [(v.double() - want).norm() for v in (plain, tg.distill(x, teacher, ids, temperature=2.0))]
+    assert off[1] <= 1.5 * off[0], off
