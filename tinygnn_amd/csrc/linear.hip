@@ -103,7 +103,7 @@ LinearPlans linear_plans(int64_t m, int64_t n, int64_t k, int type) {
 }
 
 // Few rows of x with w's rows along the contraction (few_kernel): one launch, no
-// parts.  Measured against the tiles with theirs (bf16, 1 row: 4,096 x 4,096 7.2 us
+// parts.  Measured against the tiles with theirs, each after itself (bf16, 1 row: 4,096 x 4,096 7.2 us
 // against 8.5, 512 x 8,192 4.2 against 6.0, 2,048 x 128 4.5 against 5.6; but 8,192 x
 // 1,024 11.5 against 7.1, 4,096 x 64 6.6 against 5.3, 1,024 x 32,000 17.3 against 14.8;
 // 32 rows of 4,096 x 4,096 14.6 against 13.2; fp32, 16 rows of 2,048 x 128 10.9 against

@@ -471,7 +471,8 @@ using Tall = Shape<128, 64, 2, 2>;
 // Up to 16 rows of x, w's rows along the contraction: 16 columns by the 16 wavefronts of
 // a workgroup, which take turns of 128 bytes of the contraction, loaded straight to
 // the matrix instructions' operands; their sums are added in order.  Bound by
-// reading w once: 1 x 4,096 x 4,096 bf16 7.2 us (4.7 TB/s).
+// reading w once: 1 x 4,096 x 4,096 bf16 8.9 us (3.8 TB/s) where other work ran between;
+// 7.2 after itself, when part of the 32 MB may still be in the last-level cache.
 // ---------------------------------------------------------------------------
 constexpr int kFewWaves = 16;
 

@@ -730,7 +730,8 @@ struct MyPlaces {
 
 // One row (kSegment: one segment) for each NT threads: one read of the logits, and
 // for distillation one write of the gradient.  8,192 x 32,000 bf16: log probabilities
-// 128 us (4.1 TB/s); 4,096 x 65,536 bf16 with 32 places and gradient 224 (4.8).  Top
+// 128 us (4.1 TB/s) behind the gradient of other rows, whose writes still leave the
+// caches, 92 after each other; 4,096 x 65,536 bf16 with 32 places and gradient 224 (4.8).  Top
 // classes cost beside it the largest of each thread, one sort of those and the few
 // candidates: 64 x 32,000 bf16 with 64 of them 12.7 us.  (TOPS apart: their registers,
 // 77 of 42, leave one workgroup of 1,024 a CU; 4,096 x 65,536 bf16 134 us -> 95.)
@@ -975,8 +976,8 @@ __global__ __launch_bounds__(256) void gradient_kernel(LossArgs a, int64_t spans
 // Few classes: a thread takes a row.  64 rows come through LDS (so that memory is
 // read and written in whole lines), their rows an odd number of floats apart.  A
 // workgroup is one wavefront, so that many stand at different points of load, sums and
-// store; 232,965 x 41 fp32: log probabilities 14.4 us (2.8 TB/s), their gradient 22.9
-// (3.5), distillation with its gradient 34.  What it waits for is the
+// store; 232,965 x 41 fp32: log probabilities 14.1 us (2.8 TB/s), their gradient 23.5
+// (3.4), distillation with its gradient 34.8.  What it waits for is the
 // turns of the three in a wavefront; the next rows' loads ahead of the sums spilled.
 // ---------------------------------------------------------------------------
 // e / classes: magic = 2^32 / classes rounded up (0 for one class); exact below
@@ -1260,8 +1261,8 @@ void launch_rows(const char* what, const LossArgs& all, hipStream_t s) {
         constexpr int NT = decltype(nt)::value, NV = decltype(nv)::value;
         constexpr int kBlock = NT < 256 ? 256 : NT, kRows = kBlock / NT;
         // (rows that fill the registers, read alone: LDS for four workgroups a CU.  Six
-        // have more loads in flight than the memory likes: 8,192 x 32,000 bf16 95 us ->
-        // 90, with its gradient 303 -> 296; 8,192 x 16,000 fp32 87 -> 85; but 20,000 x
+        // have more loads in flight than the memory likes: 8,192 x 32,000 bf16, the
+        // same rows again, 95 us -> 90, with its gradient 303 -> 296; 8,192 x 16,000 fp32 87 -> 85; but 20,000 x
         // 10,000 bf16, which leaves most registers empty, 71 -> 86)
         const bool four = NT == 256 && !TOPS && MODE != kDistill && length > 12 * NT * kVec<T>;
         const size_t lds = four ? 36 * 1024 : sizeof(Key) * kRows * top_keys(NT, all.top);

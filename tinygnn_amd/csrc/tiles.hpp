@@ -236,7 +236,8 @@ __device__ __forceinline__ void multiply(const RA& ra, const RB& rb, const char*
 // 256, was 8.9e-7 off with it and is 3.1e-7; 2.27 -> 2.31 ms.)  16-bit products
 // are one chain, to which the instructions add eight at a time: n of one sign are
 // off by n 2^-27 of their sum at most, n^(1/2) 2^-25 or so of random ones; the
-// result's own rounding is 2^-9 or 2^-12.
+// result's own rounding is 2^-8 or 2^-11 at most.  (The dense layers' chains stop at
+// half of it.)
 template <typename T, int N, int M>
 struct Sums {
     v4f now[N][M] = {}, all[sizeof(T) == 4 ? N : 1][sizeof(T) == 4 ? M : 1] = {};
