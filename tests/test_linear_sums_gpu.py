@@ -113,3 +113,27 @@ def test_one_sign_of_floats(gpu, m, k, n):
                 tg.linear(x.t().contiguous(), dy),
                 tg.linear(x.t().contiguous(), dy.t().contiguous(), transpose=True)):
         within(got, want, (256 + 64 + parts + 2) * U * want, "sums")
+
+
+def test_parts_at_a_time_captured(gpu):
+    """The launches of later parts in a graph: replayed on new inputs, eager calls with a
+    workspace of their own in between."""
+    import tinygnn_amd as tg
+    g, m, k, n = gen(9), 12_000, 40_000, 12_004
+    x, w = integers(g, (m, k), torch.float32), integers(g, (k, n), torch.float32)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        tg.linear(x, w)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = tg.linear(x, w)
+    for _ in range(3):
+        x.copy_(integers(g, (m, k), torch.float32))
+        want = tg.linear(x, w)
+        y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+    assert torch.equal(y, exact(x, w).float())
